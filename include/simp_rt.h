@@ -385,6 +385,134 @@ int32_t simp_rt_rope(
     float *k_alloc, float *k, int64_t k_off, int64_t k_size, int64_t k_stride,
     int64_t dim, int64_t kv_dim, int64_t head_size, int64_t pos, double theta);
 
+/* ---------------------------------------------- attention of a batch -- */
+/* No counterparts in the reference: its programs attend one token of one
+ * sequence at a time over an fp32 cache (examples/llama2/stories110M.sl:115-164).
+ * These serve several sequences of different lengths at once. */
+
+/* Causal attention of packed sequences: sequence s has the queries
+ * q[q_starts[s] .. q_starts[s+1]) and the keys and values
+ * k, v[k_starts[s] .. k_starts[s+1]), q and out [rows, heads, head_size], k and v
+ * [rows, kv_heads, head_size] (heads a multiple of kv_heads; query head h reads
+ * kv head h / (heads / kv_heads); rows may be strided, as in a fused qkv
+ * product).  The last query sees the last key: query i of nq sees the keys
+ * j <= i + nk - nq of its sequence, so that nk > nq goes on after nk - nq earlier
+ * tokens.  out = sum_j p_j v_j with p = softmax(scale * q . k_j) over the keys seen; a
+ * query that sees none (nk < nq) gets zeros; a key that a query does not see has
+ * no part in its row, whatever its values.  Rows of out that belong to no
+ * sequence stay as they are.  starts: i32, increasing, sequences + 1 of them;
+ * values outside the rows are cut off at them.  head_size 1 to 256.  out may
+ * share no memory range with the inputs.  Sums and statistics are fp32, and the
+ * products as close as fp32 ones. */
+int32_t simp_rt_attention_packed_f32(
+    const float *q_alloc, const float *q, int64_t q_off, int64_t q_s0, int64_t q_s1, int64_t q_s2,
+    int64_t q_st0, int64_t q_st1, int64_t q_st2,
+    const float *k_alloc, const float *k, int64_t k_off, int64_t k_s0, int64_t k_s1, int64_t k_s2,
+    int64_t k_st0, int64_t k_st1, int64_t k_st2,
+    const float *v_alloc, const float *v, int64_t v_off, int64_t v_s0, int64_t v_s1, int64_t v_s2,
+    int64_t v_st0, int64_t v_st1, int64_t v_st2,
+    float *out_alloc, float *out, int64_t out_off, int64_t out_s0, int64_t out_s1, int64_t out_s2,
+    int64_t out_st0, int64_t out_st1, int64_t out_st2,
+    const int32_t *qst_alloc, const int32_t *q_starts, int64_t qst_off, int64_t qst_size, int64_t qst_stride,
+    const int32_t *kst_alloc, const int32_t *k_starts, int64_t kst_off, int64_t kst_size, int64_t kst_stride,
+    double scale);
+
+/* A key/value cache of 8-bit codes for a batch of sequences, with an fp32 scale
+ * for each block of `block` tokens, head, and K or V: token t of sequence b and
+ * head h has the value k[..., d] * k_scale[..., t / block].  Code (b, h, t, d) is
+ * at b*st_seq + h*st_head + t*st_token + d, scale (b, h, j) at b*sc_seq +
+ * h*sc_head + j, in elements, for K and V alike.  Codes are -127 .. 127.  All four
+ * arrays are device memory or registered ranges (they are the caller's; the
+ * struct only says where they lie).  block is 16, 32, 64 or 128; head_size a
+ * multiple of 4 from 16 to 256; code rows start on 4-byte boundaries; tokens of a
+ * head, and heads, may be in either order ([heads, capacity] or [capacity, heads]). */
+typedef struct {
+  int8_t *k, *v;
+  float *k_scale, *v_scale; /* ceil(capacity / block) per sequence and head */
+  int64_t batch, n_kv_heads, capacity, head_size, block;
+  int64_t st_seq, st_head, st_token, sc_seq, sc_head;
+} simp_rt_kv8;
+
+/* The calls below take lengths[batch] (i32): the tokens that each sequence has
+ * in the cache, those of the call included.  Nothing here changes them: layers share
+ * them, and the caller raises them once per step.  starts[batch + 1] (i32,
+ * increasing) packs the rows of all sequences, as above. */
+
+/* Stores K and V rows [rows, kv_heads, head_size]: the n_b = starts[b+1] -
+ * starts[b] rows of sequence b go to its positions lengths[b] - n_b .. lengths[b]-1
+ * (positions outside [0, capacity) are dropped).  The scale of a block becomes
+ * s = max(its scale, where it held earlier tokens of the sequence; max|x| / 127
+ * of its new rows), new codes are x / s rounded to nearest (ties to even, of the
+ * exact quotient), and the earlier tokens' codes c become c * (s_before / s),
+ * ratio and product in 64 bits, rounded the same; a block of zeros has the scale
+ * 0.  A block that is given a NaN or an infinity has a scale that is not finite
+ * and codes 0: its values read NaN. */
+int32_t simp_rt_kv8_append(
+    const simp_rt_kv8 *cache,
+    const float *k_alloc, const float *k, int64_t k_off, int64_t k_s0, int64_t k_s1, int64_t k_s2,
+    int64_t k_st0, int64_t k_st1, int64_t k_st2,
+    const float *v_alloc, const float *v, int64_t v_off, int64_t v_s0, int64_t v_s1, int64_t v_s2,
+    int64_t v_st0, int64_t v_st1, int64_t v_st2,
+    const int32_t *st_alloc, const int32_t *starts, int64_t st_off, int64_t st_size, int64_t st_stride,
+    const int32_t *len_alloc, const int32_t *lengths, int64_t len_off, int64_t len_size, int64_t len_stride);
+
+/* The values (code * scale) of the last starts[b+1] - starts[b] tokens of each
+ * sequence into the packed rows k and v [rows, kv_heads, head_size]: what
+ * simp_rt_attention_packed_f32 needs of a prompt's earlier tokens.  Rows of
+ * positions outside [0, capacity) become zeros; rows that belong to no sequence
+ * stay as they are. */
+int32_t simp_rt_kv8_read(
+    const simp_rt_kv8 *cache,
+    const int32_t *st_alloc, const int32_t *starts, int64_t st_off, int64_t st_size, int64_t st_stride,
+    const int32_t *len_alloc, const int32_t *lengths, int64_t len_off, int64_t len_size, int64_t len_stride,
+    float *k_alloc, float *k, int64_t k_off, int64_t k_s0, int64_t k_s1, int64_t k_s2,
+    int64_t k_st0, int64_t k_st1, int64_t k_st2,
+    float *v_alloc, float *v, int64_t v_off, int64_t v_s0, int64_t v_s1, int64_t v_s2,
+    int64_t v_st0, int64_t v_st1, int64_t v_st2);
+
+/* Attention of one query per sequence (the last token's) over its tokens 0 ..
+ * lengths[b]-1 (at most capacity): q and out [batch, heads, head_size], out =
+ * sum_t p_t v_t, p = softmax(scale * q . k_t); zeros for a sequence of no tokens.
+ * seen_in and seen_out [batch, kv_heads, capacity] (both or neither: null
+ * pointers, sizes 0) add up the weight that each token receives: seen_out =
+ * seen_in + the sum of p over the heads that share the kv head, for the tokens
+ * below the length; the rest stays as it is.  They may be the same array, and
+ * share no range otherwise.  Sums and statistics are fp32; q is rounded to 24 bits of
+ * its largest element, and the products with the codes are exact. */
+int32_t simp_rt_kv8_attention(
+    const simp_rt_kv8 *cache,
+    const float *q_alloc, const float *q, int64_t q_off, int64_t q_s0, int64_t q_s1, int64_t q_s2,
+    int64_t q_st0, int64_t q_st1, int64_t q_st2,
+    const int32_t *len_alloc, const int32_t *lengths, int64_t len_off, int64_t len_size, int64_t len_stride,
+    float *out_alloc, float *out, int64_t out_off, int64_t out_s0, int64_t out_s1, int64_t out_s2,
+    int64_t out_st0, int64_t out_st1, int64_t out_st2,
+    const float *si_alloc, const float *seen_in, int64_t si_off, int64_t si_s0, int64_t si_s1, int64_t si_s2,
+    int64_t si_st0, int64_t si_st1, int64_t si_st2,
+    float *so_alloc, float *seen_out, int64_t so_off, int64_t so_s0, int64_t so_s1, int64_t so_s2,
+    int64_t so_st0, int64_t so_st1, int64_t so_st2,
+    double scale);
+
+/* Cuts every sequence to `budget` tokens per head, into another cache of the same
+ * batch, heads, head_size and block, whose arrays share no range with the first's
+ * (a layer's old cache can be the next layer's new one): the last `recent` (0 ..
+ * budget) tokens stay, and of the others those with the largest seen[batch,
+ * kv_heads, capacity] (ties: the lowest position; a NaN counts as the
+ * largest), in their order.  A sequence of up to `budget` tokens stays whole.  The new
+ * lengths are min(lengths, budget).  kept[batch, kv_heads, budget] (i32) receives
+ * the positions that stayed, then -1; new_seen[batch, kv_heads, >= budget] their
+ * weights (the rest stays as it is).  A new block's scale is the largest of its
+ * tokens' scales, and their codes are rounded to it as in simp_rt_kv8_append. */
+int32_t simp_rt_kv8_evict(
+    const simp_rt_kv8 *cache, const simp_rt_kv8 *to,
+    const int32_t *len_alloc, const int32_t *lengths, int64_t len_off, int64_t len_size, int64_t len_stride,
+    const float *se_alloc, const float *seen, int64_t se_off, int64_t se_s0, int64_t se_s1, int64_t se_s2,
+    int64_t se_st0, int64_t se_st1, int64_t se_st2,
+    float *ns_alloc, float *new_seen, int64_t ns_off, int64_t ns_s0, int64_t ns_s1, int64_t ns_s2,
+    int64_t ns_st0, int64_t ns_st1, int64_t ns_st2,
+    int32_t *kept_alloc, int32_t *kept, int64_t kept_off, int64_t kept_s0, int64_t kept_s1, int64_t kept_s2,
+    int64_t kept_st0, int64_t kept_st1, int64_t kept_st2,
+    int64_t budget, int64_t recent);
+
 /* ------------------------------------------------------- decode step -- */
 
 #define SIMP_RT_W_F32 0 /* fp32 weight matrices */

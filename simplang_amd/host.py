@@ -78,6 +78,11 @@ _sig("simp_rt_softmax", _D1 * 2 + [_I, _I, _I])
 _sig("simp_rt_silu", _D1 * 2 + [_I])
 _sig("simp_rt_swiglu", _D1 * 3 + [_I])
 _sig("simp_rt_rope", _D1 * 2 + [_I, _I, _I, _I, C.c_double])
+_sig("simp_rt_attention_packed_f32", _D3 * 4 + _D1 * 2 + [C.c_double])
+_sig("simp_rt_kv8_append", [_P] + _D3 * 2 + _D1 * 2)
+_sig("simp_rt_kv8_read", [_P] + _D1 * 2 + _D3 * 2)
+_sig("simp_rt_kv8_attention", [_P] + _D3 + _D1 + _D3 * 3 + [C.c_double])
+_sig("simp_rt_kv8_evict", [_P, _P] + _D1 + _D3 * 3 + [_I, _I])
 _sig("simp_rt_llama_create", [_P, _P, _P])
 _sig("simp_rt_llama_destroy", [_P])
 _sig("simp_rt_llama_forward", [_P, _I, _I, _P])
@@ -520,6 +525,131 @@ def rope(q, k, dim, kv_dim, head_size, pos, theta=10000.0):
     _check("simp_rt_rope", lib.simp_rt_rope(*desc1(q), *desc1(k), dim, kv_dim, head_size, pos,
                                             theta))
     return q, k
+
+
+# ----------------------------------------------------- attention of a batch
+
+def _typed(fn, name, x, dtype):
+    """x, which must be an array or tensor of the given type."""
+    if str(x.dtype).replace("torch.", "") != dtype:
+        raise TypeError(f"{fn}: {name} must be {dtype}, not {x.dtype}")
+    return x
+
+
+def _f3(fn, name, x):
+    return descn(_typed(fn, name, x, "float32"), 3)
+
+
+def _i1(fn, name, x):
+    return desc1(_typed(fn, name, x, "int32"))
+
+
+def attention_packed(q, k, v, out, q_starts, k_starts, scale=None):
+    """Causal attention of packed sequences: q and out [rows, heads, head_size], k and v
+    [rows, kv_heads, head_size], fp32; sequence s has the rows starts[s] .. starts[s + 1]
+    (int32) of each.  The last query of a sequence sees its last key, so more keys than
+    queries go on after earlier tokens; a query that sees no key gets zeros.  scale:
+    1 / sqrt(head_size) by default."""
+    fn = "attention_packed"
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    _check(fn, lib.simp_rt_attention_packed_f32(
+        *_f3(fn, "q", q), *_f3(fn, "k", k), *_f3(fn, "v", v), *_f3(fn, "out", out),
+        *_i1(fn, "q_starts", q_starts), *_i1(fn, "k_starts", k_starts), scale))
+    return out
+
+
+class _KV8(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, C.c_int64) for n in ("batch", "n_kv_heads", "capacity", "head_size", "block",
+                                 "st_seq", "st_head", "st_token", "sc_seq", "sc_head")]
+
+
+class KV8Cache:
+    """A key/value cache of 8-bit codes with one fp32 scale per block of tokens and
+    head (simp_rt_kv8) over device tensors that the caller allocates: ``k`` and ``v``
+    int8 [batch, kv_heads, capacity, head_size] (any strides whose rows do not overlap:
+    a [batch, capacity, kv_heads, head_size] array is passed transposed), ``k_scale`` and
+    ``v_scale`` float32 [batch, kv_heads, ceil(capacity / block)].  ``block``: 16, 32, 64
+    or 128.  The tensors are kept alive here.
+
+    ``lengths`` (int32 [batch]) counts the tokens that each sequence has, those of the
+    call included; no call changes it.  ``starts`` (int32 [batch + 1]) packs the rows of
+    all sequences as in :func:`attention_packed`."""
+
+    def __init__(self, k, v, k_scale, v_scale, block):
+        fn = "KV8Cache"
+        if len(k.shape) != 4 or tuple(v.shape) != tuple(k.shape):
+            raise ValueError("KV8Cache: k and v must be [batch, kv_heads, capacity, head_size]")
+        b, h, cap, hs = (int(x) for x in k.shape)
+        if tuple(k_scale.shape) != (b, h, -(-cap // block)) or tuple(v_scale.shape) != tuple(k_scale.shape):
+            raise ValueError("KV8Cache: scales must be [batch, kv_heads, ceil(capacity / block)]")
+        kd, vd = _strides4(_typed(fn, "k", k, "int8")), _strides4(_typed(fn, "v", v, "int8"))
+        ks = descn(_typed(fn, "k_scale", k_scale, "float32"), 3)
+        vs = descn(_typed(fn, "v_scale", v_scale, "float32"), 3)
+        if kd[1:] != vd[1:] or ks[3:] != vs[3:]:
+            raise ValueError("KV8Cache: k and v, and their scales, must have the same strides")
+        if kd[4] != 1 or ks[8] != 1:
+            raise ValueError("KV8Cache: the innermost stride must be 1")
+        self._tensors = (k, v, k_scale, v_scale)
+        self.batch, self.kv_heads, self.capacity, self.head_size, self.block = b, h, cap, hs, block
+        self._c = _KV8(kd[0], vd[0], ks[0], vs[0], b, h, cap, hs, block, kd[1], kd[2], kd[3],
+                       ks[6], ks[7])
+        self._ref = C.byref(self._c)
+
+    def append(self, k, v, starts, lengths) -> None:
+        """Stores packed fp32 rows [rows, kv_heads, head_size]: those of sequence b become
+        its tokens lengths[b] - n_b .. lengths[b] - 1."""
+        fn = "KV8Cache.append"
+        _check(fn, lib.simp_rt_kv8_append(self._ref, *_f3(fn, "k", k), *_f3(fn, "v", v),
+                                          *_i1(fn, "starts", starts), *_i1(fn, "lengths", lengths)))
+
+    def read(self, starts, lengths, k, v):
+        """The values of the last starts[b + 1] - starts[b] tokens of each sequence into
+        packed fp32 rows."""
+        fn = "KV8Cache.read"
+        _check(fn, lib.simp_rt_kv8_read(self._ref, *_i1(fn, "starts", starts),
+                                        *_i1(fn, "lengths", lengths), *_f3(fn, "k", k),
+                                        *_f3(fn, "v", v)))
+        return k, v
+
+    def attention(self, q, lengths, out, seen=None, seen_out=None, scale=None):
+        """Attention of one query per sequence, q and out [batch, heads, head_size] fp32, over
+        its tokens.  seen and seen_out [batch, kv_heads, capacity] (both or neither; they may
+        be the same tensor): seen_out = seen + the weight each token received."""
+        fn = "KV8Cache.attention"
+        if (seen is None) != (seen_out is None):
+            raise ValueError("KV8Cache.attention: seen and seen_out go together")
+        if scale is None:
+            scale = self.head_size ** -0.5
+        d = (_NO3, _NO3) if seen is None else (_f3(fn, "seen", seen), _f3(fn, "seen_out", seen_out))
+        _check(fn, lib.simp_rt_kv8_attention(self._ref, *_f3(fn, "q", q), *_i1(fn, "lengths", lengths),
+                                             *_f3(fn, "out", out), *d[0], *d[1], scale))
+        return out
+
+    def evict(self, to: "KV8Cache", lengths, seen, new_seen, kept, budget: int, recent: int = 0):
+        """Cuts every sequence to ``budget`` tokens per head into the cache ``to``: the last
+        ``recent`` and those that ``seen`` ranks highest.  ``new_seen`` receives their weights,
+        ``kept`` (int32 [batch, kv_heads, budget]) their positions, then -1.  The new lengths
+        are min(lengths, budget)."""
+        fn = "KV8Cache.evict"
+        _check(fn, lib.simp_rt_kv8_evict(self._ref, to._ref, *_i1(fn, "lengths", lengths),
+                                         *_f3(fn, "seen", seen), *_f3(fn, "new_seen", new_seen),
+                                         *descn(_typed(fn, "kept", kept, "int32"), 3), budget, recent))
+        return kept
+
+
+_NO3 = [None, None] + [0] * 7
+
+
+def _strides4(x):
+    """(pointer, strides...) of a rank-4 array in elements, in any order of its
+    dimensions; 0 for a dimension of one element, whose stride says nothing."""
+    if _is_torch(x):
+        p, st = x.data_ptr(), x.stride()
+    else:
+        p, st = x.ctypes.data, [s // x.itemsize for s in x.strides]
+    return [p, *(0 if n == 1 else s for n, s in zip(x.shape, st))]
 
 
 # ------------------------------------------------------------------ decode

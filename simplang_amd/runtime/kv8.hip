@@ -1,0 +1,660 @@
+// kv8.hip -- a key/value cache of 8-bit codes with an fp32 scale per block of tokens
+// and head: storing rows, reading them back, attention of one query per sequence
+// over it, and cutting sequences down to the tokens that attention used most.
+#include <cmath>
+
+#include "rt_device.h"
+#include "serve_args.h"
+
+namespace simp {
+namespace {
+
+// A simp_rt_kv8 as the kernels take it: device addresses, the block as a shift.
+struct Cache {
+  int8_t *k, *v;
+  float *ks, *vs;
+  int64_t st_seq, st_head, st_token, sc_seq, sc_head;
+  int n, hk, cap, hs, shift;
+};
+
+__device__ __forceinline__ int64_t clampl(int64_t x, int64_t lo, int64_t hi) {
+  return x < lo ? lo : x > hi ? hi : x;
+}
+
+// max that a NaN comes through
+__device__ __forceinline__ float max_nan(float a, float b) { return a != a || a > b ? a : b; }
+
+// Nearest code to x / s (ties to even, of the exact quotient), s > 0 and finite.
+__device__ __forceinline__ int code_of(float x, float s) {
+  return (int)fminf(fmaxf((float)rint((double)x / (double)s), -127.f), 127.f);
+}
+
+// ---------------------------------------------------------------- append
+
+struct AppendArgs {
+  Cache c;
+  const float *k, *v;
+  const int *starts, *lengths;
+  int64_t k_row, k_head, v_row, v_head;
+  int rows;
+};
+
+// One block of one head, K or V (blockIdx.z).  Sequence b has the slots starts[b] /
+// T + 2 b and on: n rows touch at most n / T + 2 blocks.
+__global__ void __launch_bounds__(256) kv8_append_k(const AppendArgs a) {
+  __shared__ float scratch[16];
+  __shared__ int bad;
+  const Cache &c = a.c;
+  const int t = blockIdx.x, h = blockIdx.y, T = 1 << c.shift;
+  int lo = 0, hi = c.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((int)clampl(a.starts[mid], 0, a.rows) / T + 2 * mid <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  const int b = lo;
+  const int r0 = (int)clampl(a.starts[b], 0, a.rows), r1 = (int)clampl(a.starts[b + 1], r0, a.rows);
+  const int64_t end = a.lengths[b], have = end - (r1 - r0);  // positions of the new rows
+  const int64_t from = clampl(have, 0, c.cap), to = clampl(end, 0, c.cap);
+  const int64_t blk = (from >> c.shift) + (t - (r0 / T + 2 * b));
+  const int64_t p0 = blk << c.shift, p1 = min(p0 + T, to);
+  if (t < r0 / T + 2 * b || from >= to || p0 >= to) return;
+  const int64_t first = max(p0, from);  // tokens p0 .. first-1 are there already
+  const bool is_v = blockIdx.z != 0;
+  const float *x = is_v ? a.v : a.k;
+  const int64_t row = is_v ? a.v_row : a.k_row;
+  x += (int64_t)r0 * row + h * (is_v ? a.v_head : a.k_head);
+  int8_t *codes = (is_v ? c.v : c.k) + b * c.st_seq + h * c.st_head;
+  float *sc = (is_v ? c.vs : c.ks) + b * c.sc_seq + h * c.sc_head + blk;
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  float top = 0.f;
+  bool odd = false;
+  const int nw = (int)(p1 - first) * c.hs;
+  for (int e = threadIdx.x; e < nw; e += 256) {
+    const int i = e / c.hs, d = e - i * c.hs;
+    const float f = fabsf(x[(first + i - have) * row + d]);
+    top = fmaxf(top, f);
+    odd |= !(f < INFINITY);
+  }
+  if (odd) bad = 1;
+  const float before = first > p0 ? *sc : 0.f;
+  top = block_max(top, scratch);  // its barriers order `bad` and the read of the scale too
+  float s = max_nan(before, top / 127.f);
+  if (bad) s = NAN;
+  const bool live = s > 0.f && s < INFINITY;
+  const int no = (int)(first - p0) * c.hs;
+  if (!(before == s)) {  // what the block held, to the new scale
+    const double ratio = live ? (double)before / (double)s : 0.0;
+    for (int e = threadIdx.x; e < no; e += 256) {
+      const int i = e / c.hs, d = e - i * c.hs;
+      int8_t *p = codes + (p0 + i) * c.st_token + d;
+      *p = live ? (int8_t)(int)rint(*p * ratio) : 0;
+    }
+  }
+  for (int e = threadIdx.x; e < nw; e += 256) {
+    const int i = e / c.hs, d = e - i * c.hs;
+    codes[(first + i) * c.st_token + d] =
+        live ? (int8_t)code_of(x[(first + i - have) * row + d], s) : 0;
+  }
+  if (threadIdx.x == 0) *sc = s;
+}
+
+// ------------------------------------------------------------------ read
+
+struct ReadArgs {
+  Cache c;
+  const int *starts, *lengths;
+  float *k, *v;
+  int64_t k_row, k_head, v_row, v_head;
+  int rows;
+};
+
+// One packed row of one head, K or V (blockIdx.z).
+__global__ void __launch_bounds__(64) kv8_read_k(const ReadArgs a) {
+  const Cache &c = a.c;
+  const int r = blockIdx.x, h = blockIdx.y;
+  int lo = 0, hi = c.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (clampl(a.starts[mid], 0, a.rows) <= r) lo = mid;
+    else hi = mid - 1;
+  }
+  const int b = lo;
+  const int r0 = (int)clampl(a.starts[b], 0, a.rows), r1 = (int)clampl(a.starts[b + 1], r0, a.rows);
+  if (r < r0 || r >= r1) return;
+  const int64_t p = (int64_t)a.lengths[b] - (r1 - r);
+  const bool in = p >= 0 && p < c.cap, is_v = blockIdx.z != 0;
+  const int8_t *codes = (is_v ? c.v : c.k) + b * c.st_seq + h * c.st_head + (in ? p : 0) * c.st_token;
+  const float s = in ? (is_v ? c.vs : c.ks)[b * c.sc_seq + h * c.sc_head + (p >> c.shift)] : 0.f;
+  float *out = (is_v ? a.v : a.k) + r * (is_v ? a.v_row : a.k_row) + h * (is_v ? a.v_head : a.k_head);
+  for (int d = threadIdx.x; d < c.hs; d += 64) out[d] = in ? codes[d] * s : 0.f;
+}
+
+// ------------------------------------------------------------- attention
+
+struct AttnArgs {
+  Cache c;
+  const float *q;
+  const int *lengths;
+  float *out;
+  const float *seen_in;
+  float *seen_out;
+  int64_t q_seq, q_head, o_seq, o_head, si_seq, si_head, so_seq, so_head;
+  int heads, group;
+  float scale;
+  float *scores;  // [n, heads, cap]
+  float2 *stat;   // [n, heads]: maximum and sum
+};
+
+// One query head: scores, maximum and sum, then the weighted sum of V.
+__global__ void __launch_bounds__(256) kv8_attn_k(const AttnArgs a) {
+  __shared__ float scratch[16];
+  __shared__ float q[256];
+  const Cache &c = a.c;
+  const int h = blockIdx.x, b = blockIdx.y, hk = h / a.group;
+  const int len = (int)clampl(a.lengths[b], 0, c.cap);
+  const int64_t at = b * c.st_seq + hk * c.st_head, sat = b * c.sc_seq + hk * c.sc_head;
+  float *sc = a.scores + ((int64_t)b * a.heads + h) * c.cap;
+  for (int d = threadIdx.x; d < c.hs; d += 256) q[d] = a.q[b * a.q_seq + h * a.q_head + d];
+  __syncthreads();
+  float m = -INFINITY;
+  for (int t = threadIdx.x; t < len; t += 256) {
+    const int8_t *k = c.k + at + t * c.st_token;
+    float s = 0.f;
+    for (int d = 0; d < c.hs; d++) s = fmaf(q[d], (float)k[d], s);
+    s *= c.ks[sat + (t >> c.shift)] * a.scale;
+    sc[t] = s;
+    m = fmaxf(m, s);
+  }
+  m = block_max(m, scratch);
+  const float mu = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  for (int t = threadIdx.x; t < len; t += 256) l += expf(sc[t] - mu);
+  l = block_sum(l, scratch);
+  if (threadIdx.x == 0) a.stat[b * a.heads + h] = make_float2(mu, l);
+  if ((int)threadIdx.x < c.hs) {
+    float o = 0.f;
+    for (int t = 0; t < len; t++)
+      o = fmaf(expf(sc[t] - mu) * c.vs[sat + (t >> c.shift)],
+               (float)c.v[at + t * c.st_token + threadIdx.x], o);
+    a.out[b * a.o_seq + h * a.o_head + threadIdx.x] = len ? o / l : 0.f;
+  }
+}
+
+__global__ void __launch_bounds__(256) kv8_seen_k(const AttnArgs a) {
+  const Cache &c = a.c;
+  const int t = blockIdx.x * 256 + threadIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  if (t >= (int)clampl(a.lengths[b], 0, c.cap)) return;
+  float w = a.seen_in[b * a.si_seq + hk * a.si_head + t];
+  for (int g = 0; g < a.group; g++) {
+    const int64_t row = (int64_t)b * a.heads + hk * a.group + g;
+    const float2 ml = a.stat[row];
+    w += expf(a.scores[row * c.cap + t] - ml.x) / ml.y;
+  }
+  a.seen_out[b * a.so_seq + hk * a.so_head + t] = w;
+}
+
+// ----------------------------------------------------------------- evict
+
+struct EvictArgs {
+  Cache c, to;
+  const int *lengths;
+  const float *seen;
+  float *new_seen;
+  int *kept;
+  int64_t se_seq, se_head, ns_seq, ns_head, kp_seq, kp_head;
+  int budget, recent;
+};
+
+// Unsigned order of the weights: NaN above all, both zeros alike.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  if (x != x) return 0xFFFFFFFFu;
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Which tokens stay: the weight of the last one that does, byte by byte from the top
+// (a histogram of the byte among the weights that share the bytes above it), then
+// the places in order.
+__global__ void __launch_bounds__(1024) kv8_select_k(const EvictArgs a) {
+  __shared__ int hist[256];
+  __shared__ uint32_t prefix_s;
+  __shared__ int need_s, wave_eq[16], wave_keep[16];
+  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int len = (int)clampl(a.lengths[b], 0, a.c.cap);
+  const float *seen = a.seen + b * a.se_seq + hk * a.se_head;
+  float *ns = a.new_seen + b * a.ns_seq + hk * a.ns_head;
+  int *kept = a.kept + b * a.kp_seq + hk * a.kp_head;
+  if (len <= a.budget) {
+    for (int t = tid; t < a.budget; t += 1024) {
+      kept[t] = t < len ? t : -1;
+      if (t < len) ns[t] = seen[t];
+    }
+    return;
+  }
+  const int old = len - a.recent;  // candidates 0 .. old-1
+  int need = a.budget - a.recent;  // of which so many stay (need < old)
+  uint32_t prefix = 0;
+  for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
+    if (tid < 256) hist[tid] = 0;
+    __syncthreads();
+    for (int t = tid; t < old; t += 1024) {
+      const uint32_t u = order_of(seen[t]);
+      if (shift == 24 || (u ^ prefix) >> (shift + 8) == 0)
+        atomicAdd(&hist[u >> shift & 255], 1);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int byte = 255, left = need;
+      while (byte > 0 && hist[byte] < left) left -= hist[byte--];
+      prefix_s = prefix | (uint32_t)byte << shift;
+      need_s = left;
+    }
+    __syncthreads();
+    prefix = prefix_s;
+    need = need_s;
+  }
+  // `need` of the tokens with the weight `prefix` stay, the first ones
+  const bool any = a.budget > a.recent;
+  int eq0 = 0, keep0 = 0;
+  for (int t0 = 0; t0 < len; t0 += 1024) {
+    const int t = t0 + tid;
+    const uint32_t u = t < old ? order_of(seen[t]) : 0;
+    const bool eq = any && t < old && u == prefix;
+    const unsigned long long below = (1ull << (tid & 63)) - 1, be = __ballot(eq);
+    if ((tid & 63) == 0) wave_eq[tid >> 6] = __popcll(be);
+    __syncthreads();
+    int e = eq0 + __popcll(be & below);
+    for (int w = 0; w < 16; w++) {
+      if (w < tid >> 6) e += wave_eq[w];
+      eq0 += wave_eq[w];
+    }
+    const bool keep = t < len && (t >= old || (any && u > prefix) || (eq && e < need));
+    const unsigned long long bk = __ballot(keep);
+    if ((tid & 63) == 0) wave_keep[tid >> 6] = __popcll(bk);
+    __syncthreads();
+    int k = keep0 + __popcll(bk & below);
+    for (int w = 0; w < 16; w++) {
+      if (w < tid >> 6) k += wave_keep[w];
+      keep0 += wave_keep[w];
+    }
+    if (keep && k < a.budget) {
+      kept[k] = t;
+      ns[k] = seen[t];
+    }
+    __syncthreads();
+  }
+}
+
+// One block of the new cache, one head, K or V (blockIdx.z & 1).
+__global__ void __launch_bounds__(256) kv8_move_k(const EvictArgs a) {
+  __shared__ int at[128];
+  __shared__ float sc[128];
+  const Cache &c = a.c, &o = a.to;
+  const int blk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z >> 1;
+  const bool is_v = blockIdx.z & 1;
+  const int len = min((int)clampl(a.lengths[b], 0, c.cap), a.budget);
+  const int p0 = blk << o.shift, nt = min(1 << o.shift, len - p0);
+  if (nt <= 0) return;
+  const int *kept = a.kept + b * a.kp_seq + hk * a.kp_head + p0;
+  const float *zs = (is_v ? c.vs : c.ks) + b * c.sc_seq + hk * c.sc_head;
+  for (int i = threadIdx.x; i < nt; i += 256) {
+    at[i] = (int)clampl(kept[i], 0, c.cap - 1);
+    sc[i] = zs[at[i] >> c.shift];
+  }
+  __syncthreads();
+  float s = 0.f;
+  for (int i = 0; i < nt; i++) s = max_nan(s, sc[i]);
+  const bool live = s > 0.f && s < INFINITY;
+  const int8_t *src = (is_v ? c.v : c.k) + b * c.st_seq + hk * c.st_head;
+  int8_t *dst = (is_v ? o.v : o.k) + b * o.st_seq + hk * o.st_head;
+  for (int e = threadIdx.x; e < nt * c.hs; e += 256) {
+    const int i = e / c.hs, d = e - i * c.hs;
+    const double ratio = live ? (double)sc[i] / (double)s : 0.0;
+    dst[(int64_t)(p0 + i) * o.st_token + d] = (int8_t)(int)rint(src[at[i] * c.st_token + d] * ratio);
+  }
+  if (threadIdx.x == 0) (is_v ? o.vs : o.ks)[b * o.sc_seq + hk * o.sc_head + blk] = s;
+}
+
+// ------------------------------------------------------------- host side
+
+// Element extent of one array of the cache, or -1 where rows would overlap.
+int64_t code_span(const simp_rt_kv8 &c) {
+  const int64_t in_head = c.st_head, in_tok = c.st_token, hs = c.head_size;
+  int64_t span;
+  auto step = [](int64_t n, int64_t st, int64_t inner, int64_t *out) {
+    if (n > 1 && st < inner) return false;
+    if (n > 1 && st > (INT64_MAX - inner) / (n - 1)) return false;
+    *out = inner + (n > 1 ? (n - 1) * st : 0);
+    return true;
+  };
+  int64_t a, s;
+  if (step(c.capacity, in_tok, hs, &a) && step(c.n_kv_heads, in_head, a, &s)) span = s;
+  else if (step(c.n_kv_heads, in_head, hs, &a) && step(c.capacity, in_tok, a, &s)) span = s;
+  else return -1;
+  return step(c.batch, c.st_seq, span, &s) ? s : -1;
+}
+
+int64_t scale_span(const simp_rt_kv8 &c) {
+  const int64_t nb = cdiv(c.capacity, c.block);
+  if (c.n_kv_heads > 1 && (c.sc_head < nb || c.sc_head > (INT64_MAX / 8 - nb) / (c.n_kv_heads - 1)))
+    return -1;
+  const int64_t in = nb + (c.n_kv_heads > 1 ? (c.n_kv_heads - 1) * c.sc_head : 0);
+  if (c.batch > 1 && (c.sc_seq < in || c.sc_seq > (INT64_MAX / 8 - in) / (c.batch - 1))) return -1;
+  return in + (c.batch > 1 ? (c.batch - 1) * c.sc_seq : 0);
+}
+
+struct BoundCache {
+  Operand k, v, ks, vs;
+  Cache c;
+  int64_t codes = 0, scales = 0;  // extents
+  bool empty = false;
+  int check(const simp_rt_kv8 *p, const char *fn, const char *name) {
+    if (!p) return set_error(SIMP_RT_EINVAL, "%s: %s: null pointer", fn, name);
+    if (p->batch < 0 || p->n_kv_heads < 0 || p->capacity < 0)
+      return set_error(SIMP_RT_EINVAL, "%s: %s: negative size", fn, name);
+    if (p->block != 16 && p->block != 32 && p->block != 64 && p->block != 128)
+      return set_error(SIMP_RT_EINVAL, "%s: %s: block %lld is not 16, 32, 64 or 128", fn, name,
+                       (long long)p->block);
+    if (p->head_size < 16 || p->head_size > 256 || p->head_size % 4 != 0)
+      return set_error(SIMP_RT_EUNSUPPORTED,
+                       "%s: %s: head_size %lld is not a multiple of 4 in 16..256", fn, name,
+                       (long long)p->head_size);
+    if (p->batch > 32767 || p->n_kv_heads > 32767 || p->capacity > INT32_MAX - 4096)
+      return set_error(SIMP_RT_EUNSUPPORTED, "%s: %s: batch or heads above 32767, or capacity above 2^31 - 4097",
+                       fn, name);
+    empty = p->batch == 0 || p->n_kv_heads == 0 || p->capacity == 0;
+    if (empty) return SIMP_RT_OK;
+    codes = code_span(*p);
+    scales = scale_span(*p);
+    if (codes < 0 || scales < 0)
+      return set_error(SIMP_RT_EINVAL, "%s: %s: strides let rows overlap", fn, name);
+    if (!p->k || !p->v || !p->k_scale || !p->v_scale)
+      return set_error(SIMP_RT_EINVAL, "%s: %s: null pointer", fn, name);
+    if (((uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->k_scale | (uintptr_t)p->v_scale |
+         (uintptr_t)p->st_seq | (uintptr_t)p->st_head | (uintptr_t)p->st_token) & 3)
+      return set_error(SIMP_RT_EINVAL, "%s: %s: rows and scales must start on 4-byte boundaries", fn, name);
+    return SIMP_RT_OK;
+  }
+  // Whether a byte range lies in one of the cache's arrays.
+  bool shares(const simp_rt_kv8 *p, const void *q, size_t n) const {
+    return overlap(q, n, p->k, (size_t)codes) || overlap(q, n, p->v, (size_t)codes) ||
+           overlap(q, n, p->k_scale, 4 * (size_t)scales) ||
+           overlap(q, n, p->v_scale, 4 * (size_t)scales);
+  }
+  int bind(const simp_rt_kv8 *p, Operand::Dir dir, int dev) {
+    struct { Operand *o; const void *p; size_t n; const char *name; } a[] = {
+        {&k, p->k, (size_t)codes, "cache k"}, {&v, p->v, (size_t)codes, "cache v"},
+        {&ks, p->k_scale, 4 * (size_t)scales, "cache k_scale"},
+        {&vs, p->v_scale, 4 * (size_t)scales, "cache v_scale"}};
+    for (auto &x : a) {
+      const void *d;
+      int rc;
+      if ((rc = device_view(x.p, x.n, &d, x.name)) ||  // no staging of whole caches
+          (rc = bind_here(*x.o, x.p, x.n, dir, dev, x.name)))
+        return rc;
+    }
+    c.k = (int8_t *)k.dev(), c.v = (int8_t *)v.dev();
+    c.ks = (float *)ks.dev(), c.vs = (float *)vs.dev();
+    c.st_seq = p->st_seq, c.st_head = p->st_head, c.st_token = p->st_token;
+    c.sc_seq = p->sc_seq, c.sc_head = p->sc_head;
+    c.n = (int)p->batch, c.hk = (int)p->n_kv_heads, c.cap = (int)p->capacity, c.hs = (int)p->head_size;
+    c.shift = __builtin_ctz((unsigned)p->block);
+    return SIMP_RT_OK;
+  }
+};
+
+// starts and lengths as every call takes them
+int check_lists(const simp_rt_kv8 &c, const char *fn, const int32_t *starts, int64_t st_off,
+                int64_t st_size, int64_t st_stride, const int32_t *lengths, int64_t len_off,
+                int64_t len_size, int64_t len_stride, bool with_starts) {
+  int rc;
+  if (with_starts) {
+    if ((rc = check_desc1("starts", starts, st_off, st_size, st_stride))) return rc;
+    if (st_size != c.batch + 1)
+      return set_error(SIMP_RT_EINVAL, "%s: starts must have batch + 1 entries", fn);
+  }
+  if ((rc = check_desc1("lengths", lengths, len_off, len_size, len_stride))) return rc;
+  if (len_size != c.batch)
+    return set_error(SIMP_RT_EINVAL, "%s: lengths must have batch entries", fn);
+  return SIMP_RT_OK;
+}
+
+}  // namespace
+}  // namespace simp
+
+using namespace simp;
+
+extern "C" {
+
+int32_t simp_rt_kv8_append(
+    const simp_rt_kv8 *cache, const float *k_alloc, const float *k, int64_t k_off, int64_t k_s0,
+    int64_t k_s1, int64_t k_s2, int64_t k_st0, int64_t k_st1, int64_t k_st2, const float *v_alloc,
+    const float *v, int64_t v_off, int64_t v_s0, int64_t v_s1, int64_t v_s2, int64_t v_st0,
+    int64_t v_st1, int64_t v_st2, const int32_t *st_alloc, const int32_t *starts, int64_t st_off,
+    int64_t st_size, int64_t st_stride, const int32_t *len_alloc, const int32_t *lengths,
+    int64_t len_off, int64_t len_size, int64_t len_stride) {
+  (void)k_alloc; (void)v_alloc; (void)st_alloc; (void)len_alloc;
+  static const char *fn = "kv8_append";
+  int rc;
+  BoundCache bc;
+  Desc3<const float> dk{k, k_off, {k_s0, k_s1, k_s2}, {k_st0, k_st1, k_st2}, 0};
+  Desc3<const float> dv{v, v_off, {v_s0, v_s1, v_s2}, {v_st0, v_st1, v_st2}, 0};
+  if ((rc = bc.check(cache, fn, "cache")) || (rc = dk.check("k")) || (rc = dv.check("v")) ||
+      (rc = check_lists(*cache, fn, starts, st_off, st_size, st_stride, lengths, len_off, len_size,
+                        len_stride, true)))
+    return rc;
+  if (!dk.is(k_s0, cache->n_kv_heads, cache->head_size) || !dv.is(k_s0, k_s1, k_s2))
+    return set_error(SIMP_RT_EINVAL, "kv8_append: k and v must be [rows, n_kv_heads, head_size]");
+  if (bc.empty || k_s0 == 0) return SIMP_RT_OK;
+  if (bc.shares(cache, dk.data(), dk.bytes()) || bc.shares(cache, dv.data(), dv.bytes()))
+    return set_error(SIMP_RT_EINVAL, "kv8_append: rows share memory with the cache");
+  const int64_t slots = k_s0 / cache->block + 2 * cache->batch;
+  if (k_s0 > INT32_MAX || slots * 256 > UINT32_MAX)
+    return set_error(SIMP_RT_EUNSUPPORTED, "kv8_append: more rows than the grid holds");
+  const int dev = ensure_device();
+  if (dev < 0) return dev;
+  Operand ok, ov, os, ol;
+  if ((rc = bc.bind(cache, Operand::kInOut, dev)) ||
+      (rc = bind_here(ok, dk.data(), dk.bytes(), Operand::kIn, dev, "k")) ||
+      (rc = bind_here(ov, dv.data(), dv.bytes(), Operand::kIn, dev, "v")) ||
+      (rc = bind_here(os, starts + st_off, 4 * (size_t)st_size, Operand::kIn, dev, "starts")) ||
+      (rc = bind_here(ol, lengths + len_off, 4 * (size_t)len_size, Operand::kIn, dev, "lengths")))
+    return rc;
+  const AppendArgs a{bc.c, (const float *)ok.dev(), (const float *)ov.dev(), (const int *)os.dev(),
+                     (const int *)ol.dev(), k_st0, k_st1, v_st0, v_st1, (int)k_s0};
+  hipLaunchKernelGGL(kv8_append_k, dim3((unsigned)slots, (unsigned)bc.c.hk, 2), dim3(256), 0,
+                     cur_stream(), a);
+  Operand *ops[] = {&ok, &ov, &os, &ol};
+  return finish(ops, 4);
+}
+
+int32_t simp_rt_kv8_read(
+    const simp_rt_kv8 *cache, const int32_t *st_alloc, const int32_t *starts, int64_t st_off,
+    int64_t st_size, int64_t st_stride, const int32_t *len_alloc, const int32_t *lengths,
+    int64_t len_off, int64_t len_size, int64_t len_stride, float *k_alloc, float *k, int64_t k_off,
+    int64_t k_s0, int64_t k_s1, int64_t k_s2, int64_t k_st0, int64_t k_st1, int64_t k_st2,
+    float *v_alloc, float *v, int64_t v_off, int64_t v_s0, int64_t v_s1, int64_t v_s2,
+    int64_t v_st0, int64_t v_st1, int64_t v_st2) {
+  (void)k_alloc; (void)v_alloc; (void)st_alloc; (void)len_alloc;
+  static const char *fn = "kv8_read";
+  int rc;
+  BoundCache bc;
+  Desc3<float> dk{k, k_off, {k_s0, k_s1, k_s2}, {k_st0, k_st1, k_st2}, 0};
+  Desc3<float> dv{v, v_off, {v_s0, v_s1, v_s2}, {v_st0, v_st1, v_st2}, 0};
+  if ((rc = bc.check(cache, fn, "cache")) || (rc = dk.check("k")) || (rc = dv.check("v")) ||
+      (rc = check_lists(*cache, fn, starts, st_off, st_size, st_stride, lengths, len_off, len_size,
+                        len_stride, true)))
+    return rc;
+  if (!dk.is(k_s0, cache->n_kv_heads, cache->head_size) || !dv.is(k_s0, k_s1, k_s2))
+    return set_error(SIMP_RT_EINVAL, "kv8_read: k and v must be [rows, n_kv_heads, head_size]");
+  if (cache->batch == 0 || cache->n_kv_heads == 0 || k_s0 == 0) return SIMP_RT_OK;
+  if (k_s0 > INT32_MAX || k_s0 * 64 > UINT32_MAX)
+    return set_error(SIMP_RT_EUNSUPPORTED, "kv8_read: more rows than the grid holds");
+  if (bc.empty) return set_error(SIMP_RT_EINVAL, "kv8_read: the cache has no capacity");
+  if (bc.shares(cache, dk.data(), dk.bytes()) || bc.shares(cache, dv.data(), dv.bytes()))
+    return set_error(SIMP_RT_EINVAL, "kv8_read: rows share memory with the cache");
+  const int dev = ensure_device();
+  if (dev < 0) return dev;
+  Operand ok, ov, os, ol;
+  if ((rc = bc.bind(cache, Operand::kIn, dev)) ||
+      (rc = bind_here(ok, dk.data(), dk.bytes(), Operand::kOut, dev, "k")) ||
+      (rc = bind_here(ov, dv.data(), dv.bytes(), Operand::kOut, dev, "v")) ||
+      (rc = bind_here(os, starts + st_off, 4 * (size_t)st_size, Operand::kIn, dev, "starts")) ||
+      (rc = bind_here(ol, lengths + len_off, 4 * (size_t)len_size, Operand::kIn, dev, "lengths")))
+    return rc;
+  const ReadArgs a{bc.c, (const int *)os.dev(), (const int *)ol.dev(), (float *)ok.dev(),
+                   (float *)ov.dev(), k_st0, k_st1, v_st0, v_st1, (int)k_s0};
+  hipLaunchKernelGGL(kv8_read_k, dim3((unsigned)k_s0, (unsigned)bc.c.hk, 2), dim3(64), 0,
+                     cur_stream(), a);
+  Operand *ops[] = {&ok, &ov, &os, &ol};
+  return finish(ops, 4);
+}
+
+int32_t simp_rt_kv8_attention(
+    const simp_rt_kv8 *cache, const float *q_alloc, const float *q, int64_t q_off, int64_t q_s0,
+    int64_t q_s1, int64_t q_s2, int64_t q_st0, int64_t q_st1, int64_t q_st2,
+    const int32_t *len_alloc, const int32_t *lengths, int64_t len_off, int64_t len_size,
+    int64_t len_stride, float *out_alloc, float *out, int64_t out_off, int64_t out_s0,
+    int64_t out_s1, int64_t out_s2, int64_t out_st0, int64_t out_st1, int64_t out_st2,
+    const float *si_alloc, const float *seen_in, int64_t si_off, int64_t si_s0, int64_t si_s1,
+    int64_t si_s2, int64_t si_st0, int64_t si_st1, int64_t si_st2, float *so_alloc,
+    float *seen_out, int64_t so_off, int64_t so_s0, int64_t so_s1, int64_t so_s2, int64_t so_st0,
+    int64_t so_st1, int64_t so_st2, double scale) {
+  (void)q_alloc; (void)len_alloc; (void)out_alloc; (void)si_alloc; (void)so_alloc;
+  static const char *fn = "kv8_attention";
+  int rc;
+  BoundCache bc;
+  Desc3<const float> dq{q, q_off, {q_s0, q_s1, q_s2}, {q_st0, q_st1, q_st2}, 0};
+  Desc3<float> dout{out, out_off, {out_s0, out_s1, out_s2}, {out_st0, out_st1, out_st2}, 0};
+  Desc3<const float> dsi{seen_in, si_off, {si_s0, si_s1, si_s2}, {si_st0, si_st1, si_st2}, 0};
+  Desc3<float> dso{seen_out, so_off, {so_s0, so_s1, so_s2}, {so_st0, so_st1, so_st2}, 0};
+  const bool with = seen_in || seen_out;
+  if ((rc = bc.check(cache, fn, "cache")) || (rc = dq.check("q")) || (rc = dout.check("out")) ||
+      (rc = check_lists(*cache, fn, nullptr, 0, 0, 0, lengths, len_off, len_size, len_stride, false)))
+    return rc;
+  if (with && ((rc = dsi.check("seen_in")) || (rc = dso.check("seen_out")))) return rc;
+  if (!dq.is(cache->batch, q_s1, cache->head_size) || !dout.is(q_s0, q_s1, q_s2))
+    return set_error(SIMP_RT_EINVAL, "kv8_attention: q and out must be [batch, heads, head_size]");
+  if (q_s0 == 0 || q_s1 == 0) return SIMP_RT_OK;
+  if (cache->n_kv_heads < 1 || q_s1 % cache->n_kv_heads != 0)
+    return set_error(SIMP_RT_EINVAL, "kv8_attention: %lld heads are no multiple of %lld kv heads",
+                     (long long)q_s1, (long long)cache->n_kv_heads);
+  if (bc.empty) return set_error(SIMP_RT_EINVAL, "kv8_attention: the cache has no capacity");
+  if (with && (!dsi.is(cache->batch, cache->n_kv_heads, cache->capacity) || !dso.is(si_s0, si_s1, si_s2)))
+    return set_error(SIMP_RT_EINVAL, "kv8_attention: seen_in and seen_out must be [batch, n_kv_heads, capacity]");
+  if (!std::isfinite(scale)) return set_error(SIMP_RT_EINVAL, "kv8_attention: scale must be finite");
+  if (q_s1 > 32767) return set_error(SIMP_RT_EUNSUPPORTED, "kv8_attention: heads above 32767");
+  const bool in_place = with && dsi.data() == dso.data() && si_st0 == so_st0 && si_st1 == so_st1;
+  if (overlap(dout.data(), dout.bytes(), dq.data(), dq.bytes()) ||
+      bc.shares(cache, dout.data(), dout.bytes()) ||
+      (with && bc.shares(cache, dso.data(), dso.bytes())) ||
+      (with && (overlap(dout.data(), dout.bytes(), dsi.data(), dsi.bytes()) ||
+                overlap(dout.data(), dout.bytes(), dso.data(), dso.bytes()) ||
+                overlap(dso.data(), dso.bytes(), dq.data(), dq.bytes()) ||
+                (!in_place && overlap(dsi.data(), dsi.bytes(), dso.data(), dso.bytes())))))
+    return set_error(SIMP_RT_EINVAL, "kv8_attention: an output shares memory with another operand");
+  const int dev = ensure_device();
+  if (dev < 0) return dev;
+  Operand oq, ol, oo, osi, oso;
+  if ((rc = bc.bind(cache, Operand::kIn, dev)) ||
+      (rc = bind_here(oq, dq.data(), dq.bytes(), Operand::kIn, dev, "q")) ||
+      (rc = bind_here(ol, lengths + len_off, 4 * (size_t)len_size, Operand::kIn, dev, "lengths")) ||
+      (rc = bind_here(oo, dout.data(), dout.bytes(), Operand::kOut, dev, "out")) ||
+      (with && ((rc = bind_here(osi, dsi.data(), dsi.bytes(), Operand::kIn, dev, "seen_in")) ||
+                (rc = bind_here(oso, dso.data(), dso.bytes(), Operand::kOut, dev, "seen_out")))))
+    return rc;
+  AttnArgs a{};
+  a.c = bc.c;
+  a.q = (const float *)oq.dev();
+  a.lengths = (const int *)ol.dev();
+  a.out = (float *)oo.dev();
+  a.seen_in = (const float *)osi.dev();
+  a.seen_out = (float *)oso.dev();
+  a.q_seq = q_st0, a.q_head = q_st1, a.o_seq = out_st0, a.o_head = out_st1;
+  a.si_seq = si_st0, a.si_head = si_st1, a.so_seq = so_st0, a.so_head = so_st1;
+  a.heads = (int)q_s1, a.group = (int)(q_s1 / cache->n_kv_heads);
+  a.scale = (float)scale;
+  hipStream_t st = cur_stream();
+  Workspace ws;
+  float *p = nullptr;
+  const size_t rows = (size_t)q_s0 * (size_t)q_s1;
+  if ((rc = ws.get(st, 4 * rows * (size_t)bc.c.cap + 8 * rows, (void **)&p, 8))) return rc;
+  a.stat = (float2 *)p;
+  a.scores = p + 2 * rows;
+  hipLaunchKernelGGL(kv8_attn_k, dim3((unsigned)q_s1, (unsigned)q_s0), dim3(256), 0, st, a);
+  if (with)
+    hipLaunchKernelGGL(kv8_seen_k, dim3((unsigned)cdiv(bc.c.cap, 256), (unsigned)bc.c.hk, (unsigned)q_s0),
+                       dim3(256), 0, st, a);
+  Operand *ops[] = {&oq, &ol, &oo, &osi, &oso};
+  return finish(ops, with ? 5 : 3);
+}
+
+int32_t simp_rt_kv8_evict(
+    const simp_rt_kv8 *cache, const simp_rt_kv8 *to, const int32_t *len_alloc,
+    const int32_t *lengths, int64_t len_off, int64_t len_size, int64_t len_stride,
+    const float *se_alloc, const float *seen, int64_t se_off, int64_t se_s0, int64_t se_s1,
+    int64_t se_s2, int64_t se_st0, int64_t se_st1, int64_t se_st2, float *ns_alloc,
+    float *new_seen, int64_t ns_off, int64_t ns_s0, int64_t ns_s1, int64_t ns_s2, int64_t ns_st0,
+    int64_t ns_st1, int64_t ns_st2, int32_t *kept_alloc, int32_t *kept, int64_t kept_off,
+    int64_t kept_s0, int64_t kept_s1, int64_t kept_s2, int64_t kept_st0, int64_t kept_st1,
+    int64_t kept_st2, int64_t budget, int64_t recent) {
+  (void)len_alloc; (void)se_alloc; (void)ns_alloc; (void)kept_alloc;
+  static const char *fn = "kv8_evict";
+  int rc;
+  BoundCache bc, bt;
+  Desc3<const float> ds{seen, se_off, {se_s0, se_s1, se_s2}, {se_st0, se_st1, se_st2}, 0};
+  Desc3<float> dn{new_seen, ns_off, {ns_s0, ns_s1, ns_s2}, {ns_st0, ns_st1, ns_st2}, 0};
+  Desc3<int32_t> dp{kept, kept_off, {kept_s0, kept_s1, kept_s2}, {kept_st0, kept_st1, kept_st2}, 0};
+  if ((rc = bc.check(cache, fn, "cache")) || (rc = bt.check(to, fn, "to")) ||
+      (rc = ds.check("seen")) || (rc = dn.check("new_seen")) || (rc = dp.check("kept")) ||
+      (rc = check_lists(*cache, fn, nullptr, 0, 0, 0, lengths, len_off, len_size, len_stride, false)))
+    return rc;
+  if (to->batch != cache->batch || to->n_kv_heads != cache->n_kv_heads ||
+      to->head_size != cache->head_size || to->block != cache->block)
+    return set_error(SIMP_RT_EINVAL, "kv8_evict: the caches differ in batch, heads, head_size or block");
+  if (budget < 0 || budget > to->capacity || recent < 0 || recent > budget)
+    return set_error(SIMP_RT_EINVAL, "kv8_evict: budget %lld (capacity %lld), recent %lld: "
+                     "0 <= recent <= budget <= the new cache's capacity is wanted", (long long)budget,
+                     (long long)to->capacity, (long long)recent);
+  if (!ds.is(cache->batch, cache->n_kv_heads, cache->capacity) ||
+      !dp.is(cache->batch, cache->n_kv_heads, budget) || ns_s0 != cache->batch ||
+      ns_s1 != cache->n_kv_heads || ns_s2 < budget)
+    return set_error(SIMP_RT_EINVAL, "kv8_evict: seen must be [batch, n_kv_heads, capacity], new_seen "
+                     "[batch, n_kv_heads, >= budget], kept [batch, n_kv_heads, budget]");
+  if (budget == 0 || cache->batch == 0 || cache->n_kv_heads == 0) return SIMP_RT_OK;
+  if (bc.empty) return set_error(SIMP_RT_EINVAL, "kv8_evict: the cache has no capacity");
+  const struct { const void *p; size_t n; } r[] = {
+      {to->k, (size_t)bt.codes}, {to->v, (size_t)bt.codes}, {to->k_scale, 4 * (size_t)bt.scales},
+      {to->v_scale, 4 * (size_t)bt.scales}, {dn.data(), dn.bytes()}, {dp.data(), dp.bytes()},
+      {cache->k, (size_t)bc.codes}, {cache->v, (size_t)bc.codes},
+      {cache->k_scale, 4 * (size_t)bc.scales}, {cache->v_scale, 4 * (size_t)bc.scales},
+      {ds.data(), ds.bytes()}, {lengths + len_off, 4 * (size_t)len_size}};
+  for (int i = 0; i < 6; i++)
+    for (int j = i + 1; j < 12; j++) {
+      if (i < 4 && j < 4) continue;  // the new cache's own arrays may be interleaved
+      if (overlap(r[i].p, r[i].n, r[j].p, r[j].n))
+        return set_error(SIMP_RT_EINVAL, "kv8_evict: an output shares memory with another operand");
+    }
+  const int dev = ensure_device();
+  if (dev < 0) return dev;
+  Operand ol, os, on, op;
+  if ((rc = bc.bind(cache, Operand::kIn, dev)) || (rc = bt.bind(to, Operand::kOut, dev)) ||
+      (rc = bind_here(ol, lengths + len_off, 4 * (size_t)len_size, Operand::kIn, dev, "lengths")) ||
+      (rc = bind_here(os, ds.data(), ds.bytes(), Operand::kIn, dev, "seen")) ||
+      (rc = bind_here(on, dn.data(), dn.bytes(), Operand::kOut, dev, "new_seen")) ||
+      (rc = bind_here(op, dp.data(), dp.bytes(), Operand::kOut, dev, "kept")))
+    return rc;
+  const EvictArgs a{bc.c, bt.c, (const int *)ol.dev(), (const float *)os.dev(), (float *)on.dev(),
+                    (int *)op.dev(), se_st0, se_st1, ns_st0, ns_st1, kept_st0, kept_st1,
+                    (int)budget, (int)recent};
+  hipStream_t st = cur_stream();
+  hipLaunchKernelGGL(kv8_select_k, dim3((unsigned)bc.c.hk, (unsigned)bc.c.n), dim3(1024), 0, st, a);
+  hipLaunchKernelGGL(kv8_move_k, dim3((unsigned)cdiv(budget, to->block), (unsigned)bc.c.hk,
+                                      2 * (unsigned)bc.c.n), dim3(256), 0, st, a);
+  Operand *ops[] = {&ol, &os, &on, &op};
+  return finish(ops, 4);
+}
+
+}  // extern "C"

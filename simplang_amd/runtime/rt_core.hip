@@ -147,7 +147,7 @@ static void *find_mirror(const void *p, size_t bytes, int *flags) {
   return (char *)it->second.dev + (a - it->first);
 }
 
-static bool is_device_memory(const void *p) {
+static bool is_device_memory(const void *p, int *device = nullptr) {
   hipPointerAttribute_t attr;
   std::memset(&attr, 0, sizeof attr);
   hipError_t e = hipPointerGetAttributes(&attr, p);
@@ -155,6 +155,7 @@ static bool is_device_memory(const void *p) {
     (void)hipGetLastError();  // unregistered host memory: clear the sticky error
     return false;
   }
+  if (device && attr.type == hipMemoryTypeDevice) *device = attr.device;
   return attr.type == hipMemoryTypeDevice || attr.type == hipMemoryTypeManaged;
 }
 
@@ -191,7 +192,7 @@ int Operand::bind(const void *p, size_t bytes, Dir dir, const char *name) {
     return SIMP_RT_OK;
   }
   if (!p) return set_error(SIMP_RT_EINVAL, "%s: null pointer", name);
-  if (is_device_memory(p)) {
+  if (is_device_memory(p, &device_)) {
     dev_ = const_cast<void *>(p);
     return SIMP_RT_OK;
   }

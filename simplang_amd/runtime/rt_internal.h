@@ -48,6 +48,8 @@ class Operand {
   int bind(const void *p, size_t bytes, Dir dir, const char *name);
   void *dev() const { return dev_; }
   bool staged() const { return staged_; }
+  // The GPU that the caller's device memory lies on; -1 for anything else.
+  int device() const { return device_; }
   // Copies a staged output back to its host range (on the current stream).
   int commit();
 
@@ -57,6 +59,7 @@ class Operand {
   size_t bytes_ = 0;
   Dir dir_ = kIn;
   bool staged_ = false;
+  int device_ = -1;
 };
 
 // Device address of a caller range that must already be device-resident

@@ -1,0 +1,40 @@
+// serve_args.h -- operand checks shared by the entry points that serve a batch of
+// sequences (attention.hip, kv8.hip).
+#pragma once
+
+#include "rt_internal.h"
+
+namespace simp {
+
+// A rank-3 descriptor as the entry points take it, and its element extent.
+template <class T>
+struct Desc3 {
+  T *p;
+  int64_t off, s[3], st[3], span;
+  int check(const char *name) { return check_descn(name, p, off, 3, s, st, &span); }
+  bool is(int64_t a, int64_t b, int64_t c) const { return s[0] == a && s[1] == b && s[2] == c; }
+  T *data() const { return p + off; }
+  size_t bytes() const { return (size_t)span * sizeof(T); }
+};
+
+// Device memory of another GPU than the one that the call launches on is refused.
+inline int check_here(const Operand &o, int dev, const char *name) {
+  if (o.device() >= 0 && o.device() != dev)
+    return set_error(SIMP_RT_EINVAL, "%s: lies on device %d, the call is on device %d", name,
+                     o.device(), dev);
+  return SIMP_RT_OK;
+}
+
+inline int bind_here(Operand &o, const void *p, size_t bytes, Operand::Dir dir, int dev,
+                     const char *name) {
+  const int rc = o.bind(p, bytes, dir, name);
+  return rc ? rc : check_here(o, dev, name);
+}
+
+// Whether two byte ranges share any.
+inline bool overlap(const void *a, size_t an, const void *b, size_t bn) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return an && bn && x < y + bn && y < x + an;
+}
+
+}  // namespace simp
