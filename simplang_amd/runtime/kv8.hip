@@ -1,6 +1,7 @@
 // kv8.hip -- a key/value cache of 8-bit codes with an fp32 scale per block of tokens
 // and head: storing rows, reading them back, attention of one query per sequence
 // over it, and cutting sequences down to the tokens that attention used most.
+#include <algorithm>
 #include <cmath>
 
 #include "rt_device.h"
@@ -132,6 +133,29 @@ __global__ void __launch_bounds__(64) kv8_read_k(const ReadArgs a) {
 }
 
 // ------------------------------------------------------------- attention
+//
+// Both products run on v_mfma_i32_16x16x64_i8 with the codes as they lie in memory:
+// the other factor (q, then the weights) is rounded to a whole number of 24 bits of
+// its largest element and taken apart into three signed bytes, v = l0 + 256 l1 +
+// 65536 l2, so every product and sum is exact and the fp32 work is one combination
+// of three integers.  Memory bounds the kernel (2 head_size bytes a token and kv head);
+// converting the codes to floating point would cost more VALU time than that.
+//   * A wave takes 64 tokens at a time.  S^T = K Q^T: lane (i, g) = (lane % 16, lane /
+//     16) loads 16 codes of token i, and ends with the scores of tokens 16 t + 4 g + r
+//     (t, r < 4) for query head i of the group.
+//   * O^T = V^T P^T: the order of the 64 tokens inside the product is free as long as
+//     both factors have it, so lane group g takes the tokens 16 t + 4 g + r, whose
+//     weights it holds already, and the V rows it loads 4 codes at a time are turned
+//     by 4x4 byte transposes in registers.  Neither product touches LDS.
+//   * The head dimension is free in the same way: row i of the n-th product of a
+//     64-dimension chunk is d = 4 i + n.
+// Weights: p = 2^(s - m) of the tile's own maximum m, times the V block's scale over the
+// tile's largest; the integer's unit is the largest of these products / 8.35e6, so
+// that each tile keeps 24 bits of what it contributes, whatever the scales.
+// A block of four waves takes `chunk` tokens of one kv head, its tiles in turn; the
+// rest of a row's softmax is joined by kv8_join_k.
+
+typedef int v4i __attribute__((ext_vector_type(4)));
 
 struct AttnArgs {
   Cache c;
@@ -142,57 +166,357 @@ struct AttnArgs {
   float *seen_out;
   int64_t q_seq, q_head, o_seq, o_head, si_seq, si_head, so_seq, so_head;
   int heads, group;
-  float scale;
-  float *scores;  // [n, heads, cap]
-  float2 *stat;   // [n, heads]: maximum and sum
+  int sets, width;    // sets of up to `width` (at most 16) query heads of a kv head
+  int chunk, splits;  // tokens a block takes; blocks for a full sequence
+  float scale;        // times log2(e): the scores are powers of two
+  float *scores;      // [n, heads, cap], or null
+  float *part;        // [n, heads, splits, head_size], unnormalised
+  float2 *stat;       // [n, heads, splits]: maximum and sum
 };
 
-// One query head: scores, maximum and sum, then the weighted sum of V.
+constexpr float kUnit = 8.35e6f;        // v + 0x808080 stays below 2^24 and above 0
+constexpr uint32_t kBytes = 0x808080u;  // makes the three bytes unsigned
+
+__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
+  return __builtin_amdgcn_perm(hi, lo, sel);  // bytes 0-3 of lo, 4-7 of hi
+}
+
+// The three byte planes of four numbers v + kBytes (bits above 24 are ignored).
+__device__ __forceinline__ void planes(const uint32_t (&u)[4], uint32_t &l0, uint32_t &l1, uint32_t &l2) {
+  const uint32_t a = perm(u[1], u[0], 0x05010400), b = perm(u[3], u[2], 0x05010400);
+  l0 = perm(b, a, 0x05040100) ^ 0x80808080u;
+  l1 = perm(b, a, 0x07060302) ^ 0x80808080u;
+  l2 = perm(perm(u[3], u[2], 0x0c0c0602), perm(u[1], u[0], 0x0c0c0602), 0x05040100) ^ 0x80808080u;
+}
+
+// 4x4 bytes: out[n] = byte n of in[0..3]
+__device__ __forceinline__ void turn4(const uint32_t (&in)[4], uint32_t (&out)[4]) {
+  const uint32_t a = perm(in[1], in[0], 0x05010400), b = perm(in[1], in[0], 0x07030602);
+  const uint32_t c = perm(in[3], in[2], 0x05010400), d = perm(in[3], in[2], 0x07030602);
+  out[0] = perm(c, a, 0x05040100);
+  out[1] = perm(c, a, 0x07060302);
+  out[2] = perm(d, b, 0x05040100);
+  out[3] = perm(d, b, 0x07060302);
+}
+
+// max / sum over the four lanes with the same lane % 16
+__device__ __forceinline__ float quad_max(float v) {
+  float a = v, b = v;
+  permlane16_swap(a, b);
+  a = b = fmaxf(a, b);
+  permlane32_swap(a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  float a = v, b = v;
+  permlane16_swap(a, b);
+  a = b = a + b;
+  permlane32_swap(a, b);
+  return a + b;
+}
+
+// NC: 64-dimension chunks of a head.  blockIdx: chunk of tokens, kv head and set of
+// its query heads, sequence.
+template <int NC>
 __global__ void __launch_bounds__(256) kv8_attn_k(const AttnArgs a) {
-  __shared__ float scratch[16];
-  __shared__ float q[256];
+  extern __shared__ float lds[];  // o [4][cols][hs], then m and l [4][cols]
   const Cache &c = a.c;
-  const int h = blockIdx.x, b = blockIdx.y, hk = h / a.group;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i16 = lane & 15, g = lane >> 4, hs = c.hs;
+  const int hk = blockIdx.y / a.sets, first = ((int)blockIdx.y - hk * a.sets) * a.width;
+  const int cols = min(a.width, a.group - first), h0 = hk * a.group + first;  // query heads h0 ..
+  const int b = blockIdx.z;
   const int len = (int)clampl(a.lengths[b], 0, c.cap);
-  const int64_t at = b * c.st_seq + hk * c.st_head, sat = b * c.sc_seq + hk * c.sc_head;
-  float *sc = a.scores + ((int64_t)b * a.heads + h) * c.cap;
-  for (int d = threadIdx.x; d < c.hs; d += 256) q[d] = a.q[b * a.q_seq + h * a.q_head + d];
-  __syncthreads();
-  float m = -INFINITY;
-  for (int t = threadIdx.x; t < len; t += 256) {
-    const int8_t *k = c.k + at + t * c.st_token;
-    float s = 0.f;
-    for (int d = 0; d < c.hs; d++) s = fmaf(q[d], (float)k[d], s);
-    s *= c.ks[sat + (t >> c.shift)] * a.scale;
-    sc[t] = s;
-    m = fmaxf(m, s);
+  const int from = blockIdx.x * a.chunk;
+  if (from >= len) return;
+  const int to = len - from < a.chunk ? len : from + a.chunk;
+  const int8_t *kp = c.k + b * c.st_seq + hk * c.st_head;
+  const int8_t *vp = c.v + b * c.st_seq + hk * c.st_head;
+  const float *ksp = c.ks + b * c.sc_seq + hk * c.sc_head, *vsp = c.vs + b * c.sc_seq + hk * c.sc_head;
+
+  // Query head i16's dimensions as the lane's K loads have them: 16 from doff on, of
+  // which those below 64 j + 16 g belong to the chunk before (the row's end).
+  v4i ql[NC][3];
+  int doff[NC];
+  float qf;
+  {
+    float x[NC][16], top = 0.f;
+    bool odd = false;
+    const float *qr = a.q + b * a.q_seq + (h0 + min(i16, cols - 1)) * a.q_head;
+#pragma unroll
+    for (int j = 0; j < NC; j++) {
+      const int d0 = 64 * j + 16 * g;
+      doff[j] = min(d0, hs - 16);
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        x[j][e] = qr[doff[j] + e];
+        odd |= !(fabsf(x[j][e]) < INFINITY);
+        if (doff[j] + e < d0) x[j][e] = 0.f;
+        top = fmaxf(top, fabsf(x[j][e]));
+      }
+    }
+    top = quad_max(top);
+    const unsigned long long who = __ballot(odd);  // a query that is not finite: its row is NaN
+    if ((who >> i16) & 0x0001000100010001ull) top = NAN;
+    qf = top * a.scale / kUnit;
+    const float inv = top > 0.f ? 1.f / top : 0.f;
+    const bool tiny = top < 1e-30f;  // 1 / top may overflow: divide
+#pragma unroll
+    for (int j = 0; j < NC; j++)
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        uint32_t u[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const float v = x[j][4 * w + r];
+          const float f = tiny ? (top > 0.f ? v / top : 0.f) : v * inv;
+          u[r] = (uint32_t)(__float2int_rn(f * kUnit) + (int)kBytes);
+        }
+        uint32_t l0, l1, l2;
+        planes(u, l0, l1, l2);
+        ql[j][0][w] = (int)l0;
+        ql[j][1][w] = (int)l1;
+        ql[j][2][w] = (int)l2;
+      }
   }
-  m = block_max(m, scratch);
-  const float mu = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  for (int t = threadIdx.x; t < len; t += 256) l += expf(sc[t] - mu);
-  l = block_sum(l, scratch);
-  if (threadIdx.x == 0) a.stat[b * a.heads + h] = make_float2(mu, l);
-  if ((int)threadIdx.x < c.hs) {
-    float o = 0.f;
-    for (int t = 0; t < len; t++)
-      o = fmaf(expf(sc[t] - mu) * c.vs[sat + (t >> c.shift)],
-               (float)c.v[at + t * c.st_token + threadIdx.x], o);
-    a.out[b * a.o_seq + h * a.o_head + threadIdx.x] = len ? o / l : 0.f;
+
+  float o[NC][4][4];  // [j][n][r]: d = 64 j + 16 g + 4 r + n
+#pragma unroll
+  for (int j = 0; j < NC; j++)
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) o[j][n][r] = 0.f;
+  float m = -INFINITY, l = 0.f;
+  const int last = len - 1;
+  for (int key0 = from + 64 * wave; key0 < to; key0 += 256) {
+    v4i kf[4][NC];
+    uint32_t vf[4][NC][4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      const int8_t *row = kp + (int64_t)min(key0 + 16 * t + i16, last) * c.st_token;
+#pragma unroll
+      for (int j = 0; j < NC; j++) __builtin_memcpy(&kf[t][j], __builtin_assume_aligned(row + doff[j], 4), 16);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int8_t *row = vp + (int64_t)min(key0 + 16 * t + 4 * g + r, last) * c.st_token;
+#pragma unroll
+        for (int j = 0; j < NC; j++) vf[t][j][r] = *(const uint32_t *)(row + min(64 * j + 4 * i16, hs - 4));
+      }
+    float ks[4], vs[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      const int blk = min(key0 + 16 * t, last) >> c.shift;
+      ks[t] = ksp[blk];
+      vs[t] = vsp[blk];
+    }
+    // scores
+    float s[4][4];
+    float mt = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      v4i s0 = {0, 0, 0, 0}, s1 = s0, s2 = s0;
+#pragma unroll
+      for (int j = 0; j < NC; j++) {
+        s0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][j], ql[j][0], s0, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][j], ql[j][1], s1, 0, 0, 0);
+        s2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][j], ql[j][2], s2, 0, 0, 0);
+      }
+      const float f = qf * ks[t];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float x = fmaf((float)s2[r], 65536.f, (float)(s1[r] * 256 + s0[r])) * f;
+        s[t][r] = key0 + 16 * t + 4 * g + r < to ? x : -INFINITY;
+        mt = fmaxf(mt, s[t][r]);
+      }
+    }
+    if (a.scores && i16 < cols) {
+      float *sp = a.scores + ((int64_t)b * a.heads + h0 + i16) * c.cap + key0 + 4 * g;
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          if (key0 + 16 * t + 4 * g + r < to) sp[16 * t + r] = s[t][r];
+    }
+    mt = quad_max(mt);
+    const float mu = mt == -INFINITY ? 0.f : mt;
+    // weights
+    const float vsum = (vs[0] + vs[1]) + (vs[2] + vs[3]);
+    float vtop = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+    if (!(vsum < INFINITY)) vtop = NAN;  // a block that is not finite: the row is NaN
+    float w[4][4], lt = 0.f, wt = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      const float vr = vtop > 0.f ? vs[t] / vtop : 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float p = key0 + 16 * t + 4 * g + r < to ? exp2f(s[t][r] - mu) : 0.f;
+        lt += p;
+        w[t][r] = p * vr;
+        wt = fmaxf(wt, w[t][r]);
+      }
+    }
+    wt = fmaxf(quad_max(wt), 1e-30f);
+    const float inv = kUnit / wt;
+    v4i wl[3];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      uint32_t u[4], l0, l1, l2;
+#pragma unroll
+      for (int r = 0; r < 4; r++)  // the sum with 2^23 has the rounded number in its low bits
+        u[r] = __float_as_uint(fmaf(w[t][r], inv, 8388608.f)) + kBytes;
+      planes(u, l0, l1, l2);
+      wl[0][t] = (int)l0;
+      wl[1][t] = (int)l1;
+      wl[2][t] = (int)l2;
+    }
+    const float mn = fmaxf(m, mt), mnu = mn == -INFINITY ? 0.f : mn;
+    const float alpha = exp2f(m - mnu), beta = exp2f(mt - mnu);
+    m = mn;
+    l = fmaf(l, alpha, lt * beta);
+    const float f = vtop * beta * (wt / kUnit);
+#pragma unroll
+    for (int j = 0; j < NC; j++) {
+      v4i vt[4];
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        uint32_t x[4];
+        turn4(vf[t][j], x);
+#pragma unroll
+        for (int n = 0; n < 4; n++) vt[n][t] = (int)x[n];
+      }
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+        const v4i z = {0, 0, 0, 0};
+        const v4i o0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vt[n], wl[0], z, 0, 0, 0);
+        const v4i o1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vt[n], wl[1], z, 0, 0, 0);
+        const v4i o2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vt[n], wl[2], z, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const float x = fmaf((float)o2[r], 65536.f, (float)(o1[r] * 256 + o0[r]));
+          o[j][n][r] = fmaf(x, f, o[j][n][r] * alpha);
+        }
+      }
+    }
+  }
+  // the four waves' rows together
+  l = quad_sum(l);
+  float *ml = lds + 4 * cols * hs;
+  if (i16 < cols) {
+    float *row = lds + (wave * cols + i16) * hs;
+#pragma unroll
+    for (int j = 0; j < NC; j++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int d = 64 * j + 16 * g + 4 * r;
+        if (d < hs) *(float4 *)(row + d) = make_float4(o[j][0][r], o[j][1][r], o[j][2][r], o[j][3][r]);
+      }
+    if (g == 0) {
+      ml[wave * cols + i16] = m;
+      ml[(4 + wave) * cols + i16] = l;
+    }
+  }
+  __syncthreads();
+  const int quads = hs >> 2;
+  for (int e = threadIdx.x; e < cols * quads; e += 256) {
+    const int col = e / quads, d = 4 * (e - col * quads);
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; w++) M = fmaxf(M, ml[w * cols + col]);
+    const float mu = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float f = exp2f(ml[w * cols + col] - mu);
+      const float4 y = *(const float4 *)(lds + (w * cols + col) * hs + d);
+      L = fmaf(f, ml[(4 + w) * cols + col], L);
+      x.x = fmaf(f, y.x, x.x);
+      x.y = fmaf(f, y.y, x.y);
+      x.z = fmaf(f, y.z, x.z);
+      x.w = fmaf(f, y.w, x.w);
+    }
+    const int64_t row = ((int64_t)b * a.heads + h0 + col) * a.splits + blockIdx.x;
+    *(float4 *)(a.part + row * hs + d) = x;
+    if (d == 0) a.stat[row] = make_float2(M, L);
   }
 }
 
-__global__ void __launch_bounds__(256) kv8_seen_k(const AttnArgs a) {
+constexpr int kSeenTile = 1024;
+
+// The chunks of a row together.  blockIdx.x below the group: that query head's row of
+// out; above: kSeenTile tokens of the accumulated weights.
+__global__ void __launch_bounds__(256) kv8_join_k(const AttnArgs a) {
+  extern __shared__ float lds[];
   const Cache &c = a.c;
-  const int t = blockIdx.x * 256 + threadIdx.x, hk = blockIdx.y, b = blockIdx.z;
-  if (t >= (int)clampl(a.lengths[b], 0, c.cap)) return;
-  float w = a.seen_in[b * a.si_seq + hk * a.si_head + t];
-  for (int g = 0; g < a.group; g++) {
-    const int64_t row = (int64_t)b * a.heads + hk * a.group + g;
-    const float2 ml = a.stat[row];
-    w += expf(a.scores[row * c.cap + t] - ml.x) / ml.y;
+  const int hk = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int len = (int)clampl(a.lengths[b], 0, c.cap);
+  const int ns = len ? (len - 1) / a.chunk + 1 : 0, hs = c.hs;
+  if ((int)blockIdx.x < a.group) {
+    const int h = hk * a.group + blockIdx.x;
+    float *out = a.out + b * a.o_seq + h * a.o_head;
+    if (len == 0) {
+      for (int d = threadIdx.x; d < hs; d += 256) out[d] = 0.f;
+      return;
+    }
+    const float2 *st = a.stat + ((int64_t)b * a.heads + h) * a.splits;
+    const float *part = a.part + ((int64_t)b * a.heads + h) * a.splits * hs;
+    __shared__ float scratch[16];
+    __shared__ float so[4][256];
+    float M = -INFINITY;
+    for (int s = threadIdx.x; s < ns; s += 256) M = fmaxf(M, st[s].x);
+    M = block_max(M, scratch);
+    const float mu = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    for (int s = threadIdx.x; s < ns; s += 256) {
+      const float f = exp2f(st[s].x - mu);
+      lds[s] = f;
+      L = fmaf(f, st[s].y, L);
+    }
+    L = block_sum(L, scratch);  // its barriers make lds[] visible too
+    if (4 * lane < hs) {
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int s = wave; s < ns; s += 4) {
+        const float f = lds[s];
+        const float4 y = *(const float4 *)(part + (int64_t)s * hs + 4 * lane);
+        x.x = fmaf(f, y.x, x.x);
+        x.y = fmaf(f, y.y, x.y);
+        x.z = fmaf(f, y.z, x.z);
+        x.w = fmaf(f, y.w, x.w);
+      }
+      *(float4 *)&so[wave][4 * lane] = x;
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < hs; d += 256)
+      out[d] = (so[0][d] + so[1][d] + so[2][d] + so[3][d]) / L;
+    return;
   }
-  a.seen_out[b * a.so_seq + hk * a.so_head + t] = w;
+  const int t0 = ((int)blockIdx.x - a.group) * kSeenTile;
+  if (t0 >= len) return;
+  for (int g = wave; g < a.group; g += 4) {  // each head's maximum and 1 / sum
+    const float2 *st = a.stat + ((int64_t)b * a.heads + hk * a.group + g) * a.splits;
+    float M = -INFINITY, L = 0.f;
+    for (int s = lane; s < ns; s += 64) M = fmaxf(M, st[s].x);
+    M = wave_max(M);
+    const float mu = M == -INFINITY ? 0.f : M;
+    for (int s = lane; s < ns; s += 64) L = fmaf(exp2f(st[s].x - mu), st[s].y, L);
+    L = wave_sum(L);
+    if (lane == 0) {
+      lds[2 * g] = mu;
+      lds[2 * g + 1] = 1.f / L;
+    }
+  }
+  __syncthreads();
+  const float *sc = a.scores + ((int64_t)b * a.heads + hk * a.group) * c.cap;
+  for (int t = t0 + threadIdx.x; t < min(t0 + kSeenTile, len); t += 256) {
+    float w = 0.f;
+    for (int g = 0; g < a.group; g++)
+      w = fmaf(exp2f(sc[(int64_t)g * c.cap + t] - lds[2 * g]), lds[2 * g + 1], w);
+    a.seen_out[b * a.so_seq + hk * a.so_head + t] = a.seen_in[b * a.si_seq + hk * a.si_head + t] + w;
+  }
 }
 
 // ----------------------------------------------------------------- evict
@@ -545,7 +869,8 @@ int32_t simp_rt_kv8_attention(
   if (with && (!dsi.is(cache->batch, cache->n_kv_heads, cache->capacity) || !dso.is(si_s0, si_s1, si_s2)))
     return set_error(SIMP_RT_EINVAL, "kv8_attention: seen_in and seen_out must be [batch, n_kv_heads, capacity]");
   if (!std::isfinite(scale)) return set_error(SIMP_RT_EINVAL, "kv8_attention: scale must be finite");
-  if (q_s1 > 32767) return set_error(SIMP_RT_EUNSUPPORTED, "kv8_attention: heads above 32767");
+  if (q_s1 > 32767 || q_s1 / cache->n_kv_heads > 4096)
+    return set_error(SIMP_RT_EUNSUPPORTED, "kv8_attention: heads above 32767, or 4096 to a kv head");
   const bool in_place = with && dsi.data() == dso.data() && si_st0 == so_st0 && si_st1 == so_st1;
   if (overlap(dout.data(), dout.bytes(), dq.data(), dq.bytes()) ||
       bc.shares(cache, dout.data(), dout.bytes()) ||
@@ -575,18 +900,36 @@ int32_t simp_rt_kv8_attention(
   a.q_seq = q_st0, a.q_head = q_st1, a.o_seq = out_st0, a.o_head = out_st1;
   a.si_seq = si_st0, a.si_head = si_st1, a.so_seq = so_st0, a.so_head = so_st1;
   a.heads = (int)q_s1, a.group = (int)(q_s1 / cache->n_kv_heads);
-  a.scale = (float)scale;
+  a.scale = (float)(scale * 1.4426950408889634);
   hipStream_t st = cur_stream();
+  // Four tiles of 64 tokens to a block, one per wave, and more where the full cache
+  // would have more than 2048 blocks (8 a CU).
+  a.width = bc.c.hs > 192 ? 8 : 16;  // the block's rows fit 64 KB of LDS
+  a.sets = (int)cdiv(a.group, a.width);
+  const int64_t per = (int64_t)bc.c.n * bc.c.hk * a.sets;
+  a.chunk = (int)(256 * std::max<int64_t>(1, cdiv(per * bc.c.cap, 2048 * 256)));
+  a.splits = (int)cdiv(bc.c.cap, a.chunk);
+  const size_t rows = (size_t)q_s0 * (size_t)q_s1, parts = rows * (size_t)a.splits;
   Workspace ws;
   float *p = nullptr;
-  const size_t rows = (size_t)q_s0 * (size_t)q_s1;
-  if ((rc = ws.get(st, 4 * rows * (size_t)bc.c.cap + 8 * rows, (void **)&p, 8))) return rc;
-  a.stat = (float2 *)p;
-  a.scores = p + 2 * rows;
-  hipLaunchKernelGGL(kv8_attn_k, dim3((unsigned)q_s1, (unsigned)q_s0), dim3(256), 0, st, a);
-  if (with)
-    hipLaunchKernelGGL(kv8_seen_k, dim3((unsigned)cdiv(bc.c.cap, 256), (unsigned)bc.c.hk, (unsigned)q_s0),
-                       dim3(256), 0, st, a);
+  if ((rc = ws.get(st, 4 * (parts * (size_t)bc.c.hs + 2 * parts + (with ? rows * (size_t)bc.c.cap : 0)),
+                   (void **)&p, 8)))
+    return rc;
+  a.part = p;
+  a.stat = (float2 *)(p + parts * (size_t)bc.c.hs);
+  a.scores = with ? p + parts * (size_t)(bc.c.hs + 2) : nullptr;
+  const size_t cols = (size_t)std::min(a.group, a.width);
+  const unsigned lds = (unsigned)(4 * 4 * cols * ((size_t)bc.c.hs + 2));
+  const dim3 grid((unsigned)a.splits, (unsigned)(bc.c.hk * a.sets), (unsigned)bc.c.n);
+#define ATTN(NC) hipLaunchKernelGGL(kv8_attn_k<NC>, grid, dim3(256), lds, st, a)
+  if (bc.c.hs <= 64) ATTN(1);
+  else if (bc.c.hs <= 128) ATTN(2);
+  else if (bc.c.hs <= 192) ATTN(3);
+  else ATTN(4);
+#undef ATTN
+  const unsigned jx = (unsigned)(a.group + (with ? cdiv(bc.c.cap, kSeenTile) : 0));
+  hipLaunchKernelGGL(kv8_join_k, dim3(jx, (unsigned)bc.c.hk, (unsigned)bc.c.n), dim3(256),
+                     4 * std::max(a.splits, 2 * a.group), st, a);
   Operand *ops[] = {&oq, &ol, &oo, &osi, &oso};
   return finish(ops, with ? 5 : 3);
 }
