@@ -25,12 +25,59 @@ __device__ __forceinline__ int64_t clampl(int64_t x, int64_t lo, int64_t hi) {
 // max that a NaN comes through
 __device__ __forceinline__ float max_nan(float a, float b) { return a != a || a > b ? a : b; }
 
-// Nearest code to x / s (ties to even, of the exact quotient), s > 0 and finite.
-__device__ __forceinline__ int code_of(float x, float s) {
-  return (int)fminf(fmaxf((float)rint((double)x / (double)s), -127.f), 127.f);
+__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
+  return __builtin_amdgcn_perm(hi, lo, sel);  // bytes 0-3 of lo, 4-7 of hi
+}
+
+// The last s of 0 .. n-1 for which f(s) holds, where it holds up to some s and not
+// behind it; 0 where it holds for none.  The 64 lanes look at 64 places at a time, so up
+// to 64 sequences cost one round trip to memory.  Every lane of the wave takes part.
+template <class F>
+__device__ __forceinline__ int last_of(int n, F f) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 63) >> 6;
+    const unsigned long long yes = __ballot(lane * step < n && f(lo + lane * step));
+    if (!yes) break;
+    const int k = 63 - __clzll((long long)yes);
+    lo += k * step;
+    n = min(step, n - k * step);
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
+
+// Nearest code to x / s, ties to even, of the exact quotient; s > 0 and finite, inv =
+// 1 / s rounded (or anything near it).  x - n s is exact where n is next to the
+// quotient: n has 7 bits, and what remains is a multiple of the last bit of s / 2 below s.
+__device__ __forceinline__ int code_of(float x, float s, float inv) {
+  const float n = rintf(fminf(fmaxf(x * inv, -127.f), 127.f));
+  const float r = fmaf(-n, s, x), half = 0.5f * s, a = fabsf(r);
+  const bool odd = ((int)n & 1) != 0;
+  const float to = r < 0.f ? n - 1.f : n + 1.f;  // the other neighbour
+  return (int)fminf(fmaxf(a > half || (a == half && odd) ? to : n, -127.f), 127.f);
+}
+
+// Four codes times ratio <= 1 (a NaN never: the caller clears those), rounded to the
+// nearest, ties to even: the sum with 1.5 2^52 has the rounded number in its low bits.
+__device__ __forceinline__ uint32_t rescale4(uint32_t c, double ratio) {
+  uint32_t r[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const double t = fma((double)(int)(int8_t)(c >> (8 * e)), ratio, 6755399441055744.0);
+    r[e] = (uint32_t)__double_as_longlong(t);
+  }
+  return perm(perm(r[3], r[2], 0x0c0c0400), perm(r[1], r[0], 0x0c0c0400), 0x05040100);
 }
 
 // ---------------------------------------------------------------- append
+//
+// One block of one head, K or V (blockIdx.z), to a block of threads that holds the
+// new rows in registers between their maximum and their codes (V chunks of four
+// values to a thread): x is read once and memory bounds it.  Sequence b has the slots
+// starts[b] / T + 2 b and on: n rows touch at most n / T + 2 blocks.
 
 struct AppendArgs {
   Cache c;
@@ -40,65 +87,87 @@ struct AppendArgs {
   int rows;
 };
 
-// One block of one head, K or V (blockIdx.z).  Sequence b has the slots starts[b] /
-// T + 2 b and on: n rows touch at most n / T + 2 blocks.
-__global__ void __launch_bounds__(256) kv8_append_k(const AppendArgs a) {
-  __shared__ float scratch[16];
-  __shared__ int bad;
+constexpr int kAppendChunks = 8;
+
+template <int THREADS, bool VEC>
+__global__ void __launch_bounds__(THREADS) kv8_append_k(const AppendArgs a) {
+  __shared__ float top_s[THREADS / 64];
   const Cache &c = a.c;
-  const int t = blockIdx.x, h = blockIdx.y, T = 1 << c.shift;
-  int lo = 0, hi = c.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if ((int)clampl(a.starts[mid], 0, a.rows) / T + 2 * mid <= t) lo = mid;
-    else hi = mid - 1;
-  }
-  const int b = lo;
-  const int r0 = (int)clampl(a.starts[b], 0, a.rows), r1 = (int)clampl(a.starts[b + 1], r0, a.rows);
+  const int t = blockIdx.x, h = blockIdx.y, T = 1 << c.shift, tid = threadIdx.x;
+  const int b = last_of(c.n, [&](int s) { return (clampi(a.starts[s], 0, a.rows) >> c.shift) + 2 * s <= t; });
+  const int r0 = clampi(a.starts[b], 0, a.rows), r1 = clampi(a.starts[b + 1], r0, a.rows);
   const int64_t end = a.lengths[b], have = end - (r1 - r0);  // positions of the new rows
   const int64_t from = clampl(have, 0, c.cap), to = clampl(end, 0, c.cap);
-  const int64_t blk = (from >> c.shift) + (t - (r0 / T + 2 * b));
-  const int64_t p0 = blk << c.shift, p1 = min(p0 + T, to);
-  if (t < r0 / T + 2 * b || from >= to || p0 >= to) return;
-  const int64_t first = max(p0, from);  // tokens p0 .. first-1 are there already
+  const int slot0 = (r0 >> c.shift) + 2 * b;
+  const int64_t blk = (from >> c.shift) + (t - slot0);
+  const int64_t p0 = blk << c.shift;
+  if (t < slot0 || from >= to || p0 >= to) return;
+  const int64_t p1 = p0 + T < to ? p0 + T : to;
+  const int64_t first = p0 > from ? p0 : from;  // tokens p0 .. first-1 are there already
   const bool is_v = blockIdx.z != 0;
-  const float *x = is_v ? a.v : a.k;
   const int64_t row = is_v ? a.v_row : a.k_row;
-  x += (int64_t)r0 * row + h * (is_v ? a.v_head : a.k_head);
-  int8_t *codes = (is_v ? c.v : c.k) + b * c.st_seq + h * c.st_head;
+  const float *x = (is_v ? a.v + h * a.v_head : a.k + h * a.k_head) + (r0 + first - have) * row;
+  int8_t *codes = (is_v ? c.v : c.k) + b * c.st_seq + h * c.st_head + p0 * c.st_token;
   float *sc = (is_v ? c.vs : c.ks) + b * c.sc_seq + h * c.sc_head + blk;
-  if (threadIdx.x == 0) bad = 0;
-  __syncthreads();
+  const int quads = c.hs >> 2, old = (int)(first - p0), nw = (int)(p1 - first) * quads;
+  const float before = old ? *sc : 0.f;
+
+  float4 v[kAppendChunks];
   float top = 0.f;
   bool odd = false;
-  const int nw = (int)(p1 - first) * c.hs;
-  for (int e = threadIdx.x; e < nw; e += 256) {
-    const int i = e / c.hs, d = e - i * c.hs;
-    const float f = fabsf(x[(first + i - have) * row + d]);
-    top = fmaxf(top, f);
-    odd |= !(f < INFINITY);
-  }
-  if (odd) bad = 1;
-  const float before = first > p0 ? *sc : 0.f;
-  top = block_max(top, scratch);  // its barriers order `bad` and the read of the scale too
-  float s = max_nan(before, top / 127.f);
-  if (bad) s = NAN;
-  const bool live = s > 0.f && s < INFINITY;
-  const int no = (int)(first - p0) * c.hs;
-  if (!(before == s)) {  // what the block held, to the new scale
-    const double ratio = live ? (double)before / (double)s : 0.0;
-    for (int e = threadIdx.x; e < no; e += 256) {
-      const int i = e / c.hs, d = e - i * c.hs;
-      int8_t *p = codes + (p0 + i) * c.st_token + d;
-      *p = live ? (int8_t)(int)rint(*p * ratio) : 0;
+#pragma unroll
+  for (int i = 0; i < kAppendChunks; i++) {
+    const int e = tid + i * THREADS;
+    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (e < nw) {
+      const int r = e / quads;
+      const float *p = x + r * row + 4 * (e - r * quads);
+      if (VEC) v[i] = *(const float4 *)p;
+      else v[i] = make_float4(p[0], p[1], p[2], p[3]);
     }
   }
-  for (int e = threadIdx.x; e < nw; e += 256) {
-    const int i = e / c.hs, d = e - i * c.hs;
-    codes[(first + i) * c.st_token + d] =
-        live ? (int8_t)code_of(x[(first + i - have) * row + d], s) : 0;
+#pragma unroll
+  for (int i = 0; i < kAppendChunks; i++) {
+    const float m = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+    top = fmaxf(top, m);
+    const float z = v[i].x * 0.f + v[i].y * 0.f + v[i].z * 0.f + v[i].w * 0.f;
+    odd |= z != 0.f;  // of an infinity or NaN
   }
-  if (threadIdx.x == 0) *sc = s;
+  top = wave_max_dpp(top);
+  if (__any(odd)) top = NAN;
+  if ((tid & 63) == 0) top_s[tid >> 6] = top;
+  __syncthreads();  // also: every thread has read the scale
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; i++) top = max_nan(top, top_s[i]);
+  const float s = max_nan(before, top / 127.f);
+  const bool live = s > 0.f && s < INFINITY;
+  if (old && !(before == s)) {  // what the block held, to the new scale
+    const double ratio = live ? (double)before / (double)s : 0.0;
+    for (int e = tid; e < old * quads; e += THREADS) {
+      const int r = e / quads;
+      uint32_t *p = (uint32_t *)(codes + r * c.st_token + 4 * (e - r * quads));
+      *p = live ? rescale4(*p, ratio) : 0u;
+    }
+  }
+  const float inv = live ? 1.f / s : 0.f;
+  const bool tiny = s < 1e-37f;  // 1 / s may be infinite or coarse
+#pragma unroll
+  for (int i = 0; i < kAppendChunks; i++) {
+    const int e = tid + i * THREADS;
+    if (e < nw) {
+      const int r = e / quads;
+      const float y[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      uint32_t q = 0;
+      if (live) {
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+          q |= (uint32_t)(uint8_t)(int8_t)(tiny ? (int)fmin(fmax(rint((double)y[w] / (double)s), -127.0), 127.0)
+                                                : code_of(y[w], s, inv)) << (8 * w);
+      }
+      *(uint32_t *)(codes + (old + r) * c.st_token + 4 * (e - r * quads)) = q;
+    }
+  }
+  if (tid == 0) *sc = s;
 }
 
 // ------------------------------------------------------------------ read
@@ -111,25 +180,57 @@ struct ReadArgs {
   int rows;
 };
 
-// One packed row of one head, K or V (blockIdx.z).
-__global__ void __launch_bounds__(64) kv8_read_k(const ReadArgs a) {
+constexpr int kReadRows = 32;
+
+// kReadRows packed rows of one head, K and V.
+template <bool VEC>
+__global__ void __launch_bounds__(256) kv8_read_k(const ReadArgs a) {
+  __shared__ int64_t at[kReadRows];  // the token's codes; -1: zeros; -2: nobody's row
+  __shared__ float ks[kReadRows], vs[kReadRows];
   const Cache &c = a.c;
-  const int r = blockIdx.x, h = blockIdx.y;
-  int lo = 0, hi = c.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (clampl(a.starts[mid], 0, a.rows) <= r) lo = mid;
-    else hi = mid - 1;
+  const int first = blockIdx.x * kReadRows, h = blockIdx.y, n = min(kReadRows, a.rows - first);
+  if (threadIdx.x < 64) {
+    const int r = first + min((int)threadIdx.x, n - 1);
+    int b = last_of(c.n, [&](int s) { return clampi(a.starts[s], 0, a.rows) <= first; });
+    while (b + 1 < c.n && clampi(a.starts[b + 1], 0, a.rows) <= r) b++;
+    const int r0 = clampi(a.starts[b], 0, a.rows), r1 = clampi(a.starts[b + 1], r0, a.rows);
+    if ((int)threadIdx.x < n) {
+      const int64_t p = (int64_t)a.lengths[b] - (r1 - r);
+      const bool mine = r >= r0 && r < r1, in = p >= 0 && p < c.cap;
+      at[threadIdx.x] = !mine ? -2 : !in ? -1 : b * c.st_seq + h * c.st_head + p * c.st_token;
+      const int64_t z = b * c.sc_seq + h * c.sc_head + (p >> c.shift);
+      ks[threadIdx.x] = mine && in ? c.ks[z] : 0.f;
+      vs[threadIdx.x] = mine && in ? c.vs[z] : 0.f;
+    }
   }
-  const int b = lo;
-  const int r0 = (int)clampl(a.starts[b], 0, a.rows), r1 = (int)clampl(a.starts[b + 1], r0, a.rows);
-  if (r < r0 || r >= r1) return;
-  const int64_t p = (int64_t)a.lengths[b] - (r1 - r);
-  const bool in = p >= 0 && p < c.cap, is_v = blockIdx.z != 0;
-  const int8_t *codes = (is_v ? c.v : c.k) + b * c.st_seq + h * c.st_head + (in ? p : 0) * c.st_token;
-  const float s = in ? (is_v ? c.vs : c.ks)[b * c.sc_seq + h * c.sc_head + (p >> c.shift)] : 0.f;
-  float *out = (is_v ? a.v : a.k) + r * (is_v ? a.v_row : a.k_row) + h * (is_v ? a.v_head : a.k_head);
-  for (int d = threadIdx.x; d < c.hs; d += 64) out[d] = in ? codes[d] * s : 0.f;
+  __syncthreads();
+  const int quads = c.hs >> 2;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < n * quads; e += 256) {
+    const int i = e / quads, d = 4 * (e - i * quads);
+    const int64_t o = at[i];
+    if (o == -2) continue;
+    const uint32_t kc = o < 0 ? 0u : *(const uint32_t *)(c.k + o + d);
+    const uint32_t vc = o < 0 ? 0u : *(const uint32_t *)(c.v + o + d);
+    float *kd = a.k + (int64_t)(first + i) * a.k_row + h * a.k_head + d;
+    float *vd = a.v + (int64_t)(first + i) * a.v_row + h * a.v_head + d;
+    float x[4], y[4];
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      x[w] = (float)(int8_t)(kc >> (8 * w)) * ks[i];
+      y[w] = (float)(int8_t)(vc >> (8 * w)) * vs[i];
+    }
+    if (VEC) {
+      *(float4 *)kd = make_float4(x[0], x[1], x[2], x[3]);
+      *(float4 *)vd = make_float4(y[0], y[1], y[2], y[3]);
+    } else {
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        kd[w] = x[w];
+        vd[w] = y[w];
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------- attention
@@ -176,10 +277,6 @@ struct AttnArgs {
 
 constexpr float kUnit = 8.35e6f;        // v + 0x808080 stays below 2^24 and above 0
 constexpr uint32_t kBytes = 0x808080u;  // makes the three bytes unsigned
-
-__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
-  return __builtin_amdgcn_perm(hi, lo, sel);  // bytes 0-3 of lo, 4-7 of hi
-}
 
 // The three byte planes of four numbers v + kBytes (bits above 24 are ignored).
 __device__ __forceinline__ void planes(const uint32_t (&u)[4], uint32_t &l0, uint32_t &l1, uint32_t &l2) {
@@ -538,15 +635,69 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Which tokens stay: the weight of the last one that does, byte by byte from the top
-// (a histogram of the byte among the weights that share the bytes above it), then
-// the places in order.
+// The place-from-the-top search of kv8_select_k: among the weights of 0 .. old-1 whose
+// order agrees with `prefix` above bit `shift + BITS`, a histogram of the next BITS bits;
+// then the bin that holds the need-th from the top.  Returns it, and what is left to
+// take from it in `need`, its size in `size`.
+template <int BITS>
+__device__ __forceinline__ uint32_t select_digit(const float *seen, int old, uint32_t prefix, int shift,
+                                                 int &need, int &size, int *hist, int *wave_s) {
+  constexpr int BINS = 1 << BITS, PER = BINS / 1024;  // bins of a thread
+  static_assert(PER * 1024 == BINS, "");
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+  for (int i = 0; i < PER; i++) hist[tid + 1024 * i] = 0;
+  __syncthreads();
+  const bool all = shift + BITS == 32;
+#pragma unroll 4
+  for (int t = tid; t < old; t += 1024) {
+    const uint32_t u = order_of(seen[t]);
+    if (all || ((u ^ prefix) >> (shift + BITS)) == 0) atomicAdd(&hist[u >> shift & (BINS - 1)], 1);
+  }
+  __syncthreads();
+  // thread t has the bins from the top: BINS - 1 - PER t and the PER - 1 below
+  int h[PER], sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    h[i] = hist[BINS - 1 - PER * tid - i];
+    sum += h[i];
+  }
+  int upto = sum;  // bins of this wave's threads up to this one's
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int x = __shfl_up(upto, d);
+    if (lane >= d) upto += x;
+  }
+  if (lane == 63) wave_s[wave] = upto;
+  __syncthreads();
+  for (int w = 0; w < wave; w++) upto += wave_s[w];
+  int above = upto - sum;
+  if (above < need && need <= upto) {  // one thread
+    int i = 0;
+    while (above + h[i] < need) above += h[i++];
+    wave_s[16] = BINS - 1 - PER * tid - i;
+    wave_s[17] = need - above;
+    wave_s[18] = h[i];
+  }
+  __syncthreads();
+  const uint32_t digit = (uint32_t)wave_s[16];
+  need = wave_s[17];
+  size = wave_s[18];
+  __syncthreads();
+  return digit << shift;
+}
+
+// Which tokens of one head stay, by one block: the order of the last weight that
+// does, 12 bits and twice 10 from the top, then the places.  Twelve bits first, so
+// that the weights, which share few exponents, do not all add to the same few
+// counters.  Each wave then has a run of tokens: it counts those that stay (and those
+// equal to the last one, of which the first ones do), and writes them behind the
+// other waves'.
 __global__ void __launch_bounds__(1024) kv8_select_k(const EvictArgs a) {
-  __shared__ int hist[256];
-  __shared__ uint32_t prefix_s;
-  __shared__ int need_s, wave_eq[16], wave_keep[16];
-  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int len = (int)clampl(a.lengths[b], 0, a.c.cap);
+  __shared__ int hist[4096];
+  __shared__ int wave_s[32], more_s[16], equal_s[16];
+  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int len = clampi(a.lengths[b], 0, a.c.cap);
   const float *seen = a.seen + b * a.se_seq + hk * a.se_head;
   float *ns = a.new_seen + b * a.ns_seq + hk * a.ns_head;
   int *kept = a.kept + b * a.kp_seq + hk * a.kp_head;
@@ -558,87 +709,101 @@ __global__ void __launch_bounds__(1024) kv8_select_k(const EvictArgs a) {
     return;
   }
   const int old = len - a.recent;  // candidates 0 .. old-1
-  int need = a.budget - a.recent;  // of which so many stay (need < old)
-  uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int t = tid; t < old; t += 1024) {
-      const uint32_t u = order_of(seen[t]);
-      if (shift == 24 || (u ^ prefix) >> (shift + 8) == 0)
-        atomicAdd(&hist[u >> shift & 255], 1);
+  int need = a.budget - a.recent;  // of which so many stay (fewer than there are)
+  uint32_t last = 0xFFFFFFFFu;     // the order of the last one that stays,
+  uint32_t mask = 0xFFFFFFFFu;     // in these bits
+  if (need > 0) {
+    int size;
+    last = select_digit<12>(seen, old, 0, 20, need, size, hist, wave_s);
+    mask = 0xFFF00000u;
+    if (size != need) {
+      last |= select_digit<10>(seen, old, last, 10, need, size, hist, wave_s);
+      mask = 0xFFFFFC00u;
     }
-    __syncthreads();
-    if (tid == 0) {
-      int byte = 255, left = need;
-      while (byte > 0 && hist[byte] < left) left -= hist[byte--];
-      prefix_s = prefix | (uint32_t)byte << shift;
-      need_s = left;
+    if (size != need) {
+      last |= select_digit<10>(seen, old, last, 0, need, size, hist, wave_s);
+      mask = 0xFFFFFFFFu;
     }
-    __syncthreads();
-    prefix = prefix_s;
-    need = need_s;
   }
-  // `need` of the tokens with the weight `prefix` stay, the first ones
   const bool any = a.budget > a.recent;
-  int eq0 = 0, keep0 = 0;
-  for (int t0 = 0; t0 < len; t0 += 1024) {
-    const int t = t0 + tid;
-    const uint32_t u = t < old ? order_of(seen[t]) : 0;
-    const bool eq = any && t < old && u == prefix;
-    const unsigned long long below = (1ull << (tid & 63)) - 1, be = __ballot(eq);
-    if ((tid & 63) == 0) wave_eq[tid >> 6] = __popcll(be);
-    __syncthreads();
-    int e = eq0 + __popcll(be & below);
-    for (int w = 0; w < 16; w++) {
-      if (w < tid >> 6) e += wave_eq[w];
-      eq0 += wave_eq[w];
-    }
-    const bool keep = t < len && (t >= old || (any && u > prefix) || (eq && e < need));
+  const int run = (len + 1023) / 1024 * 64, t0 = min(wave * run, len), t1 = min(t0 + run, len);
+  int more = 0, equal = 0;
+  for (int t = t0 + lane; t < t1; t += 64) {
+    const uint32_t u = order_of(seen[t]) & mask;
+    more += t >= old || (any && u > last);
+    equal += t < old && any && u == last;
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    more += __shfl_xor(more, d);
+    equal += __shfl_xor(equal, d);
+  }
+  if (lane == 0) {
+    more_s[wave] = more;
+    equal_s[wave] = equal;
+  }
+  __syncthreads();
+  int eq = 0, place = 0;  // equal ones before this wave's; where it writes
+  for (int w = 0; w < wave; w++) {
+    place += more_s[w] + min(equal_s[w], max(need - eq, 0));
+    eq += equal_s[w];
+  }
+  const unsigned long long below = (1ull << lane) - 1;
+  for (int t = t0; t < t1; t += 64) {
+    const int at = t + lane;
+    const float x = at < t1 ? seen[at] : 0.f;
+    const uint32_t u = order_of(x) & mask;
+    const bool same = at < t1 && at < old && any && u == last;
+    const unsigned long long be = __ballot(same);
+    const bool keep = at < t1 && (at >= old || (any && u > last) || (same && eq + __popcll(be & below) < need));
     const unsigned long long bk = __ballot(keep);
-    if ((tid & 63) == 0) wave_keep[tid >> 6] = __popcll(bk);
-    __syncthreads();
-    int k = keep0 + __popcll(bk & below);
-    for (int w = 0; w < 16; w++) {
-      if (w < tid >> 6) k += wave_keep[w];
-      keep0 += wave_keep[w];
-    }
+    const int k = place + __popcll(bk & below);
     if (keep && k < a.budget) {
-      kept[k] = t;
-      ns[k] = seen[t];
+      kept[k] = at;
+      ns[k] = x;
     }
-    __syncthreads();
+    eq += __popcll(be);
+    place += __popcll(bk);
   }
 }
 
 // One block of the new cache, one head, K or V (blockIdx.z & 1).
 __global__ void __launch_bounds__(256) kv8_move_k(const EvictArgs a) {
-  __shared__ int at[128];
-  __shared__ float sc[128];
+  __shared__ int64_t at[128];
+  __shared__ double ratio[128];  // of the scales; 1: the codes stay; -1: they are cleared
+  __shared__ float top_s[2];
   const Cache &c = a.c, &o = a.to;
-  const int blk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z >> 1;
+  const int blk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z >> 1, tid = threadIdx.x;
   const bool is_v = blockIdx.z & 1;
-  const int len = min((int)clampl(a.lengths[b], 0, c.cap), a.budget);
+  const int len = min(clampi(a.lengths[b], 0, c.cap), a.budget);
   const int p0 = blk << o.shift, nt = min(1 << o.shift, len - p0);
   if (nt <= 0) return;
-  const int *kept = a.kept + b * a.kp_seq + hk * a.kp_head + p0;
-  const float *zs = (is_v ? c.vs : c.ks) + b * c.sc_seq + hk * c.sc_head;
-  for (int i = threadIdx.x; i < nt; i += 256) {
-    at[i] = (int)clampl(kept[i], 0, c.cap - 1);
-    sc[i] = zs[at[i] >> c.shift];
+  float z = 0.f;
+  if (tid < nt) {
+    const int t = clampi(a.kept[b * a.kp_seq + hk * a.kp_head + p0 + tid], 0, c.cap - 1);
+    at[tid] = b * c.st_seq + hk * c.st_head + t * c.st_token;
+    z = (is_v ? c.vs : c.ks)[b * c.sc_seq + hk * c.sc_head + (t >> c.shift)];
   }
+  float s = wave_max_dpp(z);
+  if (__any(z != z)) s = NAN;
+  if (tid < 128 && (tid & 63) == 0) top_s[tid >> 6] = s;
   __syncthreads();
-  float s = 0.f;
-  for (int i = 0; i < nt; i++) s = max_nan(s, sc[i]);
+  s = max_nan(top_s[0], top_s[1]);
   const bool live = s > 0.f && s < INFINITY;
-  const int8_t *src = (is_v ? c.v : c.k) + b * c.st_seq + hk * c.st_head;
-  int8_t *dst = (is_v ? o.v : o.k) + b * o.st_seq + hk * o.st_head;
-  for (int e = threadIdx.x; e < nt * c.hs; e += 256) {
-    const int i = e / c.hs, d = e - i * c.hs;
-    const double ratio = live ? (double)sc[i] / (double)s : 0.0;
-    dst[(int64_t)(p0 + i) * o.st_token + d] = (int8_t)(int)rint(src[at[i] * c.st_token + d] * ratio);
+  if (tid < nt) ratio[tid] = !live ? -1.0 : z == s ? 1.0 : (double)z / (double)s;
+  __syncthreads();
+  const int8_t *src = is_v ? c.v : c.k;
+  int8_t *dst = (is_v ? o.v : o.k) + b * o.st_seq + hk * o.st_head + p0 * o.st_token;
+  const int quads = c.hs >> 2;
+#pragma unroll 4
+  for (int e = tid; e < nt * quads; e += 256) {
+    const int i = e / quads, d = 4 * (e - i * quads);
+    uint32_t x = *(const uint32_t *)(src + at[i] + d);
+    const double r = ratio[i];
+    if (r != 1.0) x = r < 0.0 ? 0u : rescale4(x, r);
+    *(uint32_t *)(dst + i * o.st_token + d) = x;
   }
-  if (threadIdx.x == 0) (is_v ? o.vs : o.ks)[b * o.sc_seq + hk * o.sc_head + blk] = s;
+  if (tid == 0) (is_v ? o.vs : o.ks)[b * o.sc_seq + hk * o.sc_head + blk] = s;
 }
 
 // ------------------------------------------------------------- host side
@@ -775,7 +940,7 @@ int32_t simp_rt_kv8_append(
   if (bc.shares(cache, dk.data(), dk.bytes()) || bc.shares(cache, dv.data(), dv.bytes()))
     return set_error(SIMP_RT_EINVAL, "kv8_append: rows share memory with the cache");
   const int64_t slots = k_s0 / cache->block + 2 * cache->batch;
-  if (k_s0 > INT32_MAX || slots * 256 > UINT32_MAX)
+  if (k_s0 > INT32_MAX || slots * 1024 > UINT32_MAX)
     return set_error(SIMP_RT_EUNSUPPORTED, "kv8_append: more rows than the grid holds");
   const int dev = ensure_device();
   if (dev < 0) return dev;
@@ -788,8 +953,18 @@ int32_t simp_rt_kv8_append(
     return rc;
   const AppendArgs a{bc.c, (const float *)ok.dev(), (const float *)ov.dev(), (const int *)os.dev(),
                      (const int *)ol.dev(), k_st0, k_st1, v_st0, v_st1, (int)k_s0};
-  hipLaunchKernelGGL(kv8_append_k, dim3((unsigned)slots, (unsigned)bc.c.hk, 2), dim3(256), 0,
-                     cur_stream(), a);
+  const dim3 grid((unsigned)slots, (unsigned)bc.c.hk, 2);
+  const bool vec = ((k_st0 | k_st1 | v_st0 | v_st1) & 3) == 0 && (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0;
+  const int64_t chunks = (int64_t)cache->block * bc.c.hs / 4;  // of a whole block
+#define APPEND(N)                                                                              \
+  do {                                                                                         \
+    if (vec) hipLaunchKernelGGL((kv8_append_k<N, true>), grid, dim3(N), 0, cur_stream(), a);   \
+    else hipLaunchKernelGGL((kv8_append_k<N, false>), grid, dim3(N), 0, cur_stream(), a);      \
+  } while (0)
+  if (chunks <= 64 * kAppendChunks) APPEND(64);
+  else if (chunks <= 256 * kAppendChunks) APPEND(256);
+  else APPEND(1024);
+#undef APPEND
   Operand *ops[] = {&ok, &ov, &os, &ol};
   return finish(ops, 4);
 }
@@ -814,7 +989,7 @@ int32_t simp_rt_kv8_read(
   if (!dk.is(k_s0, cache->n_kv_heads, cache->head_size) || !dv.is(k_s0, k_s1, k_s2))
     return set_error(SIMP_RT_EINVAL, "kv8_read: k and v must be [rows, n_kv_heads, head_size]");
   if (cache->batch == 0 || cache->n_kv_heads == 0 || k_s0 == 0) return SIMP_RT_OK;
-  if (k_s0 > INT32_MAX || k_s0 * 64 > UINT32_MAX)
+  if (cdiv(k_s0, kReadRows) * 256 > UINT32_MAX)
     return set_error(SIMP_RT_EUNSUPPORTED, "kv8_read: more rows than the grid holds");
   if (bc.empty) return set_error(SIMP_RT_EINVAL, "kv8_read: the cache has no capacity");
   if (bc.shares(cache, dk.data(), dk.bytes()) || bc.shares(cache, dv.data(), dv.bytes()))
@@ -830,8 +1005,11 @@ int32_t simp_rt_kv8_read(
     return rc;
   const ReadArgs a{bc.c, (const int *)os.dev(), (const int *)ol.dev(), (float *)ok.dev(),
                    (float *)ov.dev(), k_st0, k_st1, v_st0, v_st1, (int)k_s0};
-  hipLaunchKernelGGL(kv8_read_k, dim3((unsigned)k_s0, (unsigned)bc.c.hk, 2), dim3(64), 0,
-                     cur_stream(), a);
+  const dim3 grid((unsigned)cdiv(k_s0, kReadRows), (unsigned)bc.c.hk);
+  if (((k_st0 | k_st1 | v_st0 | v_st1) & 3) == 0 && (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0)
+    hipLaunchKernelGGL(kv8_read_k<true>, grid, dim3(256), 0, cur_stream(), a);
+  else
+    hipLaunchKernelGGL(kv8_read_k<false>, grid, dim3(256), 0, cur_stream(), a);
   Operand *ops[] = {&ok, &ov, &os, &ol};
   return finish(ops, 4);
 }
