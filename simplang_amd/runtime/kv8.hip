@@ -270,7 +270,8 @@ struct AttnArgs {
   int sets, width;    // sets of up to `width` (at most 16) query heads of a kv head
   int chunk, splits;  // tokens a block takes; blocks for a full sequence
   float scale;        // times log2(e): the scores are powers of two
-  float *scores;      // [n, heads, cap], or null
+  float *scores;      // [n, heads, score_row], or null
+  int64_t score_row;  // the capacity in whole tiles of 64
   float *part;        // [n, heads, splits, head_size], unnormalised
   float2 *stat;       // [n, heads, splits]: maximum and sum
 };
@@ -296,6 +297,9 @@ __device__ __forceinline__ void turn4(const uint32_t (&in)[4], uint32_t (&out)[4
   out[3] = perm(d, b, 0x07060302);
 }
 
+// 2^x, below 2^-126 as 0
+__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // max / sum over the four lanes with the same lane % 16
 __device__ __forceinline__ float quad_max(float v) {
   float a = v, b = v;
@@ -312,70 +316,127 @@ __device__ __forceinline__ float quad_sum(float v) {
   return a + b;
 }
 
-// NC: 64-dimension chunks of a head.  blockIdx: chunk of tokens, kv head and set of
-// its query heads, sequence.
-template <int NC>
-__global__ void __launch_bounds__(256) kv8_attn_k(const AttnArgs a) {
+// 16 bytes from a 4-byte boundary
+__device__ __forceinline__ void load16(void *to, const void *p) {
+  __builtin_memcpy(to, __builtin_assume_aligned(p, 4), 16);
+}
+
+// The sum over the four lanes of a quad.
+__device__ __forceinline__ float quad_add(float v) {
+  v += dpp_mov<kDppXor1>(v);
+  return v + dpp_mov<kDppXor2>(v);
+}
+
+// NC: 64-dimension chunks of a head.  QUAD: up to four query heads, lane i of the 16
+// columns with byte i % 4 of head i / 4 (the fourth of them nothing), so that one
+// product does what three do with the bytes apart, one byte plane is kept instead of
+// three, and a sum over the quad joins them; else up to 16 heads, a column each.
+// blockIdx: chunk of tokens, kv head and set of its query heads, sequence.
+template <int NC, bool QUAD>
+__global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 ? 3 : NC == 3 ? 2 : 1)
+    kv8_attn_k(const AttnArgs a) {
   extern __shared__ float lds[];  // o [4][cols][hs], then m and l [4][cols]
+  constexpr int L = QUAD ? 1 : 3;
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i16 = lane & 15, g = lane >> 4, hs = c.hs;
-  const int hk = blockIdx.y / a.sets, first = ((int)blockIdx.y - hk * a.sets) * a.width;
-  const int cols = min(a.width, a.group - first), h0 = hk * a.group + first;  // query heads h0 ..
+  const int head = QUAD ? i16 >> 2 : i16, byte = QUAD ? i16 & 3 : 0;  // of the lane's column
+  const int hk = blockIdx.y / a.sets, set0 = ((int)blockIdx.y - hk * a.sets) * a.width;
+  const int cols = min(a.width, a.group - set0), h0 = hk * a.group + set0;  // query heads h0 ..
   const int b = blockIdx.z;
-  const int len = (int)clampl(a.lengths[b], 0, c.cap);
+  const int len = clampi(a.lengths[b], 0, c.cap);
   const int from = blockIdx.x * a.chunk;
   if (from >= len) return;
   const int to = len - from < a.chunk ? len : from + a.chunk;
   const int8_t *kp = c.k + b * c.st_seq + hk * c.st_head;
   const int8_t *vp = c.v + b * c.st_seq + hk * c.st_head;
   const float *ksp = c.ks + b * c.sc_seq + hk * c.sc_head, *vsp = c.vs + b * c.sc_seq + hk * c.sc_head;
+  // What takes the lane's byte of two numbers, makes it signed, and its weight.
+  const uint32_t pick = byte == 3 ? 0x0c0c0c0cu : 0x0c0c0400u + 0x0101u * byte;
+  const uint32_t flip = byte == 3 ? 0u : 0x80808080u;
+  const float weight = byte == 0 ? 1.f : byte == 1 ? 256.f : byte == 2 ? 65536.f : 0.f;
+  auto bytes_of = [&](const uint32_t (&u)[4], uint32_t (&l)[L]) {
+    if constexpr (QUAD) l[0] = perm(perm(u[3], u[2], pick), perm(u[1], u[0], pick), 0x05040100) ^ flip;
+    else planes(u, l[0], l[1], l[2]);
+  };
+  // The number that a column's products stand for (the lane's byte's part of it).
+  auto number = [&](const v4i (&x)[L], int r) {
+    if constexpr (QUAD) return (float)x[0][r] * weight;
+    else return fmaf((float)x[2][r], 65536.f, (float)(x[1][r] * 256 + x[0][r]));
+  };
 
-  // Query head i16's dimensions as the lane's K loads have them: 16 from doff on, of
-  // which those below 64 j + 16 g belong to the chunk before (the row's end).
-  v4i ql[NC][3];
-  int doff[NC];
+  // The head's dimensions as the lane's K loads have them: 16 from doff on, of which
+  // those below 64 j + 16 g belong to the chunk before (the row's end).
+  uint32_t doff[NC];
+  v4i ql[NC][L];
   float qf;
   {
     float x[NC][16], top = 0.f;
     bool odd = false;
-    const float *qr = a.q + b * a.q_seq + (h0 + min(i16, cols - 1)) * a.q_head;
+    const float *qr = a.q + b * a.q_seq + (h0 + min(head, cols - 1)) * a.q_head;
 #pragma unroll
     for (int j = 0; j < NC; j++) {
-      const int d0 = 64 * j + 16 * g;
-      doff[j] = min(d0, hs - 16);
+      doff[j] = (uint32_t)min(64 * j + 16 * g, hs - 16);
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) load16(&x[j][e], qr + doff[j] + e);
+    }
+#pragma unroll
+    for (int j = 0; j < NC; j++)
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        x[j][e] = qr[doff[j] + e];
         odd |= !(fabsf(x[j][e]) < INFINITY);
-        if (doff[j] + e < d0) x[j][e] = 0.f;
+        if ((int)doff[j] + e < 64 * j + 16 * g) x[j][e] = 0.f;
         top = fmaxf(top, fabsf(x[j][e]));
       }
-    }
     top = quad_max(top);
     const unsigned long long who = __ballot(odd);  // a query that is not finite: its row is NaN
     if ((who >> i16) & 0x0001000100010001ull) top = NAN;
     qf = top * a.scale / kUnit;
-    const float inv = top > 0.f ? 1.f / top : 0.f;
-    const bool tiny = top < 1e-30f;  // 1 / top may overflow: divide
+    // by way of [1, 2): 1 / top alone may be too large
+    const int e2 = top > 0.f ? -ilogbf(top) : 0;
+    const float inv = top > 0.f ? kUnit / ldexpf(top, e2) : 0.f;
 #pragma unroll
     for (int j = 0; j < NC; j++)
 #pragma unroll
       for (int w = 0; w < 4; w++) {
-        uint32_t u[4];
+        uint32_t u[4], l[L];
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const float v = x[j][4 * w + r];
-          const float f = tiny ? (top > 0.f ? v / top : 0.f) : v * inv;
-          u[r] = (uint32_t)(__float2int_rn(f * kUnit) + (int)kBytes);
-        }
-        uint32_t l0, l1, l2;
-        planes(u, l0, l1, l2);
-        ql[j][0][w] = (int)l0;
-        ql[j][1][w] = (int)l1;
-        ql[j][2][w] = (int)l2;
+        for (int r = 0; r < 4; r++)
+          u[r] = (uint32_t)(__float2int_rn(ldexpf(x[j][4 * w + r], e2) * inv) + (int)kBytes);
+        bytes_of(u, l);
+#pragma unroll
+        for (int i = 0; i < L; i++) ql[j][i][w] = (int)l[i];
       }
   }
+  const int last = len - 1;
+  // Addresses: a wave-uniform base for the tile, and 24-bit row numbers times strides
+  // below 2^24 (the caller sees to that).
+  const uint32_t stride = (uint32_t)c.st_token;
+  v4i kf[4][NC];
+  uint32_t vf[4][NC][4];
+  auto load_k = [&](int key0) {
+    const int8_t *base = kp + (int64_t)key0 * c.st_token;
+    const uint32_t lim = (uint32_t)(last - key0);
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      const uint32_t row = __umul24(min((uint32_t)(16 * t + i16), lim), stride);
+#pragma unroll
+      for (int j = 0; j < NC; j++) load16(&kf[t][j], base + (row + doff[j]));
+    }
+  };
+  auto load_v = [&](int key0) {
+    const int8_t *base = vp + (int64_t)key0 * c.st_token;
+    const uint32_t lim = (uint32_t)(last - key0);
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const uint32_t row = __umul24(min((uint32_t)(16 * t + 4 * g + r), lim), stride);
+#pragma unroll
+        for (int j = 0; j < NC; j++)
+          vf[t][j][r] = *(const uint32_t *)(base + (row + (uint32_t)min(64 * j + 4 * i16, hs - 4)));
+      }
+  };
 
   float o[NC][4][4];  // [j][n][r]: d = 64 j + 16 g + 4 r + n
 #pragma unroll
@@ -385,24 +446,12 @@ __global__ void __launch_bounds__(256) kv8_attn_k(const AttnArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; r++) o[j][n][r] = 0.f;
   float m = -INFINITY, l = 0.f;
-  const int last = len - 1;
+  float *scores = a.scores ? a.scores + ((int64_t)b * a.heads + h0 + min(head, cols - 1)) * a.score_row + 4 * g
+                           : nullptr;
+  const bool keeper = head < cols && byte == 0;  // writes what its column's lanes agree on
   for (int key0 = from + 64 * wave; key0 < to; key0 += 256) {
-    v4i kf[4][NC];
-    uint32_t vf[4][NC][4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-      const int8_t *row = kp + (int64_t)min(key0 + 16 * t + i16, last) * c.st_token;
-#pragma unroll
-      for (int j = 0; j < NC; j++) __builtin_memcpy(&kf[t][j], __builtin_assume_aligned(row + doff[j], 4), 16);
-    }
-#pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int8_t *row = vp + (int64_t)min(key0 + 16 * t + 4 * g + r, last) * c.st_token;
-#pragma unroll
-        for (int j = 0; j < NC; j++) vf[t][j][r] = *(const uint32_t *)(row + min(64 * j + 4 * i16, hs - 4));
-      }
+    load_k(key0);
+    load_v(key0);
     float ks[4], vs[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
@@ -411,70 +460,71 @@ __global__ void __launch_bounds__(256) kv8_attn_k(const AttnArgs a) {
       vs[t] = vsp[blk];
     }
     // scores
+    const int left = to - key0 - 4 * g;  // tokens 16 t + r below it are there
     float s[4][4];
     float mt = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-      v4i s0 = {0, 0, 0, 0}, s1 = s0, s2 = s0;
+      v4i x[L];
 #pragma unroll
-      for (int j = 0; j < NC; j++) {
-        s0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][j], ql[j][0], s0, 0, 0, 0);
-        s1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][j], ql[j][1], s1, 0, 0, 0);
-        s2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][j], ql[j][2], s2, 0, 0, 0);
-      }
+      for (int i = 0; i < L; i++) x[i] = v4i{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < NC; j++)
+#pragma unroll
+        for (int i = 0; i < L; i++)
+          x[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][j], ql[j][i], x[i], 0, 0, 0);
       const float f = qf * ks[t];
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const float x = fmaf((float)s2[r], 65536.f, (float)(s1[r] * 256 + s0[r])) * f;
-        s[t][r] = key0 + 16 * t + 4 * g + r < to ? x : -INFINITY;
+        float y = number(x, r);
+        if (QUAD) y = quad_add(y);
+        s[t][r] = 16 * t + r < left ? y * f : -INFINITY;
         mt = fmaxf(mt, s[t][r]);
       }
     }
-    if (a.scores && i16 < cols) {
-      float *sp = a.scores + ((int64_t)b * a.heads + h0 + i16) * c.cap + key0 + 4 * g;
+    if (scores && keeper) {  // score rows are padded to whole tiles
 #pragma unroll
       for (int t = 0; t < 4; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-          if (key0 + 16 * t + 4 * g + r < to) sp[16 * t + r] = s[t][r];
+        *(float4 *)(scores + key0 + 16 * t) = make_float4(s[t][0], s[t][1], s[t][2], s[t][3]);
     }
     mt = quad_max(mt);
     const float mu = mt == -INFINITY ? 0.f : mt;
     // weights
     const float vsum = (vs[0] + vs[1]) + (vs[2] + vs[3]);
-    float vtop = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-    if (!(vsum < INFINITY)) vtop = NAN;  // a block that is not finite: the row is NaN
+    const float vtop = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+    const int ve = vtop > 0.f ? ilogbf(vtop) : 0;  // the scales over 2^ve lie below 2
     float w[4][4], lt = 0.f, wt = 0.f;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-      const float vr = vtop > 0.f ? vs[t] / vtop : 0.f;
+      const float vr = ldexpf(vs[t], -ve);
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const float p = key0 + 16 * t + 4 * g + r < to ? exp2f(s[t][r] - mu) : 0.f;
+        const float p = 16 * t + r < left ? pow2(s[t][r] - mu) : 0.f;
         lt += p;
         w[t][r] = p * vr;
         wt = fmaxf(wt, w[t][r]);
       }
     }
     wt = fmaxf(quad_max(wt), 1e-30f);
-    const float inv = kUnit / wt;
-    v4i wl[3];
+    const float inv = kUnit * __builtin_amdgcn_rcpf(wt);
+    v4i wl[L];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-      uint32_t u[4], l0, l1, l2;
+      uint32_t u[4], y[L];
 #pragma unroll
       for (int r = 0; r < 4; r++)  // the sum with 2^23 has the rounded number in its low bits
         u[r] = __float_as_uint(fmaf(w[t][r], inv, 8388608.f)) + kBytes;
-      planes(u, l0, l1, l2);
-      wl[0][t] = (int)l0;
-      wl[1][t] = (int)l1;
-      wl[2][t] = (int)l2;
+      bytes_of(u, y);
+#pragma unroll
+      for (int i = 0; i < L; i++) wl[i][t] = (int)y[i];
     }
     const float mn = fmaxf(m, mt), mnu = mn == -INFINITY ? 0.f : mn;
-    const float alpha = exp2f(m - mnu), beta = exp2f(mt - mnu);
+    const float alpha = pow2(m - mnu), beta = pow2(mt - mnu);
     m = mn;
     l = fmaf(l, alpha, lt * beta);
-    const float f = vtop * beta * (wt / kUnit);
+    float f = ldexpf(beta * wt * (1.f / kUnit), ve);
+    if (!(vsum < INFINITY)) f = NAN;  // a block that is not finite: the row is NaN
+    if (QUAD) f *= weight;
 #pragma unroll
     for (int j = 0; j < NC; j++) {
       v4i vt[4];
@@ -487,14 +537,14 @@ __global__ void __launch_bounds__(256) kv8_attn_k(const AttnArgs a) {
       }
 #pragma unroll
       for (int n = 0; n < 4; n++) {
-        const v4i z = {0, 0, 0, 0};
-        const v4i o0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vt[n], wl[0], z, 0, 0, 0);
-        const v4i o1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vt[n], wl[1], z, 0, 0, 0);
-        const v4i o2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(vt[n], wl[2], z, 0, 0, 0);
+        v4i x[L];
+#pragma unroll
+        for (int i = 0; i < L; i++)
+          x[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vt[n], wl[i], v4i{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          const float x = fmaf((float)o2[r], 65536.f, (float)(o1[r] * 256 + o0[r]));
-          o[j][n][r] = fmaf(x, f, o[j][n][r] * alpha);
+          const float y = QUAD ? (float)x[0][r] : number(x, r);
+          o[j][n][r] = fmaf(y, f, o[j][n][r] * alpha);
         }
       }
     }
@@ -502,19 +552,19 @@ __global__ void __launch_bounds__(256) kv8_attn_k(const AttnArgs a) {
   // the four waves' rows together
   l = quad_sum(l);
   float *ml = lds + 4 * cols * hs;
-  if (i16 < cols) {
-    float *row = lds + (wave * cols + i16) * hs;
+  float *row = lds + (wave * cols + min(head, cols - 1)) * hs;
 #pragma unroll
-    for (int j = 0; j < NC; j++)
+  for (int j = 0; j < NC; j++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int d = 64 * j + 16 * g + 4 * r;
-        if (d < hs) *(float4 *)(row + d) = make_float4(o[j][0][r], o[j][1][r], o[j][2][r], o[j][3][r]);
-      }
-    if (g == 0) {
-      ml[wave * cols + i16] = m;
-      ml[(4 + wave) * cols + i16] = l;
+    for (int r = 0; r < 4; r++) {
+      const int d = 64 * j + 16 * g + 4 * r;
+      float4 x = make_float4(o[j][0][r], o[j][1][r], o[j][2][r], o[j][3][r]);
+      if (QUAD) x = make_float4(quad_add(x.x), quad_add(x.y), quad_add(x.z), quad_add(x.w));
+      if (keeper && d < hs) *(float4 *)(row + d) = x;
     }
+  if (keeper && g == 0) {
+    ml[wave * cols + head] = m;
+    ml[(4 + wave) * cols + head] = l;
   }
   __syncthreads();
   const int quads = hs >> 2;
@@ -524,96 +574,110 @@ __global__ void __launch_bounds__(256) kv8_attn_k(const AttnArgs a) {
 #pragma unroll
     for (int w = 0; w < 4; w++) M = fmaxf(M, ml[w * cols + col]);
     const float mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
+    float sum = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < 4; w++) {
-      const float f = exp2f(ml[w * cols + col] - mu);
+      const float f = pow2(ml[w * cols + col] - mu);
       const float4 y = *(const float4 *)(lds + (w * cols + col) * hs + d);
-      L = fmaf(f, ml[(4 + w) * cols + col], L);
+      sum = fmaf(f, ml[(4 + w) * cols + col], sum);
       x.x = fmaf(f, y.x, x.x);
       x.y = fmaf(f, y.y, x.y);
       x.z = fmaf(f, y.z, x.z);
       x.w = fmaf(f, y.w, x.w);
     }
-    const int64_t row = ((int64_t)b * a.heads + h0 + col) * a.splits + blockIdx.x;
-    *(float4 *)(a.part + row * hs + d) = x;
-    if (d == 0) a.stat[row] = make_float2(M, L);
+    const int64_t at = ((int64_t)b * a.heads + h0 + col) * a.splits + blockIdx.x;
+    *(float4 *)(a.part + at * hs + d) = x;
+    if (d == 0) a.stat[at] = make_float2(M, sum);
   }
 }
 
 constexpr int kSeenTile = 1024;
 
 // The chunks of a row together.  blockIdx.x below the group: that query head's row of
-// out; above: kSeenTile tokens of the accumulated weights.
-__global__ void __launch_bounds__(256) kv8_join_k(const AttnArgs a) {
+// out, head_size / 4 threads to a chunk and as many chunks at a time as there are
+// threads; above: kSeenTile tokens of the accumulated weights.
+__global__ void __launch_bounds__(1024) kv8_join_k(const AttnArgs a) {
   extern __shared__ float lds[];
+  __shared__ float4 so[1024];
+  __shared__ float top_s[16], sum_s[16];
   const Cache &c = a.c;
-  const int hk = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int len = (int)clampl(a.lengths[b], 0, c.cap);
+  const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int len = clampi(a.lengths[b], 0, c.cap);
   const int ns = len ? (len - 1) / a.chunk + 1 : 0, hs = c.hs;
   if ((int)blockIdx.x < a.group) {
     const int h = hk * a.group + blockIdx.x;
     float *out = a.out + b * a.o_seq + h * a.o_head;
     if (len == 0) {
-      for (int d = threadIdx.x; d < hs; d += 256) out[d] = 0.f;
+      for (int d = tid; d < hs; d += 1024) out[d] = 0.f;
       return;
     }
     const float2 *st = a.stat + ((int64_t)b * a.heads + h) * a.splits;
     const float *part = a.part + ((int64_t)b * a.heads + h) * a.splits * hs;
-    __shared__ float scratch[16];
-    __shared__ float so[4][256];
     float M = -INFINITY;
-    for (int s = threadIdx.x; s < ns; s += 256) M = fmaxf(M, st[s].x);
-    M = block_max(M, scratch);
+    for (int s = tid; s < ns; s += 1024) M = fmaxf(M, st[s].x);
+    M = wave_max_dpp(M);
+    if (lane == 0) top_s[wave] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 16; w++) M = fmaxf(M, top_s[w]);
     const float mu = M == -INFINITY ? 0.f : M;
     float L = 0.f;
-    for (int s = threadIdx.x; s < ns; s += 256) {
-      const float f = exp2f(st[s].x - mu);
+    for (int s = tid; s < ns; s += 1024) {
+      const float f = pow2(st[s].x - mu);
       lds[s] = f;
       L = fmaf(f, st[s].y, L);
     }
-    L = block_sum(L, scratch);  // its barriers make lds[] visible too
-    if (4 * lane < hs) {
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int s = wave; s < ns; s += 4) {
+    L = wave_sum_dpp(L);
+    if (lane == 0) sum_s[wave] = L;
+    __syncthreads();
+    const int quads = hs >> 2, rows = 1024 / quads, r = tid / quads, q = tid - r * quads;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < rows) {
+#pragma unroll 4
+      for (int s = r; s < ns; s += rows) {
         const float f = lds[s];
-        const float4 y = *(const float4 *)(part + (int64_t)s * hs + 4 * lane);
+        const float4 y = *(const float4 *)(part + (int64_t)s * hs + 4 * q);
         x.x = fmaf(f, y.x, x.x);
         x.y = fmaf(f, y.y, x.y);
         x.z = fmaf(f, y.z, x.z);
         x.w = fmaf(f, y.w, x.w);
       }
-      *(float4 *)&so[wave][4 * lane] = x;
     }
+    so[tid] = x;
     __syncthreads();
-    for (int d = threadIdx.x; d < hs; d += 256)
-      out[d] = (so[0][d] + so[1][d] + so[2][d] + so[3][d]) / L;
+    if (tid < hs) {
+      float s = 0.f, l = 0.f;
+      for (int i = 0; i < min(rows, ns); i++) s += ((const float *)so)[4 * (i * quads + (tid >> 2)) + (tid & 3)];
+#pragma unroll
+      for (int w = 0; w < 16; w++) l += sum_s[w];
+      out[tid] = s / l;
+    }
     return;
   }
-  const int t0 = ((int)blockIdx.x - a.group) * kSeenTile;
-  if (t0 >= len) return;
-  for (int g = wave; g < a.group; g += 4) {  // each head's maximum and 1 / sum
+  const int t = ((int)blockIdx.x - a.group) * kSeenTile + tid;
+  if (t - tid >= len) return;
+  for (int g = wave; g < a.group; g += 16) {  // each head's maximum and 1 / sum
     const float2 *st = a.stat + ((int64_t)b * a.heads + hk * a.group + g) * a.splits;
     float M = -INFINITY, L = 0.f;
     for (int s = lane; s < ns; s += 64) M = fmaxf(M, st[s].x);
-    M = wave_max(M);
+    M = wave_max_dpp(M);
     const float mu = M == -INFINITY ? 0.f : M;
-    for (int s = lane; s < ns; s += 64) L = fmaf(exp2f(st[s].x - mu), st[s].y, L);
-    L = wave_sum(L);
+    for (int s = lane; s < ns; s += 64) L = fmaf(pow2(st[s].x - mu), st[s].y, L);
+    L = wave_sum_dpp(L);
     if (lane == 0) {
       lds[2 * g] = mu;
       lds[2 * g + 1] = 1.f / L;
     }
   }
   __syncthreads();
-  const float *sc = a.scores + ((int64_t)b * a.heads + hk * a.group) * c.cap;
-  for (int t = t0 + threadIdx.x; t < min(t0 + kSeenTile, len); t += 256) {
-    float w = 0.f;
-    for (int g = 0; g < a.group; g++)
-      w = fmaf(exp2f(sc[(int64_t)g * c.cap + t] - lds[2 * g]), lds[2 * g + 1], w);
-    a.seen_out[b * a.so_seq + hk * a.so_head + t] = a.seen_in[b * a.si_seq + hk * a.si_head + t] + w;
-  }
+  if (t >= len) return;
+  const float *sc = a.scores + ((int64_t)b * a.heads + hk * a.group) * a.score_row + t;
+  float w = 0.f;
+#pragma unroll 4
+  for (int g = 0; g < a.group; g++)
+    w = fmaf(pow2(sc[g * a.score_row] - lds[2 * g]), lds[2 * g + 1], w);
+  a.seen_out[b * a.so_seq + hk * a.so_head + t] = a.seen_in[b * a.si_seq + hk * a.si_head + t] + w;
 }
 
 // ----------------------------------------------------------------- evict
@@ -850,6 +914,8 @@ struct BoundCache {
       return set_error(SIMP_RT_EUNSUPPORTED,
                        "%s: %s: head_size %lld is not a multiple of 4 in 16..256", fn, name,
                        (long long)p->head_size);
+    if (p->st_token >= 1 << 24)
+      return set_error(SIMP_RT_EUNSUPPORTED, "%s: %s: token stride of 2^24 or more", fn, name);
     if (p->batch > 32767 || p->n_kv_heads > 32767 || p->capacity > INT32_MAX - 4096)
       return set_error(SIMP_RT_EUNSUPPORTED, "%s: %s: batch or heads above 32767, or capacity above 2^31 - 4097",
                        fn, name);
@@ -1082,7 +1148,9 @@ int32_t simp_rt_kv8_attention(
   hipStream_t st = cur_stream();
   // Four tiles of 64 tokens to a block, one per wave, and more where the full cache
   // would have more than 2048 blocks (8 a CU).
-  a.width = bc.c.hs > 192 ? 8 : 16;  // the block's rows fit 64 KB of LDS
+  // A quad of lanes to a head up to four of them; else 16, or the 8 whose rows fit 64 KB
+  // of LDS.
+  a.width = a.group <= 4 ? 4 : bc.c.hs > 192 ? 8 : 16;
   a.sets = (int)cdiv(a.group, a.width);
   const int64_t per = (int64_t)bc.c.n * bc.c.hk * a.sets;
   a.chunk = (int)(256 * std::max<int64_t>(1, cdiv(per * bc.c.cap, 2048 * 256)));
@@ -1090,23 +1158,27 @@ int32_t simp_rt_kv8_attention(
   const size_t rows = (size_t)q_s0 * (size_t)q_s1, parts = rows * (size_t)a.splits;
   Workspace ws;
   float *p = nullptr;
-  if ((rc = ws.get(st, 4 * (parts * (size_t)bc.c.hs + 2 * parts + (with ? rows * (size_t)bc.c.cap : 0)),
-                   (void **)&p, 8)))
-    return rc;
-  a.part = p;
-  a.stat = (float2 *)(p + parts * (size_t)bc.c.hs);
-  a.scores = with ? p + parts * (size_t)(bc.c.hs + 2) : nullptr;
+  a.score_row = cdiv(bc.c.cap, 64) * 64;
+  const size_t scores = with ? rows * (size_t)a.score_row : 0;
+  if ((rc = ws.get(st, 4 * (scores + parts * (size_t)(bc.c.hs + 2)), (void **)&p, 8))) return rc;
+  a.scores = with ? p : nullptr;
+  a.part = p + scores;
+  a.stat = (float2 *)(a.part + parts * (size_t)bc.c.hs);
   const size_t cols = (size_t)std::min(a.group, a.width);
   const unsigned lds = (unsigned)(4 * 4 * cols * ((size_t)bc.c.hs + 2));
   const dim3 grid((unsigned)a.splits, (unsigned)(bc.c.hk * a.sets), (unsigned)bc.c.n);
-#define ATTN(NC) hipLaunchKernelGGL(kv8_attn_k<NC>, grid, dim3(256), lds, st, a)
+#define ATTN(NC)                                                                      \
+  do {                                                                                \
+    if (a.group <= 4) hipLaunchKernelGGL((kv8_attn_k<NC, true>), grid, dim3(256), lds, st, a); \
+    else hipLaunchKernelGGL((kv8_attn_k<NC, false>), grid, dim3(256), lds, st, a);    \
+  } while (0)
   if (bc.c.hs <= 64) ATTN(1);
   else if (bc.c.hs <= 128) ATTN(2);
   else if (bc.c.hs <= 192) ATTN(3);
   else ATTN(4);
 #undef ATTN
   const unsigned jx = (unsigned)(a.group + (with ? cdiv(bc.c.cap, kSeenTile) : 0));
-  hipLaunchKernelGGL(kv8_join_k, dim3(jx, (unsigned)bc.c.hk, (unsigned)bc.c.n), dim3(256),
+  hipLaunchKernelGGL(kv8_join_k, dim3(jx, (unsigned)bc.c.hk, (unsigned)bc.c.n), dim3(1024),
                      4 * std::max(a.splits, 2 * a.group), st, a);
   Operand *ops[] = {&oq, &ol, &oo, &osi, &oso};
   return finish(ops, with ? 5 : 3);
