@@ -333,7 +333,7 @@ __device__ __forceinline__ float quad_add(float v) {
 // three, and a sum over the quad joins them; else up to 16 heads, a column each.
 // blockIdx: chunk of tokens, kv head and set of its query heads, sequence.
 template <int NC, bool QUAD>
-__global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 ? 3 : NC == 3 ? 2 : 1)
+__global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 && QUAD ? 3 : NC < 4 ? 2 : 1)
     kv8_attn_k(const AttnArgs a) {
   extern __shared__ float lds[];  // o [4][cols][hs], then m and l [4][cols]
   constexpr int L = QUAD ? 1 : 3;
@@ -438,6 +438,7 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 ? 3 : NC == 3 ? 2 :
       }
   };
 
+  if (from + 64 * wave < to) load_k(from + 64 * wave);
   float o[NC][4][4];  // [j][n][r]: d = 64 j + 16 g + 4 r + n
 #pragma unroll
   for (int j = 0; j < NC; j++)
@@ -450,7 +451,6 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 ? 3 : NC == 3 ? 2 :
                            : nullptr;
   const bool keeper = head < cols && byte == 0;  // writes what its column's lanes agree on
   for (int key0 = from + 64 * wave; key0 < to; key0 += 256) {
-    load_k(key0);
     load_v(key0);
     float ks[4], vs[4];
 #pragma unroll
@@ -482,6 +482,7 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 ? 3 : NC == 3 ? 2 :
         mt = fmaxf(mt, s[t][r]);
       }
     }
+    load_k(min(key0 + 256, last));  // the next tile's, on their way during this one's V
     if (scores && keeper) {  // score rows are padded to whole tiles
 #pragma unroll
       for (int t = 0; t < 4; t++)
@@ -592,15 +593,15 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 ? 3 : NC == 3 ? 2 :
   }
 }
 
-constexpr int kSeenTile = 1024;
+constexpr int kSeenTile = 512;
 
 // The chunks of a row together.  blockIdx.x below the group: that query head's row of
 // out, head_size / 4 threads to a chunk and as many chunks at a time as there are
 // threads; above: kSeenTile tokens of the accumulated weights.
-__global__ void __launch_bounds__(1024) kv8_join_k(const AttnArgs a) {
+__global__ void __launch_bounds__(256) kv8_join_k(const AttnArgs a) {
   extern __shared__ float lds[];
-  __shared__ float4 so[1024];
-  __shared__ float top_s[16], sum_s[16];
+  __shared__ float4 so[256];
+  __shared__ float top_s[4], sum_s[4];
   const Cache &c = a.c;
   const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int len = clampi(a.lengths[b], 0, c.cap);
@@ -609,21 +610,21 @@ __global__ void __launch_bounds__(1024) kv8_join_k(const AttnArgs a) {
     const int h = hk * a.group + blockIdx.x;
     float *out = a.out + b * a.o_seq + h * a.o_head;
     if (len == 0) {
-      for (int d = tid; d < hs; d += 1024) out[d] = 0.f;
+      for (int d = tid; d < hs; d += 256) out[d] = 0.f;
       return;
     }
     const float2 *st = a.stat + ((int64_t)b * a.heads + h) * a.splits;
     const float *part = a.part + ((int64_t)b * a.heads + h) * a.splits * hs;
     float M = -INFINITY;
-    for (int s = tid; s < ns; s += 1024) M = fmaxf(M, st[s].x);
+    for (int s = tid; s < ns; s += 256) M = fmaxf(M, st[s].x);
     M = wave_max_dpp(M);
     if (lane == 0) top_s[wave] = M;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 16; w++) M = fmaxf(M, top_s[w]);
+    for (int w = 0; w < 4; w++) M = fmaxf(M, top_s[w]);
     const float mu = M == -INFINITY ? 0.f : M;
     float L = 0.f;
-    for (int s = tid; s < ns; s += 1024) {
+    for (int s = tid; s < ns; s += 256) {
       const float f = pow2(st[s].x - mu);
       lds[s] = f;
       L = fmaf(f, st[s].y, L);
@@ -631,7 +632,7 @@ __global__ void __launch_bounds__(1024) kv8_join_k(const AttnArgs a) {
     L = wave_sum_dpp(L);
     if (lane == 0) sum_s[wave] = L;
     __syncthreads();
-    const int quads = hs >> 2, rows = 1024 / quads, r = tid / quads, q = tid - r * quads;
+    const int quads = hs >> 2, rows = 256 / quads, r = tid / quads, q = tid - r * quads;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < rows) {
 #pragma unroll 4
@@ -646,18 +647,18 @@ __global__ void __launch_bounds__(1024) kv8_join_k(const AttnArgs a) {
     }
     so[tid] = x;
     __syncthreads();
-    if (tid < hs) {
+    for (int d = tid; d < hs; d += 256) {
       float s = 0.f, l = 0.f;
-      for (int i = 0; i < min(rows, ns); i++) s += ((const float *)so)[4 * (i * quads + (tid >> 2)) + (tid & 3)];
+      for (int i = 0; i < min(rows, ns); i++) s += ((const float *)so)[4 * (i * quads + (d >> 2)) + (d & 3)];
 #pragma unroll
-      for (int w = 0; w < 16; w++) l += sum_s[w];
-      out[tid] = s / l;
+      for (int w = 0; w < 4; w++) l += sum_s[w];
+      out[d] = s / l;
     }
     return;
   }
-  const int t = ((int)blockIdx.x - a.group) * kSeenTile + tid;
-  if (t - tid >= len) return;
-  for (int g = wave; g < a.group; g += 16) {  // each head's maximum and 1 / sum
+  const int t0 = ((int)blockIdx.x - a.group) * kSeenTile;
+  if (t0 >= len) return;
+  for (int g = wave; g < a.group; g += 4) {  // each head's maximum and 1 / sum
     const float2 *st = a.stat + ((int64_t)b * a.heads + hk * a.group + g) * a.splits;
     float M = -INFINITY, L = 0.f;
     for (int s = lane; s < ns; s += 64) M = fmaxf(M, st[s].x);
@@ -671,13 +672,14 @@ __global__ void __launch_bounds__(1024) kv8_join_k(const AttnArgs a) {
     }
   }
   __syncthreads();
-  if (t >= len) return;
-  const float *sc = a.scores + ((int64_t)b * a.heads + hk * a.group) * a.score_row + t;
-  float w = 0.f;
+  for (int t = t0 + tid; t < min(t0 + kSeenTile, len); t += 256) {
+    const float *sc = a.scores + ((int64_t)b * a.heads + hk * a.group) * a.score_row + t;
+    float w = 0.f;
 #pragma unroll 4
-  for (int g = 0; g < a.group; g++)
-    w = fmaf(pow2(sc[g * a.score_row] - lds[2 * g]), lds[2 * g + 1], w);
-  a.seen_out[b * a.so_seq + hk * a.so_head + t] = a.seen_in[b * a.si_seq + hk * a.si_head + t] + w;
+    for (int g = 0; g < a.group; g++)
+      w = fmaf(pow2(sc[g * a.score_row] - lds[2 * g]), lds[2 * g + 1], w);
+    a.seen_out[b * a.so_seq + hk * a.so_head + t] = a.seen_in[b * a.si_seq + hk * a.si_head + t] + w;
+  }
 }
 
 // ----------------------------------------------------------------- evict
@@ -1146,14 +1148,17 @@ int32_t simp_rt_kv8_attention(
   a.heads = (int)q_s1, a.group = (int)(q_s1 / cache->n_kv_heads);
   a.scale = (float)(scale * 1.4426950408889634);
   hipStream_t st = cur_stream();
-  // Four tiles of 64 tokens to a block, one per wave, and more where the full cache
-  // would have more than 2048 blocks (8 a CU).
+  // Four tiles of 64 tokens to a block, one per wave, and more where the full cache would
+  // have more than 512 blocks (2 a CU): what a block does once (lengths, q, its rows
+  // joined and written) costs it as much as several tiles.  16 ragged sequences of up to
+  // 4096: 23.9 us with 2048 blocks, 22.5 with 1024, 18.7 with 512; 131072 tokens of one: the
+  // same with each.
   // A quad of lanes to a head up to four of them; else 16, or the 8 whose rows fit 64 KB
   // of LDS.
   a.width = a.group <= 4 ? 4 : bc.c.hs > 192 ? 8 : 16;
   a.sets = (int)cdiv(a.group, a.width);
   const int64_t per = (int64_t)bc.c.n * bc.c.hk * a.sets;
-  a.chunk = (int)(256 * std::max<int64_t>(1, cdiv(per * bc.c.cap, 2048 * 256)));
+  a.chunk = (int)(256 * std::max<int64_t>(1, cdiv(per * bc.c.cap, 512 * 256)));
   a.splits = (int)cdiv(bc.c.cap, a.chunk);
   const size_t rows = (size_t)q_s0 * (size_t)q_s1, parts = rows * (size_t)a.splits;
   Workspace ws;
@@ -1178,7 +1183,7 @@ int32_t simp_rt_kv8_attention(
   else ATTN(4);
 #undef ATTN
   const unsigned jx = (unsigned)(a.group + (with ? cdiv(bc.c.cap, kSeenTile) : 0));
-  hipLaunchKernelGGL(kv8_join_k, dim3(jx, (unsigned)bc.c.hk, (unsigned)bc.c.n), dim3(1024),
+  hipLaunchKernelGGL(kv8_join_k, dim3(jx, (unsigned)bc.c.hk, (unsigned)bc.c.n), dim3(256),
                      4 * std::max(a.splits, 2 * a.group), st, a);
   Operand *ops[] = {&oq, &ol, &oo, &osi, &oso};
   return finish(ops, with ? 5 : 3);
