@@ -5,11 +5,11 @@
 // and sum l: o and l are scaled by e^(m_old - m_new) when a tile raises m.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
+#include <type_traits>
 #include <utility>
 
-#include "rt_device.h"
 #include "serve_args.h"
+#include "serve_device.h"
 
 namespace simp {
 namespace {
@@ -25,20 +25,20 @@ struct PackedArgs {
   float scale;
 };
 
-__device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
-
-// The sequence of tile slot `t`, where sequence s has the slots q_starts[s] / R + s
-// and on: R rows a tile, so at most n_q / R + 1 of them, and the next one's begin
-// behind.  Ends with 0 <= s < n whatever the starts hold.
+// Tile slots: sequence s has the slots starts[s] / R + s and on, R rows a tile: at most
+// n / R + 1 of them for n rows, so the next one's begin behind.
 template <int R>
 __device__ __forceinline__ int seq_of_slot(const int *starts, int n, int rows, int t) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (clampi(starts[mid], 0, rows) / R + mid <= t) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
+  return last_of(n, [&](int s) { return clampi(starts[s], 0, rows) / R + s <= t; });
+}
+
+// The rows and keys of one sequence.
+struct Seq {
+  int qb, nq, kb, nk;  // first query row, queries, first key row, keys
+};
+__device__ __forceinline__ Seq seq_of(const PackedArgs &a, int s) {
+  const int qb = clampi(a.q_starts[s], 0, a.tq), kb = clampi(a.k_starts[s], 0, a.tk);
+  return Seq{qb, clampi(a.q_starts[s + 1], qb, a.tq) - qb, kb, clampi(a.k_starts[s + 1], kb, a.tk) - kb};
 }
 
 // Up to four values of a row from dimension d on, 0 past its end.
@@ -160,118 +160,85 @@ __device__ __forceinline__ void attend16(const PackedArgs &a, const float *qr, c
   l = x + y;
 }
 
-template <int HB>
-struct TileLds {
-  float o[4][16 * HB][17];
-  float m[4][16], l[4][16];
-};
-
-// A block takes 16 queries of one head (tile slot t); its four waves take the 16-key
-// tiles in turn, each with its own running maximum, sum and output, combined through LDS
-// at the end.  only: sequences to take part (n of them, kv heads apart), or null.
-template <int HB, bool VEC>
-__device__ __forceinline__ void f32_tile(const PackedArgs &a, int t, int h, const int *only,
-                                         TileLds<HB> &lds) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r16 = lane & 15, g = lane >> 4, hs = a.hs;
-  const int s = seq_of_slot<16>(a.q_starts, a.n, a.tq, t);
-  const int qb = clampi(a.q_starts[s], 0, a.tq), qe = clampi(a.q_starts[s + 1], qb, a.tq);
-  const int kb = clampi(a.k_starts[s], 0, a.tk), ke = clampi(a.k_starts[s + 1], kb, a.tk);
-  const int nq = qe - qb, nk = ke - kb;
-  const int slot0 = qb / 16 + s;
-  if (t < slot0 || t - slot0 >= (nq + 15) / 16) return;
-  if (only && !only[(int64_t)(h / a.group) * a.n + s]) return;
-  const int q0 = 16 * (t - slot0), row = min(q0 + r16, nq - 1);
-  v4f o[HB];
-  float m, l;
-  attend16<HB, VEC>(a, a.q + (int64_t)(qb + row) * a.q_row + h * a.q_head,
-                    a.k + (int64_t)kb * a.k_row + (h / a.group) * a.k_head,
-                    a.v + (int64_t)kb * a.v_row + (h / a.group) * a.v_head, row + nk - nq,
-                    q0 + nk - nq, min(q0 + 15, nq - 1) + nk - nq, 16 * wave, 64, o, m, l);
-  if (g == 0) {
-    lds.m[wave][r16] = m;
-    lds.l[wave][r16] = l;
-  }
-#pragma unroll
-  for (int j = 0; j < HB; j++)
-#pragma unroll
-    for (int r = 0; r < 4; r++) lds.o[wave][16 * j + 4 * g + r][r16] = o[j][r];
-  __syncthreads();
-  for (int e = threadIdx.x; e < 16 * hs; e += 256) {
-    const int qi = e / hs, d = e - qi * hs;
-    if (q0 + qi >= nq) break;  // queries in increasing order
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; w++) M = fmaxf(M, lds.m[w][qi]);
-    const float mu = M == -INFINITY ? 0.f : M;
-    float num = 0.f, den = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-      const float f = expf(lds.m[w][qi] - mu);
-      num = fmaf(f, lds.o[w][d][qi], num);
-      den = fmaf(f, lds.l[w][qi], den);
-    }
-    const bool none = q0 + qi + nk - nq < 0;
-    a.out[(int64_t)(qb + q0 + qi) * a.o_row + h * a.o_head + d] = none ? 0.f : num / den;
-  }
-}
-
-template <int HB, bool VEC>
-__global__ void __launch_bounds__(256) attn_f32_k(const PackedArgs a) {
-  __shared__ TileLds<HB> lds;
-  f32_tile<HB, VEC>(a, (int)(gridDim.x - 1 - blockIdx.x), blockIdx.y, nullptr, lds);
-}
-
 // ---- the split form
 //
-// Longer inputs run both products on v_mfma_f32_32x32x16_f16.  A number x, scaled by
-// a power of two to below 2^15, is hi + lo + r with hi = f16(x), lo = f16(x - hi) and
-// |r| <= 2^-22 |x| (2^-40 of the scaling's unit for the smallest); x y is taken as
-// hi hi + hi lo + lo hi, each product exact and each sum fp32.  That is as close as
-// an fp32 product, at three times an f16 product's cost instead of the fp32 matrix
-// instruction's sixteen.
-//   attn_split_k  takes K and V apart once: per 32 keys of a kv head a stage of
-//                 1 KB operand fragments in the order that the matrix instruction's
-//                 lanes want them, so that attn_f16_k moves them to LDS as they
-//                 are; and the two scalings (NaN where a value is not finite).
+// Both products on v_mfma_f32_32x32x16_f16.  A number x, scaled by a power of two to
+// below 2^15, is hi + lo + r with hi = f16(x), lo = f16(x - hi) and |r| <= 2^-22 |x|
+// (2^-40 of the scaling's unit for the smallest); x y is taken as hi hi + hi lo + lo hi,
+// each product exact and each sum fp32.  That is as close as an fp32 product, at three
+// times an f16 product's cost instead of the fp32 matrix instruction's sixteen.
+// A stage is 32 keys of a kv head in the form of 1 KB operand fragments, in the order
+// that the matrix instruction's lanes want them: K's hi and lo, 16 dimensions each, then
+// V's, 16 keys by 32 dimensions each.  S^T = K Q^T leaves a lane with 16 keys of one
+// query, which are the B operand of O^T += V^T P^T in the order that V's keys have
+// there, so no weight moves between lanes.
 //   attn_f16_k    a block of NW waves takes NW units (32 queries of one head) of one kv
-//                 head, so that the query heads of a group share the fragments, and
-//                 walks the stages through a ring in LDS.  S^T = K Q^T leaves a lane
-//                 with 16 keys of one query, which are the B operand of O^T +=
-//                 V^T P^T in the order that attn_split_k laid the keys of V.
+//                 head, so that the query heads of a group share the stages, and
+//                 walks them through LDS.  It makes them itself from K and V rows, or
+//                 (STORED) fetches what attn_split_k has made once for all blocks.
+//   attn_split_k  makes the stages.
 //   attn_join_k   where there are few units the keys are split over several blocks; this
 //                 joins what they leave.
-//   attn_again_k  computes the sequences in fp32 whose keys the split form does not serve.
+// A block whose keys the split form does not serve (a value that is not finite, or sizes
+// too far apart) computes its rows in fp32 instead.
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
-#ifndef AHEAD
-#define AHEAD 4
-#endif
 constexpr int kStageKeys = 32;
-// Where keys differ in size by more than this, the smaller ones' parts lie too low in
-// the larger ones' scaling (they keep at least 24 bits up to here), and a key that a
-// query does not see would cost the row bits: those rows are computed in fp32.
-constexpr float kSpread = 1.f / 16384;
+// A key that is smaller than the largest of its stage by more than this, or a stage that
+// is smaller than the largest before it, would lie too low in the other's scaling (up
+// to here 24 bits of it are kept), and a key that a query does not see would cost the
+// query's row bits.
+constexpr int kSpread = 14;
 
-struct SplitArgs {
+struct F16Args {
   PackedArgs p;
-  uint4 *frags;    // [slots, kv heads] stages
-  float4 *scales;  // [kv heads, slots]: 1 / the scaling of K, of V, and the smallest key's
-  int *any;        // whether some sequence goes to attn_again_k
-  int *again;      // [kv heads, n]: which
-  int hk, slots;
+  int hk;               // kv heads
+  int blocks;           // of one kv head and one split
+  int splits, chunk;    // of the keys: stages a split takes
+  float *part;          // [splits, tq, heads, head_size], with splits > 1
+  float2 *stat;         // [splits, tq, heads]: maximum and sum
+  uint4 *frags;         // STORED: [slots, kv heads] stages, slots as of tiles of 32 keys
+  float4 *scales;       // STORED: [kv heads, slots]: 1 / the scaling of K and of V (NaN: not
+  int slots;            // served), the largest value of V's smallest key
 };
 
-// 2^x, below 2^-126 as 0
-__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
+// The exponent that brings a largest magnitude (its bits) into [2^14, 2^15); the
+// smallest ones as far as a power of two goes.
+__device__ __forceinline__ int lift(uint32_t top) {
+  return top ? min(14 + 127 - (int)(top >> 23), 126) : 0;
+}
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-// The exponent that brings a largest magnitude into [2^14, 2^15)
-__device__ __forceinline__ int lift(float top) {
-  const int e = top > 0.f ? 14 - ilogbf(top) : 0;
-  return min(e, 126);
+// The lanes' largest number of bits of a magnitude: floats in order, NaN above all.
+__device__ __forceinline__ uint32_t bits_of(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+  const auto both = [](uint32_t a, float b) { return max(a, __float_as_uint(b)); };
+  v = both(v, dpp_mov<kDppXor1>(__uint_as_float(v)));
+  v = both(v, dpp_mov<kDppXor2>(__uint_as_float(v)));
+  v = both(v, dpp_mov<kDppHalfMirror>(__uint_as_float(v)));
+  v = both(v, dpp_mov<kDppMirror>(__uint_as_float(v)));
+  float a = __uint_as_float(v), b = a;
+  permlane16_swap(a, b);
+  v = both(__float_as_uint(a), b);
+  a = b = __uint_as_float(v);
+  permlane32_swap(a, b);
+  return both(__float_as_uint(a), b);
+}
+
+// x - h for the low and the high half of a pair of f16 (one instruction each; the compiler
+// takes two)
+__device__ __forceinline__ float rest_lo(h2 h, float x) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+  return r;
+}
+__device__ __forceinline__ float rest_hi(h2 h, float x) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+  return r;
 }
 
 __device__ __forceinline__ void split8(const float (&x)[8], h8 &hi, h8 &lo) {
@@ -279,180 +246,352 @@ __device__ __forceinline__ void split8(const float (&x)[8], h8 &hi, h8 &lo) {
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
     const h2 h = __builtin_convertvector((f2{x[e], x[e + 1]}), h2);
-    const f2 r = {fmaf((float)h[0], -1.f, x[e]), fmaf((float)h[1], -1.f, x[e + 1])};
+    const f2 r = {rest_lo(h, x[e]), rest_hi(h, x[e + 1])};
     const h2 l = __builtin_convertvector(r, h2);
     hi[e] = h[0], hi[e + 1] = h[1];
     lo[e] = l[0], lo[e + 1] = l[1];
   }
 }
+__device__ __forceinline__ h8 split8(const float (&x)[8], float by, uint4 *hi, uint4 *lo) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) y[i] = x[i] * by;
+  h8 h, l;
+  split8(y, h, l);
+  *hi = __builtin_bit_cast(uint4, h);
+  *lo = __builtin_bit_cast(uint4, l);
+  return h;
+}
+
+// A lane's part of K fragment f of a stage, 8 dimensions of one key, and of V fragment
+// f = NB i + db, 8 keys of one dimension.  Keys behind the sequence's last one repeat it:
+// no query sees them.  So do dimensions behind a row's last one: q is 0 there, and O's are
+// not stored.  The lane's place in the fragment is a 32-bit offset (the caller sees to
+// strides below 2^23), so that a whole stage costs no address arithmetic.
+__device__ __forceinline__ int v_key(int i, int h, int e) { return 16 * i + 8 * (e >> 2) + 4 * h + (e & 3); }
+template <int NB, bool VEC>
+struct Part {
+  uint32_t kd[2], vd, ko, vo;  // bytes
+  __device__ __forceinline__ void init(const PackedArgs &a, int f) {
+    const int lane = threadIdx.x & 63, h = lane >> 5, d = 16 * f + 8 * h;
+    kd[0] = 4u * (uint32_t)min(d, VEC ? a.hs - 4 : a.hs - 1);
+    kd[1] = 4u * (uint32_t)min(d + 4, VEC ? a.hs - 4 : a.hs - 1);
+    vd = 4u * (uint32_t)min(32 * (f % NB) + (lane & 31), a.hs - 1);
+    ko = (uint32_t)(lane & 31) * (4u * (uint32_t)a.k_row);
+    vo = (uint32_t)(4 * h) * (4u * (uint32_t)a.v_row) + vd;
+  }
+  // kp, vp: the stage's first key; last: its last key's number in the stage
+  __device__ __forceinline__ void load(const PackedArgs &a, const float *kp, const float *vp, int last,
+                                       int f, float (&k)[8], float (&v)[8]) const {
+    const int lane = threadIdx.x & 63, h = lane >> 5, i = f / NB;
+    const char *kb = (const char *)kp, *vb = (const char *)vp;
+    const bool whole = last >= kStageKeys - 1;
+    const uint32_t row = whole ? ko : (uint32_t)min(lane & 31, last) * (4u * (uint32_t)a.k_row);
+    if (VEC) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const float4 x = *(const float4 *)(kb + (row + kd[e]));
+        k[4 * e] = x.x, k[4 * e + 1] = x.y, k[4 * e + 2] = x.z, k[4 * e + 3] = x.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        k[e] = *(const float *)(kb + (row + min(kd[e >> 2] + 4u * (e & 3), 4u * (uint32_t)(a.hs - 1))));
+    }
+    if (whole) {
+      const char *vi = vb + (int64_t)(16 * i) * (4 * a.v_row);
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = *(const float *)(vi + (int64_t)v_key(0, 0, e) * (4 * a.v_row) + vo);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        v[e] = *(const float *)(vb + ((uint32_t)min(v_key(i, h, e), last) * (4u * (uint32_t)a.v_row) + vd));
+    }
+  }
+};
+
+// The largest magnitude of eight numbers, its bits: positive ones are in order as signed
+// integers, negative ones as unsigned ones, NaN above all.
+__device__ __forceinline__ uint32_t top8(const float (&x)[8]) {
+  int p = 0;
+  uint32_t n = 0;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    p = max(p, __float_as_int(x[e]));
+    n = max(n, __float_as_uint(x[e]));
+  }
+  return max((uint32_t)p, n & 0x7fffffffu & (uint32_t)((int)n >> 31));
+}
+
+// The largest magnitude of each of a V part's eight keys over the 32 lanes that share
+// them (one half of the wave), as bits of f16 of the scaled numbers (their hi): a lane has
+// keys 2 (lane & 3) and the next one.
+__device__ __forceinline__ uint32_t top_keys(h8 hi) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  typedef uint16_t s2 __attribute__((ext_vector_type(2)));
+  u4 x = __builtin_bit_cast(u4, hi) & 0x7fff7fffu;
+  const auto both = [](uint32_t a, uint32_t b) {
+    const s2 p = __builtin_bit_cast(s2, a), q = __builtin_bit_cast(s2, b);
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(p, q));
+  };
+  const auto from = [](uint32_t v, auto c) { return __float_as_uint(dpp_mov<decltype(c)::value>(__uint_as_float(v))); };
+  const int lane = threadIdx.x & 63;
+  const bool odd1 = lane & 1, odd2 = lane & 2;
+  const uint32_t a = both(odd1 ? x[1] : x[0], from(odd1 ? x[0] : x[1], std::integral_constant<int, kDppXor1>()));
+  const uint32_t b = both(odd1 ? x[3] : x[2], from(odd1 ? x[2] : x[3], std::integral_constant<int, kDppXor1>()));
+  uint32_t c = both(odd2 ? b : a, from(odd2 ? a : b, std::integral_constant<int, kDppXor2>()));
+  // lanes that have the same pair are those of the same lane & 3
+  c = both(c, from(c, std::integral_constant<int, 0x124>()));  // row_ror:4
+  c = both(c, from(c, std::integral_constant<int, kDppRor8>()));
+  float u = __uint_as_float(c), v = u;
+  permlane16_swap(u, v);
+  return both(__float_as_uint(u), __float_as_uint(v));
+}
 
 // One stage.  NB: 32-dimension blocks of a head.
 template <int NB, bool VEC>
-__global__ void __launch_bounds__(256) attn_split_k(const SplitArgs a) {
-  constexpr int DP = 32 * NB, LD = DP + 4;
-  __shared__ float tile[2][32][LD];
-  __shared__ float most[4], least[4];
+__global__ void __launch_bounds__(256) attn_split_k(const F16Args a) {
+  __shared__ uint32_t key_s[2][32];  // each key's largest magnitude: K, V
   const PackedArgs &p = a.p;
-  const int slot = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x;
-  if (slot == 0 && hk == 0 && tid == 0) *a.any = 0;
+  const int slot = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int s = seq_of_slot<kStageKeys>(p.k_starts, p.n, p.tk, slot);
-  const int kb = clampi(p.k_starts[s], 0, p.tk), ke = clampi(p.k_starts[s + 1], kb, p.tk);
-  const int slot0 = kb / kStageKeys + s;
-  if (slot < slot0) return;
-  const int64_t key0 = (int64_t)(slot - slot0) * kStageKeys;
-  if (key0 >= ke - kb) return;
-  const int nk = (int)min((int64_t)kStageKeys, ke - kb - key0);
-  bool odd = false;
+  const Seq z = seq_of(p, s);
+  const int key0 = kStageKeys * (slot - (z.kb / kStageKeys + s));
+  if (key0 < 0 || key0 >= z.nk) return;
+  const int last = z.nk - 1 - key0;
+  if (tid < 64) key_s[tid >> 5][tid & 31] = 0;
+  __syncthreads();
+  const float *kp = p.k + (int64_t)(z.kb + key0) * p.k_row + hk * p.k_head;
+  const float *vp = p.v + (int64_t)(z.kb + key0) * p.v_row + hk * p.v_head;
+  constexpr int CH = (2 * NB + 3) / 4;
+  float k[CH][8], v[CH][8];
 #pragma unroll
-  for (int w = 0; w < 2; w++) {
-    const float *x = w ? p.v + (kb + key0) * p.v_row + hk * p.v_head
-                       : p.k + (kb + key0) * p.k_row + hk * p.k_head;
-    const int64_t row = w ? p.v_row : p.k_row;
-    for (int e = tid; e < 32 * DP / 4; e += 256) {
-      const int r = e / (DP / 4), d = 4 * (e - r * (DP / 4));
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < nk) v = load4<VEC>(x + r * row, d, p.hs);
-      *(float4 *)&tile[w][r][d] = v;
-      odd |= !(fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.z) < INFINITY &&
-               fabsf(v.w) < INFINITY);
-    }
+  for (int c = 0; c < CH; c++) {
+    const int f = wave + 4 * c;
+    if (f >= 2 * NB) break;
+    Part<NB, VEC> part;
+    part.init(p, f);
+    part.load(p, kp, vp, last, f, k[c], v[c]);
   }
-  const bool bad = __syncthreads_or(odd);
-  {  // the largest of each key, four threads to one
-    const int w = tid >> 7, r = (tid >> 2) & 31, c = tid & 3;
-    float t = 0.f;
-    for (int d = 4 * c; d < DP; d += 16) {
-      const float4 v = *(const float4 *)&tile[w][r][d];
-      t = fmaxf(t, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-    }
-    t = fmaxf(t, __shfl_xor(t, 1));
-    t = fmaxf(t, __shfl_xor(t, 2));
-    float lowest = t > 0.f ? t : INFINITY;
-    t = wave_max(t);
-    lowest = -wave_max(-lowest);
-    if ((tid & 63) == 0) {
-      most[tid >> 6] = t;
-      least[tid >> 6] = lowest;
+#pragma unroll
+  for (int c = 0; c < CH; c++) {
+    const int f = wave + 4 * c;
+    if (f >= 2 * NB) break;
+    uint32_t t = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) t = max(t, bits_of(k[c][e]));
+    atomicMax(&key_s[0][lane & 31], t);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      uint32_t u = bits_of(v[c][e]);  // over the 32 lanes of a key
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) u = max(u, (uint32_t)__shfl_xor((int)u, d));
+      if ((lane & 31) == 0) atomicMax(&key_s[1][v_key(f / NB, lane >> 5, e)], u);
     }
   }
   __syncthreads();
-  const float kt = fmaxf(most[0], most[1]), vt = fmaxf(most[2], most[3]);
-  const float kl = fminf(least[0], least[1]), vl = fminf(least[2], least[3]);
+  uint32_t kt = 0, vt = 0, kl = ~0u, vl = ~0u;  // largest, and smallest that is not 0
+#pragma unroll 8
+  for (int i = 0; i < 32; i++) {
+    const uint32_t x = key_s[0][i], y = key_s[1][i];
+    kt = max(kt, x), kl = min(kl, x - 1);
+    vt = max(vt, y), vl = min(vl, y - 1);
+  }
+  kl++, vl++;  // (0 - 1 is the largest number: a key of zeros does not count)
   const int ek = lift(kt), ev = lift(vt);
   if (tid == 0) {
-    const bool wide = bad || kl < kt * kSpread;
-    a.scales[(int64_t)hk * a.slots + slot] =
-        make_float4(ldexpf(1.f, -ek), wide ? NAN : vt > 0.f ? ldexpf(1.f, -ev) : 0.f, vl, 0.f);
+    const bool bad = max(kt, vt) >= 0x7f800000u || (kl && (int)(kt >> 23) - (int)(kl >> 23) > kSpread) ||
+                     (vl && (int)(vt >> 23) - (int)(vl >> 23) > kSpread);
+    a.scales[(int64_t)hk * a.slots + slot] = make_float4(power(-ek), bad ? NAN : vt ? power(-ev) : 0.f, 0.f, 0.f);
   }
-  if (bad) return;
   uint4 *out = a.frags + ((int64_t)slot * a.hk + hk) * (NB * 8 * 64);
-  const int lane = tid & 63, r32 = lane & 31, h = lane >> 5;
-  for (int f = tid >> 6; f < 2 * NB; f += 4) {  // K: 16 dimensions, 32 keys
-    float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = ldexpf(tile[0][r32][16 * f + 8 * h + e], ek);
-    h8 hi, lo;
-    split8(x, hi, lo);
-    out[(2 * f) * 64 + lane] = __builtin_bit_cast(uint4, hi);
-    out[(2 * f + 1) * 64 + lane] = __builtin_bit_cast(uint4, lo);
-  }
-  for (int f = tid >> 6; f < 2 * NB; f += 4) {  // V: 16 keys (f / NB), 32 dimensions
-    const int i = f / NB, db = f - i * NB;
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-      x[e] = ldexpf(tile[1][16 * i + 8 * (e >> 2) + 4 * h + (e & 3)][32 * db + r32], ev);
-    h8 hi, lo;
-    split8(x, hi, lo);
-    out[(4 * NB + 2 * f) * 64 + lane] = __builtin_bit_cast(uint4, hi);
-    out[(4 * NB + 2 * f + 1) * 64 + lane] = __builtin_bit_cast(uint4, lo);
+  for (int c = 0; c < CH; c++) {
+    const int f = wave + 4 * c;
+    if (f >= 2 * NB) break;
+    split8(k[c], power(ek), out + (2 * f) * 64 + lane, out + (2 * f + 1) * 64 + lane);
+    split8(v[c], power(ev), out + (4 * NB + 2 * f) * 64 + lane, out + (4 * NB + 2 * f + 1) * 64 + lane);
   }
 }
 
-struct F16Args {
-  SplitArgs s;
-  int blocks;   // of one kv head and one split
-  int splits, chunk;  // of the keys: stages a split takes
-  float *part;  // [splits, tq, heads, head_size], scaled by the row's sum; with splits
-  float2 *stat; // [splits, tq, heads]
-};
+// The blocks of one kv head: sequence s has ((q_starts[s] / 32 + s) G / NW) + s and on.
+template <int NW>
+__device__ __forceinline__ int first_block(const PackedArgs &a, int s) {
+  return (int)(((int64_t)(clampi(a.q_starts[s], 0, a.tq) / 32 + s) * a.group) / NW) + s;
+}
 
-// NB: 32-dimension blocks; NW: waves; NS: stages in the ring.
-template <int NB, int NW, int NS, bool VEC>
-__global__ void __launch_bounds__(64 * NW) attn_f16_k(const F16Args args) {
-  constexpr int kFrags = 8 * NB, FPW = kFrags / NW;  // fragments of a stage; loaded by a wave
-  static_assert(kFrags % NW == 0, "each wave loads as many fragments");
+// The 32 queries of a head that wave w of a block takes (tile >= tiles: none).
+struct Unit {
+  int tile, head;
+};
+template <int NW>
+__device__ __forceinline__ Unit unit_of(const PackedArgs &a, int block, int wave, int hk) {
+  const int64_t u = (int64_t)block * NW + wave;  // of the sequence
+  const int tile = (int)min(u / a.group, (int64_t)INT32_MAX);
+  return Unit{tile, hk * a.group + (int)(u % a.group)};
+}
+
+// One stage of one wave: S^T, weights and O^T.  f: what turns a product sum into a power
+// of two; er: V's scaling over O's, a power 2^er <= 1; all: the last key that every
+// query of the wave sees.
+template <int NB>
+__device__ __forceinline__ void stage(const h8 *frag, const h8 (&qh)[2 * NB], const h8 (&ql)[2 * NB],
+                                      float f, int key0, int my, int all, int h, int er,
+                                      v16f (&o)[NB], float &m, float &l) {
+  v16f s;
+#pragma unroll
+  for (int r = 0; r < 16; r++) s[r] = 0.f;
+  // Two fragments are read ahead of the products that use two others: under the other
+  // waves' reads one alone comes later than three products take.
+  constexpr int kReads = 0x100, kProducts = 0x008;
+  {
+    h8 k[2 * NB][2];
+#pragma unroll
+    for (int ds = 0; ds < 2 * NB; ds++) {
+      k[ds][0] = frag[(2 * ds) * 64];
+      k[ds][1] = frag[(2 * ds + 1) * 64];
+    }
+#pragma unroll
+    for (int ds = 0; ds < 2 * NB; ds++) {
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[ds][0], qh[ds], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[ds][0], ql[ds], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[ds][1], qh[ds], s, 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kReads, 4, 0);
+#pragma unroll
+    for (int ds = 0; ds < 2 * NB; ds++) {
+      __builtin_amdgcn_sched_group_barrier(kProducts, 3, 0);
+      __builtin_amdgcn_sched_group_barrier(kReads, 2, 0);
+    }
+  }
+  if (key0 + kStageKeys - 1 > all) {  // some query does not see all of them
+#pragma unroll
+    for (int r = 0; r < 16; r++)
+      s[r] = key0 + 8 * (r >> 2) + 4 * h + (r & 3) <= my ? s[r] * f : -INFINITY;
+    f = 1.f;
+  }
+  float mt = s[0];
+#pragma unroll
+  for (int r = 1; r < 16; r++) mt = fmaxf(mt, s[r]);
+  {
+    float u = mt, v = mt;
+    permlane32_swap(u, v);
+    mt = fmaxf(u, v) * f;
+  }
+  // The maximum is raised only where a weight would pass 4: weights of 2^13 to the largest
+  // one's 1 still fit f16 then.
+  if (__any(mt > m + 2.f)) {
+    const float mn = fmaxf(m, mt), alpha = pow2(m - mn);
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < NB; d++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) o[d][r] *= alpha;
+  }
+  const float off = (float)(13 + er) - m;
+  float pl = 0.f;
+  {
+    h8 ph[2], pw[2], v[2][NB][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int d = 0; d < NB; d++) {
+        v[i][d][0] = frag[(4 * NB + 2 * (i * NB + d)) * 64];
+        v[i][d][1] = frag[(4 * NB + 2 * (i * NB + d) + 1) * 64];
+      }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        x[e] = pow2(fmaf(s[8 * i + e], f, off));
+        pl += x[e];
+      }
+      split8(x, ph[i], pw[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int d = 0; d < NB; d++) {
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i][d][0], ph[i], o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i][d][0], pw[i], o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i][d][1], ph[i], o[d], 0, 0, 0);
+      }
+    __builtin_amdgcn_sched_group_barrier(kReads, 4, 1);
+#pragma unroll
+    for (int d = 0; d < 2 * NB; d++) {
+      __builtin_amdgcn_sched_group_barrier(kProducts, 3, 1);
+      __builtin_amdgcn_sched_group_barrier(kReads, 2, 1);
+    }
+  }
+  l = fmaf(pl, power(-13 - er), l);
+}
+
+// NB: 32-dimension blocks; NW: waves; NS: stages in LDS.
+template <int NB, int NW, int NS, bool VEC, bool STORED>
+__global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : NB == 2 ? 3 : NB <= 4 ? 2 : 1)
+    attn_f16_k(const F16Args args) {
+  constexpr int kFrags = 8 * NB, FPW = kFrags / NW;  // fragments of a stage; fetched by a wave
+  constexpr int CH = (2 * NB + NW - 1) / NW;         // made by a wave, of K and of V
+  static_assert(kFrags % NW == 0, "each wave fetches as many fragments");
   __shared__ uint4 ring[NS][kFrags * 64];
-  __shared__ float vtop_s[NW], vlow_s[NW];
-  const SplitArgs &sa = args.s;
-  const PackedArgs &a = sa.p;
+  __shared__ uint2 top_s[2][NW];
+  __shared__ uint32_t key_s[2][2][32];  // each key's largest of a made stage
+  const PackedArgs &a = args.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r32 = lane & 31, h = lane >> 5;
   // the last rows of a sequence, which see most keys, come first
-  const int hk = blockIdx.x % sa.hk, split = blockIdx.y;
-  const int w = args.blocks - 1 - blockIdx.x / sa.hk;
-  // Sequence s has the blocks ((q_starts[s] / 32 + s) G / NW) + s and on.
-  const int G = a.group;
-  auto base = [&](int s) {
-    return (int)(((int64_t)(clampi(a.q_starts[s], 0, a.tq) / 32 + s) * G) / NW) + s;
-  };
-  int lo = 0, hi = a.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (base(mid) <= w) lo = mid;
-    else hi = mid - 1;
-  }
-  const int seq = lo, b0 = base(seq);
-  const int qb = clampi(a.q_starts[seq], 0, a.tq), qe = clampi(a.q_starts[seq + 1], qb, a.tq);
-  const int kb = clampi(a.k_starts[seq], 0, a.tk), ke = clampi(a.k_starts[seq + 1], kb, a.tk);
-  const int nq = qe - qb, nk = ke - kb, tiles = (nq + 31) / 32;
-  if (w < b0 || (int64_t)(w - b0) * NW >= (int64_t)tiles * G) return;
-  const int64_t unit = (int64_t)(w - b0) * NW + wave;
-  const int tile = (int)(unit / G), head = hk * G + (int)(unit - (int64_t)tile * G);
-  const bool idle = tile >= tiles;
-  const int row0 = 32 * tile, row = min(row0 + r32, nq - 1);  // this lane's query
-  const int my = row + nk - nq;                               // its last key, or negative
-  const int first = row0 + nk - nq;                           // what every query sees, at least
-  const int wend = idle ? -1 : min(row0 + 31, nq - 1) + nk - nq;  // the wave's last key
-  const int top_tile = min(tiles - 1, (int)(((int64_t)(w - b0) * NW + NW - 1) / G));
-  const int bend = min(32 * top_tile + 31, nq - 1) + nk - nq;     // the block's
+  const int hk = blockIdx.x % args.hk, split = blockIdx.y;
+  const int w = args.blocks - 1 - blockIdx.x / args.hk;
+  const int seq = last_of(a.n, [&](int s) { return first_block<NW>(a, s) <= w; });
+  const int block = w - first_block<NW>(a, seq);
+  const Seq z = seq_of(a, seq);
+  const int tiles = (z.nq + 31) / 32, off = z.nk - z.nq;
+  const Unit un = unit_of<NW>(a, block, wave, hk);
+  // the block's last key, and its stages
+  const int top_tile = min(tiles - 1, unit_of<NW>(a, block, NW - 1, hk).tile);
+  const int bend = min(32 * top_tile + 31, z.nq - 1) + off;
   const int st0 = split * args.chunk;
   const int st1 = min(bend < 0 ? 0 : bend / kStageKeys + 1, st0 + args.chunk);
-  if (split > 0 && st0 >= st1) return;  // attn_join_k does not read it
-  const int slot0 = kb / kStageKeys + seq;
-
-  // The largest scaling of V in the block's stages is the unit of O.
-  const float4 *scales = sa.scales + (int64_t)hk * sa.slots + slot0;
-  float vt = 0.f, vl = INFINITY;
+  // (the last: attn_join_k reads nothing of it)
+  if (block < 0 || unit_of<NW>(a, block, 0, hk).tile >= tiles || (split > 0 && st0 >= st1)) return;
+  const bool idle = un.tile >= tiles;
+  const int row0 = 32 * min(un.tile, tiles), row = min(row0 + r32, z.nq - 1);  // the lane's query
+  const int my = row + off;                                     // its last key, or negative
+  const int all = row0 + off;                                   // what every query sees
+  const int wend = idle ? -1 : min(row0 + 31, z.nq - 1) + off;  // the wave's last key
+  const int slot0 = z.kb / kStageKeys + seq;
   bool odd = false;
-  for (int i = threadIdx.x; i < (nk + kStageKeys - 1) / kStageKeys; i += 64 * NW) {
-    const float4 v = scales[i];
-    odd |= v.y != v.y;
-    vt = fmaxf(vt, v.y);
-    vl = fminf(vl, v.z);
-  }
-  vt = wave_max(vt);
-  vl = -wave_max(-vl);
-  if (lane == 0) {
-    vtop_s[wave] = vt;
-    vlow_s[wave] = vl;
-  }
-  odd = __syncthreads_or(odd);
-#pragma unroll
-  for (int i = 0; i < NW; i++) {
-    vt = fmaxf(vt, vtop_s[i]);
-    vl = fminf(vl, vlow_s[i]);
-  }
-  odd |= vl < vt * (32768.f * kSpread);  // the largest value is below 2^15 vt
-  if (split == 0 && threadIdx.x == 0) {
-    sa.again[(int64_t)hk * a.n + seq] = odd;  // the same from each of its blocks
-    if (odd) *sa.any = 1;
-  }
-  if (odd) return;
 
+  // O's scaling over V's: the largest of the stages before (made), or of all (STORED)
+  const float4 *scales = args.scales + (int64_t)hk * args.slots + slot0;
+  int unit = -1000;
+  if constexpr (STORED) {
+    float hi = 0.f, lo = INFINITY;
+    for (int i = threadIdx.x; i < (bend < 0 ? 0 : bend / kStageKeys + 1); i += 64 * NW) {
+      const float v = scales[i].y;
+      odd |= v != v;
+      hi = fmaxf(hi, v);
+      lo = fminf(lo, v > 0.f ? v : INFINITY);
+    }
+    hi = wave_max_dpp(hi);
+    lo = -wave_max_dpp(-lo);
+    if (lane == 0) top_s[0][wave] = make_uint2(__float_as_uint(hi), __float_as_uint(lo));
+    odd = __syncthreads_or(odd);
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+      hi = fmaxf(hi, __uint_as_float(top_s[0][i].x));
+      lo = fminf(lo, __uint_as_float(top_s[0][i].y));
+    }
+    odd |= lo < hi * (1.f / (1 << kSpread));
+    unit = (__float_as_int(hi) >> 23) - 127;
+  }
+  const float *kp = a.k + (int64_t)z.kb * a.k_row + hk * a.k_head;
+  const float *vp = a.v + (int64_t)z.kb * a.v_row + hk * a.v_head;
   const uint32_t lds0 = lds_offset(&ring[0][0]);
   auto fetch = [&](int st) {
-    const uint4 *src = sa.frags + ((int64_t)(slot0 + st) * sa.hk + hk) * (kFrags * 64) + lane;
+    const uint4 *src = args.frags + ((int64_t)(slot0 + st) * args.hk + hk) * (kFrags * 64) + lane;
     const uint32_t dst = lds0 + (uint32_t)((st - st0) % NS) * (kFrags * 1024);
 #pragma unroll
     for (int i = 0; i < FPW; i++) {
@@ -460,39 +599,52 @@ __global__ void __launch_bounds__(64 * NW) attn_f16_k(const F16Args args) {
       dma16(src + f * 64, dst + f * 1024);
     }
   };
+  float kx[CH][8], vx[CH][8];
+  Part<NB, VEC> part[CH];
+  if constexpr (!STORED)
 #pragma unroll
-  for (int i = 0; i < NS - 1; i++)
-    if (st0 + i < st1) fetch(st0 + i);
+    for (int c = 0; c < CH; c++) part[c].init(a, wave + c * NW);
+  auto load = [&](int st) {
+    const int key0 = kStageKeys * st, last = z.nk - 1 - key0;
+#pragma unroll
+    for (int c = 0; c < CH; c++) {
+      const int f = wave + c * NW;
+      if (2 * NB % NW != 0 && f >= 2 * NB) break;
+      part[c].load(a, kp + (int64_t)key0 * a.k_row, vp + (int64_t)key0 * a.v_row, last, f, kx[c], vx[c]);
+    }
+  };
+  if constexpr (STORED) {
+#pragma unroll
+    for (int i = 0; i < NS - 1; i++)
+      if (!odd && st0 + i < st1) fetch(st0 + i);
+  } else if (st0 < st1) {
+    load(st0);
+    if (threadIdx.x < 64) key_s[0][h][r32] = 0;  // seen by all behind the first barrier
+  }
 
   h8 qh[2 * NB], ql[2 * NB];
   float qf;
   {
-    const float *qr = a.q + (int64_t)(qb + row) * a.q_row + head * a.q_head;
-    float top = 0.f;
+    const float *qr = a.q + (int64_t)(z.qb + row) * a.q_row + un.head * a.q_head;
+    uint32_t top = 0;
     float x[2 * NB][8];
 #pragma unroll
     for (int ds = 0; ds < 2 * NB; ds++) {
       const int d0 = 16 * ds + 8 * h;
-      if (VEC) {
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (!idle && d0 + e < a.hs) v = *(const float4 *)(qr + d0 + e);
-          x[ds][e] = v.x, x[ds][e + 1] = v.y, x[ds][e + 2] = v.z, x[ds][e + 3] = v.w;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[ds][e] = !idle && d0 + e < a.hs ? qr[d0 + e] : 0.f;
+      for (int e = 0; e < 8; e += 4) {
+        const float4 v = idle ? make_float4(0.f, 0.f, 0.f, 0.f) : load4<VEC>(qr, d0 + e, a.hs);
+        x[ds][e] = v.x, x[ds][e + 1] = v.y, x[ds][e + 2] = v.z, x[ds][e + 3] = v.w;
       }
 #pragma unroll
-      for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[ds][e]));
+      for (int e = 0; e < 8; e++) top = max(top, bits_of(x[ds][e]));
     }
     {
-      float u = top, v = top;
+      float u = __uint_as_float(top), v = u;
       permlane32_swap(u, v);
-      top = fmaxf(u, v);
+      top = max(__float_as_uint(u), __float_as_uint(v));
     }
-    const int eq = top < INFINITY ? lift(top) : 0;  // infinities and NaN come through
+    const int eq = top < 0x7f800000u ? lift(top) : 0;  // infinities and NaN come through
     const float sign = a.scale < 0.f ? -1.f : 1.f;
     qf = ldexpf(fabsf(a.scale) * 1.44269504f, -eq);
 #pragma unroll
@@ -509,128 +661,132 @@ __global__ void __launch_bounds__(64 * NW) attn_f16_k(const F16Args args) {
 #pragma unroll
     for (int r = 0; r < 16; r++) o[d][r] = 0.f;
   float m = -3.402823466e38f, l = 0.f;  // finite: a difference of two is no NaN
-  const int vexp = __float_as_int(vt) >> 23;
-  // Read as constants, through the scalar cache: a vector load here would wait for the
-  // stages on their way.
-  const auto *uniform = (const __attribute__((address_space(4))) float *)scales;
-  for (int st = st0; st < st1; st++) {
-    wait_vm_le<FPW, NS - 2>(min(NS - 2, st1 - 1 - st));
-    block_barrier();
-    if (st + NS - 1 < st1) fetch(st + NS - 1);
-    if (kStageKeys * st > wend) continue;  // nothing here is seen by this wave
-    const float kinv = uniform[4 * st], vinv = uniform[4 * st + 1];
-    const h8 *frag = (const h8 *)ring[(st - st0) % NS] + lane;
-    v16f s;
+  if constexpr (STORED) {
+    // Read as constants, through the scalar cache: a vector load in the loop would wait
+    // for the stages on their way.
+    const auto *uniform = (const __attribute__((address_space(4))) float *)scales;
+    for (int st = st0; st < (odd ? st0 : st1); st++) {
+      wait_vm_le<FPW, NS - 2>(min(NS - 2, st1 - 1 - st));
+      block_barrier();
+      if (st + NS - 1 < st1) fetch(st + NS - 1);
+      if (kStageKeys * st > wend) continue;  // nothing here is seen by this wave
+      const float kinv = uniform[4 * st], vinv = uniform[4 * st + 1];
+      const int er = vinv > 0.f ? (__float_as_int(vinv) >> 23) - 127 - unit : 0;
+      stage<NB>((const h8 *)ring[(st - st0) % NS] + lane, qh, ql, qf * kinv, kStageKeys * st, my, all,
+                h, er, o, m, l);
+    }
+  } else {
+    for (int st = st0; st < st1; st++) {
+      const int at = (st - st0) & 1;
+      uint32_t kt = 0, vt = 0, key_top[CH];
 #pragma unroll
-    for (int r = 0; r < 16; r++) s[r] = 0.f;
-    // Two fragments are read ahead of the products that use two others: under the
-    // other waves' reads one alone comes later than three products take.
-    constexpr int kReads = 0x100, kProducts = 0x008;
-    {
-      h8 k[2 * NB][2];
-#pragma unroll
-      for (int ds = 0; ds < 2 * NB; ds++) {
-        k[ds][0] = frag[(2 * ds) * 64];
-        k[ds][1] = frag[(2 * ds + 1) * 64];
+      for (int c = 0; c < CH; c++) {
+        if (2 * NB % NW != 0 && wave + c * NW >= 2 * NB) break;
+        key_top[c] = top8(kx[c]);
+        kt = max(kt, key_top[c]);
+        vt = max(vt, top8(vx[c]));
       }
+      kt = wave_max_bits(kt);
+      vt = wave_max_bits(vt);
+      if (lane == 0) top_s[at][wave] = make_uint2(kt, vt);
+      lds_barrier();  // also: every wave is done with this slot's stage before the last
 #pragma unroll
-      for (int ds = 0; ds < 2 * NB; ds++) {
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[ds][0], qh[ds], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[ds][0], ql[ds], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[ds][1], qh[ds], s, 0, 0, 0);
+      for (int i = 0; i < NW; i++) {
+        kt = max(kt, top_s[at][i].x);
+        vt = max(vt, top_s[at][i].y);
       }
-      __builtin_amdgcn_sched_group_barrier(kReads, AHEAD, 0);
+      kt = __builtin_amdgcn_readfirstlane(kt);
+      vt = __builtin_amdgcn_readfirstlane(vt);
+      const int ek = lift(kt), ev = lift(vt);
+      odd |= max(kt, vt) >= 0x7f800000u;
+      // each key's largest: K's as it is, V's scaled
 #pragma unroll
-      for (int ds = 0; ds < 2 * NB; ds++) {
-        __builtin_amdgcn_sched_group_barrier(kProducts, 3, 0);
-        __builtin_amdgcn_sched_group_barrier(kReads, 2, 0);
-      }
-    }
-    float f = qf * kinv;
-    if (kStageKeys * st + 31 > first) {  // some query does not see all of them
-#pragma unroll
-      for (int r = 0; r < 16; r++)
-        s[r] = kStageKeys * st + 8 * (r >> 2) + 4 * h + (r & 3) <= my ? s[r] * f : -INFINITY;
-      f = 1.f;
-    }
-    float mt = s[0];
-#pragma unroll
-    for (int r = 1; r < 16; r++) mt = fmaxf(mt, s[r]);
-    {
-      float u = mt, v = mt;
-      permlane32_swap(u, v);
-      mt = fmaxf(u, v) * f;
-    }
-    // The maximum is raised only where a weight would pass 4: weights of 2^13 to the
-    // largest one's 1 still fit f16 then.
-    if (__any(mt > m + 2.f)) {
-      const float mn = fmaxf(m, mt), alpha = pow2(m - mn);
-      m = mn;
-      l *= alpha;
-#pragma unroll
-      for (int d = 0; d < NB; d++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) o[d][r] *= alpha;
-    }
-    // V's scaling over the unit, a power of two 2^er <= 1
-    const int er = vinv > 0.f ? (__float_as_int(vinv) >> 23) - vexp : 0;
-    const float off = (float)(13 + er) - m;
-    float pl = 0.f;
-    {
-      h8 ph[2], pw[2], v[2][NB][2];
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int d = 0; d < NB; d++) {
-          v[i][d][0] = frag[(4 * NB + 2 * (i * NB + d)) * 64];
-          v[i][d][1] = frag[(4 * NB + 2 * (i * NB + d) + 1) * 64];
+      for (int c = 0; c < CH; c++) {
+        const int f = wave + c * NW;
+        if (2 * NB % NW != 0 && f >= 2 * NB) break;
+        uint4 *dst = ring[at];
+        split8(kx[c], power(ek), dst + (2 * f) * 64 + lane, dst + (2 * f + 1) * 64 + lane);
+        const h8 hi = split8(vx[c], power(ev), dst + (4 * NB + 2 * f) * 64 + lane, dst + (4 * NB + 2 * f + 1) * 64 + lane);
+        atomicMax(&key_s[at][0][r32], key_top[c]);
+        const uint32_t t = top_keys(hi);
+        if ((r32 & ~3) == 0) {  // keys 2 (lane & 3) and the next of the half's eight
+          uint32_t *key = &key_s[at][1][v_key(f / NB, h, 2 * (lane & 3))];
+          atomicMax(key, t & 0xffffu);
+          atomicMax(key + 1, t >> 16);
         }
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          x[e] = pow2(fmaf(s[8 * i + e], f, off));
-          pl += x[e];
-        }
-        split8(x, ph[i], pw[i]);
       }
-#pragma unroll
-      for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int d = 0; d < NB; d++) {
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i][d][0], ph[i], o[d], 0, 0, 0);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i][d][0], pw[i], o[d], 0, 0, 0);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i][d][1], ph[i], o[d], 0, 0, 0);
+      if (threadIdx.x < 64) key_s[at ^ 1][h][r32] = 0;  // for the next stage
+      if (st + 1 < st1) load(st + 1);
+      lds_barrier();
+      {  // far below the largest, and not 0; V is scaled to 2^14, and 0x3c00 is f16's 1
+        const uint32_t x = key_s[at][0][r32], y = key_s[at][1][r32];
+        bool low = (x && x + (kSpread << 23) < kt) || (y && y < 0x3c00u);
+        if (vt && __any(y == 0)) {  // zeros, or what f16 has no number for
+          const float *v = vp + (int64_t)min(kStageKeys * st + r32, z.nk - 1) * a.v_row;
+          for (int d = 0; y == 0 && !low && d < a.hs; d++) low = v[d] != 0.f;
         }
-      __builtin_amdgcn_sched_group_barrier(kReads, AHEAD, 1);
-#pragma unroll
-      for (int d = 0; d < 2 * NB; d++) {
-        __builtin_amdgcn_sched_group_barrier(kProducts, 3, 1);
-        __builtin_amdgcn_sched_group_barrier(kReads, 2, 1);
+        odd |= __any(low);
       }
+      const int e = vt ? -ev : unit;  // a stage of zeros has no size
+      if (e > unit) {
+        if (unit > -1000) {
+          const float down = ldexpf(1.f, unit - e);
+#pragma unroll
+          for (int d = 0; d < NB; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] *= down;
+        }
+        unit = e;
+      }
+      const int er = e - unit;  // (-1000 less itself where V has been 0 so far)
+      odd |= er < -kSpread;
+      if (kStageKeys * st > wend) continue;  // nothing here is seen by this wave
+      stage<NB>((const h8 *)ring[at] + lane, qh, ql, qf * power(-ek), kStageKeys * st, my, all, h,
+                max(er, -kSpread), o, m, l);
     }
-    l = fmaf(pl, __int_as_float((127 - 13 - er) << 23), l);
   }
-  if (idle || row0 + r32 >= nq) return;
+  const int64_t part_row = ((int64_t)split * a.tq + z.qb) * (args.hk * a.group) + un.head;
+  const int part_step = args.hk * a.group;
+  if (odd) {
+    // In fp32, the wave's 32 queries 16 at a time over the block's keys.
+    for (int q0 = row0; !idle && q0 < min(row0 + 32, z.nq); q0 += 16) {
+      const int r16 = lane & 15, g = lane >> 4, r = min(q0 + r16, z.nq - 1);
+      v4f y[2 * NB];
+      attend16<2 * NB, VEC>(a, a.q + (int64_t)(z.qb + r) * a.q_row + un.head * a.q_head, kp, vp, r + off,
+                            q0 + off, min(min(q0 + 15, z.nq - 1) + off, kStageKeys * st1 - 1),
+                            kStageKeys * st0, 16, y, m, l);
+      if (q0 + r16 >= z.nq) continue;
+      const int64_t at = part_row + (int64_t)r * part_step;
+      float *out = args.splits > 1 ? args.part + at * a.hs
+                                   : a.out + (int64_t)(z.qb + r) * a.o_row + un.head * a.o_head;
+      if (args.splits > 1 && g == 0) args.stat[at] = make_float2(m * 1.44269504f, l);
+      const float f = args.splits > 1 ? 1.f : r + off < 0 ? 0.f : 1.f / l;
+#pragma unroll
+      for (int j = 0; j < 2 * NB; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (16 * j + 4 * g + e < a.hs) out[16 * j + 4 * g + e] = y[j][e] * f;
+    }
+    return;
+  }
+  if (idle || row0 + r32 >= z.nq) return;
   {
     float u = l, v = l;
     permlane32_swap(u, v);
     l = u + v;
   }
-  const float o_unit = vt * (1.f / 8192.f);
+  const float scale = unit > -1000 ? ldexpf(1.f, unit - 13) : 0.f;
+  const bool none = args.splits == 1 && my < 0;
   float *out;
-  float f;
+  float f = scale;
   if (args.splits > 1) {
-    const int64_t at = ((int64_t)split * a.tq + qb + row) * (sa.hk * G) + head;
+    const int64_t at = part_row + (int64_t)row * part_step;
     out = args.part + at * a.hs;
-    f = o_unit;
     if (h == 0) args.stat[at] = make_float2(m, l);
   } else {
-    out = a.out + (int64_t)(qb + row) * a.o_row + head * a.o_head;
-    f = my < 0 ? 0.f : o_unit / l;
+    out = a.out + (int64_t)(z.qb + row) * a.o_row + un.head * a.o_head;
+    f = scale / l;
   }
-  const bool none = args.splits == 1 && my < 0;
 #pragma unroll
   for (int d = 0; d < NB; d++)
 #pragma unroll
@@ -649,123 +805,143 @@ __global__ void __launch_bounds__(64 * NW) attn_f16_k(const F16Args args) {
     }
 }
 
-// One row of one head: its splits together, four rows to a block.
-__global__ void __launch_bounds__(256) attn_join_k(const F16Args args) {
-  const PackedArgs &a = args.s.p;
-  const int lane = threadIdx.x & 63, heads = args.s.hk * a.group;
-  const int64_t e = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), row = e / heads;
-  const int head = (int)(e - row * heads);
-  if (row >= a.tq) return;
-  int lo = 0, hi = a.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (clampi(a.q_starts[mid], 0, a.tq) <= row) lo = mid;
-    else hi = mid - 1;
-  }
-  const int qb = clampi(a.q_starts[lo], 0, a.tq), qe = clampi(a.q_starts[lo + 1], qb, a.tq);
-  const int kb = clampi(a.k_starts[lo], 0, a.tk), ke = clampi(a.k_starts[lo + 1], kb, a.tk);
-  if (row < qb || row >= qe) return;
-  const int last = (int)(row - qb) + (ke - kb) - (qe - qb);  // the row's last key
-  float *out = a.out + row * a.o_row + head * a.o_head;
-  if (last < 0) {
-    for (int d = lane; d < a.hs; d += 64) out[d] = 0.f;
-    return;
-  }
-  const int ns = last / (kStageKeys * args.chunk) + 1;
-  const int64_t step = (int64_t)a.tq * heads, at = row * heads + head;
-  float M = -INFINITY;
-  for (int s = 0; s < ns; s++) M = fmaxf(M, args.stat[at + s * step].x);
-  const float mu = M == -INFINITY ? 0.f : M;
-  float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < ns; s++) {
-    const float2 ml = args.stat[at + s * step];
-    const float f = pow2(ml.x - mu);
-    L = fmaf(f, ml.y, L);
-    const float *part = args.part + (at + s * step) * a.hs;
-#pragma unroll
-    for (int c = 0; c < 4; c++)
-      if (lane + 64 * c < a.hs) o[c] = fmaf(f, part[lane + 64 * c], o[c]);
-  }
-#pragma unroll
-  for (int c = 0; c < 4; c++)
-    if (lane + 64 * c < a.hs) out[lane + 64 * c] = o[c] / L;
-}
-
-// The sequences that attn_f16_k left out.
-template <int HB, bool VEC>
-__global__ void __launch_bounds__(256) attn_again_k(const SplitArgs a, int tiles) {
-  __shared__ TileLds<HB> lds;
-  if (!*a.any) return;
-  const int64_t items = (int64_t)tiles * a.hk * a.p.group;
-  for (int64_t e = blockIdx.x; e < items; e += gridDim.x) {
-    f32_tile<HB, VEC>(a.p, (int)(e % tiles), (int)(e / tiles), a.again, lds);
-    __syncthreads();
-  }
-}
-
+// 1024 values of one row, heads side by side: their splits together, four to a thread.
 template <bool VEC>
-void launch_f32(const PackedArgs &a, dim3 grid, hipStream_t st) {
-#define ATTN(HB) hipLaunchKernelGGL((attn_f32_k<HB, VEC>), grid, dim3(256), 0, st, a)
-  if (a.hs <= 32) ATTN(2);
-  else if (a.hs <= 64) ATTN(4);
-  else if (a.hs <= 128) ATTN(8);
-  else ATTN(16);
-#undef ATTN
+__global__ void __launch_bounds__(256) attn_join_k(const F16Args args) {
+  extern __shared__ float weight[];  // [heads of the block, ns]
+  const PackedArgs &a = args.p;
+  const int heads = args.hk * a.group, row = blockIdx.x, tid = threadIdx.x;
+  const int s = last_of(a.n, [&](int i) { return clampi(a.q_starts[i], 0, a.tq) <= row; });
+  const Seq z = seq_of(a, s);
+  if (row < z.qb || row >= z.qb + z.nq) return;
+  const int last = row - z.qb + z.nk - z.nq;  // the row's last key
+  const int ns = last < 0 ? 0 : last / kStageKeys / args.chunk + 1;
+  const int64_t step = (int64_t)a.tq * heads;
+  const int e0 = 1024 * (int)blockIdx.y, h0 = e0 / a.hs, h1 = min(heads, (e0 + 1023) / a.hs + 1);
+  for (int t = tid; h0 + t < h1; t += 256) {
+    const float2 *stat = args.stat + (int64_t)row * heads + h0 + t;
+    float M = -INFINITY, L = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < ns; i++) M = fmaxf(M, stat[i * step].x);
+    if (M == -INFINITY) M = 0.f;  // every score is -inf: the sums are 0 too
+#pragma unroll 8
+    for (int i = 0; i < ns; i++) {
+      const float2 ml = stat[i * step];
+      const float f = pow2(ml.x - M);
+      weight[t * ns + i] = f;
+      L = fmaf(f, ml.y, L);
+    }
+    for (int i = 0; i < ns; i++) weight[t * ns + i] /= L;
+  }
+  __syncthreads();
+  const float *part = args.part + (int64_t)row * heads * a.hs;
+  float *out = a.out + row * a.o_row;
+  if (VEC) {
+    const int e = e0 + 4 * tid, h = e / a.hs;
+    if (h >= heads) return;
+    const float *w = weight + (h - h0) * ns;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int i = 0; i < ns; i++) {
+      const float4 x = *(const float4 *)(part + i * step * a.hs + e);
+      o.x = fmaf(w[i], x.x, o.x);
+      o.y = fmaf(w[i], x.y, o.y);
+      o.z = fmaf(w[i], x.z, o.z);
+      o.w = fmaf(w[i], x.w, o.w);
+    }
+    *(float4 *)(out + h * a.o_head + (e - h * a.hs)) = o;
+  } else {
+    for (int e = e0 + tid; e < min(e0 + 1024, heads * a.hs); e += 256) {
+      const int h = e / a.hs;
+      float o = 0.f;
+#pragma unroll 8
+      for (int i = 0; i < ns; i++) o = fmaf(weight[(h - h0) * ns + i], part[i * step * a.hs + e], o);
+      out[h * a.o_head + (e - h * a.hs)] = o;
+    }
+  }
 }
 
-template <int NB, int NW, int NS, bool VEC>
-void launch_f16_(const F16Args &a, hipStream_t st) {
-  const PackedArgs &p = a.s.p;
-  hipLaunchKernelGGL((attn_split_k<NB, VEC>), dim3((unsigned)a.s.slots, (unsigned)a.s.hk), dim3(256),
-                     0, st, a.s);
-  hipLaunchKernelGGL((attn_f16_k<NB, NW, NS, VEC>), dim3((unsigned)(a.blocks * a.s.hk), (unsigned)a.splits),
+template <int NB, int NW, int NS, bool VEC, bool STORED>
+void launch_f16(const F16Args &a, hipStream_t st) {
+  const int heads = a.hk * a.p.group;
+  if (STORED)
+    hipLaunchKernelGGL((attn_split_k<NB, VEC>), dim3((unsigned)a.slots, (unsigned)a.hk), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((attn_f16_k<NB, NW, NS, VEC, STORED>), dim3((unsigned)(a.blocks * a.hk), (unsigned)a.splits),
                      dim3(64 * NW), 0, st, a);
-  const int64_t heads = (int64_t)a.s.hk * p.group;
   if (a.splits > 1)
-    hipLaunchKernelGGL(attn_join_k, dim3((unsigned)cdiv(p.tq * heads, 4)), dim3(256), 0, st, a);
-  const int tiles = p.tq / 16 + p.n;
-  hipLaunchKernelGGL((attn_again_k<2 * NB, VEC>), dim3((unsigned)std::min<int64_t>(tiles * heads, 1024)),
-                     dim3(256), 0, st, a.s, tiles);
+    hipLaunchKernelGGL(attn_join_k<VEC>, dim3((unsigned)a.p.tq, (unsigned)cdiv((int64_t)heads * a.p.hs, 1024)),
+                       dim3(256), (unsigned)(4 * a.splits * std::min<int64_t>(heads, 1024 / a.p.hs + 2)), st, a);
 }
 
-// Waves of a block: eight share the fragments where a wave's registers leave room for
-// two waves on a SIMD.
-int f16_waves(int hs) { return hs <= 128 ? 8 : 4; }
-
-int launch_f16(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
+int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
   const int nb = p.hs <= 32 ? 1 : p.hs <= 64 ? 2 : p.hs <= 96 ? 3 : p.hs <= 128 ? 4 : p.hs <= 192 ? 6 : 8;
-  const int nw = f16_waves(p.hs);
   F16Args a{};
-  a.s.p = p;
-  a.s.hk = heads / p.group;
-  a.s.slots = p.tk / kStageKeys + p.n;
+  a.p = p;
+  a.hk = heads / p.group;
+  // attn_split_k and its traffic pay where about 24 blocks of four waves or more would
+  // make each stage: 1024 tokens of 32 heads over 8, 128 wide (32 blocks) 67 us against 80,
+  // 4096 (128) 380 against 560; 512 (16) 48 against 40, 2048 of 16 over 16, 64 wide (16) 67
+  // against 65.
+  const int64_t rows = cdiv(p.tq, p.n), keys = cdiv(p.tk, p.n);  // of a sequence, on average
+  const bool stored = rows * p.group >= 24 * 128;
+  // Eight waves share a fetched stage where their registers leave room for two on a SIMD.
+  const int nw = stored && p.hs <= 128 ? 8 : 4;
+  a.slots = p.tk / kStageKeys + p.n;
   a.blocks = (int)((int64_t)(p.tq / 32 + p.n) * p.group / nw) + p.n;
+  // The keys are split where the blocks (each with about `stages`, the last one of a row
+  // half used) would not fill the chip's room for them, one or two a CU, and the rows are
+  // long enough to be worth joining: 17 queries after 2983 tokens 33 us against 235, 273
+  // of the 3B heads after up to 1500 60 against 145.
   a.splits = 1;
   a.chunk = INT32_MAX / 2;
-  const size_t rows = a.splits > 1 ? (size_t)a.splits * p.tq * heads : 0;
+  const int64_t room = (int64_t)num_cus() * (nw == 8 || p.hs > 128 ? 1 : 2);
+  const int64_t wgs = cdiv(cdiv(rows, 32) * p.group, nw) * p.n * a.hk;
+  const int64_t stages = cdiv(std::max<int64_t>(keys - rows / 2, 1), kStageKeys);
+  if (wgs < room) {
+    const int64_t chunk = std::max<int64_t>(4, cdiv(cdiv(wgs * stages, room - wgs / 2), 2) * 2);
+    const int64_t splits = cdiv(cdiv(p.tk, kStageKeys), chunk);  // one sequence may have all keys
+    if (cdiv(keys, kStageKeys) >= 2 * chunk && splits * p.tq * heads * p.hs <= int64_t(1) << 25 && splits <= 1024) {
+      a.chunk = (int)chunk;
+      a.splits = (int)splits;
+    }
+  }
+  if ((int64_t)a.blocks * a.hk * 64 * nw > UINT32_MAX || (int64_t)a.slots * 256 > UINT32_MAX)
+    return set_error(SIMP_RT_EUNSUPPORTED, "attention_packed: more rows, heads or sequences than the grid holds");
+  const size_t parts = a.splits > 1 ? (size_t)a.splits * p.tq * heads : 0;
   size_t bytes = 0;
   auto take = [&](size_t n) { return std::exchange(bytes, bytes + (n + 15) / 16 * 16); };
-  const size_t frags = take((size_t)a.s.slots * a.s.hk * nb * 8 * 1024);
-  const size_t scales = take((size_t)a.s.slots * a.s.hk * sizeof(float4));
-  const size_t part = take(rows * p.hs * 4), stat = take(rows * sizeof(float2));
-  const size_t any = take(4), again = take((size_t)p.n * a.s.hk * 4);
+  const size_t frags = take(stored ? (size_t)a.slots * a.hk * nb * 8 * 1024 : 0);
+  const size_t scales = take(stored ? (size_t)a.slots * a.hk * sizeof(float4) : 0);
+  const size_t part = take(parts * p.hs * 4), stat = take(parts * sizeof(float2));
   Workspace ws;
-  char *w;
-  if (int rc = ws.get(st, bytes, (void **)&w, 9)) return rc;
-  a.s.frags = (uint4 *)(w + frags);
-  a.s.scales = (float4 *)(w + scales);
-  a.part = (float *)(w + part);
-  a.stat = (float2 *)(w + stat);
-  a.s.any = (int *)(w + any);
-  a.s.again = (int *)(w + again);
-#define F16(NB, NW, NS) vec ? launch_f16_<NB, NW, NS, true>(a, st) : launch_f16_<NB, NW, NS, false>(a, st)
-  switch (nb) {
-    case 1: F16(1, 8, 4); break;
-    case 2: F16(2, 8, 4); break;
-    case 3: F16(3, 8, 4); break;
-    case 4: F16(4, 8, 4); break;
-    case 6: F16(6, 4, 3); break;
-    default: F16(8, 4, 2);
+  if (bytes) {
+    char *w;
+    if (int rc = ws.get(st, bytes, (void **)&w, 9)) return rc;
+    a.frags = (uint4 *)(w + frags);
+    a.scales = (float4 *)(w + scales);
+    a.part = (float *)(w + part);
+    a.stat = (float2 *)(w + stat);
+  }
+#define F16(NB, NW, NS, STORED) \
+  vec ? launch_f16<NB, NW, NS, true, STORED>(a, st) : launch_f16<NB, NW, NS, false, STORED>(a, st)
+  if (stored) {
+    switch (nb) {
+      case 1: F16(1, 8, 4, true); break;
+      case 2: F16(2, 8, 4, true); break;
+      case 3: F16(3, 8, 4, true); break;
+      case 4: F16(4, 8, 4, true); break;
+      case 6: F16(6, 4, 3, true); break;
+      default: F16(8, 4, 2, true);
+    }
+  } else {
+    switch (nb) {
+      case 1: F16(1, 4, 2, false); break;
+      case 2: F16(2, 4, 2, false); break;
+      case 3: F16(3, 4, 2, false); break;
+      case 4: F16(4, 4, 2, false); break;
+      case 6: F16(6, 4, 2, false); break;
+      default: F16(8, 4, 2, false);
+    }
   }
 #undef F16
   return SIMP_RT_OK;
@@ -813,9 +989,10 @@ int32_t simp_rt_attention_packed_f32(
                      (long long)q_s1, (long long)k_s1);
   const int64_t n = qst_size - 1;
   if (q_s0 == 0 || q_s1 == 0 || n == 0) return SIMP_RT_OK;
-  if (q_s0 > INT32_MAX || k_s0 > INT32_MAX || q_s1 > 65535 || n > INT32_MAX - 1 ||
-      (q_s0 / 16 + n) * 256 > UINT32_MAX)
+  if (q_s0 > INT32_MAX - 64 || k_s0 > INT32_MAX - 64 || q_s1 > 65535 || n > INT32_MAX / 65536)
     return set_error(SIMP_RT_EUNSUPPORTED, "attention_packed: more rows, heads or sequences than the grid holds");
+  if (k_st0 >= 1 << 23 || v_st0 >= 1 << 23)  // 32-bit offsets within 32 rows
+    return set_error(SIMP_RT_EUNSUPPORTED, "attention_packed: rows of k or v 2^23 elements or more apart");
   if (overlap(dout.data(), dout.bytes(), dq.data(), dq.bytes()) ||
       overlap(dout.data(), dout.bytes(), dk.data(), dk.bytes()) ||
       overlap(dout.data(), dout.bytes(), dv.data(), dv.bytes()))
@@ -845,13 +1022,7 @@ int32_t simp_rt_attention_packed_f32(
   const bool vec = a.hs % 4 == 0 &&
                    ((q_st0 | q_st1 | k_st0 | k_st1 | v_st0 | v_st1 | out_st0 | out_st1) & 3) == 0 &&
                    (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) & 15) == 0;
-  if (getenv("F16")) {
-    if ((rc = launch_f16(a, (int)q_s1, vec, cur_stream()))) return rc;
-  } else {
-    const dim3 grid((unsigned)(q_s0 / 16 + n), (unsigned)q_s1);
-    if (vec) launch_f32<true>(a, grid, cur_stream());
-    else launch_f32<false>(a, grid, cur_stream());
-  }
+  if ((rc = launch_packed(a, (int)q_s1, vec, cur_stream()))) return rc;
   Operand *ops[] = {&oq, &ok, &ov, &oo, &oqs, &oks};
   return finish(ops, 6);
 }

@@ -4,8 +4,8 @@
 #include <algorithm>
 #include <cmath>
 
-#include "rt_device.h"
 #include "serve_args.h"
+#include "serve_device.h"
 
 namespace simp {
 namespace {
@@ -28,26 +28,6 @@ __device__ __forceinline__ float max_nan(float a, float b) { return a != a || a 
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
   return __builtin_amdgcn_perm(hi, lo, sel);  // bytes 0-3 of lo, 4-7 of hi
 }
-
-// The last s of 0 .. n-1 for which f(s) holds, where it holds up to some s and not
-// behind it; 0 where it holds for none.  The 64 lanes look at 64 places at a time, so up
-// to 64 sequences cost one round trip to memory.  Every lane of the wave takes part.
-template <class F>
-__device__ __forceinline__ int last_of(int n, F f) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0;
-  while (n > 1) {
-    const int step = (n + 63) >> 6;
-    const unsigned long long yes = __ballot(lane * step < n && f(lo + lane * step));
-    if (!yes) break;
-    const int k = 63 - __clzll((long long)yes);
-    lo += k * step;
-    n = min(step, n - k * step);
-  }
-  return __builtin_amdgcn_readfirstlane(lo);
-}
-
-__device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
 // Nearest code to x / s, ties to even, of the exact quotient; s > 0 and finite, inv =
 // 1 / s rounded (or anything near it).  x - n s is exact where n is next to the
@@ -296,9 +276,6 @@ __device__ __forceinline__ void turn4(const uint32_t (&in)[4], uint32_t (&out)[4
   out[2] = perm(d, b, 0x05040100);
   out[3] = perm(d, b, 0x07060302);
 }
-
-// 2^x, below 2^-126 as 0
-__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // max / sum over the four lanes with the same lane % 16
 __device__ __forceinline__ float quad_max(float v) {
