@@ -529,18 +529,31 @@ def rope(q, k, dim, kv_dim, head_size, pos, theta=10000.0):
 
 # ----------------------------------------------------- attention of a batch
 
+_DTYPES = {}  # dtype object -> its name without "torch."
+
+
 def _typed(fn, name, x, dtype):
     """x, which must be an array or tensor of the given type."""
-    if str(x.dtype).replace("torch.", "") != dtype:
-        raise TypeError(f"{fn}: {name} must be {dtype}, not {x.dtype}")
+    dt = x.dtype
+    if _DTYPES.get(dt) != dtype:
+        _DTYPES[dt] = str(dt).replace("torch.", "")
+        if _DTYPES[dt] != dtype:
+            raise TypeError(f"{fn}: {name} must be {dtype}, not {dt}")
     return x
 
 
-def _f3(fn, name, x):
-    return descn(_typed(fn, name, x, "float32"), 3)
+def _rows(fn, name, x, dtype="float32"):
+    """The rank-3 descriptor of an operand of the given type."""
+    _typed(fn, name, x, dtype)
+    if not _is_torch(x):
+        return descn(x, 3)
+    shape, p = x.shape, x.data_ptr()
+    if len(shape) != 3:
+        raise ValueError(f"expected a rank-3 tensor, got shape {tuple(shape)}")
+    return (p, p, 0, *shape, *x.stride())
 
 
-def _i1(fn, name, x):
+def _list(fn, name, x):
     return desc1(_typed(fn, name, x, "int32"))
 
 
@@ -554,8 +567,8 @@ def attention_packed(q, k, v, out, q_starts, k_starts, scale=None):
     if scale is None:
         scale = q.shape[-1] ** -0.5
     _check(fn, lib.simp_rt_attention_packed_f32(
-        *_f3(fn, "q", q), *_f3(fn, "k", k), *_f3(fn, "v", v), *_f3(fn, "out", out),
-        *_i1(fn, "q_starts", q_starts), *_i1(fn, "k_starts", k_starts), scale))
+        *_rows(fn, "q", q), *_rows(fn, "k", k), *_rows(fn, "v", v), *_rows(fn, "out", out),
+        *_list(fn, "q_starts", q_starts), *_list(fn, "k_starts", k_starts), scale))
     return out
 
 
@@ -601,16 +614,16 @@ class KV8Cache:
         """Stores packed fp32 rows [rows, kv_heads, head_size]: those of sequence b become
         its tokens lengths[b] - n_b .. lengths[b] - 1."""
         fn = "KV8Cache.append"
-        _check(fn, lib.simp_rt_kv8_append(self._ref, *_f3(fn, "k", k), *_f3(fn, "v", v),
-                                          *_i1(fn, "starts", starts), *_i1(fn, "lengths", lengths)))
+        _check(fn, lib.simp_rt_kv8_append(self._ref, *_rows(fn, "k", k), *_rows(fn, "v", v),
+                                          *_list(fn, "starts", starts), *_list(fn, "lengths", lengths)))
 
     def read(self, starts, lengths, k, v):
         """The values of the last starts[b + 1] - starts[b] tokens of each sequence into
         packed fp32 rows."""
         fn = "KV8Cache.read"
-        _check(fn, lib.simp_rt_kv8_read(self._ref, *_i1(fn, "starts", starts),
-                                        *_i1(fn, "lengths", lengths), *_f3(fn, "k", k),
-                                        *_f3(fn, "v", v)))
+        _check(fn, lib.simp_rt_kv8_read(self._ref, *_list(fn, "starts", starts),
+                                        *_list(fn, "lengths", lengths), *_rows(fn, "k", k),
+                                        *_rows(fn, "v", v)))
         return k, v
 
     def attention(self, q, lengths, out, seen=None, seen_out=None, scale=None):
@@ -622,9 +635,9 @@ class KV8Cache:
             raise ValueError("KV8Cache.attention: seen and seen_out go together")
         if scale is None:
             scale = self.head_size ** -0.5
-        d = (_NO3, _NO3) if seen is None else (_f3(fn, "seen", seen), _f3(fn, "seen_out", seen_out))
-        _check(fn, lib.simp_rt_kv8_attention(self._ref, *_f3(fn, "q", q), *_i1(fn, "lengths", lengths),
-                                             *_f3(fn, "out", out), *d[0], *d[1], scale))
+        d = (_NO3, _NO3) if seen is None else (_rows(fn, "seen", seen), _rows(fn, "seen_out", seen_out))
+        _check(fn, lib.simp_rt_kv8_attention(self._ref, *_rows(fn, "q", q), *_list(fn, "lengths", lengths),
+                                             *_rows(fn, "out", out), *d[0], *d[1], scale))
         return out
 
     def evict(self, to: "KV8Cache", lengths, seen, new_seen, kept, budget: int, recent: int = 0):
@@ -633,9 +646,9 @@ class KV8Cache:
         ``kept`` (int32 [batch, kv_heads, budget]) their positions, then -1.  The new lengths
         are min(lengths, budget)."""
         fn = "KV8Cache.evict"
-        _check(fn, lib.simp_rt_kv8_evict(self._ref, to._ref, *_i1(fn, "lengths", lengths),
-                                         *_f3(fn, "seen", seen), *_f3(fn, "new_seen", new_seen),
-                                         *descn(_typed(fn, "kept", kept, "int32"), 3), budget, recent))
+        _check(fn, lib.simp_rt_kv8_evict(self._ref, to._ref, *_list(fn, "lengths", lengths),
+                                         *_rows(fn, "seen", seen), *_rows(fn, "new_seen", new_seen),
+                                         *_rows(fn, "kept", kept, "int32"), budget, recent))
         return kept
 
 

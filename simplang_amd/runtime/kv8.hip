@@ -922,13 +922,8 @@ struct BoundCache {
         {&k, p->k, (size_t)codes, "cache k"}, {&v, p->v, (size_t)codes, "cache v"},
         {&ks, p->k_scale, 4 * (size_t)scales, "cache k_scale"},
         {&vs, p->v_scale, 4 * (size_t)scales, "cache v_scale"}};
-    for (auto &x : a) {
-      const void *d;
-      int rc;
-      if ((rc = device_view(x.p, x.n, &d, x.name)) ||  // no staging of whole caches
-          (rc = bind_here(*x.o, x.p, x.n, dir, dev, x.name)))
-        return rc;
-    }
+    for (auto &x : a)  // no staging of whole caches
+      if (int rc = bind_here(*x.o, x.p, x.n, dir, dev, x.name, false)) return rc;
     c.k = (int8_t *)k.dev(), c.v = (int8_t *)v.dev();
     c.ks = (float *)ks.dev(), c.vs = (float *)vs.dev();
     c.st_seq = p->st_seq, c.st_head = p->st_head, c.st_token = p->st_token;

@@ -183,7 +183,7 @@ Operand::~Operand() {
   if (staged_ && dev_) (void)hipFree(dev_);
 }
 
-int Operand::bind(const void *p, size_t bytes, Dir dir, const char *name) {
+int Operand::bind(const void *p, size_t bytes, Dir dir, const char *name, bool stage) {
   host_ = p;
   bytes_ = bytes;
   dir_ = dir;
@@ -204,6 +204,7 @@ int Operand::bind(const void *p, size_t bytes, Dir dir, const char *name) {
     dev_ = m;
     return SIMP_RT_OK;
   }
+  if (!stage) return set_error(SIMP_RT_EINVAL, "%s: must be device memory or inside a simp_rt_register'd range", name);
   hipError_t e = hipMalloc(&dev_, bytes);
   if (e != hipSuccess) {
     dev_ = nullptr;

@@ -44,8 +44,8 @@ class Operand {
   Operand(const Operand &) = delete;
   Operand &operator=(const Operand &) = delete;
   ~Operand();
-  // Returns SIMP_RT_OK or a negative status.
-  int bind(const void *p, size_t bytes, Dir dir, const char *name);
+  // Returns SIMP_RT_OK or a negative status.  stage = false: plain host memory is refused.
+  int bind(const void *p, size_t bytes, Dir dir, const char *name, bool stage = true);
   void *dev() const { return dev_; }
   bool staged() const { return staged_; }
   // The GPU that the caller's device memory lies on; -1 for anything else.

@@ -26,8 +26,8 @@ inline int check_here(const Operand &o, int dev, const char *name) {
 }
 
 inline int bind_here(Operand &o, const void *p, size_t bytes, Operand::Dir dir, int dev,
-                     const char *name) {
-  const int rc = o.bind(p, bytes, dir, name);
+                     const char *name, bool stage = true) {
+  const int rc = o.bind(p, bytes, dir, name, stage);
   return rc ? rc : check_here(o, dev, name);
 }
 
