@@ -544,17 +544,23 @@ def _typed(fn, name, x, dtype):
 
 def _rows(fn, name, x, dtype="float32"):
     """The rank-3 descriptor of an operand of the given type."""
-    _typed(fn, name, x, dtype)
-    if not _is_torch(x):
+    if _DTYPES.get(x.dtype) != dtype:
+        _typed(fn, name, x, dtype)
+    try:
+        p = x.data_ptr()
+    except AttributeError:
         return descn(x, 3)
-    shape, p = x.shape, x.data_ptr()
-    if len(shape) != 3:
-        raise ValueError(f"expected a rank-3 tensor, got shape {tuple(shape)}")
-    return (p, p, 0, *shape, *x.stride())
+    d = (p, p, 0) + x.shape + x.stride()
+    if len(d) != 9:
+        raise ValueError(f"expected a rank-3 tensor, got shape {tuple(x.shape)}")
+    return d
 
 
 def _list(fn, name, x):
-    return desc1(_typed(fn, name, x, "int32"))
+    """The rank-1 descriptor of an int32 operand."""
+    if _DTYPES.get(x.dtype) != "int32":
+        _typed(fn, name, x, "int32")
+    return desc1(x)
 
 
 def attention_packed(q, k, v, out, q_starts, k_starts, scale=None):

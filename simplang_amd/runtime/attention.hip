@@ -889,16 +889,17 @@ int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
   a.slots = p.tk / kStageKeys + p.n;
   a.blocks = (int)((int64_t)(p.tq / 32 + p.n) * p.group / nw) + p.n;
   // The keys are split where the blocks (each with about `stages`, the last one of a row
-  // half used) would not fill the chip's room for them, one or two a CU, and the rows are
-  // long enough to be worth joining: 17 queries after 2983 tokens 33 us against 235, 273
-  // of the 3B heads after up to 1500 60 against 145.
+  // half used) would not fill the chip, and the rows are long enough to be worth joining:
+  // 17 queries after 2983 tokens 29 us against 235, 273 of the 3B heads after up to 1500 56
+  // against 145, 2048 tokens of 16 heads 65 against 105.  Shorter pieces than 6 stages cost
+  // more in joining than they spare.
   a.splits = 1;
   a.chunk = INT32_MAX / 2;
-  const int64_t room = (int64_t)num_cus() * (nw == 8 || p.hs > 128 ? 1 : 2);
+  const int64_t cus = num_cus(), room = nw == 8 || p.hs > 128 ? cus : cus * 5 / 2;
   const int64_t wgs = cdiv(cdiv(rows, 32) * p.group, nw) * p.n * a.hk;
   const int64_t stages = cdiv(std::max<int64_t>(keys - rows / 2, 1), kStageKeys);
   if (wgs < room) {
-    const int64_t chunk = std::max<int64_t>(4, cdiv(cdiv(wgs * stages, room - wgs / 2), 2) * 2);
+    const int64_t chunk = std::max<int64_t>(6, cdiv(cdiv(wgs * stages, room - wgs / 2), 2) * 2);
     const int64_t splits = cdiv(cdiv(p.tk, kStageKeys), chunk);  // one sequence may have all keys
     if (cdiv(keys, kStageKeys) >= 2 * chunk && splits * p.tq * heads * p.hs <= int64_t(1) << 25 && splits <= 1024) {
       a.chunk = (int)chunk;

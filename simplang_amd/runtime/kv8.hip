@@ -678,12 +678,32 @@ __device__ __forceinline__ uint32_t order_of(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// The tokens of a wave's run, [t0, t1): f(token, order of its weight).  Up to 512 of
+// them (8192 of the sequence) are in registers; more are read again.
+struct Run {
+  const float *seen;
+  int t0, t1;
+  bool held;
+  uint32_t u[8];
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    const int lane = threadIdx.x & 63;
+    if (held) {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (t0 + 64 * i < t1) f(t0 + 64 * i + lane, u[i]);
+    } else {
+      for (int t = t0; t < t1; t += 64) f(t + lane, t + lane < t1 ? order_of(seen[t + lane]) : 0u);
+    }
+  }
+};
+
 // The place-from-the-top search of kv8_select_k: among the weights of 0 .. old-1 whose
 // order agrees with `prefix` above bit `shift + BITS`, a histogram of the next BITS bits;
 // then the bin that holds the need-th from the top.  Returns it, and what is left to
 // take from it in `need`, its size in `size`.
 template <int BITS>
-__device__ __forceinline__ uint32_t select_digit(const float *seen, int old, uint32_t prefix, int shift,
+__device__ __forceinline__ uint32_t select_digit(const Run &run, int old, uint32_t prefix, int shift,
                                                  int &need, int &size, int *hist, int *wave_s) {
   constexpr int BINS = 1 << BITS, PER = BINS / 1024;  // bins of a thread
   static_assert(PER * 1024 == BINS, "");
@@ -691,12 +711,11 @@ __device__ __forceinline__ uint32_t select_digit(const float *seen, int old, uin
 #pragma unroll
   for (int i = 0; i < PER; i++) hist[tid + 1024 * i] = 0;
   __syncthreads();
-  const bool all = shift + BITS == 32;
-#pragma unroll 4
-  for (int t = tid; t < old; t += 1024) {
-    const uint32_t u = order_of(seen[t]);
-    if (all || ((u ^ prefix) >> (shift + BITS)) == 0) atomicAdd(&hist[u >> shift & (BINS - 1)], 1);
-  }
+  const int above_bits = min(shift + BITS, 31);
+  const uint32_t same = shift + BITS == 32 ? 0u : 0xFFFFFFFFu << above_bits;
+  run.each([&](int t, uint32_t u) {
+    if (t < min(old, run.t1) && ((u ^ prefix) & same) == 0) atomicAdd(&hist[u >> shift & (BINS - 1)], 1);
+  });
   __syncthreads();
   // thread t has the bins from the top: BINS - 1 - PER t and the PER - 1 below
   int h[PER], sum = 0;
@@ -713,7 +732,8 @@ __device__ __forceinline__ uint32_t select_digit(const float *seen, int old, uin
   }
   if (lane == 63) wave_s[wave] = upto;
   __syncthreads();
-  for (int w = 0; w < wave; w++) upto += wave_s[w];
+#pragma unroll
+  for (int w = 0; w < 16; w++) upto += w < wave ? wave_s[w] : 0;
   int above = upto - sum;
   if (above < need && need <= upto) {  // one thread
     int i = 0;
@@ -733,9 +753,8 @@ __device__ __forceinline__ uint32_t select_digit(const float *seen, int old, uin
 // Which tokens of one head stay, by one block: the order of the last weight that
 // does, 12 bits and twice 10 from the top, then the places.  Twelve bits first, so
 // that the weights, which share few exponents, do not all add to the same few
-// counters.  Each wave then has a run of tokens: it counts those that stay (and those
-// equal to the last one, of which the first ones do), and writes them behind the
-// other waves'.
+// counters.  Each wave has a run of tokens: it counts those that stay (and those equal
+// to the last one, of which the first ones do), and writes them behind the other waves'.
 __global__ void __launch_bounds__(1024) kv8_select_k(const EvictArgs a) {
   __shared__ int hist[4096];
   __shared__ int wave_s[32], more_s[16], equal_s[16];
@@ -751,31 +770,41 @@ __global__ void __launch_bounds__(1024) kv8_select_k(const EvictArgs a) {
     }
     return;
   }
+  Run run;
+  const int each = (len + 1023) / 1024 * 64;  // tokens of a wave
+  run.seen = seen;
+  run.t0 = min(wave * each, len);
+  run.t1 = min(run.t0 + each, len);
+  run.held = each <= 512;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int t = run.t0 + 64 * i + lane;
+    run.u[i] = run.held && t < run.t1 ? order_of(seen[t]) : 0u;
+  }
   const int old = len - a.recent;  // candidates 0 .. old-1
   int need = a.budget - a.recent;  // of which so many stay (fewer than there are)
   uint32_t last = 0xFFFFFFFFu;     // the order of the last one that stays,
   uint32_t mask = 0xFFFFFFFFu;     // in these bits
   if (need > 0) {
     int size;
-    last = select_digit<12>(seen, old, 0, 20, need, size, hist, wave_s);
+    last = select_digit<12>(run, old, 0, 20, need, size, hist, wave_s);
     mask = 0xFFF00000u;
     if (size != need) {
-      last |= select_digit<10>(seen, old, last, 10, need, size, hist, wave_s);
+      last |= select_digit<10>(run, old, last, 10, need, size, hist, wave_s);
       mask = 0xFFFFFC00u;
     }
     if (size != need) {
-      last |= select_digit<10>(seen, old, last, 0, need, size, hist, wave_s);
+      last |= select_digit<10>(run, old, last, 0, need, size, hist, wave_s);
       mask = 0xFFFFFFFFu;
     }
   }
   const bool any = a.budget > a.recent;
-  const int run = (len + 1023) / 1024 * 64, t0 = min(wave * run, len), t1 = min(t0 + run, len);
   int more = 0, equal = 0;
-  for (int t = t0 + lane; t < t1; t += 64) {
-    const uint32_t u = order_of(seen[t]) & mask;
-    more += t >= old || (any && u > last);
-    equal += t < old && any && u == last;
-  }
+  run.each([&](int t, uint32_t x) {
+    const uint32_t u = x & mask;
+    more += t < run.t1 && (t >= old || (any && u > last));
+    equal += t < min(old, run.t1) && any && u == last;
+  });
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     more += __shfl_xor(more, d);
@@ -792,61 +821,63 @@ __global__ void __launch_bounds__(1024) kv8_select_k(const EvictArgs a) {
     eq += equal_s[w];
   }
   const unsigned long long below = (1ull << lane) - 1;
-  for (int t = t0; t < t1; t += 64) {
-    const int at = t + lane;
-    const float x = at < t1 ? seen[at] : 0.f;
-    const uint32_t u = order_of(x) & mask;
-    const bool same = at < t1 && at < old && any && u == last;
+  run.each([&](int t, uint32_t x) {
+    const uint32_t u = x & mask;
+    const bool same = t < min(old, run.t1) && any && u == last;
     const unsigned long long be = __ballot(same);
-    const bool keep = at < t1 && (at >= old || (any && u > last) || (same && eq + __popcll(be & below) < need));
+    const bool keep = t < run.t1 && (t >= old || (any && u > last) || (same && eq + __popcll(be & below) < need));
     const unsigned long long bk = __ballot(keep);
     const int k = place + __popcll(bk & below);
     if (keep && k < a.budget) {
-      kept[k] = at;
-      ns[k] = x;
+      kept[k] = t;
+      ns[k] = seen[t];
     }
     eq += __popcll(be);
     place += __popcll(bk);
-  }
+  });
 }
 
-// One block of the new cache, one head, K or V (blockIdx.z & 1).
+// One block of the new cache, one head, K and V.  W: 4-byte words to a thread.
+template <int W>
 __global__ void __launch_bounds__(256) kv8_move_k(const EvictArgs a) {
   __shared__ int64_t at[128];
-  __shared__ double ratio[128];  // of the scales; 1: the codes stay; -1: they are cleared
-  __shared__ float top_s[2];
+  __shared__ double ratio[2][128];  // of the scales; 1: the codes stay; -1: they are cleared
+  __shared__ float top_s[4];
   const Cache &c = a.c, &o = a.to;
-  const int blk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z >> 1, tid = threadIdx.x;
-  const bool is_v = blockIdx.z & 1;
+  const int blk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const int len = min(clampi(a.lengths[b], 0, c.cap), a.budget);
   const int p0 = blk << o.shift, nt = min(1 << o.shift, len - p0);
   if (nt <= 0) return;
+  const int i = tid & 127, w = tid >> 7;  // K for half of the threads, V for the others
   float z = 0.f;
-  if (tid < nt) {
-    const int t = clampi(a.kept[b * a.kp_seq + hk * a.kp_head + p0 + tid], 0, c.cap - 1);
-    at[tid] = b * c.st_seq + hk * c.st_head + t * c.st_token;
-    z = (is_v ? c.vs : c.ks)[b * c.sc_seq + hk * c.sc_head + (t >> c.shift)];
+  if (i < nt) {
+    const int t = clampi(a.kept[b * a.kp_seq + hk * a.kp_head + p0 + i], 0, c.cap - 1);
+    if (w == 0) at[i] = b * c.st_seq + hk * c.st_head + t * c.st_token;
+    z = (w ? c.vs : c.ks)[b * c.sc_seq + hk * c.sc_head + (t >> c.shift)];
   }
   float s = wave_max_dpp(z);
   if (__any(z != z)) s = NAN;
-  if (tid < 128 && (tid & 63) == 0) top_s[tid >> 6] = s;
+  if ((tid & 63) == 0) top_s[tid >> 6] = s;
   __syncthreads();
-  s = max_nan(top_s[0], top_s[1]);
+  s = max_nan(top_s[2 * w], top_s[2 * w + 1]);
   const bool live = s > 0.f && s < INFINITY;
-  if (tid < nt) ratio[tid] = !live ? -1.0 : z == s ? 1.0 : (double)z / (double)s;
+  if (i < nt) ratio[w][i] = !live ? -1.0 : z == s ? 1.0 : (double)z / (double)s;
+  if (i == 0) (w ? o.vs : o.ks)[b * o.sc_seq + hk * o.sc_head + blk] = s;
   __syncthreads();
-  const int8_t *src = is_v ? c.v : c.k;
-  int8_t *dst = (is_v ? o.v : o.k) + b * o.st_seq + hk * o.st_head + p0 * o.st_token;
-  const int quads = c.hs >> 2;
-#pragma unroll 4
-  for (int e = tid; e < nt * quads; e += 256) {
-    const int i = e / quads, d = 4 * (e - i * quads);
-    uint32_t x = *(const uint32_t *)(src + at[i] + d);
-    const double r = ratio[i];
-    if (r != 1.0) x = r < 0.0 ? 0u : rescale4(x, r);
-    *(uint32_t *)(dst + i * o.st_token + d) = x;
+  const int64_t to = b * o.st_seq + hk * o.st_head + p0 * o.st_token;
+  const int parts = c.hs / (4 * W), n = nt * parts;
+#pragma unroll 2
+  for (int e = tid; e < 2 * n; e += 256) {
+    const bool v = e >= n;
+    const int f = v ? e - n : e, r = f / parts, d = 4 * W * (f - r * parts);
+    uint32_t x[W];
+    __builtin_memcpy(x, __builtin_assume_aligned((v ? c.v : c.k) + at[r] + d, 4 * W), 4 * W);
+    const double q = ratio[v][r];
+    if (q != 1.0)
+#pragma unroll
+      for (int g = 0; g < W; g++) x[g] = q < 0.0 ? 0u : rescale4(x[g], q);
+    __builtin_memcpy(__builtin_assume_aligned((v ? o.v : o.k) + to + r * o.st_token + d, 4 * W), x, 4 * W);
   }
-  if (tid == 0) (is_v ? o.vs : o.ks)[b * o.sc_seq + hk * o.sc_head + blk] = s;
 }
 
 // ------------------------------------------------------------- host side
@@ -1221,8 +1252,12 @@ int32_t simp_rt_kv8_evict(
                     (int)budget, (int)recent};
   hipStream_t st = cur_stream();
   hipLaunchKernelGGL(kv8_select_k, dim3((unsigned)bc.c.hk, (unsigned)bc.c.n), dim3(1024), 0, st, a);
-  hipLaunchKernelGGL(kv8_move_k, dim3((unsigned)cdiv(budget, to->block), (unsigned)bc.c.hk,
-                                      2 * (unsigned)bc.c.n), dim3(256), 0, st, a);
+  const dim3 grid((unsigned)cdiv(budget, to->block), (unsigned)bc.c.hk, (unsigned)bc.c.n);
+  auto wide = [](const Cache &c) {
+    return ((c.hs | c.st_seq | c.st_head | c.st_token | (int64_t)(uintptr_t)c.k | (int64_t)(uintptr_t)c.v) & 15) == 0;
+  };
+  if (wide(bc.c) && wide(bt.c)) hipLaunchKernelGGL(kv8_move_k<4>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(kv8_move_k<1>, grid, dim3(256), 0, st, a);
   Operand *ops[] = {&ol, &os, &on, &op};
   return finish(ops, 4);
 }
