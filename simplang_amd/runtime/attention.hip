@@ -899,11 +899,15 @@ int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
   const int64_t wgs = cdiv(cdiv(rows, 32) * p.group, nw) * p.n * a.hk;
   const int64_t stages = cdiv(std::max<int64_t>(keys - rows / 2, 1), kStageKeys);
   if (wgs < room) {
-    const int64_t chunk = std::max<int64_t>(6, cdiv(cdiv(wgs * stages, room - wgs / 2), 2) * 2);
-    const int64_t splits = cdiv(cdiv(p.tk, kStageKeys), chunk);  // one sequence may have all keys
-    if (cdiv(keys, kStageKeys) >= 2 * chunk && splits * p.tq * heads * p.hs <= int64_t(1) << 25 && splits <= 1024) {
+    // One sequence may have all keys.  The pieces' rows take up to 128 MB, and the weights of
+    // a block of attn_join_k up to 48 KB.
+    const int64_t most = cdiv(p.tk, kStageKeys), row = (int64_t)heads * p.hs;
+    const int64_t join_heads = std::min<int64_t>(heads, 1024 / p.hs + 2);
+    const int64_t chunk = std::max({int64_t(6), cdiv(cdiv(wgs * stages, room - wgs / 2), 2) * 2,
+                                    cdiv(most * join_heads, 12288), cdiv(most * p.tq * row, int64_t(1) << 25)});
+    if (cdiv(keys, kStageKeys) >= 2 * chunk) {
       a.chunk = (int)chunk;
-      a.splits = (int)splits;
+      a.splits = (int)cdiv(most, chunk);
     }
   }
   if ((int64_t)a.blocks * a.hk * 64 * nw > UINT32_MAX || (int64_t)a.slots * 256 > UINT32_MAX)

@@ -55,7 +55,7 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t c, double ratio) {
 // ---------------------------------------------------------------- append
 //
 // One block of one head, K or V (blockIdx.z), to a block of threads that holds the
-// new rows in registers between their maximum and their codes (V chunks of four
+// new rows in registers between their maximum and their codes (kAppendChunks times four
 // values to a thread): x is read once and memory bounds it.  Sequence b has the slots
 // starts[b] / T + 2 b and on: n rows touch at most n / T + 2 blocks.
 
@@ -172,7 +172,11 @@ __global__ void __launch_bounds__(256) kv8_read_k(const ReadArgs a) {
   if (threadIdx.x < 64) {
     const int r = first + min((int)threadIdx.x, n - 1);
     int b = last_of(c.n, [&](int s) { return clampi(a.starts[s], 0, a.rows) <= first; });
-    while (b + 1 < c.n && clampi(a.starts[b + 1], 0, a.rows) <= r) b++;
+    for (int hi = c.n - 1; b < hi && clampi(a.starts[b + 1], 0, a.rows) <= r;) {  // this row's
+      const int mid = (b + hi + 1) >> 1;
+      if (clampi(a.starts[mid], 0, a.rows) <= r) b = mid;
+      else hi = mid - 1;
+    }
     const int r0 = clampi(a.starts[b], 0, a.rows), r1 = clampi(a.starts[b + 1], r0, a.rows);
     if ((int)threadIdx.x < n) {
       const int64_t p = (int64_t)a.lengths[b] - (r1 - r);
@@ -385,7 +389,7 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 && QUAD ? 3 : NC < 
         for (int i = 0; i < L; i++) ql[j][i][w] = (int)l[i];
       }
   }
-  const int last = len - 1;
+  const int last = to - 1;  // rows behind it repeat it, and are masked
   // Addresses: a wave-uniform base for the tile, and 24-bit row numbers times strides
   // below 2^24 (the caller sees to that).
   const uint32_t stride = (uint32_t)c.st_token;
@@ -1161,7 +1165,8 @@ int32_t simp_rt_kv8_attention(
   a.width = a.group <= 4 ? 4 : bc.c.hs > 192 ? 8 : 16;
   a.sets = (int)cdiv(a.group, a.width);
   const int64_t per = (int64_t)bc.c.n * bc.c.hk * a.sets;
-  a.chunk = (int)(256 * std::max<int64_t>(1, cdiv(per * bc.c.cap, 512 * 256)));
+  a.chunk = (int)std::min<int64_t>(256 * std::max<int64_t>(1, cdiv(per * bc.c.cap, 512 * 256)),
+                                   cdiv(bc.c.cap, 256) * 256);
   a.splits = (int)cdiv(bc.c.cap, a.chunk);
   const size_t rows = (size_t)q_s0 * (size_t)q_s1, parts = rows * (size_t)a.splits;
   Workspace ws;

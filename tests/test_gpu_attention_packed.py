@@ -66,6 +66,23 @@ def test_long(dev, heads, kv, hs, nq, nk):
     _check(_run(dev, *a), *a)
 
 
+@pytest.mark.parametrize("heads, kv, hs, nq, nk", [(8, 1, 128, 500, 520), (8, 2, 64, 800, 800), (8, 1, 32, 450, 450),
+                                                   (6, 1, 96, 600, 640), (4, 1, 192, 800, 811), (5, 1, 256, 650, 700),
+                                                   (4, 1, 100, 801, 900), (4, 1, 63, 800, 830)])
+def test_many_queries(dev, heads, kv, hs, nq, nk):
+    """Enough queries to a key that K and V are taken apart once, ahead of the products."""
+    a = _case([nq], [nk], heads, kv, hs, seed=nq)
+    _check(_run(dev, *a), *a)
+
+
+@pytest.mark.parametrize("heads, kv, hs, nq, nk", [(4, 1, 64, 2, 6000), (66, 2, 16, 1, 20000), (2, 1, 128, 33, 4000),
+                                                   (3, 3, 7, 5, 3000), (1, 1, 256, 9, 2000), (300, 1, 2, 1, 2500)])
+def test_few_queries_over_many_keys(dev, heads, kv, hs, nq, nk):
+    """The keys are split over blocks, and the pieces joined."""
+    a = _case([nq, 1, 0, 1], [nk, 1, 2, 0], heads, kv, hs, seed=nk)
+    _check(_run(dev, *a), *a)
+
+
 def test_fewer_keys_than_queries_leaves_rows_empty(dev):
     a = _case([40, 20, 5], [10, 0, 5], 4, 2, 64)
     got = _run(dev, *a)
@@ -148,6 +165,42 @@ def test_hidden_keys_may_hold_anything(dev, which, bad, n):
     else:
         assert not np.isfinite(got[n - 4:n, :2, 5:9]).any()
         assert np.isfinite(got[n - 4:n, :2, 9:]).all()
+
+
+@pytest.mark.parametrize("nq, nk, heads", [(850, 850, 4), (40, 2500, 2)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, 1e30])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_hidden_keys_of_long_inputs(dev, which, bad, nq, nk, heads):
+    """The same where the keys are taken apart ahead, and where they are split over blocks."""
+    a = _case([nq], [nk], heads, 1, 64)
+    q, k, v, qs, ks = a
+    (k if which == "k" else v)[nk - 4, 0, 5:9] = bad
+    got = _run(dev, *a)
+    want, tol = S.packed(*(np.where(np.abs(x) < 1e20, x, 0) for x in (q, k, v)), qs, ks, 0.125, heads)
+    assert (np.abs(got - want) <= tol[..., None])[:nq - 4].all()
+    if which == "v":
+        assert np.abs(got[nq - 4:, :, 5:9]).max() > 1e20 or not np.isfinite(got[nq - 4:, :, 5:9]).any()
+        assert (np.abs(got - want)[..., 9:] <= tol[..., None]).all()
+
+
+@pytest.mark.parametrize("nq, nk, heads", [(850, 850, 4), (40, 2500, 2), (90, 90, 2)])
+@pytest.mark.parametrize("at", [0, 5, 31, 40])
+def test_keys_of_zeros_and_tiny_keys(dev, nq, nk, heads, at):
+    """Some keys and values are 0, some so small that they are next to nothing beside their
+    neighbours: the queries that see only those get them in full."""
+    q, k, v, qs, ks = _case([nq, 50], [nk, 50], heads, 1, 64)
+    k[at:at + 3] = 0
+    v[at:at + 2] = 0
+    _check(_run(dev, q, k, v, qs, ks), q, k, v, qs, ks)
+    v[:6] *= np.float32(1e-13)
+    v[nk:nk + 7] *= np.float32(1e-30)
+    got = _run(dev, q, k, v, qs, ks)
+    _check(got, q, k, v, qs, ks)
+    # relative to what the first queries see, not to the values they do not
+    want, _ = S.packed(q, k, v, qs, ks, 0.125, heads)
+    for r in [*range(0, 6 if nq == nk else 0), *range(nq, nq + 7)]:
+        size = np.abs(want[r]).max()
+        assert np.abs(got[r] - want[r]).max() <= 1e-5 * size, r
 
 
 def test_large_and_small_values(dev):

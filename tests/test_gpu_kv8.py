@@ -456,6 +456,77 @@ def test_graph_and_streams(dev):
         sa.set_stream(torch.cuda.current_stream())
 
 
+def test_capture_without_a_warm_up_call_is_refused(dev):
+    """The attention wants scratch, which a captured call does not allocate; the rest wants none."""
+    import torch
+    p = Pair(dev, 2, 1, 5000, 32, 16)
+    q, out = torch.zeros((2, 2, 32), device=dev), torch.zeros((2, 2, 32), device=dev)
+    k, v, st, ln = p.up(*_rows(2, 1, 32), S.starts([1, 1]), np.array([100, 7], np.int32))
+    p.np.append(k.cpu().numpy(), v.cpu().numpy(), st.cpu().numpy(), [100, 7])
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    try:
+        sa.set_stream(stream)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            with pytest.raises(sa.SimpRTError, match="workspace"):
+                p.gpu.attention(q, ln, out)
+            p.gpu.append(k, v, st, ln)
+        g.replay()
+        torch.cuda.synchronize()
+        p.same()
+    finally:
+        sa.set_stream(torch.cuda.current_stream())
+
+
+def test_two_threads(dev):
+    """Two threads at once on one stream: each finds its own results."""
+    import threading
+    import torch
+    ps = [Pair(dev, 2, 2, 3000, 64, 32, seed=i) for i in range(2)]
+    r = np.random.default_rng(1)
+    qs = [r.standard_normal((2, 4, 64)).astype(np.float32) for _ in ps]
+    ln = np.array([3000, 1700], np.int32)
+    want = [p.np.attention(q, ln, 0.125) for p, q in zip(ps, qs)]
+    fails = []
+
+    def work(i):
+        torch.cuda.set_device(0)
+        sa.set_stream(torch.cuda.current_stream())
+        q, lt = ps[i].up(qs[i], ln)
+        for _ in range(30):
+            out = torch.zeros_like(q)
+            ps[i].gpu.attention(q, lt, out)
+            torch.cuda.synchronize()
+            if (np.abs(out.cpu().numpy() - want[i][0]) > want[i][2][..., None]).any():
+                fails.append(i)
+                return
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not fails
+
+
+def test_read_over_many_empty_sequences(dev):
+    import torch
+    n = 3000
+    p = Pair(dev, n, 1, 16, 16, 16)
+    lens = np.zeros(n, int)
+    lens[[0, 1, 1500, n - 1]] = [3, 16, 5, 9]
+    st, ln = S.starts(lens), np.full(n, 16, np.int32)
+    k = np.zeros((33, 1, 16), np.float32)
+    v = np.zeros_like(k)
+    p.np.read(st, ln, k, v)
+    kt, vt = torch.zeros((33, 1, 16), device=dev), torch.zeros((33, 1, 16), device=dev)
+    p.gpu.read(*p.up(st, ln), kt, vt)
+    assert np.array_equal(kt.cpu().numpy(), k) and np.array_equal(vt.cpu().numpy(), v)
+    p.append(*_rows(33, 1, 16), lens, ln)
+    p.same()
+
+
 def test_a_serving_loop(dev):
     """Prompts in two chunks, decode steps, an eviction, more steps: the operators together,
     against the same loop in numpy."""
