@@ -401,9 +401,10 @@ int32_t simp_rt_rope(
  * query that sees none (nk < nq) gets zeros; a key that a query does not see has
  * no part in its row, whatever its values.  Rows of out that belong to no
  * sequence stay as they are.  starts: i32, increasing, sequences + 1 of them;
- * values outside the rows are cut off at them.  head_size 1 to 256.  out may
- * share no memory range with the inputs.  Sums and statistics are fp32, and the
- * products as close as fp32 ones. */
+ * values outside the rows are cut off at them.  head_size 1 to 256; rows of k and v
+ * less than 2^23 elements apart.  out may share no memory range with the inputs.
+ * Sums and statistics are fp32, and the products as close as fp32 ones; the values
+ * of a query's keys, added up, have to stay below fp32's largest number. */
 int32_t simp_rt_attention_packed_f32(
     const float *q_alloc, const float *q, int64_t q_off, int64_t q_s0, int64_t q_s1, int64_t q_s2,
     int64_t q_st0, int64_t q_st1, int64_t q_st2,
@@ -425,7 +426,8 @@ int32_t simp_rt_attention_packed_f32(
  * arrays are device memory or registered ranges (they are the caller's; the
  * struct only says where they lie).  block is 16, 32, 64 or 128; head_size a
  * multiple of 4 from 16 to 256; code rows start on 4-byte boundaries; tokens of a
- * head, and heads, may be in either order ([heads, capacity] or [capacity, heads]). */
+ * head, and heads, may be in either order ([heads, capacity] or [capacity, heads]),
+ * tokens less than 2^24 apart.  batch and heads up to 32767. */
 typedef struct {
   int8_t *k, *v;
   float *k_scale, *v_scale; /* ceil(capacity / block) per sequence and head */
@@ -460,7 +462,7 @@ int32_t simp_rt_kv8_append(
  * sequence into the packed rows k and v [rows, kv_heads, head_size]: what
  * simp_rt_attention_packed_f32 needs of a prompt's earlier tokens.  Rows of
  * positions outside [0, capacity) become zeros; rows that belong to no sequence
- * stay as they are. */
+ * stay as they are.  k and v share no element (one may lie between the other's rows). */
 int32_t simp_rt_kv8_read(
     const simp_rt_kv8 *cache,
     const int32_t *st_alloc, const int32_t *starts, int64_t st_off, int64_t st_size, int64_t st_stride,
@@ -478,7 +480,8 @@ int32_t simp_rt_kv8_read(
  * seen_in + the sum of p over the heads that share the kv head, for the tokens
  * below the length; the rest stays as it is.  They may be the same array, and
  * share no range otherwise.  Sums and statistics are fp32; q is rounded to 24 bits of
- * its largest element, and the products with the codes are exact. */
+ * its largest element, and the products with the codes are exact.  At most 4096
+ * query heads to a kv head. */
 int32_t simp_rt_kv8_attention(
     const simp_rt_kv8 *cache,
     const float *q_alloc, const float *q, int64_t q_off, int64_t q_s0, int64_t q_s1, int64_t q_s2,

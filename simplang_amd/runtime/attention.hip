@@ -198,7 +198,7 @@ struct F16Args {
   int hk;               // kv heads
   int blocks;           // of one kv head and one split
   int splits, chunk;    // of the keys: stages a split takes
-  float *part;          // [splits, tq, heads, head_size], with splits > 1
+  float *part;          // [splits, tq, heads, head_size], each divided by its sum; with splits > 1
   float2 *stat;         // [splits, tq, heads]: maximum and sum
   uint4 *frags;         // STORED: [slots, kv heads] stages, slots as of tiles of 32 keys
   float4 *scales;       // STORED: [kv heads, slots]: 1 / the scaling of K and of V (NaN: not
@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
       float *out = args.splits > 1 ? args.part + at * a.hs
                                    : a.out + (int64_t)(z.qb + r) * a.o_row + un.head * a.o_head;
       if (args.splits > 1 && g == 0) args.stat[at] = make_float2(m * 1.44269504f, l);
-      const float f = args.splits > 1 ? 1.f : r + off < 0 ? 0.f : 1.f / l;
+      const float f = args.splits == 1 && r + off < 0 ? 0.f : 1.f / l;
 #pragma unroll
       for (int j = 0; j < 2 * NB; j++)
 #pragma unroll
@@ -775,17 +775,18 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
     permlane32_swap(u, v);
     l = u + v;
   }
+  // Two factors: the scaling, exact, and 1 / l.  One number for both would lose bits to
+  // gradual underflow where V is tiny.
   const float scale = unit > -1000 ? ldexpf(1.f, unit - 13) : 0.f;
   const bool none = args.splits == 1 && my < 0;
+  const float f = 1.f / l;
   float *out;
-  float f = scale;
   if (args.splits > 1) {
     const int64_t at = part_row + (int64_t)row * part_step;
     out = args.part + at * a.hs;
     if (h == 0) args.stat[at] = make_float2(m, l);
   } else {
     out = a.out + (int64_t)(z.qb + row) * a.o_row + un.head * a.o_head;
-    f = scale / l;
   }
 #pragma unroll
   for (int d = 0; d < NB; d++)
@@ -794,7 +795,7 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
       const int at = 32 * d + 2 * r + 4 * h;
       float y[4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) y[e] = none ? 0.f : o[d][r + e] * f;
+      for (int e = 0; e < 4; e++) y[e] = none ? 0.f : o[d][r + e] * f * scale;
       if (VEC) {
         if (at < a.hs) *(float4 *)(out + at) = make_float4(y[0], y[1], y[2], y[3]);
       } else {
@@ -827,9 +828,9 @@ __global__ void __launch_bounds__(256) attn_join_k(const F16Args args) {
 #pragma unroll 8
     for (int i = 0; i < ns; i++) {
       const float2 ml = stat[i * step];
-      const float f = pow2(ml.x - M);
+      const float f = pow2(ml.x - M) * ml.y;
       weight[t * ns + i] = f;
-      L = fmaf(f, ml.y, L);
+      L += f;
     }
     for (int i = 0; i < ns; i++) weight[t * ns + i] /= L;
   }
@@ -886,8 +887,11 @@ int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
   const bool stored = rows * p.group >= 24 * 128;
   // Eight waves share a fetched stage where their registers leave room for two on a SIMD.
   const int nw = stored && p.hs <= 128 ? 8 : 4;
-  a.slots = p.tk / kStageKeys + p.n;
-  a.blocks = (int)((int64_t)(p.tq / 32 + p.n) * p.group / nw) + p.n;
+  const int64_t slots = p.tk / kStageKeys + p.n, blocks = (int64_t)(p.tq / 32 + p.n) * p.group / nw + p.n;
+  if (blocks > UINT32_MAX / a.hk / (64 * nw) || slots > UINT32_MAX / 256)
+    return set_error(SIMP_RT_EUNSUPPORTED, "attention_packed: more rows, heads or sequences than the grid holds");
+  a.slots = (int)slots;
+  a.blocks = (int)blocks;
   // The keys are split where the blocks (each with about `stages`, the last one of a row
   // half used) would not fill the chip, and the rows are long enough to be worth joining:
   // 17 queries after 2983 tokens 29 us against 235, 273 of the 3B heads after up to 1500 56
@@ -910,8 +914,6 @@ int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
       a.splits = (int)cdiv(most, chunk);
     }
   }
-  if ((int64_t)a.blocks * a.hk * 64 * nw > UINT32_MAX || (int64_t)a.slots * 256 > UINT32_MAX)
-    return set_error(SIMP_RT_EUNSUPPORTED, "attention_packed: more rows, heads or sequences than the grid holds");
   const size_t parts = a.splits > 1 ? (size_t)a.splits * p.tq * heads : 0;
   size_t bytes = 0;
   auto take = [&](size_t n) { return std::exchange(bytes, bytes + (n + 15) / 16 * 16); };
@@ -1000,7 +1002,9 @@ int32_t simp_rt_attention_packed_f32(
     return set_error(SIMP_RT_EUNSUPPORTED, "attention_packed: rows of k or v 2^23 elements or more apart");
   if (overlap(dout.data(), dout.bytes(), dq.data(), dq.bytes()) ||
       overlap(dout.data(), dout.bytes(), dk.data(), dk.bytes()) ||
-      overlap(dout.data(), dout.bytes(), dv.data(), dv.bytes()))
+      overlap(dout.data(), dout.bytes(), dv.data(), dv.bytes()) ||
+      overlap(dout.data(), dout.bytes(), q_starts + qst_off, 4 * (size_t)qst_size) ||
+      overlap(dout.data(), dout.bytes(), k_starts + kst_off, 4 * (size_t)kst_size))
     return set_error(SIMP_RT_EINVAL, "attention_packed: out shares memory with an input");
   const int dev = ensure_device();
   if (dev < 0) return dev;

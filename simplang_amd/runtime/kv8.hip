@@ -941,6 +941,8 @@ struct BoundCache {
       return set_error(SIMP_RT_EINVAL, "%s: %s: strides let rows overlap", fn, name);
     if (!p->k || !p->v || !p->k_scale || !p->v_scale)
       return set_error(SIMP_RT_EINVAL, "%s: %s: null pointer", fn, name);
+    if (p->k == p->v || p->k_scale == p->v_scale)
+      return set_error(SIMP_RT_EINVAL, "%s: %s: K and V are the same memory", fn, name);
     if (((uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->k_scale | (uintptr_t)p->v_scale |
          (uintptr_t)p->st_seq | (uintptr_t)p->st_head | (uintptr_t)p->st_token) & 3)
       return set_error(SIMP_RT_EINVAL, "%s: %s: rows and scales must start on 4-byte boundaries", fn, name);
@@ -1012,8 +1014,10 @@ int32_t simp_rt_kv8_append(
   if (!dk.is(k_s0, cache->n_kv_heads, cache->head_size) || !dv.is(k_s0, k_s1, k_s2))
     return set_error(SIMP_RT_EINVAL, "kv8_append: k and v must be [rows, n_kv_heads, head_size]");
   if (bc.empty || k_s0 == 0) return SIMP_RT_OK;
-  if (bc.shares(cache, dk.data(), dk.bytes()) || bc.shares(cache, dv.data(), dv.bytes()))
-    return set_error(SIMP_RT_EINVAL, "kv8_append: rows share memory with the cache");
+  if (bc.shares(cache, dk.data(), dk.bytes()) || bc.shares(cache, dv.data(), dv.bytes()) ||
+      bc.shares(cache, starts + st_off, 4 * (size_t)st_size) ||
+      bc.shares(cache, lengths + len_off, 4 * (size_t)len_size))
+    return set_error(SIMP_RT_EINVAL, "kv8_append: rows or lists share memory with the cache");
   const int64_t slots = k_s0 / cache->block + 2 * cache->batch;
   if (k_s0 > INT32_MAX || slots * 1024 > UINT32_MAX)
     return set_error(SIMP_RT_EUNSUPPORTED, "kv8_append: more rows than the grid holds");
@@ -1069,6 +1073,11 @@ int32_t simp_rt_kv8_read(
   if (bc.empty) return set_error(SIMP_RT_EINVAL, "kv8_read: the cache has no capacity");
   if (bc.shares(cache, dk.data(), dk.bytes()) || bc.shares(cache, dv.data(), dv.bytes()))
     return set_error(SIMP_RT_EINVAL, "kv8_read: rows share memory with the cache");
+  if (share(dk, dv) || overlap(dk.data(), dk.bytes(), starts + st_off, 4 * (size_t)st_size) ||
+      overlap(dv.data(), dv.bytes(), starts + st_off, 4 * (size_t)st_size) ||
+      overlap(dk.data(), dk.bytes(), lengths + len_off, 4 * (size_t)len_size) ||
+      overlap(dv.data(), dv.bytes(), lengths + len_off, 4 * (size_t)len_size))
+    return set_error(SIMP_RT_EINVAL, "kv8_read: k or v shares memory with another operand");
   const int dev = ensure_device();
   if (dev < 0) return dev;
   Operand ok, ov, os, ol;
@@ -1125,8 +1134,10 @@ int32_t simp_rt_kv8_attention(
   if (q_s1 > 32767 || q_s1 / cache->n_kv_heads > 4096)
     return set_error(SIMP_RT_EUNSUPPORTED, "kv8_attention: heads above 32767, or 4096 to a kv head");
   const bool in_place = with && dsi.data() == dso.data() && si_st0 == so_st0 && si_st1 == so_st1;
+  const auto with_lengths = [&](const void *p, size_t n) { return overlap(p, n, lengths + len_off, 4 * (size_t)len_size); };
   if (overlap(dout.data(), dout.bytes(), dq.data(), dq.bytes()) ||
-      bc.shares(cache, dout.data(), dout.bytes()) ||
+      bc.shares(cache, dout.data(), dout.bytes()) || with_lengths(dout.data(), dout.bytes()) ||
+      (with && with_lengths(dso.data(), dso.bytes())) ||
       (with && bc.shares(cache, dso.data(), dso.bytes())) ||
       (with && (overlap(dout.data(), dout.bytes(), dsi.data(), dsi.bytes()) ||
                 overlap(dout.data(), dout.bytes(), dso.data(), dso.bytes()) ||

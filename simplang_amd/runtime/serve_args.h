@@ -37,4 +37,20 @@ inline bool overlap(const void *a, size_t an, const void *b, size_t bn) {
   return an && bn && x < y + bn && y < x + an;
 }
 
+// Whether two arrays of one shape share elements.  One may lie between the rows or the
+// heads of the other, as the parts of a fused product do.
+template <class T>
+bool share(const Desc3<T> &a, const Desc3<T> &b) {
+  if (!overlap(a.data(), a.bytes(), b.data(), b.bytes())) return false;
+  if (((uintptr_t)a.data() ^ (uintptr_t)b.data()) % sizeof(T)) return true;
+  const auto apart = [&](int64_t period, int64_t n) {  // runs of n elements, one each period
+    const int64_t d = ((int64_t)((uintptr_t)b.data() - (uintptr_t)a.data()) / (int64_t)sizeof(T)) % period;
+    const int64_t to = d < 0 ? d + period : d;
+    return to >= n && period - to >= n;
+  };
+  if (a.st[0] != b.st[0] || a.st[1] != b.st[1]) return true;
+  return !apart(a.st[0], (a.s[1] - 1) * a.st[1] + a.s[2]) &&
+         !(a.st[0] % a.st[1] == 0 && apart(a.st[1], a.s[2]));
+}
+
 }  // namespace simp

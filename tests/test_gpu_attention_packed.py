@@ -203,6 +203,18 @@ def test_keys_of_zeros_and_tiny_keys(dev, nq, nk, heads, at):
         assert np.abs(got[r] - want[r]).max() <= 1e-5 * size, r
 
 
+@pytest.mark.parametrize("size", [1e-36, 1e-33, 1e34])
+@pytest.mark.parametrize("nq, nk, heads", [(850, 850, 4), (40, 2500, 2), (90, 90, 2)])
+def test_tiny_and_huge_values_keep_their_bits(dev, nq, nk, heads, size):
+    """The result is linear in V, and so is its bound as long as no value is subnormal (the
+    smallest here are 5e-37): the bound at size 1, times the size."""
+    q, k, v, qs, ks = _case([nq], [nk], heads, 1, 64)
+    v[:] = (np.abs(v) + np.float32(0.5)) * np.float32(size)
+    got = _run(dev, q, k, v, qs, ks).astype(np.float64)
+    want, tol = S.packed(q, k, v / np.float64(np.float32(size)), qs, ks, 0.125, heads)
+    assert (np.abs(got / np.float64(np.float32(size)) - want) <= tol[..., None]).all()
+
+
 def test_large_and_small_values(dev):
     a = _case([90], [90], 2, 2, 64, amp=1.0)
     q, k, v, qs, ks = a

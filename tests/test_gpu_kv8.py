@@ -510,6 +510,21 @@ def test_two_threads(dev):
     assert not fails
 
 
+def test_read_into_parts_of_one_tensor(dev):
+    """K and V between each other's rows, or heads."""
+    import torch
+    p = Pair(dev, 2, 3, 40, 32, 16)
+    st, ln = S.starts([9, 20]), np.array([30, 33], np.int32)
+    p.append(*_rows(29, 3, 32), [9, 20], ln)
+    k, v = np.zeros((29, 3, 32), np.float32), np.zeros((29, 3, 32), np.float32)
+    p.np.read(st, ln, k, v)
+    for axis in (1, 2):
+        x = torch.zeros((29, 2, 3, 32) if axis == 1 else (29, 3, 2, 32), device=dev)
+        kt, vt = x.unbind(axis)
+        p.gpu.read(*p.up(st, ln), kt, vt)
+        assert np.array_equal(kt.cpu().numpy(), k) and np.array_equal(vt.cpu().numpy(), v)
+
+
 def test_read_over_many_empty_sequences(dev):
     import torch
     n = 3000

@@ -154,6 +154,61 @@ def test_evict_refusals():
         c.evict(to, ln, seen, ns, kept.astype(np.int64), 20)
 
 
+def test_lists_and_outputs_in_one_memory_are_refused():
+    a = _prompt(tq=8)
+    flat = a["out"].reshape(-1).view(I)
+    for name in ("q_starts", "k_starts"):
+        with pytest.raises(sa.SimpRTError, match="shares memory"):
+            sa.attention_packed(**{**a, name: flat[3:5]})
+    arrays = _cache()
+    c = sa.KV8Cache(*arrays, 16)
+    k, v = _rows()
+    with pytest.raises(sa.SimpRTError, match="shares memory"):
+        c.read(np.zeros(3, I), np.zeros(2, I), k, k)
+    with pytest.raises(sa.SimpRTError, match="shares memory"):
+        c.read(v.reshape(-1).view(I)[:3], np.zeros(2, I), k, v)
+    with pytest.raises(sa.SimpRTError, match="shares memory"):
+        c.read(np.zeros(3, I), k.reshape(-1).view(I)[5:7], k, v)
+    w = np.zeros((5, 2, 32), F)
+    with pytest.raises(sa.SimpRTError, match="shares memory"):  # a row on
+        c.read(np.zeros(3, I), np.zeros(2, I), w[:4], w[1:])
+    w = np.zeros((4, 2, 96), F)
+    with pytest.raises(sa.SimpRTError, match="shares memory"):  # the end of a head's row over the next one's
+        c.read(np.zeros(3, I), np.zeros(2, I), w[..., :32], w[..., 31:63])
+    q = np.zeros((2, 4, 32), F)
+    out = q.copy()
+    seen = np.zeros((2, 2, 40), F)
+    with pytest.raises(sa.SimpRTError, match="shares memory"):
+        c.attention(q, out.reshape(-1).view(I)[7:9], out)
+    with pytest.raises(sa.SimpRTError, match="shares memory"):
+        c.attention(q, seen.reshape(-1).view(I)[7:9], out, seen, seen)
+    with pytest.raises(sa.SimpRTError, match="share memory"):
+        c.append(k, v, np.zeros(3, I), arrays[2].reshape(-1).view(I)[:2])
+
+
+def test_one_array_for_k_and_v_is_refused():
+    a = _cache()
+    k, v = _rows()
+    for c in (sa.KV8Cache(a[0], a[0], a[2], a[3], 16), sa.KV8Cache(a[0], a[1], a[2], a[2], 16)):
+        with pytest.raises(sa.SimpRTError, match="same memory"):
+            c.append(k, v, np.zeros(3, I), np.zeros(2, I))
+
+
+def test_far_rows_are_refused():
+    """Strides beyond what the kernels' offsets hold, without the memory."""
+    from numpy.lib.stride_tricks import as_strided
+    a = _prompt(tq=2, tk=2)
+    x = as_strided(np.zeros(1, F), (2, 2, 32), (4 << 23, 128, 4))
+    with pytest.raises(sa.SimpRTError, match="2\\^23"):
+        sa.attention_packed(**{**a, "k": x})
+    with pytest.raises(sa.SimpRTError, match="2\\^23"):
+        sa.attention_packed(**{**a, "v": x})
+    y = as_strided(np.zeros(4, np.int8), (2, 2, 40, 32), (40 << 24, 32, 1 << 24, 1))
+    z = as_strided(np.zeros(4, np.int8), (2, 2, 40, 32), (40 << 24, 32, 1 << 24, 1))
+    with pytest.raises(sa.SimpRTError, match="2\\^24"):
+        sa.KV8Cache(y, z, *_cache()[2:], 16).append(*_rows(), np.zeros(3, I), np.zeros(2, I))
+
+
 def test_null_cache():
     from simplang_amd import host
     z = [None, None] + [0] * 7
