@@ -480,8 +480,10 @@ int32_t simp_rt_kv8_read(
  * seen_in + the sum of p over the heads that share the kv head, for the tokens
  * below the length; the rest stays as it is.  They may be the same array, and
  * share no range otherwise.  Sums and statistics are fp32; q is rounded to 24 bits of
- * its largest element, and the products with the codes are exact.  At most 4096
- * query heads to a kv head. */
+ * its largest element, and the products with the codes are exact; the values
+ * of a sequence's tokens, added up, have to stay below fp32's largest number, and
+ * those below 2^-90 lose bits to gradual underflow.  At most 4096 query heads to a kv
+ * head. */
 int32_t simp_rt_kv8_attention(
     const simp_rt_kv8 *cache,
     const float *q_alloc, const float *q, int64_t q_off, int64_t q_s0, int64_t q_s1, int64_t q_s2,
