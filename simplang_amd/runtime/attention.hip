@@ -175,8 +175,8 @@ __device__ __forceinline__ void attend16(const PackedArgs &a, const float *qr, c
 //   attn_f16_k    a block of NW waves takes NW units (32 queries of one head) of one kv
 //                 head, so that the query heads of a group share the stages, and
 //                 walks them through LDS.  It makes them itself from K and V rows, or
-//                 (STORED) fetches what attn_split_k has made once for all blocks.
-//   attn_split_k  makes the stages.
+//                 (STORED) fetches what attn_stages_k has made once for all blocks.
+//   attn_stages_k  makes the stages.
 //   attn_join_k   where there are few units the keys are split over several blocks; this
 //                 joins what they leave.
 // A block whose keys the split form does not serve (a value that is not finite, or sizes
@@ -252,6 +252,15 @@ __device__ __forceinline__ void split8(const float (&x)[8], h8 &hi, h8 &lo) {
     lo[e] = l[0], lo[e + 1] = l[1];
   }
 }
+__device__ __forceinline__ void split4(const float4 &x, float by, uint2 *hi, uint2 *lo) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  const f2 a = {x.x * by, x.y * by}, b = {x.z * by, x.w * by};
+  const h2 p = __builtin_convertvector(a, h2), q = __builtin_convertvector(b, h2);
+  const f2 r = {rest_lo(p, a[0]), rest_hi(p, a[1])}, s = {rest_lo(q, b[0]), rest_hi(q, b[1])};
+  *hi = make_uint2(__builtin_bit_cast(uint32_t, p), __builtin_bit_cast(uint32_t, q));
+  *lo = make_uint2(__builtin_bit_cast(uint32_t, __builtin_convertvector(r, h2)),
+                   __builtin_bit_cast(uint32_t, __builtin_convertvector(s, h2)));
+}
 __device__ __forceinline__ h8 split8(const float (&x)[8], float by, uint4 *hi, uint4 *lo) {
   float y[8];
 #pragma unroll
@@ -263,42 +272,77 @@ __device__ __forceinline__ h8 split8(const float (&x)[8], float by, uint4 *hi, u
   return h;
 }
 
-// A lane's part of K fragment f of a stage, 8 dimensions of one key, and of V fragment
-// f = NB i + db, 8 keys of one dimension.  Keys behind the sequence's last one repeat it:
-// no query sees them.  So do dimensions behind a row's last one: q is 0 there, and O's are
-// not stored.  The lane's place in the fragment is a 32-bit offset (the caller sees to
-// strides below 2^23), so that a whole stage costs no address arithmetic.
+// A wave's part of the making of a stage by four waves.  K: the eight keys from 8 w on,
+// whole rows, four dimensions to a lane and 32 (128 bytes of a row) to a piece, so that a load
+// takes whole cache lines; eight lanes share a key.  V: fragments f = NB i + db, 8 keys of one
+// dimension to a lane.  Keys behind the sequence's last one repeat it: no query sees
+// them.  So do dimensions behind a row's last one: q is 0 there, and O's are not stored.
+// The lane's place in the stage is a 32-bit offset (the caller sees to strides below
+// 2^23), so that a whole stage costs no address arithmetic.
 __device__ __forceinline__ int v_key(int i, int h, int e) { return 16 * i + 8 * (e >> 2) + 4 * h + (e & 3); }
+// The smallest head_size that NB serves.
+constexpr int least_head(int nb) { return nb <= 4 ? 32 * nb - 31 : 32 * nb - 63; }
 template <int NB, bool VEC>
-struct Part {
-  uint32_t kd[2], vd, ko, vo;  // bytes
+struct KPart {
+  int key, d;         // of the lane
+  uint32_t ko;        // bytes
+  uint32_t at;        // in a stage, bytes: of piece 0's hi
+  __device__ __forceinline__ void init(const PackedArgs &a, int wave) {
+    const int lane = threadIdx.x & 63, c = lane & 7;
+    key = 8 * wave + (lane >> 3);
+    d = 4 * c;
+    ko = (uint32_t)key * (4u * (uint32_t)a.k_row);
+    at = (uint32_t)((2 * (c >> 2)) * 1024 + (32 * (c >> 1 & 1) + key) * 16 + 8 * (c & 1));
+  }
+  // kp: the stage's first key; last: its last key's number in the stage
+  __device__ __forceinline__ void load(const PackedArgs &a, const float *kp, int last, float4 (&k)[NB]) const {
+    const uint32_t row = last >= kStageKeys - 1 ? ko : (uint32_t)min(key, last) * (4u * (uint32_t)a.k_row);
+    const char *kb = (const char *)kp;
+#pragma unroll
+    for (int p = 0; p < NB; p++) {
+      const bool sure = 32 * p + 32 <= least_head(NB);
+      const uint32_t end = 4u * (uint32_t)(a.hs - (VEC ? 4 : 1)), x = 4u * (uint32_t)d + 128u * p;
+      if (VEC) {
+        k[p] = *(const float4 *)(kb + (row + (sure ? x : min(x, end))));
+      } else {
+        k[p].x = *(const float *)(kb + (row + min(x, end)));
+        k[p].y = *(const float *)(kb + (row + min(x + 4, end)));
+        k[p].z = *(const float *)(kb + (row + min(x + 8, end)));
+        k[p].w = *(const float *)(kb + (row + min(x + 12, end)));
+      }
+    }
+  }
+  // The key's largest magnitude, its bits, in all of its lanes.
+  __device__ __forceinline__ static uint32_t top(const float4 (&k)[NB]) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int p = 0; p < NB; p++)
+      t = max(t, max(max(bits_of(k[p].x), bits_of(k[p].y)), max(bits_of(k[p].z), bits_of(k[p].w))));
+    const auto both = [](uint32_t x, float y) { return max(x, __float_as_uint(y)); };
+    t = both(t, dpp_mov<kDppXor1>(__uint_as_float(t)));
+    t = both(t, dpp_mov<kDppXor2>(__uint_as_float(t)));
+    return both(t, dpp_mov<kDppHalfMirror>(__uint_as_float(t)));
+  }
+  __device__ __forceinline__ void split(const float4 &k, int p, float by, void *stage) const {
+    uint2 hi, lo;
+    split4(k, by, &hi, &lo);
+    char *dst = (char *)stage + (at + 4096u * p);
+    *(uint2 *)dst = hi;
+    *(uint2 *)(dst + 1024) = lo;
+  }
+};
+template <int NB>
+struct VPart {
+  uint32_t vd, vo;  // bytes
   __device__ __forceinline__ void init(const PackedArgs &a, int f) {
-    const int lane = threadIdx.x & 63, h = lane >> 5, d = 16 * f + 8 * h;
-    kd[0] = 4u * (uint32_t)min(d, VEC ? a.hs - 4 : a.hs - 1);
-    kd[1] = 4u * (uint32_t)min(d + 4, VEC ? a.hs - 4 : a.hs - 1);
+    const int lane = threadIdx.x & 63, h = lane >> 5;
     vd = 4u * (uint32_t)min(32 * (f % NB) + (lane & 31), a.hs - 1);
-    ko = (uint32_t)(lane & 31) * (4u * (uint32_t)a.k_row);
     vo = (uint32_t)(4 * h) * (4u * (uint32_t)a.v_row) + vd;
   }
-  // kp, vp: the stage's first key; last: its last key's number in the stage
-  __device__ __forceinline__ void load(const PackedArgs &a, const float *kp, const float *vp, int last,
-                                       int f, float (&k)[8], float (&v)[8]) const {
+  __device__ __forceinline__ void load(const PackedArgs &a, const float *vp, int last, int f, float (&v)[8]) const {
     const int lane = threadIdx.x & 63, h = lane >> 5, i = f / NB;
-    const char *kb = (const char *)kp, *vb = (const char *)vp;
-    const bool whole = last >= kStageKeys - 1;
-    const uint32_t row = whole ? ko : (uint32_t)min(lane & 31, last) * (4u * (uint32_t)a.k_row);
-    if (VEC) {
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const float4 x = *(const float4 *)(kb + (row + kd[e]));
-        k[4 * e] = x.x, k[4 * e + 1] = x.y, k[4 * e + 2] = x.z, k[4 * e + 3] = x.w;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        k[e] = *(const float *)(kb + (row + min(kd[e >> 2] + 4u * (e & 3), 4u * (uint32_t)(a.hs - 1))));
-    }
-    if (whole) {
+    const char *vb = (const char *)vp;
+    if (last >= kStageKeys - 1) {
       const char *vi = vb + (int64_t)(16 * i) * (4 * a.v_row);
 #pragma unroll
       for (int e = 0; e < 8; e++) v[e] = *(const float *)(vi + (int64_t)v_key(0, 0, e) * (4 * a.v_row) + vo);
@@ -350,7 +394,7 @@ __device__ __forceinline__ uint32_t top_keys(h8 hi) {
 
 // One stage.  NB: 32-dimension blocks of a head.
 template <int NB, bool VEC>
-__global__ void __launch_bounds__(256) attn_split_k(const F16Args a) {
+__global__ void __launch_bounds__(256) attn_stages_k(const F16Args a) {
   __shared__ uint32_t key_s[2][32];  // each key's largest magnitude: K, V
   const PackedArgs &p = a.p;
   const int slot = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -359,28 +403,29 @@ __global__ void __launch_bounds__(256) attn_split_k(const F16Args a) {
   const int key0 = kStageKeys * (slot - (z.kb / kStageKeys + s));
   if (key0 < 0 || key0 >= z.nk) return;
   const int last = z.nk - 1 - key0;
-  if (tid < 64) key_s[tid >> 5][tid & 31] = 0;
+  if (tid < 32) key_s[1][tid] = 0;
   __syncthreads();
   const float *kp = p.k + (int64_t)(z.kb + key0) * p.k_row + hk * p.k_head;
   const float *vp = p.v + (int64_t)(z.kb + key0) * p.v_row + hk * p.v_head;
   constexpr int CH = (2 * NB + 3) / 4;
-  float k[CH][8], v[CH][8];
+  float4 k[NB];
+  float v[CH][8];
+  KPart<NB, VEC> kpart;
+  kpart.init(p, wave);
+  kpart.load(p, kp, last, k);
 #pragma unroll
   for (int c = 0; c < CH; c++) {
     const int f = wave + 4 * c;
     if (f >= 2 * NB) break;
-    Part<NB, VEC> part;
-    part.init(p, f);
-    part.load(p, kp, vp, last, f, k[c], v[c]);
+    VPart<NB> vpart;
+    vpart.init(p, f);
+    vpart.load(p, vp, last, f, v[c]);
   }
+  key_s[0][kpart.key] = kpart.top(k);
 #pragma unroll
   for (int c = 0; c < CH; c++) {
     const int f = wave + 4 * c;
     if (f >= 2 * NB) break;
-    uint32_t t = 0;
-#pragma unroll
-    for (int e = 0; e < 8; e++) t = max(t, bits_of(k[c][e]));
-    atomicMax(&key_s[0][lane & 31], t);
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       uint32_t u = bits_of(v[c][e]);  // over the 32 lanes of a key
@@ -406,10 +451,11 @@ __global__ void __launch_bounds__(256) attn_split_k(const F16Args a) {
   }
   uint4 *out = a.frags + ((int64_t)slot * a.hk + hk) * (NB * 8 * 64);
 #pragma unroll
+  for (int i = 0; i < NB; i++) kpart.split(k[i], i, power(ek), out);
+#pragma unroll
   for (int c = 0; c < CH; c++) {
     const int f = wave + 4 * c;
     if (f >= 2 * NB) break;
-    split8(k[c], power(ek), out + (2 * f) * 64 + lane, out + (2 * f + 1) * 64 + lane);
     split8(v[c], power(ev), out + (4 * NB + 2 * f) * 64 + lane, out + (4 * NB + 2 * f + 1) * 64 + lane);
   }
 }
@@ -433,18 +479,39 @@ __device__ __forceinline__ Unit unit_of(const PackedArgs &a, int block, int wave
 
 // One stage of one wave: S^T, weights and O^T.  f: what turns a product sum into a power
 // of two; er: V's scaling over O's, a power 2^er <= 1; all: the last key that every
-// query of the wave sees.
-template <int NB>
+// query of the wave sees.  beside(ds): a part of other work, which goes between the
+// products of S^T; behind: what follows them.
+template <int NB, bool MADE, class Beside, class Behind>
 __device__ __forceinline__ void stage(const h8 *frag, const h8 (&qh)[2 * NB], const h8 (&ql)[2 * NB],
                                       float f, int key0, int my, int all, int h, int er,
-                                      v16f (&o)[NB], float &m, float &l) {
+                                      v16f (&o)[NB], float &m, float &l, Beside beside, Behind behind) {
   v16f s;
 #pragma unroll
   for (int r = 0; r < 16; r++) s[r] = 0.f;
   // Two fragments are read ahead of the products that use two others: under the other
   // waves' reads one alone comes later than three products take.
   constexpr int kReads = 0x100, kProducts = 0x008;
-  {
+  if constexpr (MADE) {
+    h8 k[3][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      k[i][0] = frag[(2 * i) * 64];
+      k[i][1] = frag[(2 * i + 1) * 64];
+    }
+#pragma unroll
+    for (int ds = 0; ds < 2 * NB; ds++) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (ds + 2 < 2 * NB) {
+        k[(ds + 2) % 3][0] = frag[(2 * ds + 4) * 64];
+        k[(ds + 2) % 3][1] = frag[(2 * ds + 5) * 64];
+      }
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[ds % 3][0], qh[ds], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[ds % 3][0], ql[ds], s, 0, 0, 0);
+      s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[ds % 3][1], qh[ds], s, 0, 0, 0);
+      beside(ds);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  } else {
     h8 k[2 * NB][2];
 #pragma unroll
     for (int ds = 0; ds < 2 * NB; ds++) {
@@ -464,6 +531,7 @@ __device__ __forceinline__ void stage(const h8 *frag, const h8 (&qh)[2 * NB], co
       __builtin_amdgcn_sched_group_barrier(kReads, 2, 0);
     }
   }
+  behind();
   if (key0 + kStageKeys - 1 > all) {  // some query does not see all of them
 #pragma unroll
     for (int r = 0; r < 16; r++)
@@ -537,7 +605,7 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
   static_assert(kFrags % NW == 0, "each wave fetches as many fragments");
   __shared__ uint4 ring[NS][kFrags * 64];
   __shared__ uint2 top_s[2][NW];
-  __shared__ uint32_t key_s[2][2][32];  // each key's largest of a made stage
+  __shared__ uint32_t key_s[3][2][32];  // each key's largest of a made stage
   const PackedArgs &a = args.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r32 = lane & 31, h = lane >> 5;
@@ -599,18 +667,65 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
       dma16(src + f * 64, dst + f * 1024);
     }
   };
-  float kx[CH][8], vx[CH][8];
-  Part<NB, VEC> part[CH];
-  if constexpr (!STORED)
+  // (some waves repeat the last fragment)
+  const auto frag_of = [&](int c) { return 2 * NB % NW ? min(wave + c * NW, 2 * NB - 1) : wave + c * NW; };
+  float4 kx[NB];
+  float vx[CH][8];
+  uint32_t key_top;
+  KPart<NB, VEC> kpart;
+  VPart<NB> vpart[CH];
+  if constexpr (!STORED) {
+    kpart.init(a, wave);
 #pragma unroll
-    for (int c = 0; c < CH; c++) part[c].init(a, wave + c * NW);
+    for (int c = 0; c < CH; c++) vpart[c].init(a, frag_of(c));
+  }
   auto load = [&](int st) {
     const int key0 = kStageKeys * st, last = z.nk - 1 - key0;
+    kpart.load(a, kp + (int64_t)key0 * a.k_row, last, kx);
+#pragma unroll
+    for (int c = 0; c < CH; c++) vpart[c].load(a, vp + (int64_t)key0 * a.v_row, last, frag_of(c), vx[c]);
+  };
+  // What is loaded: its largest magnitudes, for all waves; then in its fragments, with
+  // the scalings 2^ek and 2^ev; then each key's largest, K's as it is, V's scaled.
+  auto post = [&](int at) {
+    uint32_t vt = 0;
+    key_top = kpart.top(kx);
+#pragma unroll
+    for (int c = 0; c < CH; c++) vt = max(vt, top8(vx[c]));
+    const uint32_t kt = wave_max_bits(key_top);
+    vt = wave_max_bits(vt);
+    if (lane == 0) top_s[at][wave] = make_uint2(kt, vt);
+  };
+  auto tops = [&](int at) {
+    uint2 t = top_s[at][0];
+#pragma unroll
+    for (int i = 1; i < NW; i++) {
+      t.x = max(t.x, top_s[at][i].x);
+      t.y = max(t.y, top_s[at][i].y);
+    }
+    t.x = __builtin_amdgcn_readfirstlane(t.x);
+    t.y = __builtin_amdgcn_readfirstlane(t.y);
+    return t;
+  };
+  h8 v_hi[CH];
+  auto make = [&](uint4 *dst, uint2 t, int part) {  // part: of 2 NB
+    if (part % 2 == 0) {
+      kpart.split(kx[part / 2], part / 2, power(lift(t.x)), dst);
+    } else if (part / 2 < CH) {
+      const int c = part / 2, f = frag_of(c);
+      v_hi[c] = split8(vx[c], power(lift(t.y)), dst + (4 * NB + 2 * f) * 64 + lane, dst + (4 * NB + 2 * f + 1) * 64 + lane);
+    }
+  };
+  auto key_tops = [&](int at) {
+    key_s[at][0][kpart.key] = key_top;
 #pragma unroll
     for (int c = 0; c < CH; c++) {
-      const int f = wave + c * NW;
-      if (2 * NB % NW != 0 && f >= 2 * NB) break;
-      part[c].load(a, kp + (int64_t)key0 * a.k_row, vp + (int64_t)key0 * a.v_row, last, f, kx[c], vx[c]);
+      const uint32_t t = top_keys(v_hi[c]);
+      if ((r32 & ~3) == 0) {  // keys 2 (lane & 3) and the next of the half's eight
+        uint32_t *key = &key_s[at][1][v_key(frag_of(c) / NB, h, 2 * (lane & 3))];
+        atomicMax(key, t & 0xffffu);
+        atomicMax(key + 1, t >> 16);
+      }
     }
   };
   if constexpr (STORED) {
@@ -619,7 +734,7 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
       if (!odd && st0 + i < st1) fetch(st0 + i);
   } else if (st0 < st1) {
     load(st0);
-    if (threadIdx.x < 64) key_s[0][h][r32] = 0;  // seen by all behind the first barrier
+    if (threadIdx.x < 32) key_s[0][1][r32] = key_s[1][1][r32] = 0;
   }
 
   h8 qh[2 * NB], ql[2 * NB];
@@ -672,54 +787,30 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
       if (kStageKeys * st > wend) continue;  // nothing here is seen by this wave
       const float kinv = uniform[4 * st], vinv = uniform[4 * st + 1];
       const int er = vinv > 0.f ? (__float_as_int(vinv) >> 23) - 127 - unit : 0;
-      stage<NB>((const h8 *)ring[(st - st0) % NS] + lane, qh, ql, qf * kinv, kStageKeys * st, my, all,
-                h, er, o, m, l);
+      stage<NB, false>((const h8 *)ring[(st - st0) % NS] + lane, qh, ql, qf * kinv, kStageKeys * st, my, all,
+                   h, er, o, m, l, [](int) {}, [] {});
     }
-  } else {
-    for (int st = st0; st < st1; st++) {
-      const int at = (st - st0) & 1;
-      uint32_t kt = 0, vt = 0, key_top[CH];
+  } else if (st0 < st1) {
+    // While a stage is used the next one is made, between the products, and the one
+    // behind that is loaded: one barrier a stage.
+    post(0);
+    lds_barrier();
+    uint2 top = tops(0);
 #pragma unroll
-      for (int c = 0; c < CH; c++) {
-        if (2 * NB % NW != 0 && wave + c * NW >= 2 * NB) break;
-        key_top[c] = top8(kx[c]);
-        kt = max(kt, key_top[c]);
-        vt = max(vt, top8(vx[c]));
-      }
-      kt = wave_max_bits(kt);
-      vt = wave_max_bits(vt);
-      if (lane == 0) top_s[at][wave] = make_uint2(kt, vt);
-      lds_barrier();  // also: every wave is done with this slot's stage before the last
-#pragma unroll
-      for (int i = 0; i < NW; i++) {
-        kt = max(kt, top_s[at][i].x);
-        vt = max(vt, top_s[at][i].y);
-      }
-      kt = __builtin_amdgcn_readfirstlane(kt);
-      vt = __builtin_amdgcn_readfirstlane(vt);
-      const int ek = lift(kt), ev = lift(vt);
+    for (int i = 0; i < 2 * NB; i++) make(ring[0], top, i);
+    key_tops(0);
+    if (st0 + 1 < st1) {
+      load(st0 + 1);
+      post(1);
+    }
+    for (int st = st0, slot = 0; st < st1; st++) {
+      const int at = (st - st0) & 1, slot1 = slot == 2 ? 0 : slot + 1, slot2 = slot1 == 2 ? 0 : slot1 + 1;
+      lds_barrier();  // this stage and the sizes of the next are there, the last one's slot is free
+      const uint2 next = tops(at ^ 1);
+      const uint32_t kt = top.x, vt = top.y;
       odd |= max(kt, vt) >= 0x7f800000u;
-      // each key's largest: K's as it is, V's scaled
-#pragma unroll
-      for (int c = 0; c < CH; c++) {
-        const int f = wave + c * NW;
-        if (2 * NB % NW != 0 && f >= 2 * NB) break;
-        uint4 *dst = ring[at];
-        split8(kx[c], power(ek), dst + (2 * f) * 64 + lane, dst + (2 * f + 1) * 64 + lane);
-        const h8 hi = split8(vx[c], power(ev), dst + (4 * NB + 2 * f) * 64 + lane, dst + (4 * NB + 2 * f + 1) * 64 + lane);
-        atomicMax(&key_s[at][0][r32], key_top[c]);
-        const uint32_t t = top_keys(hi);
-        if ((r32 & ~3) == 0) {  // keys 2 (lane & 3) and the next of the half's eight
-          uint32_t *key = &key_s[at][1][v_key(f / NB, h, 2 * (lane & 3))];
-          atomicMax(key, t & 0xffffu);
-          atomicMax(key + 1, t >> 16);
-        }
-      }
-      if (threadIdx.x < 64) key_s[at ^ 1][h][r32] = 0;  // for the next stage
-      if (st + 1 < st1) load(st + 1);
-      lds_barrier();
       {  // far below the largest, and not 0; V is scaled to 2^14, and 0x3c00 is f16's 1
-        const uint32_t x = key_s[at][0][r32], y = key_s[at][1][r32];
+        const uint32_t x = key_s[slot][0][r32], y = key_s[slot][1][r32];
         bool low = (x && x + (kSpread << 23) < kt) || (y && y < 0x3c00u);
         if (vt && __any(y == 0)) {  // zeros, or what f16 has no number for
           const float *v = vp + (int64_t)min(kStageKeys * st + r32, z.nk - 1) * a.v_row;
@@ -727,7 +818,7 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
         }
         odd |= __any(low);
       }
-      const int e = vt ? -ev : unit;  // a stage of zeros has no size
+      const int e = vt ? -lift(vt) : unit;  // a stage of zeros has no size
       if (e > unit) {
         if (unit > -1000) {
           const float down = ldexpf(1.f, unit - e);
@@ -740,9 +831,17 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
       }
       const int er = e - unit;  // (-1000 less itself where V has been 0 so far)
       odd |= er < -kSpread;
-      if (kStageKeys * st > wend) continue;  // nothing here is seen by this wave
-      stage<NB>((const h8 *)ring[at] + lane, qh, ql, qf * power(-ek), kStageKeys * st, my, all, h,
-                max(er, -kSpread), o, m, l);
+      // (waves that see nothing of the stage have weights of 0; behind the last stage it is made again)
+      stage<NB, true>((const h8 *)ring[at] + lane, qh, ql, qf * power(-lift(kt)), kStageKeys * st, my, all, h,
+                    max(er, -kSpread), o, m, l, [&](int i) { make(ring[at ^ 1], next, i); },
+                    [&] {
+                      key_tops(slot1);
+                      if (threadIdx.x < 32) key_s[slot2][1][r32] = 0;  // for the stage behind the next
+                      if (st + 2 < st1) load(st + 2);
+                    });
+      if (st + 2 < st1) post(at);
+      top = next;
+      slot = slot1;
     }
   }
   const int64_t part_row = ((int64_t)split * a.tq + z.qb) * (args.hk * a.group) + un.head;
@@ -866,7 +965,7 @@ template <int NB, int NW, int NS, bool VEC, bool STORED>
 void launch_f16(const F16Args &a, hipStream_t st) {
   const int heads = a.hk * a.p.group;
   if (STORED)
-    hipLaunchKernelGGL((attn_split_k<NB, VEC>), dim3((unsigned)a.slots, (unsigned)a.hk), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((attn_stages_k<NB, VEC>), dim3((unsigned)a.slots, (unsigned)a.hk), dim3(256), 0, st, a);
   hipLaunchKernelGGL((attn_f16_k<NB, NW, NS, VEC, STORED>), dim3((unsigned)(a.blocks * a.hk), (unsigned)a.splits),
                      dim3(64 * NW), 0, st, a);
   if (a.splits > 1)
@@ -879,7 +978,7 @@ int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
   F16Args a{};
   a.p = p;
   a.hk = heads / p.group;
-  // attn_split_k and its traffic pay where about 24 blocks of four waves or more would
+  // attn_stages_k and its traffic pay where about 24 blocks of four waves or more would
   // make each stage: 1024 tokens of 32 heads over 8, 128 wide (32 blocks) 67 us against 80,
   // 4096 (128) 380 against 560; 512 (16) 48 against 40, 2048 of 16 over 16, 64 wide (16) 67
   // against 65.
