@@ -40,6 +40,29 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
   return (int)fminf(fmaxf(a > half || (a == half && odd) ? to : n, -127.f), 127.f);
 }
 
+// The codes of four numbers, in bytes.  The sum of x inv with 1.5 2^23 has the nearest
+// whole number in its low bits, and x inv is within 127 2^-24 of the quotient: only
+// where it comes that close to the middle of two codes does the exact way decide.
+__device__ __forceinline__ uint32_t codes4(const float4 &x, float s, float inv) {
+  constexpr float kShift = 12582912.f;
+  const float a = fmaf(x.x, inv, kShift), b = fmaf(x.y, inv, kShift);
+  const float c = fmaf(x.z, inv, kShift), d = fmaf(x.w, inv, kShift);
+  const float off = fmaxf(fmaxf(fabsf(fmaf(x.x, inv, kShift - a)), fabsf(fmaf(x.y, inv, kShift - b))),
+                          fmaxf(fabsf(fmaf(x.z, inv, kShift - c)), fabsf(fmaf(x.w, inv, kShift - d))));
+  uint32_t r[4] = {__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d)};
+  if (off > 0.4999f) {
+    r[0] = (uint32_t)code_of(x.x, s, inv);
+    r[1] = (uint32_t)code_of(x.y, s, inv);
+    r[2] = (uint32_t)code_of(x.z, s, inv);
+    r[3] = (uint32_t)code_of(x.w, s, inv);
+  }
+  return perm(perm(r[3], r[2], 0x0c0c0400), perm(r[1], r[0], 0x0c0c0400), 0x05040100);
+}
+
+// i / n by way of per = ceil(2^20 / n): exact for i < 4096 n (n up to 64).
+inline uint32_t per_of(int64_t n) { return (uint32_t)cdiv(int64_t(1) << 20, n); }
+__device__ __forceinline__ int over(int i, uint32_t per) { return (int)((uint32_t)i * per >> 20); }
+
 // Four codes times ratio <= 1 (a NaN never: the caller clears those), rounded to the
 // nearest, ties to even: the sum with 1.5 2^52 has the rounded number in its low bits.
 __device__ __forceinline__ uint32_t rescale4(uint32_t c, double ratio) {
@@ -65,6 +88,7 @@ struct AppendArgs {
   const int *starts, *lengths;
   int64_t k_row, k_head, v_row, v_head;
   int rows;
+  uint32_t per;  // of head_size / 4
 };
 
 constexpr int kAppendChunks = 8;
@@ -100,7 +124,7 @@ __global__ void __launch_bounds__(THREADS) kv8_append_k(const AppendArgs a) {
     const int e = tid + i * THREADS;
     v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (e < nw) {
-      const int r = e / quads;
+      const int r = over(e, a.per);
       const float *p = x + r * row + 4 * (e - r * quads);
       if (VEC) v[i] = *(const float4 *)p;
       else v[i] = make_float4(p[0], p[1], p[2], p[3]);
@@ -124,25 +148,26 @@ __global__ void __launch_bounds__(THREADS) kv8_append_k(const AppendArgs a) {
   if (old && !(before == s)) {  // what the block held, to the new scale
     const double ratio = live ? (double)before / (double)s : 0.0;
     for (int e = tid; e < old * quads; e += THREADS) {
-      const int r = e / quads;
+      const int r = over(e, a.per);
       uint32_t *p = (uint32_t *)(codes + r * c.st_token + 4 * (e - r * quads));
       *p = live ? rescale4(*p, ratio) : 0u;
     }
   }
   const float inv = live ? 1.f / s : 0.f;
-  const bool tiny = s < 1e-37f;  // 1 / s may be infinite or coarse
+  const bool tiny = live && s < 1e-37f;  // 1 / s may be infinite or coarse
 #pragma unroll
   for (int i = 0; i < kAppendChunks; i++) {
     const int e = tid + i * THREADS;
     if (e < nw) {
-      const int r = e / quads;
-      const float y[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      const int r = over(e, a.per);
       uint32_t q = 0;
-      if (live) {
+      if (tiny) {
+        const float y[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
         for (int w = 0; w < 4; w++)
-          q |= (uint32_t)(uint8_t)(int8_t)(tiny ? (int)fmin(fmax(rint((double)y[w] / (double)s), -127.0), 127.0)
-                                                : code_of(y[w], s, inv)) << (8 * w);
+          q |= (uint32_t)(uint8_t)(int8_t)(int)fmin(fmax(rint((double)y[w] / (double)s), -127.0), 127.0) << (8 * w);
+      } else if (live) {
+        q = codes4(v[i], s, inv);
       }
       *(uint32_t *)(codes + (old + r) * c.st_token + 4 * (e - r * quads)) = q;
     }
@@ -673,6 +698,7 @@ struct EvictArgs {
   int *kept;
   int64_t se_seq, se_head, ns_seq, ns_head, kp_seq, kp_head;
   int budget, recent;
+  uint32_t per;  // of the words of a row that kv8_move_k takes at a time
 };
 
 // Unsigned order of the weights: NaN above all, both zeros alike.
@@ -873,7 +899,7 @@ __global__ void __launch_bounds__(256) kv8_move_k(const EvictArgs a) {
 #pragma unroll 2
   for (int e = tid; e < 2 * n; e += 256) {
     const bool v = e >= n;
-    const int f = v ? e - n : e, r = f / parts, d = 4 * W * (f - r * parts);
+    const int f = v ? e - n : e, r = over(f, a.per), d = 4 * W * (f - r * parts);
     uint32_t x[W];
     __builtin_memcpy(x, __builtin_assume_aligned((v ? c.v : c.k) + at[r] + d, 4 * W), 4 * W);
     const double q = ratio[v][r];
@@ -1031,7 +1057,7 @@ int32_t simp_rt_kv8_append(
       (rc = bind_here(ol, lengths + len_off, 4 * (size_t)len_size, Operand::kIn, dev, "lengths")))
     return rc;
   const AppendArgs a{bc.c, (const float *)ok.dev(), (const float *)ov.dev(), (const int *)os.dev(),
-                     (const int *)ol.dev(), k_st0, k_st1, v_st0, v_st1, (int)k_s0};
+                     (const int *)ol.dev(), k_st0, k_st1, v_st0, v_st1, (int)k_s0, per_of(bc.c.hs / 4)};
   const dim3 grid((unsigned)slots, (unsigned)bc.c.hk, 2);
   const bool vec = ((k_st0 | k_st1 | v_st0 | v_st1) & 3) == 0 && (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0;
   const int64_t chunks = (int64_t)cache->block * bc.c.hs / 4;  // of a whole block
@@ -1263,16 +1289,18 @@ int32_t simp_rt_kv8_evict(
       (rc = bind_here(on, dn.data(), dn.bytes(), Operand::kOut, dev, "new_seen")) ||
       (rc = bind_here(op, dp.data(), dp.bytes(), Operand::kOut, dev, "kept")))
     return rc;
-  const EvictArgs a{bc.c, bt.c, (const int *)ol.dev(), (const float *)os.dev(), (float *)on.dev(),
+  EvictArgs a{bc.c, bt.c, (const int *)ol.dev(), (const float *)os.dev(), (float *)on.dev(),
                     (int *)op.dev(), se_st0, se_st1, ns_st0, ns_st1, kept_st0, kept_st1,
-                    (int)budget, (int)recent};
+                    (int)budget, (int)recent, 0};
   hipStream_t st = cur_stream();
   hipLaunchKernelGGL(kv8_select_k, dim3((unsigned)bc.c.hk, (unsigned)bc.c.n), dim3(1024), 0, st, a);
   const dim3 grid((unsigned)cdiv(budget, to->block), (unsigned)bc.c.hk, (unsigned)bc.c.n);
   auto wide = [](const Cache &c) {
     return ((c.hs | c.st_seq | c.st_head | c.st_token | (int64_t)(uintptr_t)c.k | (int64_t)(uintptr_t)c.v) & 15) == 0;
   };
-  if (wide(bc.c) && wide(bt.c)) hipLaunchKernelGGL(kv8_move_k<4>, grid, dim3(256), 0, st, a);
+  const bool quads = wide(bc.c) && wide(bt.c);
+  a.per = per_of(bc.c.hs / (quads ? 16 : 4));
+  if (quads) hipLaunchKernelGGL(kv8_move_k<4>, grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL(kv8_move_k<1>, grid, dim3(256), 0, st, a);
   Operand *ops[] = {&ol, &os, &on, &op};
   return finish(ops, 4);
