@@ -268,12 +268,13 @@ __global__ void __launch_bounds__(256) kv8_read_k(const ReadArgs a) {
 // Weights: p = 2^(s - m) of the tile's own maximum m, times the V block's scale over the
 // tile's largest; the integer's unit is the largest of these products / 8.35e6, so
 // that each tile keeps 24 bits of what it contributes, whatever the scales.
-// A block of four waves takes `chunk` tokens of one kv head, its tiles in turn; the
+// A block of four waves takes a piece of one kv head's tokens, its tiles in turn; the
 // rest of a row's softmax is joined by kv8_join_k.
 // 131072 tokens of 8 heads, 128 wide: 57 us for 268 MB of codes, 4.7 TB/s, and 17 MB of scores.
-// 16 sequences of 1 to 4096 tokens: 19.8 us for 60 MB, 3.0 TB/s: the longest sequences'
-// blocks run on when the others are done, and shorter ones cost more than they even out.
-// Eight waves to a block: 24.2 us.
+// 16 sequences of 1 to 4096 tokens: 16 us for 57 MB, 3.6 TB/s (19.6 with pieces of one length
+// for each sequence's place in the grid, whose empty blocks leave CUs with two full
+// ones next to idle ones; 26 with exactly equal shares, which span sequences); half of it is the
+// latency of lengths, q and the first tile, and of the join of the waves.
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
@@ -287,12 +288,102 @@ struct AttnArgs {
   int64_t q_seq, q_head, o_seq, o_head, si_seq, si_head, so_seq, so_head;
   int heads, group;
   int sets, width;    // sets of up to `width` (at most 16) query heads of a kv head
-  int chunk, splits;  // tokens a block takes; blocks for a full sequence
+  int blocks;         // that full pieces should come to
   float scale;        // times log2(e): the scores are powers of two
   float *scores;      // [n, heads, score_row], or null
   int64_t score_row;  // the capacity in whole tiles of 64
-  float *part;        // [n, heads, splits, head_size], unnormalised
-  float2 *stat;       // [n, heads, splits]: maximum and sum
+  float *part;        // [units' first pieces, width, pieces of a unit, head_size], unnormalised
+  float2 *stat;       // the same without head_size: maximum and sum
+  int *starts;        // [n + 1]: pieces of a unit in the sequences before
+};
+
+// Sums of whole numbers over the wave, and running sums over its lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+  const int lane = threadIdx.x & 63;
+  // within rows of 16 lanes (lanes without a neighbour add 0), then the rows before
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  const int a = __builtin_amdgcn_readlane(x, 15), b = __builtin_amdgcn_readlane(x, 31), c = __builtin_amdgcn_readlane(x, 47);
+  return x + (lane < 16 ? 0 : lane < 32 ? a : lane < 48 ? a + b : a + b + c);
+}
+__device__ __forceinline__ int wave_total(int scanned) { return __builtin_amdgcn_readlane(scanned, 63); }
+
+// The work: rounds of 256 tokens (a tile for each wave).  A piece is up to `share` rounds of
+// one unit (a set of the query heads of a kv head, of one sequence), with a share that makes
+// about `blocks` pieces of all, whatever the lengths.  Pieces follow each other sequence after sequence, and in a sequence
+// unit after unit; block i has piece i.
+constexpr int kRound = 256;
+struct Work {
+  const int *lengths;
+  int n, cap, units;  // units: of a sequence
+  int m, share, upto; // a lane has m sequences; pieces of a unit of its and the lanes' before
+
+  __device__ __forceinline__ int rounds_of(int b) const {
+    return b < n ? (clampi(lengths[b], 0, cap) + kRound - 1) / kRound : 0;
+  }
+  __device__ __forceinline__ int pieces_of(int b) const { return (rounds_of(b) + share - 1) / share; }
+  __device__ __forceinline__ void init(const AttnArgs &a) {
+    lengths = a.lengths, n = a.c.n, cap = a.c.cap, units = a.c.hk * a.sets;
+    m = (n + 63) >> 6;
+    const int lane = threadIdx.x & 63;
+    int sum = 0;
+    if (m == 1) sum = rounds_of(lane);
+    else
+      for (int i = 0; i < m; i++) sum += rounds_of(lane * m + i);
+    share = max((wave_total(wave_scan(sum)) * units + a.blocks - 1) / a.blocks, 1);
+    if (m == 1) sum = (sum + share - 1) / share;
+    else {
+      sum = 0;
+      for (int i = 0; i < m; i++) sum += pieces_of(lane * m + i);
+    }
+    upto = wave_scan(sum);
+  }
+  // For kv8_join_k: the pieces of a unit in the sequences before each, and in all.
+  __device__ __forceinline__ void store(int *starts) const {
+    const int lane = threadIdx.x;
+    int sum = upto;
+    if (m == 1) {
+      if (lane < n) starts[lane + 1] = sum;
+    } else {
+      for (int b = min((lane + 1) * m, n) - 1; b >= lane * m; b--) {
+        starts[b + 1] = sum;
+        sum -= pieces_of(b);
+      }
+    }
+    if (lane == 0) starts[0] = 0;
+  }
+  // The sequence of piece x, its unit, the place among the unit's and their count; false:
+  // there is none.
+  __device__ __forceinline__ bool find(int x, int &b, int &unit, int &place, int &count) const {
+    const int lane = threadIdx.x & 63;
+    const unsigned long long who = __ballot(upto > x / units);
+    if (!who) return false;
+    const int l = __ffsll(who) - 1;
+    int sum = l ? __builtin_amdgcn_readlane(upto, l - 1) : 0;
+    if (m == 1) {
+      b = l;
+      count = __builtin_amdgcn_readlane(upto, l) - sum;
+    } else {
+      for (int s0 = l * m;; s0 += 64) {
+        const int p = s0 + lane < (l + 1) * m ? pieces_of(s0 + lane) : 0, to = wave_scan(p);
+        const unsigned long long there = __ballot(sum + to > x / units);
+        if (there) {
+          const int k = __ffsll(there) - 1;
+          b = s0 + k;
+          count = __builtin_amdgcn_readlane(p, k);
+          sum += __builtin_amdgcn_readlane(to, k) - count;
+          break;
+        }
+        sum += wave_total(to);
+      }
+    }
+    const int y = x - sum * units;
+    unit = y / count;
+    place = y - unit * count;
+    return true;
+  }
 };
 
 constexpr float kUnit = 8.35e6f;        // v + 0x808080 stays below 2^24 and above 0
@@ -347,7 +438,6 @@ __device__ __forceinline__ float quad_add(float v) {
 // columns with byte i % 4 of head i / 4 (the fourth of them nothing), so that one
 // product does what three do with the bytes apart, one byte plane is kept instead of
 // three, and a sum over the quad joins them; else up to 16 heads, a column each.
-// blockIdx: chunk of tokens, kv head and set of its query heads, sequence.
 template <int NC, bool QUAD>
 __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 && QUAD ? 3 : NC < 4 ? 2 : 1)
     kv8_attn_k(const AttnArgs a) {
@@ -357,13 +447,15 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 && QUAD ? 3 : NC < 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i16 = lane & 15, g = lane >> 4, hs = c.hs;
   const int head = QUAD ? i16 >> 2 : i16, byte = QUAD ? i16 & 3 : 0;  // of the lane's column
-  const int hk = blockIdx.y / a.sets, set0 = ((int)blockIdx.y - hk * a.sets) * a.width;
+  Work work;
+  work.init(a);
+  if (blockIdx.x == 0 && threadIdx.x < 64) work.store(a.starts);
+  int b, unit, place, count;
+  if (!work.find((int)blockIdx.x, b, unit, place, count)) return;
+  const int hk = unit / a.sets, set0 = (unit - hk * a.sets) * a.width;
   const int cols = min(a.width, a.group - set0), h0 = hk * a.group + set0;  // query heads h0 ..
-  const int b = blockIdx.z;
-  const int len = clampi(a.lengths[b], 0, c.cap);
-  const int from = blockIdx.x * a.chunk;
-  if (from >= len) return;
-  const int to = len - from < a.chunk ? len : from + a.chunk;
+  const int len = clampi(a.lengths[b], 0, c.cap), chunk = work.share * kRound;
+  const int from = place * chunk, to = len - from < chunk ? len : from + chunk;
   const int8_t *kp = c.k + b * c.st_seq + hk * c.st_head;
   const int8_t *vp = c.v + b * c.st_seq + hk * c.st_head;
   const float *ksp = c.ks + b * c.sc_seq + hk * c.sc_head, *vsp = c.vs + b * c.sc_seq + hk * c.sc_head;
@@ -603,7 +695,7 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 && QUAD ? 3 : NC < 
       x.z = fmaf(f, y.z, x.z);
       x.w = fmaf(f, y.w, x.w);
     }
-    const int64_t at = ((int64_t)b * a.heads + h0 + col) * a.splits + blockIdx.x;
+    const int64_t at = ((int64_t)blockIdx.x - place) * a.width + (int64_t)col * count + place;
     *(float4 *)(a.part + at * hs + d) = x;
     if (d == 0) a.stat[at] = make_float2(M, sum);
   }
@@ -623,7 +715,14 @@ __global__ void __launch_bounds__(256) kv8_join_k(const AttnArgs a) {
   const Cache &c = a.c;
   const int hk = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int len = clampi(a.lengths[b], 0, c.cap);
-  const int ns = len ? (len - 1) / a.chunk + 1 : 0, hs = c.hs;
+  const auto *starts = (const __attribute__((address_space(4))) int *)a.starts;  // a scalar load
+  const int before = starts[b], ns = starts[b + 1] - before, hs = c.hs, wd = a.width;
+  const int64_t first = ((int64_t)before * c.hk * a.sets) + (int64_t)hk * a.sets * ns;
+  // A head's first row.
+  const auto row_of = [&](int g) {
+    const int set = g / wd;
+    return (first + (int64_t)set * ns) * wd + (int64_t)(g - set * wd) * ns;
+  };
   if ((int)blockIdx.x < a.group) {
     const int h = hk * a.group + blockIdx.x;
     float *out = a.out + b * a.o_seq + h * a.o_head;
@@ -631,8 +730,8 @@ __global__ void __launch_bounds__(256) kv8_join_k(const AttnArgs a) {
       for (int d = tid; d < hs; d += 256) out[d] = 0.f;
       return;
     }
-    const float2 *st = a.stat + ((int64_t)b * a.heads + h) * a.splits;
-    const float *part = a.part + ((int64_t)b * a.heads + h) * a.splits * hs;
+    const float2 *st = a.stat + row_of(blockIdx.x);
+    const float *part = a.part + row_of(blockIdx.x) * hs;
     float M = -INFINITY;
     for (int s = tid; s < ns; s += 256) M = fmaxf(M, st[s].x);
     M = wave_max_dpp(M);
@@ -643,9 +742,10 @@ __global__ void __launch_bounds__(256) kv8_join_k(const AttnArgs a) {
     const float mu = M == -INFINITY ? 0.f : M;
     float L = 0.f;
     for (int s = tid; s < ns; s += 256) {
-      const float f = pow2(st[s].x - mu);
+      const float2 ml = st[s];
+      const float f = pow2(ml.x - mu);
       lds[s] = f;
-      L = fmaf(f, st[s].y, L);
+      L = fmaf(f, ml.y, L);
     }
     L = wave_sum_dpp(L);
     if (lane == 0) sum_s[wave] = L;
@@ -677,7 +777,7 @@ __global__ void __launch_bounds__(256) kv8_join_k(const AttnArgs a) {
   const int t0 = ((int)blockIdx.x - a.group) * kSeenTile;
   if (t0 >= len) return;
   for (int g = wave; g < a.group; g += 4) {  // each head's maximum and 1 / sum
-    const float2 *st = a.stat + ((int64_t)b * a.heads + hk * a.group + g) * a.splits;
+    const float2 *st = a.stat + row_of(g);
     float M = -INFINITY, L = 0.f;
     for (int s = lane; s < ns; s += 64) M = fmaxf(M, st[s].x);
     M = wave_max_dpp(M);
@@ -1209,31 +1309,33 @@ int32_t simp_rt_kv8_attention(
   a.heads = (int)q_s1, a.group = (int)(q_s1 / cache->n_kv_heads);
   a.scale = (float)(scale * 1.4426950408889634);
   hipStream_t st = cur_stream();
-  // Four tiles of 64 tokens to a block, one per wave, and more where the full cache would
-  // have more than 512 blocks (2 a CU): what a block does once (lengths, q, its rows
-  // joined and written) costs it as much as several tiles.  16 ragged sequences of up to
-  // 4096: 23.9 us with 2048 blocks, 22.5 with 1024, 18.7 with 512; 131072 tokens of one: the
-  // same with each.
+  // Pieces for two blocks a CU, three where four waves fit a SIMD: what a block does once
+  // (lengths, q, its rows joined and written) costs it as much as several tiles.  16
+  // ragged sequences of up to 4096, 128 wide: 19.4 us with 256 pieces, 15.9 with 512, 16.2
+  // with 768, 18.2 with 1024; 64 of them, 64 wide: 49, 37, 33.6 and 34.7 us; 131072 tokens of
+  // one: 58.5, 58.8, 62 and 58.
   // A quad of lanes to a head up to four of them; else 16, or the 8 whose rows fit 64 KB
   // of LDS.
   a.width = a.group <= 4 ? 4 : bc.c.hs > 192 ? 8 : 16;
   a.sets = (int)cdiv(a.group, a.width);
-  const int64_t per = (int64_t)bc.c.n * bc.c.hk * a.sets;
-  a.chunk = (int)std::min<int64_t>(256 * std::max<int64_t>(1, cdiv(per * bc.c.cap, 512 * 256)),
-                                   cdiv(bc.c.cap, 256) * 256);
-  a.splits = (int)cdiv(bc.c.cap, a.chunk);
-  const size_t rows = (size_t)q_s0 * (size_t)q_s1, parts = rows * (size_t)a.splits;
+  const int64_t units = (int64_t)bc.c.n * bc.c.hk * a.sets, most = units * cdiv(bc.c.cap, kRound);
+  a.blocks = num_cus() * (bc.c.hs <= 64 ? 3 : 2);
+  const int64_t pieces = std::min(units + a.blocks, most);  // every unit may have one that is not full
+  if (most > INT32_MAX - a.blocks || pieces > UINT32_MAX / 256)
+    return set_error(SIMP_RT_EUNSUPPORTED, "kv8_attention: more heads and tokens than the kernels count");
+  const size_t rows = (size_t)q_s0 * (size_t)q_s1, parts = (size_t)pieces * (size_t)a.width;
   Workspace ws;
   float *p = nullptr;
   a.score_row = cdiv(bc.c.cap, 64) * 64;
   const size_t scores = with ? rows * (size_t)a.score_row : 0;
-  if ((rc = ws.get(st, 4 * (scores + parts * (size_t)(bc.c.hs + 2)), (void **)&p, 8))) return rc;
+  if ((rc = ws.get(st, 4 * (scores + parts * (size_t)(bc.c.hs + 2) + (size_t)bc.c.n + 1), (void **)&p, 8))) return rc;
   a.scores = with ? p : nullptr;
   a.part = p + scores;
   a.stat = (float2 *)(a.part + parts * (size_t)bc.c.hs);
+  a.starts = (int *)(a.stat + parts);
   const size_t cols = (size_t)std::min(a.group, a.width);
   const unsigned lds = (unsigned)(4 * 4 * cols * ((size_t)bc.c.hs + 2));
-  const dim3 grid((unsigned)a.splits, (unsigned)(bc.c.hk * a.sets), (unsigned)bc.c.n);
+  const dim3 grid((unsigned)pieces);
 #define ATTN(NC)                                                                      \
   do {                                                                                \
     if (a.group <= 4) hipLaunchKernelGGL((kv8_attn_k<NC, true>), grid, dim3(256), lds, st, a); \
@@ -1246,7 +1348,7 @@ int32_t simp_rt_kv8_attention(
 #undef ATTN
   const unsigned jx = (unsigned)(a.group + (with ? cdiv(bc.c.cap, kSeenTile) : 0));
   hipLaunchKernelGGL(kv8_join_k, dim3(jx, (unsigned)bc.c.hk, (unsigned)bc.c.n), dim3(256),
-                     4 * std::max(a.splits, 2 * a.group), st, a);
+                     4 * std::max<int64_t>(std::min<int64_t>(a.blocks, cdiv(bc.c.cap, kRound)), 2 * a.group), st, a);
   Operand *ops[] = {&oq, &ol, &oo, &osi, &oso};
   return finish(ops, with ? 5 : 3);
 }

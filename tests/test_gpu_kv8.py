@@ -209,6 +209,19 @@ def test_attention_long(dev, n, b, heads, h, hs, block):
             seen=r.random((b, h, n + 7)).astype(np.float32))
 
 
+@pytest.mark.parametrize("n, h, cap, hs", [(64, 3, 600, 32), (65, 1, 600, 16), (200, 2, 3000, 16), (1, 1, 3000, 256),
+                                           (4200, 1, 300, 16)])
+def test_attention_many_sequences(dev, n, h, cap, hs):
+    """More sequences than a wave has lanes, some empty, in one to several pieces each."""
+    r = np.random.default_rng(n)
+    lengths = r.integers(0, cap + 1, n).astype(np.int32)
+    lengths[r.integers(0, n, n // 3)] = 0
+    lengths[-1] = cap
+    p = Pair(dev, n, h, cap, hs, 64, seed=n)
+    q = r.standard_normal((n, 2 * h, hs)).astype(np.float32)
+    _attend(p, q, lengths, seen=np.abs(r.standard_normal((n, h, cap))).astype(np.float32))
+
+
 def test_attention_one_token_matters(dev):
     """A weight near one among thousands of nothing, and equal scores everywhere."""
     p = Pair(dev, 2, 1, 3000, 64, 32)
