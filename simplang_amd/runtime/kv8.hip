@@ -813,19 +813,21 @@ struct EvictArgs {
   uint32_t per;  // of the words of a row that kv8_move_k takes at a time
 };
 
-// Unsigned order of the weights: NaN above all, both zeros alike.
+// Unsigned order of the weights: NaN above all, both zeros alike.  None has the order 0.
 __device__ __forceinline__ uint32_t order_of(float x) {
   if (x != x) return 0xFFFFFFFFu;
   const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// The tokens of a wave's run, [t0, t1): f(token, order of its weight).  Up to 512 of
-// them (8192 of the sequence) are in registers; more are read again.
+// The tokens of a wave's run, [t0, t1): f(token, its weight, the weight's order, or 0 from
+// `old` on).  Up to 512 of them (8192 of the sequence) are in registers; more are read
+// again.  Sixteen waves share four SIMDs here, so every instruction of f counts.
 struct Run {
   const float *seen;
-  int t0, t1;
+  int t0, t1, old;
   bool held;
+  float x[8];
   uint32_t u[8];
   template <class F>
   __device__ __forceinline__ void each(F f) const {
@@ -833,49 +835,45 @@ struct Run {
     if (held) {
 #pragma unroll
       for (int i = 0; i < 8; i++)
-        if (t0 + 64 * i < t1) f(t0 + 64 * i + lane, u[i]);
+        if (t0 + 64 * i < t1) f(t0 + 64 * i + lane, x[i], u[i]);
     } else {
-      for (int t = t0; t < t1; t += 64) f(t + lane, t + lane < t1 ? order_of(seen[t + lane]) : 0u);
+      for (int t = t0 + lane; t - lane < t1; t += 64) {
+        const float y = t < t1 ? seen[t] : 0.f;
+        f(t, y, t < min(old, t1) ? order_of(y) : 0u);
+      }
     }
   }
 };
 
-// The place-from-the-top search of kv8_select_k: among the weights of 0 .. old-1 whose
-// order agrees with `prefix` above bit `shift + BITS`, a histogram of the next BITS bits;
-// then the bin that holds the need-th from the top.  Returns it, and what is left to
-// take from it in `need`, its size in `size`.
+// The place-from-the-top search of kv8_select_k: among the weights whose order agrees with `prefix` above bit `shift + BITS`, a histogram of the next BITS bits
+// (hist is 0 before and after); then the bin that holds the need-th from the top.
+// Returns it, and what is left to take from it in `need`, its size in `size`.
 template <int BITS>
-__device__ __forceinline__ uint32_t select_digit(const Run &run, int old, uint32_t prefix, int shift,
+__device__ __forceinline__ uint32_t select_digit(const Run &run, uint32_t prefix, int shift,
                                                  int &need, int &size, int *hist, int *wave_s) {
   constexpr int BINS = 1 << BITS, PER = BINS / 1024;  // bins of a thread
   static_assert(PER * 1024 == BINS, "");
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-  for (int i = 0; i < PER; i++) hist[tid + 1024 * i] = 0;
-  __syncthreads();
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int above_bits = min(shift + BITS, 31);
   const uint32_t same = shift + BITS == 32 ? 0u : 0xFFFFFFFFu << above_bits;
-  run.each([&](int t, uint32_t u) {
-    if (t < min(old, run.t1) && ((u ^ prefix) & same) == 0) atomicAdd(&hist[u >> shift & (BINS - 1)], 1);
+  run.each([&](int, float, uint32_t u) {
+    if (u && ((u ^ prefix) & same) == 0) atomicAdd(&hist[u >> shift & (BINS - 1)], 1);
   });
   __syncthreads();
   // thread t has the bins from the top: BINS - 1 - PER t and the PER - 1 below
   int h[PER], sum = 0;
 #pragma unroll
   for (int i = 0; i < PER; i++) {
-    h[i] = hist[BINS - 1 - PER * tid - i];
+    int &bin = hist[BINS - 1 - PER * tid - i];
+    h[i] = bin;
+    bin = 0;
     sum += h[i];
   }
-  int upto = sum;  // bins of this wave's threads up to this one's
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int x = __shfl_up(upto, d);
-    if (lane >= d) upto += x;
-  }
+  int upto = wave_scan(sum);  // bins of this wave's threads up to this one's
   if (lane == 63) wave_s[wave] = upto;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 16; w++) upto += w < wave ? wave_s[w] : 0;
+  const int waves = wave_scan(lane < 16 ? wave_s[lane] : 0);
+  if (wave > 0) upto += __builtin_amdgcn_readlane(waves, wave - 1);
   int above = upto - sum;
   if (above < need && need <= upto) {  // one thread
     int i = 0;
@@ -888,7 +886,6 @@ __device__ __forceinline__ uint32_t select_digit(const Run &run, int old, uint32
   const uint32_t digit = (uint32_t)wave_s[16];
   need = wave_s[17];
   size = wave_s[18];
-  __syncthreads();
   return digit << shift;
 }
 
@@ -897,12 +894,15 @@ __device__ __forceinline__ uint32_t select_digit(const Run &run, int old, uint32
 // that the weights, which share few exponents, do not all add to the same few
 // counters.  Each wave has a run of tokens: it counts those that stay (and those equal
 // to the last one, of which the first ones do), and writes them behind the other waves'.
-// 128 heads of up to 8192 tokens: 17 us (20 with the weights read again for each search), on
-// half of the CUs: the searches follow each other, each with its atomics in LDS.
+// 128 heads of up to 8192 tokens: 11 us on half of the CUs (17 with the orders formed anew
+// in each pass and the weights read again for the writing): three searches with their
+// atomics in LDS, the count and the writing follow each other, and the 16 waves' issue
+// bounds each.
 __global__ void __launch_bounds__(1024) kv8_select_k(const EvictArgs a) {
   __shared__ int hist[4096];
   __shared__ int wave_s[32], more_s[16], equal_s[16];
-  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int len = clampi(a.lengths[b], 0, a.c.cap);
   const float *seen = a.seen + b * a.se_seq + hk * a.se_head;
   float *ns = a.new_seen + b * a.ns_seq + hk * a.ns_head;
@@ -920,61 +920,66 @@ __global__ void __launch_bounds__(1024) kv8_select_k(const EvictArgs a) {
   run.t0 = min(wave * each, len);
   run.t1 = min(run.t0 + each, len);
   run.held = each <= 512;
+  const int old = run.old = len - a.recent;  // candidates 0 .. old-1
 #pragma unroll
   for (int i = 0; i < 8; i++) {
     const int t = run.t0 + 64 * i + lane;
-    run.u[i] = run.held && t < run.t1 ? order_of(seen[t]) : 0u;
+    run.x[i] = run.held && t < run.t1 ? seen[t] : 0.f;
   }
-  const int old = len - a.recent;  // candidates 0 .. old-1
+#pragma unroll
+  for (int i = 0; i < 8; i++) run.u[i] = run.t0 + 64 * i + lane < min(old, run.t1) ? order_of(run.x[i]) : 0u;
+#pragma unroll
+  for (int i = 0; i < 4; i++) hist[tid + 1024 * i] = 0;
+  __syncthreads();
   int need = a.budget - a.recent;  // of which so many stay (fewer than there are)
   uint32_t last = 0xFFFFFFFFu;     // the order of the last one that stays,
   uint32_t mask = 0xFFFFFFFFu;     // in these bits
   if (need > 0) {
     int size;
-    last = select_digit<12>(run, old, 0, 20, need, size, hist, wave_s);
+    last = select_digit<12>(run, 0, 20, need, size, hist, wave_s);
     mask = 0xFFF00000u;
     if (size != need) {
-      last |= select_digit<10>(run, old, last, 10, need, size, hist, wave_s);
+      last |= select_digit<10>(run, last, 10, need, size, hist, wave_s);
       mask = 0xFFFFFC00u;
     }
     if (size != need) {
-      last |= select_digit<10>(run, old, last, 0, need, size, hist, wave_s);
+      last |= select_digit<10>(run, last, 0, need, size, hist, wave_s);
       mask = 0xFFFFFFFFu;
     }
   }
-  const bool any = a.budget > a.recent;
-  int more = 0, equal = 0;
-  run.each([&](int t, uint32_t x) {
-    const uint32_t u = x & mask;
-    more += t < run.t1 && (t >= old || (any && u > last));
-    equal += t < min(old, run.t1) && any && u == last;
+  // Above `high` an order is larger than the last one in its bits, and from `last` to it equal.
+  const uint32_t high = last | ~mask, range = ~mask;
+  int more = max(run.t1 - max(run.t0, old), 0), equal = 0;  // of the wave
+  run.each([&](int, float, uint32_t u) {
+    more += __popcll(__ballot(u > high));
+    equal += __popcll(__ballot(u - last <= range));
   });
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    more += __shfl_xor(more, d);
-    equal += __shfl_xor(equal, d);
-  }
   if (lane == 0) {
     more_s[wave] = more;
     equal_s[wave] = equal;
   }
   __syncthreads();
   int eq = 0, place = 0;  // equal ones before this wave's; where it writes
-  for (int w = 0; w < wave; w++) {
-    place += more_s[w] + min(equal_s[w], max(need - eq, 0));
-    eq += equal_s[w];
+  {
+    const int m = lane < 16 ? more_s[lane] : 0, e = lane < 16 ? equal_s[lane] : 0;  // of a wave
+    const int es = wave_scan(e), ps = wave_scan(m + min(e, max(need - (es - e), 0)));
+    if (wave > 0) {
+      eq = __builtin_amdgcn_readlane(es, wave - 1);
+      place = __builtin_amdgcn_readlane(ps, wave - 1);
+    }
   }
-  const unsigned long long below = (1ull << lane) - 1;
-  run.each([&](int t, uint32_t x) {
-    const uint32_t u = x & mask;
-    const bool same = t < min(old, run.t1) && any && u == last;
+  const auto below = [](unsigned long long who) {  // lanes before this one
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+  };
+  run.each([&](int t, float x, uint32_t u) {
+    const bool same = u - last <= range;
     const unsigned long long be = __ballot(same);
-    const bool keep = t < run.t1 && (t >= old || (any && u > last) || (same && eq + __popcll(be & below) < need));
+    const bool keep = u > high || (t >= old && t < run.t1) || (same && eq + below(be) < need);
     const unsigned long long bk = __ballot(keep);
-    const int k = place + __popcll(bk & below);
+    const int k = place + below(bk);
     if (keep && k < a.budget) {
       kept[k] = t;
-      ns[k] = seen[t];
+      ns[k] = x;
     }
     eq += __popcll(be);
     place += __popcll(bk);
