@@ -294,7 +294,7 @@ struct AttnArgs {
   int64_t score_row;  // the capacity in whole tiles of 64
   float *part;        // [units' first pieces, width, pieces of a unit, head_size], unnormalised
   float2 *stat;       // the same without head_size: maximum and sum
-  int *starts;        // [n + 1]: pieces of a unit in the sequences before
+  int *starts;        // [n + 2]: pieces of a unit in the sequences before; the share (n > 64)
 };
 
 // Sums of whole numbers over the wave, and running sums over its lanes.
@@ -312,79 +312,81 @@ __device__ __forceinline__ int wave_total(int scanned) { return __builtin_amdgcn
 
 // The work: rounds of 256 tokens (a tile for each wave).  A piece is up to `share` rounds of
 // one unit (a set of the query heads of a kv head, of one sequence), with a share that makes
-// about `blocks` pieces of all, whatever the lengths.  Pieces follow each other sequence after sequence, and in a sequence
-// unit after unit; block i has piece i.
+// about `blocks` pieces of all, whatever the lengths.  Pieces follow each other sequence
+// after sequence, and in a sequence unit after unit; block i has piece i.  Up to 64
+// sequences, one to a lane, are counted by every wave for itself; more by kv8_plan_k.
 constexpr int kRound = 256;
-struct Work {
-  const int *lengths;
-  int n, cap, units;  // units: of a sequence
-  int m, share, upto; // a lane has m sequences; pieces of a unit of its and the lanes' before
-
-  __device__ __forceinline__ int rounds_of(int b) const {
-    return b < n ? (clampi(lengths[b], 0, cap) + kRound - 1) / kRound : 0;
-  }
-  __device__ __forceinline__ int pieces_of(int b) const { return (rounds_of(b) + share - 1) / share; }
-  __device__ __forceinline__ void init(const AttnArgs &a) {
-    lengths = a.lengths, n = a.c.n, cap = a.c.cap, units = a.c.hk * a.sets;
-    m = (n + 63) >> 6;
-    const int lane = threadIdx.x & 63;
-    int sum = 0;
-    if (m == 1) sum = rounds_of(lane);
-    else
-      for (int i = 0; i < m; i++) sum += rounds_of(lane * m + i);
-    share = max((wave_total(wave_scan(sum)) * units + a.blocks - 1) / a.blocks, 1);
-    if (m == 1) sum = (sum + share - 1) / share;
-    else {
-      sum = 0;
-      for (int i = 0; i < m; i++) sum += pieces_of(lane * m + i);
+__device__ __forceinline__ int rounds_of(const AttnArgs &a, int b) {
+  return b < a.c.n ? (clampi(a.lengths[b], 0, a.c.cap) + kRound - 1) / kRound : 0;
+}
+__device__ __forceinline__ int share_of(const AttnArgs &a, int rounds) {
+  return max((rounds * (a.c.hk * a.sets) + a.blocks - 1) / a.blocks, 1);
+}
+struct Piece {
+  int b, unit;       // sequence, unit in it
+  int place, count;  // among the unit's pieces
+  int share;
+};
+__device__ __forceinline__ bool find_piece(const AttnArgs &a, int x, Piece &p) {
+  const int lane = threadIdx.x & 63, n = a.c.n, units = a.c.hk * a.sets;
+  int before;
+  if (n <= 64) {
+    const int r = rounds_of(a, lane);
+    p.share = share_of(a, wave_total(wave_scan(r)));
+    const int own = (r + p.share - 1) / p.share, upto = wave_scan(own);
+    if (x == 0 && threadIdx.x < 64) {  // for kv8_join_k
+      if (lane < n) a.starts[lane + 1] = upto;
+      if (lane == 0) a.starts[0] = 0;
     }
-    upto = wave_scan(sum);
-  }
-  // For kv8_join_k: the pieces of a unit in the sequences before each, and in all.
-  __device__ __forceinline__ void store(int *starts) const {
-    const int lane = threadIdx.x;
-    int sum = upto;
-    if (m == 1) {
-      if (lane < n) starts[lane + 1] = sum;
-    } else {
-      for (int b = min((lane + 1) * m, n) - 1; b >= lane * m; b--) {
-        starts[b + 1] = sum;
-        sum -= pieces_of(b);
-      }
-    }
-    if (lane == 0) starts[0] = 0;
-  }
-  // The sequence of piece x, its unit, the place among the unit's and their count; false:
-  // there is none.
-  __device__ __forceinline__ bool find(int x, int &b, int &unit, int &place, int &count) const {
-    const int lane = threadIdx.x & 63;
     const unsigned long long who = __ballot(upto > x / units);
     if (!who) return false;
-    const int l = __ffsll(who) - 1;
-    int sum = l ? __builtin_amdgcn_readlane(upto, l - 1) : 0;
-    if (m == 1) {
-      b = l;
-      count = __builtin_amdgcn_readlane(upto, l) - sum;
-    } else {
-      for (int s0 = l * m;; s0 += 64) {
-        const int p = s0 + lane < (l + 1) * m ? pieces_of(s0 + lane) : 0, to = wave_scan(p);
-        const unsigned long long there = __ballot(sum + to > x / units);
-        if (there) {
-          const int k = __ffsll(there) - 1;
-          b = s0 + k;
-          count = __builtin_amdgcn_readlane(p, k);
-          sum += __builtin_amdgcn_readlane(to, k) - count;
-          break;
-        }
-        sum += wave_total(to);
-      }
-    }
-    const int y = x - sum * units;
-    unit = y / count;
-    place = y - unit * count;
-    return true;
+    p.b = __ffsll(who) - 1;
+    p.count = __builtin_amdgcn_readlane(own, p.b);
+    before = __builtin_amdgcn_readlane(upto, p.b) - p.count;
+  } else {
+    const auto *starts = (const __attribute__((address_space(4))) int *)a.starts;
+    p.share = starts[n + 1];
+    if (starts[n] <= x / units) return false;
+    p.b = last_of(n, [&](int s) { return a.starts[s] <= x / units; });
+    before = starts[p.b];
+    p.count = starts[p.b + 1] - before;
   }
-};
+  const int y = x - before * units;
+  p.unit = y / p.count;
+  p.place = y - p.unit * p.count;
+  return true;
+}
+
+// The pieces of a unit in the sequences before each of more than 64, and in all; then the
+// share.  65 sequences: 2.4 us and 14.9 for kv8_attn_k, against 15.9 where its waves count for
+// themselves; 200: 3-5 and 36.9 against 38.5; 1024: 3-5 and 24 against 59.
+__global__ void __launch_bounds__(1024) kv8_plan_k(const AttnArgs a) {
+  __shared__ int wave_s[2][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = a.c.n;
+  // the running sum of x over the block's threads, and its total
+  const auto block_scan = [&](int x, int slot, int &total) {
+    x = wave_scan(x);
+    if (lane == 63) wave_s[slot][wave] = x;
+    __syncthreads();
+    const int waves = wave_scan(lane < 16 ? wave_s[slot][lane] : 0);
+    total = __builtin_amdgcn_readlane(waves, 15);
+    return x + (wave ? __builtin_amdgcn_readlane(waves, wave - 1) : 0);
+  };
+  int rounds = 0, total;
+  for (int b = tid; b < n; b += 1024) rounds += rounds_of(a, b);
+  block_scan(rounds, 0, total);
+  const int share = share_of(a, total);
+  int before = 0, slot = 1;
+  for (int b0 = 0; b0 < n; b0 += 1024, slot ^= 1) {
+    const int upto = before + block_scan((rounds_of(a, b0 + tid) + share - 1) / share, slot, total);
+    if (b0 + tid < n) a.starts[b0 + tid + 1] = upto;
+    before += total;
+  }
+  if (tid == 0) {
+    a.starts[0] = 0;
+    a.starts[n + 1] = share;
+  }
+}
 
 constexpr float kUnit = 8.35e6f;        // v + 0x808080 stays below 2^24 and above 0
 constexpr uint32_t kBytes = 0x808080u;  // makes the three bytes unsigned
@@ -447,15 +449,12 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 && QUAD ? 3 : NC < 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i16 = lane & 15, g = lane >> 4, hs = c.hs;
   const int head = QUAD ? i16 >> 2 : i16, byte = QUAD ? i16 & 3 : 0;  // of the lane's column
-  Work work;
-  work.init(a);
-  if (blockIdx.x == 0 && threadIdx.x < 64) work.store(a.starts);
-  int b, unit, place, count;
-  if (!work.find((int)blockIdx.x, b, unit, place, count)) return;
-  const int hk = unit / a.sets, set0 = (unit - hk * a.sets) * a.width;
+  Piece piece;
+  if (!find_piece(a, (int)blockIdx.x, piece)) return;
+  const int b = piece.b, hk = piece.unit / a.sets, set0 = (piece.unit - hk * a.sets) * a.width;
   const int cols = min(a.width, a.group - set0), h0 = hk * a.group + set0;  // query heads h0 ..
-  const int len = clampi(a.lengths[b], 0, c.cap), chunk = work.share * kRound;
-  const int from = place * chunk, to = len - from < chunk ? len : from + chunk;
+  const int len = clampi(a.lengths[b], 0, c.cap), chunk = piece.share * kRound;
+  const int from = piece.place * chunk, to = len - from < chunk ? len : from + chunk;
   const int8_t *kp = c.k + b * c.st_seq + hk * c.st_head;
   const int8_t *vp = c.v + b * c.st_seq + hk * c.st_head;
   const float *ksp = c.ks + b * c.sc_seq + hk * c.sc_head, *vsp = c.vs + b * c.sc_seq + hk * c.sc_head;
@@ -695,7 +694,7 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 && QUAD ? 3 : NC < 
       x.z = fmaf(f, y.z, x.z);
       x.w = fmaf(f, y.w, x.w);
     }
-    const int64_t at = ((int64_t)blockIdx.x - place) * a.width + (int64_t)col * count + place;
+    const int64_t at = ((int64_t)blockIdx.x - piece.place) * a.width + (int64_t)col * piece.count + piece.place;
     *(float4 *)(a.part + at * hs + d) = x;
     if (d == 0) a.stat[at] = make_float2(M, sum);
   }
@@ -1333,13 +1332,14 @@ int32_t simp_rt_kv8_attention(
   float *p = nullptr;
   a.score_row = cdiv(bc.c.cap, 64) * 64;
   const size_t scores = with ? rows * (size_t)a.score_row : 0;
-  if ((rc = ws.get(st, 4 * (scores + parts * (size_t)(bc.c.hs + 2) + (size_t)bc.c.n + 1), (void **)&p, 8))) return rc;
+  if ((rc = ws.get(st, 4 * (scores + parts * (size_t)(bc.c.hs + 2) + (size_t)bc.c.n + 2), (void **)&p, 8))) return rc;
   a.scores = with ? p : nullptr;
   a.part = p + scores;
   a.stat = (float2 *)(a.part + parts * (size_t)bc.c.hs);
   a.starts = (int *)(a.stat + parts);
   const size_t cols = (size_t)std::min(a.group, a.width);
   const unsigned lds = (unsigned)(4 * 4 * cols * ((size_t)bc.c.hs + 2));
+  if (bc.c.n > 64) hipLaunchKernelGGL(kv8_plan_k, dim3(1), dim3(1024), 0, st, a);
   const dim3 grid((unsigned)pieces);
 #define ATTN(NC)                                                                      \
   do {                                                                                \
