@@ -291,3 +291,38 @@ def test_another_stream_and_a_graph(dev, n):
             assert torch.equal(first, o)
     finally:
         sa.set_stream(torch.cuda.current_stream())
+
+
+@pytest.mark.parametrize("nq, nk, heads", [(1700, 1700, 4), (41, 5200, 2)])
+def test_replays_with_other_packings(dev, nq, nk, heads):
+    """A graph of a call that takes the keys apart ahead, and of one that splits them: each
+    replay with other sequences in the same rows, empty and overlong ones among them."""
+    import torch
+    q, k, v, _, _ = _case([nq], [nk], heads, 1, 32)
+    t = [torch.from_numpy(x).to(dev) for x in (q, k, v)]
+    qs, ks = torch.zeros(3, dtype=torch.int32, device=dev), torch.zeros(3, dtype=torch.int32, device=dev)
+    o = torch.zeros_like(t[0])
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    try:
+        sa.set_stream(st)
+        sa.attention_packed(*t, o, qs, ks)
+        st.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            sa.attention_packed(*t, o, qs, ks)
+        h = nq // 2
+        for a, b in (([0, nq, nq], [0, nk, nk]), ([0, 0, nq], [0, 33, nk]), ([0, h, nq], [0, nk - 40, nk]),
+                     ([0, h, h], [0, 5, nk]), ([0, nq, nq], [0, 1, nk])):
+            a, b = np.array(a, np.int32), np.array(b, np.int32)
+            qs.copy_(torch.from_numpy(a))
+            ks.copy_(torch.from_numpy(b))
+            o.fill_(4)
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            got = o.cpu().numpy()
+            assert (got[a[-1]:] == 4).all()
+            _check(got[:a[-1]], q[:a[-1]], k, v, a, b)
+    finally:
+        sa.set_stream(torch.cuda.current_stream())

@@ -469,6 +469,41 @@ def test_graph_and_streams(dev):
         sa.set_stream(torch.cuda.current_stream())
 
 
+@pytest.mark.parametrize("n", [3, 70])
+def test_replays_with_other_lengths(dev, n):
+    """One graph for short, long, empty and full sequences: the pieces follow the lengths."""
+    import torch
+    cap = 2900
+    p = Pair(dev, n, 1, cap, 32, 64, seed=n)
+    r = np.random.default_rng(n)
+    q = r.standard_normal((n, 3, 32)).astype(np.float32)
+    qt, ln = p.up(q, np.zeros(n, np.int32))
+    out, seen = torch.zeros_like(qt), torch.zeros((n, 1, cap), device=dev)
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    try:
+        sa.set_stream(st)
+        p.gpu.attention(qt, ln, out, seen, seen)
+        st.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            p.gpu.attention(qt, ln, out, seen, seen)
+        full, one = np.full(n, cap), np.ones(n)
+        for lengths in (full, one, np.zeros(n), r.integers(0, cap + 1, n), np.where(r.random(n) < 0.8, 0, cap)):
+            lengths = lengths.astype(np.int32)
+            ln.copy_(torch.from_numpy(lengths))
+            seen.zero_()
+            out.fill_(3)
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            want, ws, tol, stol = p.np.attention(q, lengths, 32 ** -0.5, np.zeros((n, 1, cap), np.float32))
+            assert (np.abs(out.cpu().numpy() - want) <= tol[..., None]).all()
+            assert (np.abs(seen.cpu().numpy() - ws) <= stol).all()
+    finally:
+        sa.set_stream(torch.cuda.current_stream())
+
+
 def test_capture_without_a_warm_up_call_is_refused(dev):
     """The attention wants scratch, which a captured call does not allocate; the rest wants none."""
     import torch
