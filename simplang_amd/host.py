@@ -550,7 +550,7 @@ def _rows(fn, name, x, dtype="float32"):
         p = x.data_ptr()
     except AttributeError:
         return descn(x, 3)
-    d = (p, p, 0) + x.shape + x.stride()
+    d = (p, p, 0, *x.shape, *x.stride())
     if len(d) != 9:
         raise ValueError(f"expected a rank-3 tensor, got shape {tuple(x.shape)}")
     return d
@@ -560,7 +560,12 @@ def _list(fn, name, x):
     """The rank-1 descriptor of an int32 operand."""
     if _DTYPES.get(x.dtype) != "int32":
         _typed(fn, name, x, "int32")
-    return desc1(x)
+    try:
+        p = x.data_ptr()
+    except AttributeError:
+        return desc1(x)
+    d = (p, p, 0, *x.shape, *x.stride())
+    return d if len(d) == 5 and d[4] == 1 else desc1(x)
 
 
 def attention_packed(q, k, v, out, q_starts, k_starts, scale=None):
