@@ -1009,9 +1009,9 @@ int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
   a.p = p;
   a.hk = heads / p.group;
   // attn_stages_k and its traffic pay where about 24 blocks of four waves or more would
-  // make each stage: 1024 tokens of 32 heads over 8, 128 wide (32 blocks) 67 us against 80,
-  // 4096 (128) 380 against 560; 512 (16) 48 against 40, 2048 of 16 over 16, 64 wide (16) 67
-  // against 65.
+  // make each stage: 1024 tokens of 32 heads over 8, 128 wide (32 blocks) 63 us against 77,
+  // 4096 (128) 400 against 537; 512 (16) 46 against 39, 2048 of 16 over 16, 64 wide (16) 75
+  // against 66.
   const int64_t rows = cdiv(p.tq, p.n), keys = cdiv(p.tk, p.n);  // of a sequence, on average
   const bool stored = rows * p.group >= 24 * 128;
   // Eight waves share a fetched stage where their registers leave room for two on a SIMD.
@@ -1023,9 +1023,9 @@ int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
   a.blocks = (int)blocks;
   // The keys are split where the blocks (each with about `stages`, the last one of a row
   // half used) would not fill the chip, and the rows are long enough to be worth joining:
-  // 17 queries after 2983 tokens 29 us against 235, 273 of the 3B heads after up to 1500 56
-  // against 145, 2048 tokens of 16 heads 65 against 105.  Shorter pieces than 6 stages cost
-  // more in joining than they spare.
+  // 17 queries after 2983 tokens 28 us against 203, 273 of the 3B heads after up to 1500 56
+  // against 126, 2048 tokens of 16 heads 66 against 100.  Shorter pieces than 6 stages cost
+  // more in joining than they spare (512 tokens of 32 heads 39 us, 42 with four).
   a.splits = 1;
   a.chunk = INT32_MAX / 2;
   const int64_t cus = num_cus(), room = nw == 8 || p.hs > 128 ? cus : cus * 5 / 2;
