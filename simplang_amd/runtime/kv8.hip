@@ -700,13 +700,12 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 && QUAD ? 3 : NC < 
   }
 }
 
-constexpr int kSeenTile = 512;
-
-// 16 sequences of up to 4096 tokens, 32 heads, with the accumulated weights: 5 us;
-// 131072 tokens of one: 10.5 us for 25 MB.
+// 16 sequences of up to 4096 tokens, 32 heads, with the accumulated weights: 4.8 us;
+// 131072 tokens of one: 8 us for 25 MB.
 // The chunks of a row together.  blockIdx.x below the group: that query head's row of
 // out, head_size / 4 threads to a chunk and as many chunks at a time as there are
-// threads; above: kSeenTile tokens of the accumulated weights.
+// threads; above: TILE tokens of the accumulated weights.
+template <int TILE>
 __global__ void __launch_bounds__(256) kv8_join_k(const AttnArgs a) {
   extern __shared__ float lds[];
   __shared__ float4 so[256];
@@ -773,8 +772,20 @@ __global__ void __launch_bounds__(256) kv8_join_k(const AttnArgs a) {
     }
     return;
   }
-  const int t0 = ((int)blockIdx.x - a.group) * kSeenTile;
+  const int t0 = ((int)blockIdx.x - a.group) * TILE;
   if (t0 >= len) return;
+  // A thread has the tokens t0 + tid and 256 on.  What it adds to and up to four heads'
+  // scores are asked for first: the pieces' sums take their time meanwhile.
+  constexpr int kMine = TILE / 256, kAhead = 4;
+  const float *sc = a.scores + ((int64_t)b * a.heads + hk * a.group) * a.score_row;
+  float was[kMine], ahead[kAhead][kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; i++) {
+    const int t = min(t0 + tid + 256 * i, len - 1);
+    was[i] = a.seen_in[b * a.si_seq + hk * a.si_head + t];
+#pragma unroll
+    for (int g = 0; g < kAhead; g++) ahead[g][i] = sc[min(g, a.group - 1) * a.score_row + t];
+  }
   for (int g = wave; g < a.group; g += 4) {  // each head's maximum and 1 / sum
     const float2 *st = a.stat + row_of(g);
     float M = -INFINITY, L = 0.f;
@@ -789,13 +800,18 @@ __global__ void __launch_bounds__(256) kv8_join_k(const AttnArgs a) {
     }
   }
   __syncthreads();
-  for (int t = t0 + tid; t < min(t0 + kSeenTile, len); t += 256) {
-    const float *sc = a.scores + ((int64_t)b * a.heads + hk * a.group) * a.score_row + t;
+#pragma unroll
+  for (int i = 0; i < kMine; i++) {
+    const int t = t0 + tid + 256 * i;
+    if (t >= len) break;
     float w = 0.f;
+#pragma unroll
+    for (int g = 0; g < kAhead; g++)
+      if (g < a.group) w = fmaf(pow2(ahead[g][i] - lds[2 * g]), lds[2 * g + 1], w);
 #pragma unroll 4
-    for (int g = 0; g < a.group; g++)
-      w = fmaf(pow2(sc[g * a.score_row] - lds[2 * g]), lds[2 * g + 1], w);
-    a.seen_out[b * a.so_seq + hk * a.so_head + t] = a.seen_in[b * a.si_seq + hk * a.si_head + t] + w;
+    for (int g = kAhead; g < a.group; g++)
+      w = fmaf(pow2(sc[g * a.score_row + t] - lds[2 * g]), lds[2 * g + 1], w);
+    a.seen_out[b * a.so_seq + hk * a.so_head + t] = was[i] + w;
   }
 }
 
@@ -1351,9 +1367,15 @@ int32_t simp_rt_kv8_attention(
   else if (bc.c.hs <= 192) ATTN(3);
   else ATTN(4);
 #undef ATTN
-  const unsigned jx = (unsigned)(a.group + (with ? cdiv(bc.c.cap, kSeenTile) : 0));
-  hipLaunchKernelGGL(kv8_join_k, dim3(jx, (unsigned)bc.c.hk, (unsigned)bc.c.n), dim3(256),
-                     4 * std::max<int64_t>(std::min<int64_t>(a.blocks, cdiv(bc.c.cap, kRound)), 2 * a.group), st, a);
+  // The accumulated weights 512 tokens to a block, and twice as many where that would make
+  // more than four blocks a CU: 16 sequences of up to 4096 tokens (1024 blocks) 4.8 us
+  // against 5.4, 131072 tokens of one (2048) 10.1 against 8.0.
+  const int64_t tiles = with ? cdiv(bc.c.cap, 512) : 0;
+  const bool wide = tiles * bc.c.hk * bc.c.n > 4 * num_cus();
+  const dim3 joins((unsigned)(a.group + (wide ? cdiv(tiles, 2) : tiles)), (unsigned)bc.c.hk, (unsigned)bc.c.n);
+  const unsigned sums = (unsigned)(4 * std::max<int64_t>(std::min<int64_t>(a.blocks, cdiv(bc.c.cap, kRound)), 2 * a.group));
+  if (wide) hipLaunchKernelGGL(kv8_join_k<1024>, joins, dim3(256), sums, st, a);
+  else hipLaunchKernelGGL(kv8_join_k<512>, joins, dim3(256), sums, st, a);
   Operand *ops[] = {&oq, &ol, &oo, &osi, &oso};
   return finish(ops, with ? 5 : 3);
 }
