@@ -462,6 +462,13 @@ __global__ void __launch_bounds__(256) attn_stages_k(const F16Args a) {
   }
 }
 
+// What a row, or its part of a piece, is divided by.  A piece in which every score is -inf
+// has the sum 0 and leaves zeros, for its weight in the row is 0 too; a whole row of
+// such scores stays 0 / 0.
+__device__ __forceinline__ float one_over(float l, int splits) {
+  return splits > 1 && l == 0.f ? 0.f : 1.f / l;
+}
+
 // The blocks of one kv head: sequence s has ((q_starts[s] / 32 + s) G / NW) + s and on.
 template <int NW>
 __device__ __forceinline__ int first_block(const PackedArgs &a, int s) {
@@ -889,7 +896,7 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
       float *out = args.splits > 1 ? args.part + at * a.hs
                                    : a.out + (int64_t)(z.qb + r) * a.o_row + un.head * a.o_head;
       if (args.splits > 1 && g == 0) args.stat[at] = make_float2(m * 1.44269504f, l);
-      const float f = args.splits == 1 && r + off < 0 ? 0.f : 1.f / l;
+      const float f = args.splits == 1 && r + off < 0 ? 0.f : one_over(l, args.splits);
 #pragma unroll
       for (int j = 0; j < 2 * NB; j++)
 #pragma unroll
@@ -908,7 +915,7 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
   // gradual underflow where V is tiny.
   const float scale = unit > -1000 ? ldexpf(1.f, unit - 13) : 0.f;
   const bool none = args.splits == 1 && my < 0;
-  const float f = 1.f / l;
+  const float f = one_over(l, args.splits);
   float *out;
   if (args.splits > 1) {
     const int64_t at = part_row + (int64_t)row * part_step;
@@ -954,7 +961,7 @@ __global__ void __launch_bounds__(256) attn_join_k(const F16Args args) {
     float M = -INFINITY, L = 0.f;
 #pragma unroll 8
     for (int i = 0; i < ns; i++) M = fmaxf(M, stat[i * step].x);
-    if (M == -INFINITY) M = 0.f;  // every score is -inf: the sums are 0 too
+    if (M == -INFINITY) M = 0.f;  // every score is -inf: the sums are 0 too, and the row 0 / 0
 #pragma unroll 8
     for (int i = 0; i < ns; i++) {
       const float2 ml = stat[i * step];

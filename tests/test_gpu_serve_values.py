@@ -1,0 +1,81 @@
+"""The batch attention operators at values that only some of their forms meet: pieces of a
+row in which every score is -inf."""
+import numpy as np
+import pytest
+
+import simplang_amd as sa
+import _serve as S
+
+pytestmark = pytest.mark.gpu
+
+# made in the block, taken apart ahead, split over blocks (made), split over blocks (wide)
+FORMS = [(90, 300, 2, 1, 64), (850, 900, 4, 1, 64), (40, 2500, 2, 1, 64), (9, 2000, 1, 1, 256)]
+
+
+def _inputs(nq, nk, heads, kv, hs, seed=0):
+    r = np.random.default_rng(seed + nq + nk)
+    f = lambda *s: r.standard_normal(s).astype(np.float32)  # noqa: E731
+    return f(nq, heads, hs), f(nk, kv, hs), f(nk, kv, hs)
+
+
+def _run(dev, q, k, v, scale=None):
+    import torch
+    t = [torch.from_numpy(x).to(dev) for x in (q, k, v)]
+    st = [torch.tensor([0, len(x)], dtype=torch.int32, device=dev) for x in (q, k)]
+    out = torch.full(q.shape, 7.0, device=dev)
+    sa.attention_packed(*t, out, *st, scale)
+    return out.cpu().numpy()
+
+
+def _want(q, k, v, gone):
+    """(out, bound) in 64 bits, with the keys in `gone` left out."""
+    nq, nk, group = len(q), len(k), q.shape[1] // k.shape[1]
+    hidden = np.arange(nk)[None, :] > np.arange(nq)[:, None] + nk - nq
+    hidden = hidden | gone[None, :]
+    out, tol = np.zeros(q.shape), np.zeros(q.shape[:2])
+    for h in range(q.shape[1]):
+        x = [np.where(gone[:, None], 0, y[:, h // group]).astype(np.float64) for y in (k, v)]
+        qq = q[:, h].astype(np.float64)
+        out[:, h], _ = S.attention(qq, *x, q.shape[2] ** -0.5, hidden)
+        tol[:, h] = S.row_bound(qq, *x, q.shape[2] ** -0.5, hidden)
+    return out, tol
+
+
+@pytest.mark.parametrize("where", ["first", "last"])
+@pytest.mark.parametrize("gone", [192, 224, 400])
+@pytest.mark.parametrize("how", ["channel", "overflow"])
+@pytest.mark.parametrize("nq, nk, heads, kv, hs", FORMS)
+def test_pieces_of_nothing_but_minus_infinity(dev, nq, nk, heads, kv, hs, how, gone, where):
+    """Keys that score -inf have the weight 0, also where they fill a piece of the row:
+    through a channel of -inf, and finite ones through products below -3.4e38."""
+    gone = min(gone, nk - 64)
+    q, k, v = _inputs(nq, nk, heads, kv, hs)
+    at = np.zeros(nk, bool)
+    at[:gone] = True
+    if where == "last":
+        at = np.roll(at, nk - gone)
+    if how == "channel":
+        q[..., 0], k[..., 0] = 1, 0
+        k[at, :, 0] = -np.inf
+    else:
+        q = (np.abs(q) + np.float32(0.5)) * np.float32(1e19)
+        k *= np.float32(1e-19)
+        k[at] = -1e20
+    got = _run(dev, q, k, v)
+    want, tol = _want(q, k, v, at)
+    seen = (~at)[None, :] & (np.arange(nk)[None, :] <= np.arange(nq)[:, None] + nk - nq)
+    some = seen.any(1)
+    assert np.isnan(got[~some]).all()
+    assert (np.abs(got - want) <= tol[..., None])[some].all(), np.argwhere(~(np.abs(got - want) <= tol[..., None]))[:4]
+
+
+@pytest.mark.parametrize("nq, nk, heads, kv, hs", FORMS)
+def test_rows_of_nothing_but_minus_infinity(dev, nq, nk, heads, kv, hs):
+    """No weight to share out: 0 / 0, in whichever form."""
+    q, k, v = _inputs(nq, nk, heads, kv, hs)
+    k[:] = -1e20
+    assert np.isnan(_run(dev, (np.abs(q) + np.float32(0.5)) * np.float32(1e20), k, v)).all()
+    k[..., 1:] = 0
+    k[..., 0] = -np.inf
+    q[..., 0] = 1
+    assert np.isnan(_run(dev, q, k, v)).all()
