@@ -193,6 +193,10 @@ constexpr int kStageKeys = 32;
 // to here 24 bits of it are kept), and a key that a query does not see would cost the
 // query's row bits.
 constexpr int kSpread = 14;
+// O is kept in the scaling of the largest stage so far.  A row that sees only the first
+// stages has a sum of 2^13 there or more, and 24 bits below its largest value stay above fp32's
+// subnormals as long as the scaling does not rise by more than this behind its last key.
+constexpr int kClimb = 64;
 
 struct F16Args {
   PackedArgs p;
@@ -829,6 +833,7 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
     post(0);
     lds_barrier();
     uint2 top = tops(0);
+    int first = -1000;  // O's first scaling
 #pragma unroll
     for (int i = 0; i < 2 * NB; i++) make(ring[0], top, i);
     key_tops(0);
@@ -866,8 +871,9 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
         unit = e;
       }
       keep(o);
+      if (first == -1000) first = unit;
       const int er = e - unit;  // (-1000 less itself where V has been 0 so far)
-      odd |= er < -kSpread;
+      odd |= er < -kSpread || unit - first > kClimb;
       // (waves that see nothing of the stage have weights of 0; behind the last stage it is made again)
       stage<NB, true>((const h8 *)ring[at] + lane, qh, ql, qf * power(-lift(kt)), kStageKeys * st, my, all, h,
                     max(er, -kSpread), o, m, l, [&](int i) { make(ring[at ^ 1], next, i); },

@@ -1,5 +1,5 @@
 """The batch attention operators at values that only some of their forms meet: pieces of a
-row in which every score is -inf."""
+row in which every score is -inf, values that grow by many powers of ten."""
 import numpy as np
 import pytest
 
@@ -79,3 +79,20 @@ def test_rows_of_nothing_but_minus_infinity(dev, nq, nk, heads, kv, hs):
     k[..., 0] = -np.inf
     q[..., 0] = 1
     assert np.isnan(_run(dev, q, k, v)).all()
+
+
+@pytest.mark.parametrize("powers", [(-25, 25), (-30, -10, 10, 30), (-36, 35), (25, -25), (-3, 3)], ids=str)
+@pytest.mark.parametrize("nq, heads, kv, hs", [(128, 2, 2, 64), (130, 1, 1, 100), (128, 2, 1, 192), (850, 4, 1, 64)])
+def test_rows_before_much_larger_values(dev, nq, heads, kv, hs, powers):
+    """Values that grow by many powers of ten every 32 keys: a row that sees only the first
+    ones has them in full."""
+    q, k, v = _inputs(nq, nq, heads, kv, hs)
+    v = np.abs(v) + np.float32(0.5)
+    step = np.minimum(np.arange(nq) // 32, len(powers) - 1)
+    v *= (10.0 ** np.array(powers, np.float64)[step]).astype(np.float32)[:, None, None]
+    got = _run(dev, q, k, v)
+    want, _ = _want(q, k, v, np.zeros(nq, bool))
+    # every value is above 0, so the bound of a row of ones is relative to the row
+    _, tol = _want(q, k, np.ones_like(v), np.zeros(nq, bool))
+    bad = np.abs(got - want) > tol[..., None] * want
+    assert not bad.any(), np.argwhere(bad)[:4]
