@@ -476,7 +476,8 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 && QUAD ? 3 : NC < 
   // those below 64 j + 16 g belong to the chunk before (the row's end).
   uint32_t doff[NC];
   v4i ql[NC][L];
-  float qf;
+  float qf;  // times 2^qe: what a unit of q's whole numbers is worth
+  int qe;
   {
     float x[NC][16], top = 0.f;
     bool odd = false;
@@ -498,10 +499,12 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 && QUAD ? 3 : NC < 
     top = quad_max(top);
     const unsigned long long who = __ballot(odd);  // a query that is not finite: its row is NaN
     if ((who >> i16) & 0x0001000100010001ull) top = NAN;
-    qf = top * a.scale / kUnit;
-    // by way of [1, 2): 1 / top alone may be too large
+    // by way of [1, 2): 1 / top alone may be too large, and top / kUnit subnormal
     const int e2 = top > 0.f ? -ilogbf(top) : 0;
-    const float inv = top > 0.f ? kUnit / ldexpf(top, e2) : 0.f;
+    const float top1 = ldexpf(top, e2);
+    const float inv = top > 0.f ? kUnit / top1 : 0.f;
+    qf = top1 * a.scale * (8388608.f / kUnit);  // over 2^qe
+    qe = -23 - e2;
 #pragma unroll
     for (int j = 0; j < NC; j++)
 #pragma unroll
@@ -580,7 +583,7 @@ __global__ void __launch_bounds__(256, NC == 1 ? 4 : NC == 2 && QUAD ? 3 : NC < 
 #pragma unroll
         for (int i = 0; i < L; i++)
           x[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf[t][j], ql[j][i], x[i], 0, 0, 0);
-      const float f = qf * ks[t];
+      const float f = ldexpf(qf * ks[t], qe);
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         float y = number(x, r);

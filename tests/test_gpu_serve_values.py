@@ -1,5 +1,6 @@
 """The batch attention operators at values that only some of their forms meet: pieces of a
-row in which every score is -inf, values that grow by many powers of ten."""
+row in which every score is -inf, values that grow by many powers of
+ten, queries that are tiny beside the keys."""
 import numpy as np
 import pytest
 
@@ -96,3 +97,33 @@ def test_rows_before_much_larger_values(dev, nq, heads, kv, hs, powers):
     _, tol = _want(q, k, np.ones_like(v), np.zeros(nq, bool))
     bad = np.abs(got - want) > tol[..., None] * want
     assert not bad.any(), np.argwhere(bad)[:4]
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-34, 1e-36])
+@pytest.mark.parametrize("heads", [2, 5])
+def test_tiny_queries_keep_their_bits(dev, heads, size):
+    """q . k is what counts, however the size is shared between them (values of 5e-38 and
+    above, none subnormal)."""
+    import torch
+    from test_gpu_kv8 import Pair, _attend
+    p = Pair(dev, 2, 1, 300, 64, 32)
+    q = np.random.default_rng(5).standard_normal((2, heads, 64))
+    q = (np.sign(q) * (np.abs(q) + 0.05) * size).astype(np.float32)
+    p.np.ks *= np.float32(1 / size)
+    p.t[2].copy_(torch.from_numpy(p.np.ks))
+    _attend(p, q, [300, 77], seen=np.zeros((2, 1, 300), np.float32))
+
+
+@pytest.mark.parametrize("heads", [2, 5])
+def test_huge_queries_over_tiny_codes(dev, heads):
+    """The largest element of a query may meet codes of 0 only: its size alone is no score."""
+    import torch
+    from test_gpu_kv8 import Pair, _attend
+    p = Pair(dev, 2, 1, 300, 64, 32)
+    p.np.kc[..., 0] = 0
+    p.t[0].copy_(torch.from_numpy(p.np.kc))
+    p.np.ks *= np.float32(1e5)
+    p.t[2].copy_(torch.from_numpy(p.np.ks))
+    q = np.zeros((2, heads, 64), np.float32)
+    q[..., 0] = 1e36
+    _attend(p, q, [300, 77], seen=np.zeros((2, 1, 300), np.float32))
