@@ -1130,8 +1130,8 @@ int32_t simp_rt_attention_packed_f32(
                      (long long)k_s0, (long long)k_s1, (long long)k_s2);
   if (qst_size < 1 || kst_size != qst_size)
     return set_error(SIMP_RT_EINVAL, "attention_packed: q_starts and k_starts must have sequences + 1 entries");
-  if (!std::isfinite(scale))
-    return set_error(SIMP_RT_EINVAL, "attention_packed: scale must be finite");
+  if (!scale_fits(scale))
+    return set_error(SIMP_RT_EINVAL, "attention_packed: scale must be finite, also in fp32 and times log2(e)");
   if (q_s2 < 1 || q_s2 > 256)
     return set_error(SIMP_RT_EUNSUPPORTED, "attention_packed: head_size %lld is not in 1..256", (long long)q_s2);
   if (k_s1 < 1 || q_s1 % k_s1 != 0)

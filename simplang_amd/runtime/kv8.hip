@@ -1296,7 +1296,7 @@ int32_t simp_rt_kv8_attention(
   if (bc.empty) return set_error(SIMP_RT_EINVAL, "kv8_attention: the cache has no capacity");
   if (with && (!dsi.is(cache->batch, cache->n_kv_heads, cache->capacity) || !dso.is(si_s0, si_s1, si_s2)))
     return set_error(SIMP_RT_EINVAL, "kv8_attention: seen_in and seen_out must be [batch, n_kv_heads, capacity]");
-  if (!std::isfinite(scale)) return set_error(SIMP_RT_EINVAL, "kv8_attention: scale must be finite");
+  if (!scale_fits(scale)) return set_error(SIMP_RT_EINVAL, "kv8_attention: scale must be finite, also in fp32 and times log2(e)");
   if (q_s1 > 32767 || q_s1 / cache->n_kv_heads > 4096)
     return set_error(SIMP_RT_EUNSUPPORTED, "kv8_attention: heads above 32767, or 4096 to a kv head");
   const bool in_place = with && dsi.data() == dso.data() && si_st0 == so_st0 && si_st1 == so_st1;

@@ -2,6 +2,9 @@
 // sequences (attention.hip, kv8.hip).
 #pragma once
 
+#include <cfloat>
+#include <cmath>
+
 #include "rt_internal.h"
 
 namespace simp {
@@ -16,6 +19,9 @@ struct Desc3 {
   T *data() const { return p + off; }
   size_t bytes() const { return (size_t)span * sizeof(T); }
 };
+
+// The kernels take the scale in fp32, times log2(e) for powers of two.
+inline bool scale_fits(double scale) { return std::fabs(scale) * 1.4426950408889634 <= FLT_MAX; }
 
 // Device memory of another GPU than the one that the call launches on is refused.
 inline int check_here(const Operand &o, int dev, const char *name) {
