@@ -424,7 +424,8 @@ int32_t simp_rt_attention_packed_f32(
  * at b*st_seq + h*st_head + t*st_token + d, scale (b, h, j) at b*sc_seq +
  * h*sc_head + j, in elements, for K and V alike.  Codes are -127 .. 127.  All four
  * arrays are device memory or registered ranges (they are the caller's; the
- * struct only says where they lie).  block is 16, 32, 64 or 128; head_size a
+ * struct only says where they lie) and share no element; one may lie between the
+ * rows of another.  block is 16, 32, 64 or 128; head_size a
  * multiple of 4 from 16 to 256; code rows start on 4-byte boundaries; tokens of a
  * head, and heads, may be in either order ([heads, capacity] or [capacity, heads]),
  * tokens less than 2^24 apart.  batch and heads up to 32767. */

@@ -1078,6 +1078,22 @@ int64_t scale_span(const simp_rt_kv8 &c) {
   return in + (c.batch > 1 ? (c.batch - 1) * c.sc_seq : 0);
 }
 
+// Whether K and V share codes or scales.  One may lie between the other's rows, heads or
+// sequences, as the parts of one tensor do.
+bool one_memory(const simp_rt_kv8 &c, int64_t codes, int64_t scales) {
+  if (overlap(c.k, (size_t)codes, c.v, (size_t)codes)) {
+    const Level seq{c.batch, c.st_seq}, head{c.n_kv_heads, c.st_head}, token{c.capacity, c.st_token}, d{c.head_size, 1};
+    const bool heads_outside = c.n_kv_heads == 1 || c.capacity == 1 || c.st_head > c.st_token;
+    const Level l[] = {seq, heads_outside ? head : token, heads_outside ? token : head, d};
+    if (meet(l, 4, (int64_t)((uintptr_t)c.v - (uintptr_t)c.k))) return true;
+  }
+  if (overlap(c.k_scale, 4 * (size_t)scales, c.v_scale, 4 * (size_t)scales)) {
+    const Level l[] = {{c.batch, c.sc_seq}, {c.n_kv_heads, c.sc_head}, {cdiv(c.capacity, c.block), 1}};
+    if (meet(l, 3, (int64_t)((uintptr_t)c.v_scale - (uintptr_t)c.k_scale) / 4)) return true;
+  }
+  return false;
+}
+
 struct BoundCache {
   Operand k, v, ks, vs;
   Cache c;
@@ -1107,11 +1123,11 @@ struct BoundCache {
       return set_error(SIMP_RT_EINVAL, "%s: %s: strides let rows overlap", fn, name);
     if (!p->k || !p->v || !p->k_scale || !p->v_scale)
       return set_error(SIMP_RT_EINVAL, "%s: %s: null pointer", fn, name);
-    if (p->k == p->v || p->k_scale == p->v_scale)
-      return set_error(SIMP_RT_EINVAL, "%s: %s: K and V are the same memory", fn, name);
     if (((uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->k_scale | (uintptr_t)p->v_scale |
          (uintptr_t)p->st_seq | (uintptr_t)p->st_head | (uintptr_t)p->st_token) & 3)
       return set_error(SIMP_RT_EINVAL, "%s: %s: rows and scales must start on 4-byte boundaries", fn, name);
+    if (one_memory(*p, codes, scales))
+      return set_error(SIMP_RT_EINVAL, "%s: %s: K and V share elements: the same memory", fn, name);
     return SIMP_RT_OK;
   }
   // Whether a byte range lies in one of the cache's arrays.

@@ -43,6 +43,26 @@ inline bool overlap(const void *a, size_t an, const void *b, size_t bn) {
   return an && bn && x < y + bn && y < x + an;
 }
 
+// Dimensions of an array, the outer ones first, each with a stride of at least the span of
+// those inside it.  One of size 1 has any stride.
+struct Level {
+  int64_t n, stride;
+};
+
+// Whether two arrays with these dimensions share an element, the second's first one
+// `delta` elements behind the first's: sum (i - j) stride = delta has a solution.  What the
+// inner dimensions add is less than a stride, so only two differences come into question.
+inline bool meet(const Level *level, int levels, int64_t delta) {
+  if (levels == 0) return delta == 0;
+  const Level &l = *level;
+  if (l.n <= 1) return l.n == 1 && meet(level + 1, levels - 1, delta);
+  int64_t d = delta / l.stride;
+  if (delta % l.stride < 0) d--;  // rounded down
+  for (int i = 0; i < 2; i++, d++)
+    if (d > -l.n && d < l.n && meet(level + 1, levels - 1, delta - d * l.stride)) return true;
+  return false;
+}
+
 // Whether two arrays of one shape share elements.  One may lie between the rows or the
 // heads of the other, as the parts of a fused product do.
 template <class T>

@@ -22,3 +22,71 @@ def test_scales_beyond_fp32_are_refused(scale):
 @pytest.mark.parametrize("scale", [0.0, 1e-300, -2e38])
 def test_scales_within_fp32_pass(scale):
     sa.attention_packed(**_prompt(tq=0), scale=scale)
+
+
+def _views(layout):
+    """K and V of a cache in one tensor, and the offset of V's first element behind K's."""
+    b, h, cap, hs = 2, 3, 40, 32
+    if layout == "row":        # K and V rows in turn
+        x = np.zeros((b, h, cap, 2, hs), np.int8)
+        return x[:, :, :, 0], x[:, :, :, 1]
+    if layout == "token":      # [batch, capacity, K and V, heads, head_size]
+        x = np.zeros((b, cap, 2, h, hs), np.int8)
+        return x[:, :, 0].transpose(0, 2, 1, 3), x[:, :, 1].transpose(0, 2, 1, 3)
+    if layout == "head":       # a head's K, then its V
+        x = np.zeros((b, h, 2, cap, hs), np.int8)
+        return x[:, :, 0], x[:, :, 1]
+    if layout == "seq":
+        x = np.zeros((b, 2, h, cap, hs), np.int8)
+        return x[:, 0], x[:, 1]
+    x = np.zeros((2, b, h, cap, hs), np.int8)
+    return x[0], x[1]
+
+
+@pytest.mark.parametrize("layout", ["row", "token", "head", "seq", "apart"])
+def test_k_and_v_between_each_other_pass(layout):
+    k, v = _views(layout)
+    s = np.zeros((2, 2, 3, 3), F)
+    for x, y in ((k, v), (v, k)):
+        c = sa.KV8Cache(x, y, s[0], s[1], 16)
+        c.append(*_rows(n=0, h=3), np.zeros(3, I), np.zeros(2, I))
+
+
+def _part(x, by):
+    """x, its first element moved by so many bytes (the memory behind it is not touched)."""
+    from numpy.lib.stride_tricks import as_strided
+    whole = x.base if x.base is not None else x
+    at = x.ctypes.data - whole.ctypes.data + by * x.itemsize
+    flat = whole.reshape(-1).view(x.dtype)[at // x.itemsize:]
+    return as_strided(flat[:1], x.shape, x.strides)
+
+
+@pytest.mark.parametrize("by", [4, 28, -4, 32 * 40, 32, -32 * 40 * 3, 32 * 40 * 2 + 32 * 39])
+def test_k_and_v_that_share_codes_are_refused(by):
+    x = np.zeros((4, 3, 40, 32), np.int8)
+    k = x[1:3]
+    s = np.zeros((2, 2, 3, 3), F)
+    with pytest.raises(sa.SimpRTError, match="same memory"):
+        sa.KV8Cache(k, _part(k, by), s[0], s[1], 16).append(*_rows(h=3), np.zeros(3, I), np.zeros(2, I))
+
+
+@pytest.mark.parametrize("layout, by", [("row", 4), ("row", -4), ("row", 96), ("token", 32), ("token", 100),
+                                        ("head", 32 * 39), ("head", -32), ("seq", 32), ("seq", -4)])
+def test_k_and_v_that_overlap_between_each_other_are_refused(layout, by):
+    """One is between the other's rows, heads or sequences, and reaches into them."""
+    k, v = _views(layout)
+    s = np.zeros((2, 2, 3, 3), F)
+    with pytest.raises(sa.SimpRTError, match="same memory"):
+        sa.KV8Cache(k, _part(v, by), s[0], s[1], 16).append(*_rows(h=3), np.zeros(3, I), np.zeros(2, I))
+
+
+def test_scales_that_share_memory_are_refused():
+    k, v = _views("apart")
+    s = np.zeros((4, 3, 3), F)
+    for by in (1, 3, -3, 9):
+        with pytest.raises(sa.SimpRTError, match="same memory"):
+            sa.KV8Cache(k, v, s[1:3], _part(s[1:3], by), 16).append(*_rows(h=3), np.zeros(3, I), np.zeros(2, I))
+    z = np.zeros((2, 3, 2, 3), F)
+    sa.KV8Cache(k, v, z[:, :, 0], z[:, :, 1], 16).append(*_rows(n=0, h=3), np.zeros(3, I), np.zeros(2, I))
+    with pytest.raises(sa.SimpRTError, match="same memory"):
+        sa.KV8Cache(k, v, z[:, :, 0], _part(z[:, :, 1], 1), 16).append(*_rows(h=3), np.zeros(3, I), np.zeros(2, I))
