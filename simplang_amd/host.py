@@ -563,9 +563,11 @@ def _list(fn, name, x):
     try:
         p = x.data_ptr()
     except AttributeError:
-        return desc1(x)
+        return [x.ctypes.data, x.ctypes.data, 0, 1, 1] if x.shape == (1,) else desc1(x)
     d = (p, p, 0, *x.shape, *x.stride())
-    return d if len(d) == 5 and d[4] == 1 else desc1(x)
+    if len(d) != 5 or (d[4] != 1 and d[3] != 1):
+        return desc1(x)
+    return d if d[4] == 1 else (*d[:4], 1)
 
 
 def attention_packed(q, k, v, out, q_starts, k_starts, scale=None):
@@ -608,17 +610,16 @@ class KV8Cache:
         b, h, cap, hs = (int(x) for x in k.shape)
         if tuple(k_scale.shape) != (b, h, -(-cap // block)) or tuple(v_scale.shape) != tuple(k_scale.shape):
             raise ValueError("KV8Cache: scales must be [batch, kv_heads, ceil(capacity / block)]")
-        kd, vd = _strides4(_typed(fn, "k", k, "int8")), _strides4(_typed(fn, "v", v, "int8"))
-        ks = descn(_typed(fn, "k_scale", k_scale, "float32"), 3)
-        vs = descn(_typed(fn, "v_scale", v_scale, "float32"), 3)
-        if kd[1:] != vd[1:] or ks[3:] != vs[3:]:
+        kd, vd = _strides(_typed(fn, "k", k, "int8")), _strides(_typed(fn, "v", v, "int8"))
+        ks, vs = _strides(_typed(fn, "k_scale", k_scale, "float32")), _strides(_typed(fn, "v_scale", v_scale, "float32"))
+        if kd[1:] != vd[1:] or ks[1:] != vs[1:]:
             raise ValueError("KV8Cache: k and v, and their scales, must have the same strides")
-        if kd[4] != 1 or ks[8] != 1:
+        if kd[4] != 1 or ks[3] > 1:
             raise ValueError("KV8Cache: the innermost stride must be 1")
         self._tensors = (k, v, k_scale, v_scale)
         self.batch, self.kv_heads, self.capacity, self.head_size, self.block = b, h, cap, hs, block
         self._c = _KV8(kd[0], vd[0], ks[0], vs[0], b, h, cap, hs, block, kd[1], kd[2], kd[3],
-                       ks[6], ks[7])
+                       ks[1], ks[2])
         self._ref = C.byref(self._c)
 
     def append(self, k, v, starts, lengths) -> None:
@@ -666,12 +667,14 @@ class KV8Cache:
 _NO3 = [None, None] + [0] * 7
 
 
-def _strides4(x):
-    """(pointer, strides...) of a rank-4 array in elements, in any order of its
-    dimensions; 0 for a dimension of one element, whose stride says nothing."""
+def _strides(x):
+    """(pointer, strides...) of an array in elements, in any order of its dimensions; 0 for
+    a dimension of one element, whose stride says nothing."""
     if _is_torch(x):
         p, st = x.data_ptr(), x.stride()
     else:
+        if any(s % x.itemsize for s in x.strides):
+            raise ValueError("strides must be whole elements")
         p, st = x.ctypes.data, [s // x.itemsize for s in x.strides]
     return [p, *(0 if n == 1 else s for n, s in zip(x.shape, st))]
 

@@ -1141,7 +1141,7 @@ int32_t simp_rt_attention_packed_f32(
   if (q_s0 == 0 || q_s1 == 0 || n == 0) return SIMP_RT_OK;
   if (q_s0 > INT32_MAX - 64 || k_s0 > INT32_MAX - 64 || q_s1 > 65535 || n > INT32_MAX / 65536)
     return set_error(SIMP_RT_EUNSUPPORTED, "attention_packed: more rows, heads or sequences than the grid holds");
-  if (k_st0 >= 1 << 23 || v_st0 >= 1 << 23)  // 32-bit offsets within 32 rows
+  if (dk.st[0] >= 1 << 23 || dv.st[0] >= 1 << 23)  // 32-bit offsets within 32 rows
     return set_error(SIMP_RT_EUNSUPPORTED, "attention_packed: rows of k or v 2^23 elements or more apart");
   if (overlap(dout.data(), dout.bytes(), dq.data(), dq.bytes()) ||
       overlap(dout.data(), dout.bytes(), dk.data(), dk.bytes()) ||
@@ -1166,13 +1166,13 @@ int32_t simp_rt_attention_packed_f32(
   a.out = (float *)oo.dev();
   a.q_starts = (const int *)oqs.dev();
   a.k_starts = (const int *)oks.dev();
-  a.q_row = q_st0, a.q_head = q_st1, a.k_row = k_st0, a.k_head = k_st1;
-  a.v_row = v_st0, a.v_head = v_st1, a.o_row = out_st0, a.o_head = out_st1;
+  a.q_row = dq.st[0], a.q_head = dq.st[1], a.k_row = dk.st[0], a.k_head = dk.st[1];
+  a.v_row = dv.st[0], a.v_head = dv.st[1], a.o_row = dout.st[0], a.o_head = dout.st[1];
   a.tq = (int)q_s0, a.tk = (int)k_s0, a.n = (int)n;
   a.group = (int)(q_s1 / k_s1), a.hs = (int)q_s2;
   a.scale = (float)scale;
   const bool vec = a.hs % 4 == 0 &&
-                   ((q_st0 | q_st1 | k_st0 | k_st1 | v_st0 | v_st1 | out_st0 | out_st1) & 3) == 0 &&
+                   ((a.q_row | a.q_head | a.k_row | a.k_head | a.v_row | a.v_head | a.o_row | a.o_head) & 3) == 0 &&
                    (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) & 15) == 0;
   if ((rc = launch_packed(a, (int)q_s1, vec, cur_stream()))) return rc;
   Operand *ops[] = {&oq, &ok, &ov, &oo, &oqs, &oks};

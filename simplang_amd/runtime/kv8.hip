@@ -1213,9 +1213,9 @@ int32_t simp_rt_kv8_append(
       (rc = bind_here(ol, lengths + len_off, 4 * (size_t)len_size, Operand::kIn, dev, "lengths")))
     return rc;
   const AppendArgs a{bc.c, (const float *)ok.dev(), (const float *)ov.dev(), (const int *)os.dev(),
-                     (const int *)ol.dev(), k_st0, k_st1, v_st0, v_st1, (int)k_s0, per_of(bc.c.hs / 4)};
+                     (const int *)ol.dev(), dk.st[0], dk.st[1], dv.st[0], dv.st[1], (int)k_s0, per_of(bc.c.hs / 4)};
   const dim3 grid((unsigned)slots, (unsigned)bc.c.hk, 2);
-  const bool vec = ((k_st0 | k_st1 | v_st0 | v_st1) & 3) == 0 && (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0;
+  const bool vec = ((a.k_row | a.k_head | a.v_row | a.v_head) & 3) == 0 && (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0;
   const int64_t chunks = (int64_t)cache->block * bc.c.hs / 4;  // of a whole block
 #define APPEND(N)                                                                              \
   do {                                                                                         \
@@ -1270,9 +1270,9 @@ int32_t simp_rt_kv8_read(
       (rc = bind_here(ol, lengths + len_off, 4 * (size_t)len_size, Operand::kIn, dev, "lengths")))
     return rc;
   const ReadArgs a{bc.c, (const int *)os.dev(), (const int *)ol.dev(), (float *)ok.dev(),
-                   (float *)ov.dev(), k_st0, k_st1, v_st0, v_st1, (int)k_s0};
+                   (float *)ov.dev(), dk.st[0], dk.st[1], dv.st[0], dv.st[1], (int)k_s0};
   const dim3 grid((unsigned)cdiv(k_s0, kReadRows), (unsigned)bc.c.hk);
-  if (((k_st0 | k_st1 | v_st0 | v_st1) & 3) == 0 && (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0)
+  if (((a.k_row | a.k_head | a.v_row | a.v_head) & 3) == 0 && (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0)
     hipLaunchKernelGGL(kv8_read_k<true>, grid, dim3(256), 0, cur_stream(), a);
   else
     hipLaunchKernelGGL(kv8_read_k<false>, grid, dim3(256), 0, cur_stream(), a);
@@ -1315,7 +1315,7 @@ int32_t simp_rt_kv8_attention(
   if (!scale_fits(scale)) return set_error(SIMP_RT_EINVAL, "kv8_attention: scale must be finite, also in fp32 and times log2(e)");
   if (q_s1 > 32767 || q_s1 / cache->n_kv_heads > 4096)
     return set_error(SIMP_RT_EUNSUPPORTED, "kv8_attention: heads above 32767, or 4096 to a kv head");
-  const bool in_place = with && dsi.data() == dso.data() && si_st0 == so_st0 && si_st1 == so_st1;
+  const bool in_place = with && dsi.data() == dso.data() && dsi.st[0] == dso.st[0] && dsi.st[1] == dso.st[1];
   const auto with_lengths = [&](const void *p, size_t n) { return overlap(p, n, lengths + len_off, 4 * (size_t)len_size); };
   if (overlap(dout.data(), dout.bytes(), dq.data(), dq.bytes()) ||
       bc.shares(cache, dout.data(), dout.bytes()) || with_lengths(dout.data(), dout.bytes()) ||
@@ -1343,8 +1343,8 @@ int32_t simp_rt_kv8_attention(
   a.out = (float *)oo.dev();
   a.seen_in = (const float *)osi.dev();
   a.seen_out = (float *)oso.dev();
-  a.q_seq = q_st0, a.q_head = q_st1, a.o_seq = out_st0, a.o_head = out_st1;
-  a.si_seq = si_st0, a.si_head = si_st1, a.so_seq = so_st0, a.so_head = so_st1;
+  a.q_seq = dq.st[0], a.q_head = dq.st[1], a.o_seq = dout.st[0], a.o_head = dout.st[1];
+  a.si_seq = dsi.st[0], a.si_head = dsi.st[1], a.so_seq = dso.st[0], a.so_head = dso.st[1];
   a.heads = (int)q_s1, a.group = (int)(q_s1 / cache->n_kv_heads);
   a.scale = (float)(scale * 1.4426950408889634);
   hipStream_t st = cur_stream();
@@ -1455,7 +1455,7 @@ int32_t simp_rt_kv8_evict(
       (rc = bind_here(op, dp.data(), dp.bytes(), Operand::kOut, dev, "kept")))
     return rc;
   EvictArgs a{bc.c, bt.c, (const int *)ol.dev(), (const float *)os.dev(), (float *)on.dev(),
-                    (int *)op.dev(), se_st0, se_st1, ns_st0, ns_st1, kept_st0, kept_st1,
+                    (int *)op.dev(), ds.st[0], ds.st[1], dn.st[0], dn.st[1], dp.st[0], dp.st[1],
                     (int)budget, (int)recent, 0};
   hipStream_t st = cur_stream();
   hipLaunchKernelGGL(kv8_select_k, dim3((unsigned)bc.c.hk, (unsigned)bc.c.n), dim3(1024), 0, st, a);

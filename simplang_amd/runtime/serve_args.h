@@ -14,7 +14,15 @@ template <class T>
 struct Desc3 {
   T *p;
   int64_t off, s[3], st[3], span;
-  int check(const char *name) { return check_descn(name, p, off, 3, s, st, &span); }
+  // A dimension of one element may have any stride: it gets the span of those inside it.
+  int check(const char *name) {
+    uint64_t inner = 1;  // (what overflows is refused below)
+    for (int i = 2; i >= 0; i--) {
+      if (s[i] == 1) st[i] = (int64_t)inner;
+      inner += (uint64_t)(s[i] - 1) * (uint64_t)st[i];
+    }
+    return check_descn(name, p, off, 3, s, st, &span);
+  }
   bool is(int64_t a, int64_t b, int64_t c) const { return s[0] == a && s[1] == b && s[2] == c; }
   T *data() const { return p + off; }
   size_t bytes() const { return (size_t)span * sizeof(T); }
@@ -68,15 +76,10 @@ inline bool meet(const Level *level, int levels, int64_t delta) {
 template <class T>
 bool share(const Desc3<T> &a, const Desc3<T> &b) {
   if (!overlap(a.data(), a.bytes(), b.data(), b.bytes())) return false;
-  if (((uintptr_t)a.data() ^ (uintptr_t)b.data()) % sizeof(T)) return true;
-  const auto apart = [&](int64_t period, int64_t n) {  // runs of n elements, one each period
-    const int64_t d = ((int64_t)((uintptr_t)b.data() - (uintptr_t)a.data()) / (int64_t)sizeof(T)) % period;
-    const int64_t to = d < 0 ? d + period : d;
-    return to >= n && period - to >= n;
-  };
-  if (a.st[0] != b.st[0] || a.st[1] != b.st[1]) return true;
-  return !apart(a.st[0], (a.s[1] - 1) * a.st[1] + a.s[2]) &&
-         !(a.st[0] % a.st[1] == 0 && apart(a.st[1], a.s[2]));
+  const int64_t bytes = (int64_t)((uintptr_t)b.data() - (uintptr_t)a.data());
+  if (bytes % (int64_t)sizeof(T) || a.st[0] != b.st[0] || a.st[1] != b.st[1]) return true;
+  const Level l[] = {{a.s[0], a.st[0]}, {a.s[1], a.st[1]}, {a.s[2], 1}};
+  return meet(l, 3, bytes / (int64_t)sizeof(T));
 }
 
 }  // namespace simp

@@ -127,3 +127,34 @@ def test_huge_queries_over_tiny_codes(dev, heads):
     q = np.zeros((2, heads, 64), np.float32)
     q[..., 0] = 1e36
     _attend(p, q, [300, 77], seen=np.zeros((2, 1, 300), np.float32))
+
+
+@pytest.mark.parametrize("odd", [0, 3, 1 << 40])
+def test_strides_of_one_row_and_one_head(dev, odd):
+    """One row, one head: their strides are any number."""
+    import torch
+    from test_gpu_kv8 import Pair, _rows
+    p = Pair(dev, 1, 1, 40, 64, 16)
+
+    def one(x):
+        return torch.as_strided(x, x.shape, (odd, odd, 1)) if odd < 99 else torch.as_strided(x, x.shape, (odd, odd + 1, 1))
+
+    k, v = _rows(1, 1, 64)
+    st, ln = np.array([0, 1], np.int32), np.array([21], np.int32)
+    p.np.append(k, v, st, ln)
+    up = p.up(k, v, st, ln)
+    p.gpu.append(one(up[0]), one(up[1]), *up[2:])
+    p.same()
+    back = [torch.zeros((1, 1, 64), device=dev) for _ in range(2)]
+    want = np.zeros((2, 1, 1, 64), np.float32)
+    p.np.read(st, ln, *want)
+    p.gpu.read(*up[2:], one(back[0]), one(back[1]))
+    assert all(np.array_equal(b.cpu().numpy(), w) for b, w in zip(back, want))
+    q = p.up(k)[0]
+    out = torch.zeros_like(q)
+    p.gpu.attention(one(q), up[3], one(out))
+    ref, _, tol, _ = p.np.attention(k, ln, 0.125)
+    assert (np.abs(out.cpu().numpy() - ref) <= tol[..., None]).all()
+    out.fill_(7)
+    sa.attention_packed(one(q), one(back[0]), one(back[1]), one(out), up[2], up[2])
+    assert np.abs(out.cpu().numpy() - want[1]).max() <= 4 * S.EPS * np.abs(want[1]).max()

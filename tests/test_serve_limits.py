@@ -90,3 +90,46 @@ def test_scales_that_share_memory_are_refused():
     sa.KV8Cache(k, v, z[:, :, 0], z[:, :, 1], 16).append(*_rows(n=0, h=3), np.zeros(3, I), np.zeros(2, I))
     with pytest.raises(sa.SimpRTError, match="same memory"):
         sa.KV8Cache(k, v, z[:, :, 0], _part(z[:, :, 1], 1), 16).append(*_rows(h=3), np.zeros(3, I), np.zeros(2, I))
+
+
+def test_strides_of_dimensions_of_one_element_say_nothing():
+    """One sequence, one head, one block of scales, one row: numpy gives a new dimension the
+    stride 0, and a part of a larger tensor keeps the larger one's."""
+    k, v, ks, vs = _cache(b=1, h=1, cap=16)
+    whole = np.zeros((1, 1, 7), F)
+    c = sa.KV8Cache(k, v, whole[:, :, 3:4], vs[0, 0][None, None], 16)
+    c.append(*_rows(n=0, h=1), np.zeros(2, I), np.zeros(1, I))
+    c = sa.KV8Cache(k, v, np.zeros((1, 1, 9), F)[:, :, ::9], vs, 16)
+    c.append(*_rows(n=0, h=1), np.zeros(2, I), np.zeros(1, I))
+    q = np.zeros((4, 32), F)
+    # as far as the first check behind the descriptors'
+    a = dict(q=q[None], k=q[:2][None], v=q[:2][None], out=q.copy()[None], q_starts=np.zeros(2, I), k_starts=np.zeros(2, I))
+    with pytest.raises(sa.SimpRTError, match="finite"):
+        sa.attention_packed(**a, scale=float("nan"))
+    a = dict(q=q[:, None], k=q[:, None], v=q[:, None], out=q.copy()[:, None], q_starts=np.zeros(2, I), k_starts=np.zeros(2, I))
+    with pytest.raises(sa.SimpRTError, match="finite"):
+        sa.attention_packed(**a, scale=float("nan"))
+    for x in (q[None, :1], q[:1, None], q[:1][None]):
+        with pytest.raises(sa.SimpRTError, match="finite"):
+            c.attention(x, np.zeros(1, I), x.copy(), scale=float("nan"))
+
+
+def test_read_of_one_row_between_the_heads():
+    """K and V of one token, head by head in turn: as far as the cache's own check."""
+    x = np.zeros((1, 2, 2, 32), F)
+    c = sa.KV8Cache(*_cache(b=1), 16)
+    st, ln = np.zeros(2, I), np.zeros(1, I)
+    for k, v in ((x[:, :, 0], x[:, :, 1]), (x[0, :, 0][None], x[0, :, 1][None])):
+        with pytest.raises(sa.SimpRTError) as e:
+            c.read(st, ln, k, v)
+        assert "shares memory" not in str(e.value)
+        with pytest.raises(sa.SimpRTError, match="shares memory"):
+            c.read(st, ln, k, _part(v, 1))
+
+
+def test_lists_of_one_element_have_any_stride():
+    x = np.zeros((5, 3), I)
+    c = sa.KV8Cache(*_cache(b=1), 16)
+    c.append(*_rows(n=0), np.zeros(2, I), x[2:3, 1])
+    with pytest.raises(ValueError, match="contiguous"):
+        c.append(*_rows(n=0), x[1:3, 1], x[2:3, 1])
