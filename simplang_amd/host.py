@@ -578,7 +578,7 @@ def attention_packed(q, k, v, out, q_starts, k_starts, scale=None):
     1 / sqrt(head_size) by default."""
     fn = "attention_packed"
     if scale is None:
-        scale = q.shape[-1] ** -0.5
+        scale = max(q.shape[-1], 1) ** -0.5
     _check(fn, lib.simp_rt_attention_packed_f32(
         *_rows(fn, "q", q), *_rows(fn, "k", k), *_rows(fn, "v", v), *_rows(fn, "out", out),
         *_list(fn, "q_starts", q_starts), *_list(fn, "k_starts", k_starts), scale))
@@ -608,6 +608,8 @@ class KV8Cache:
         if len(k.shape) != 4 or tuple(v.shape) != tuple(k.shape):
             raise ValueError("KV8Cache: k and v must be [batch, kv_heads, capacity, head_size]")
         b, h, cap, hs = (int(x) for x in k.shape)
+        if block < 1:
+            raise ValueError("KV8Cache: block must be 16, 32, 64 or 128")
         if tuple(k_scale.shape) != (b, h, -(-cap // block)) or tuple(v_scale.shape) != tuple(k_scale.shape):
             raise ValueError("KV8Cache: scales must be [batch, kv_heads, ceil(capacity / block)]")
         kd, vd = _strides(_typed(fn, "k", k, "int8")), _strides(_typed(fn, "v", v, "int8"))

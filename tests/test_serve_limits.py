@@ -92,6 +92,14 @@ def test_scales_that_share_memory_are_refused():
         sa.KV8Cache(k, v, z[:, :, 0], _part(z[:, :, 1], 1), 16).append(*_rows(h=3), np.zeros(3, I), np.zeros(2, I))
 
 
+@pytest.mark.parametrize("block", [0, -16, 8, 24, 256])
+def test_blocks_that_are_none_are_refused(block):
+    a = _cache()
+    with pytest.raises(ValueError, match="block"):
+        sa.KV8Cache(*a[:2], np.zeros((2, 2, 3), F), np.zeros((2, 2, 3), F), block).append(
+            *_rows(n=0), np.zeros(3, I), np.zeros(2, I))
+
+
 def test_strides_of_dimensions_of_one_element_say_nothing():
     """One sequence, one head, one block of scales, one row: numpy gives a new dimension the
     stride 0, and a part of a larger tensor keeps the larger one's."""
@@ -133,3 +141,8 @@ def test_lists_of_one_element_have_any_stride():
     c.append(*_rows(n=0), np.zeros(2, I), x[2:3, 1])
     with pytest.raises(ValueError, match="contiguous"):
         c.append(*_rows(n=0), x[1:3, 1], x[2:3, 1])
+
+
+def test_no_head_size_is_refused():
+    with pytest.raises(sa.SimpRTError, match="1..256"):
+        sa.attention_packed(**_prompt(hs=0))
