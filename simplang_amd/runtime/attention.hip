@@ -1017,9 +1017,17 @@ void launch_f16(const F16Args &a, hipStream_t st) {
                        dim3(256), (unsigned)(4 * a.splits * std::min<int64_t>(heads, 1024 / a.p.hs + 2)), st, a);
 }
 
-int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
-  const int nb = p.hs <= 32 ? 1 : p.hs <= 64 ? 2 : p.hs <= 96 ? 3 : p.hs <= 128 ? 4 : p.hs <= 192 ? 6 : 8;
-  F16Args a{};
+// How a call is computed, and where in its scratch what lies.
+struct Plan {
+  F16Args a;
+  int nb;
+  bool stored;
+  size_t frags, scales, part, stat, bytes;  // offsets, and all of it
+};
+
+int plan_packed(const PackedArgs &p, int heads, bool may_store, Plan &plan) {
+  plan.nb = p.hs <= 32 ? 1 : p.hs <= 64 ? 2 : p.hs <= 96 ? 3 : p.hs <= 128 ? 4 : p.hs <= 192 ? 6 : 8;
+  F16Args &a = plan.a = F16Args{};
   a.p = p;
   a.hk = heads / p.group;
   // attn_stages_k and its traffic pay where about 24 blocks of four waves or more would
@@ -1027,7 +1035,7 @@ int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
   // 4096 (128) 400 against 537; 512 (16) 46 against 39, 2048 of 16 over 16, 64 wide (16) 75
   // against 66.
   const int64_t rows = cdiv(p.tq, p.n), keys = cdiv(p.tk, p.n);  // of a sequence, on average
-  const bool stored = rows * p.group >= 24 * 128;
+  const bool stored = plan.stored = may_store && rows * p.group >= 24 * 128;
   // Eight waves share a fetched stage where their registers leave room for two on a SIMD.
   const int nw = stored && p.hs <= 128 ? 8 : 4;
   const int64_t slots = p.tk / kStageKeys + p.n, blocks = (int64_t)(p.tq / 32 + p.n) * p.group / nw + p.n;
@@ -1058,24 +1066,38 @@ int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
     }
   }
   const size_t parts = a.splits > 1 ? (size_t)a.splits * p.tq * heads : 0;
-  size_t bytes = 0;
-  auto take = [&](size_t n) { return std::exchange(bytes, bytes + (n + 15) / 16 * 16); };
-  const size_t frags = take(stored ? (size_t)a.slots * a.hk * nb * 8 * 1024 : 0);
-  const size_t scales = take(stored ? (size_t)a.slots * a.hk * sizeof(float4) : 0);
-  const size_t part = take(parts * p.hs * 4), stat = take(parts * sizeof(float2));
+  plan.bytes = 0;
+  auto take = [&](size_t n) { return std::exchange(plan.bytes, plan.bytes + (n + 15) / 16 * 16); };
+  plan.frags = take(stored ? (size_t)a.slots * a.hk * plan.nb * 8 * 1024 : 0);
+  plan.scales = take(stored ? (size_t)a.slots * a.hk * sizeof(float4) : 0);
+  plan.part = take(parts * p.hs * 4);
+  plan.stat = take(parts * sizeof(float2));
+  return SIMP_RT_OK;
+}
+
+int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
+  Plan plan;
+  int rc = plan_packed(p, heads, true, plan);
+  if (rc) return rc;
   Workspace ws;
-  if (bytes) {
-    char *w;
-    if (int rc = ws.get(st, bytes, (void **)&w, 9)) return rc;
-    a.frags = (uint4 *)(w + frags);
-    a.scales = (float4 *)(w + scales);
-    a.part = (float *)(w + part);
-    a.stat = (float2 *)(w + stat);
+  char *w = nullptr;
+  // The stages take as much memory as K and V.  Where there is none, or a captured call's
+  // warm-up left none, the blocks make them for themselves.
+  if (plan.stored && !ws.try_get(st, plan.bytes, (void **)&w, 9) &&
+      (rc = plan_packed(p, heads, false, plan)))
+    return rc;
+  if (!plan.stored && plan.bytes && (rc = ws.get(st, plan.bytes, (void **)&w, 9))) return rc;
+  F16Args &a = plan.a;
+  if (w) {
+    a.frags = (uint4 *)(w + plan.frags);
+    a.scales = (float4 *)(w + plan.scales);
+    a.part = (float *)(w + plan.part);
+    a.stat = (float2 *)(w + plan.stat);
   }
 #define F16(NB, NW, NS, STORED) \
   vec ? launch_f16<NB, NW, NS, true, STORED>(a, st) : launch_f16<NB, NW, NS, false, STORED>(a, st)
-  if (stored) {
-    switch (nb) {
+  if (plan.stored) {
+    switch (plan.nb) {
       case 1: F16(1, 8, 4, true); break;
       case 2: F16(2, 8, 4, true); break;
       case 3: F16(3, 8, 4, true); break;
@@ -1084,7 +1106,7 @@ int launch_packed(const PackedArgs &p, int heads, bool vec, hipStream_t st) {
       default: F16(8, 4, 2, true);
     }
   } else {
-    switch (nb) {
+    switch (plan.nb) {
       case 1: F16(1, 4, 2, false); break;
       case 2: F16(2, 4, 2, false); break;
       case 3: F16(3, 4, 2, false); break;

@@ -158,3 +158,41 @@ def test_strides_of_one_row_and_one_head(dev, odd):
     out.fill_(7)
     sa.attention_packed(one(q), one(back[0]), one(back[1]), one(out), up[2], up[2])
     assert np.abs(out.cpu().numpy() - want[1]).max() <= 4 * S.EPS * np.abs(want[1]).max()
+
+
+def test_capture_of_a_long_prompt_without_a_warm_up_call(dev):
+    """Where the scratch for K and V taken apart ahead cannot be had, the blocks take them
+    apart for themselves; after a warm-up call it is had."""
+    import torch
+    q, k, v = _inputs(900, 900, 4, 1, 64)
+    more = _inputs(900, 900, 4, 1, 64, seed=1)
+    want = [_want(*x, np.zeros(900, bool)) for x in ((q, k, v), more)]
+    t = [torch.from_numpy(x).to(dev) for x in (q, k, v)]
+    up = [torch.from_numpy(x).to(dev) for x in more]
+    n = 32  # as many sequences of the same rows: enough blocks without splitting the keys
+    wide = [x.repeat(n, 1, 1) for x in t]
+    starts = torch.arange(0, 900 * n + 1, 900, dtype=torch.int32, device=dev)
+    out = torch.zeros_like(wide[0])
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    try:
+        sa.set_stream(stream)
+        g = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+        for i in range(2):
+            with torch.cuda.graph(g[i], stream=stream):
+                sa.attention_packed(*wide, out, starts, starts)
+            if i == 0:
+                sa.attention_packed(*wide, out, starts, starts)
+                stream.synchronize()
+        for x, (ref, tol) in zip((t, up, t), (want[0], want[1], want[0])):
+            for a, b in zip(wide, x):
+                a.copy_(b.repeat(n, 1, 1))
+            for y in g:
+                out.fill_(5)
+                torch.cuda.synchronize()
+                y.replay()
+                torch.cuda.synchronize()
+                got = out.view(n, *q.shape).cpu().numpy()
+                assert (np.abs(got - ref) <= tol[..., None]).all()
+    finally:
+        sa.set_stream(torch.cuda.current_stream())
