@@ -180,8 +180,9 @@ __device__ __forceinline__ void attend16(const PackedArgs &a, const float *qr, c
 //   attn_join_k    where there are few units the keys are split over several blocks; this
 //                  joins what they leave.
 // A block whose keys the split form does not serve (a value that is not finite, or sizes
-// too far apart) computes its rows in fp32 instead (2048 tokens of 32 heads over 8, 128 wide,
-// with a NaN in the last value and 1e30 in the first: 979 us for 170).
+// too far apart), and a wave whose queries it does not, compute their rows in fp32 instead
+// (2048 tokens of 32 heads over 8, 128 wide, with a NaN in the last value and 1e30 in the
+// first: 979 us for 170).
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -197,6 +198,8 @@ constexpr int kSpread = 14;
 // stages has a sum of 2^13 there or more, and 24 bits below its largest value stay above fp32's
 // subnormals as long as the scaling does not rise by more than this behind its last key.
 constexpr int kClimb = 64;
+// What lies this far below the largest element of its query keeps 23 bits or fewer.
+constexpr int kWide = 16;
 
 struct F16Args {
   PackedArgs p;
@@ -775,6 +778,7 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
 
   h8 qh[2 * NB], ql[2 * NB];
   float qf;
+  bool wide = false;  // some query of the wave spreads too far
   {
     const float *qr = a.q + (int64_t)(z.qb + row) * a.q_row + un.head * a.q_head;
     uint32_t top = 0;
@@ -794,6 +798,20 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
       float u = __uint_as_float(top), v = u;
       permlane32_swap(u, v);
       top = max(__float_as_uint(u), __float_as_uint(v));
+    }
+    // A query most of whose elements lie far below its largest: one channel masks keys, say,
+    // and the others, which decide, would keep few bits in its scaling.
+    {
+      const uint32_t limit = (uint32_t)max((int)top - (kWide << 23), 1) - 1;
+      int low = 0;
+#pragma unroll
+      for (int ds = 0; ds < 2 * NB; ds++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) low += bits_of(x[ds][e]) - 1 < limit;
+      float u = __int_as_float(low), v = u;
+      permlane32_swap(u, v);
+      low = __float_as_int(u) + __float_as_int(v);
+      wide = __any(2 * low > a.hs && low > 1);
     }
     const int eq = top < 0x7f800000u ? lift(top) : 0;  // infinities and NaN come through
     const float sign = a.scale < 0.f ? -1.f : 1.f;
@@ -889,7 +907,7 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
   }
   const int64_t part_row = ((int64_t)split * a.tq + z.qb) * (args.hk * a.group) + un.head;
   const int part_step = args.hk * a.group;
-  if (odd) {
+  if (odd || wide) {
     // In fp32, the wave's 32 queries 16 at a time over the block's keys.
     for (int q0 = row0; !idle && q0 < min(row0 + 32, z.nq); q0 += 16) {
       const int r16 = lane & 15, g = lane >> 4, r = min(q0 + r16, z.nq - 1);

@@ -28,17 +28,18 @@ def _run(dev, q, k, v, scale=None):
     return out.cpu().numpy()
 
 
-def _want(q, k, v, gone):
+def _want(q, k, v, gone, scale=None):
     """(out, bound) in 64 bits, with the keys in `gone` left out."""
+    scale = q.shape[2] ** -0.5 if scale is None else scale
     nq, nk, group = len(q), len(k), q.shape[1] // k.shape[1]
     hidden = np.arange(nk)[None, :] > np.arange(nq)[:, None] + nk - nq
     hidden = hidden | gone[None, :]
-    out, tol = np.zeros(q.shape), np.zeros(q.shape[:2])
+    out, tol = np.zeros((*q.shape[:2], v.shape[2])), np.zeros(q.shape[:2])
     for h in range(q.shape[1]):
         x = [np.where(gone[:, None], 0, y[:, h // group]).astype(np.float64) for y in (k, v)]
         qq = q[:, h].astype(np.float64)
-        out[:, h], _ = S.attention(qq, *x, q.shape[2] ** -0.5, hidden)
-        tol[:, h] = S.row_bound(qq, *x, q.shape[2] ** -0.5, hidden)
+        out[:, h], _ = S.attention(qq, *x, scale, hidden)
+        tol[:, h] = S.row_bound(qq, *x, scale, hidden)
     return out, tol
 
 
@@ -196,3 +197,22 @@ def test_capture_of_a_long_prompt_without_a_warm_up_call(dev):
                 assert (np.abs(got - ref) <= tol[..., None]).all()
     finally:
         sa.set_stream(torch.cuda.current_stream())
+
+
+@pytest.mark.parametrize("size", [1e5, 1e9, 1e20])
+@pytest.mark.parametrize("nq, nk, heads, kv, hs", FORMS + [(5, 5, 1, 1, 33)])
+def test_a_channel_that_masks_keys(dev, nq, nk, heads, kv, hs, size):
+    """Channel 0 of a query is far above the others, and 0 in the keys that are not masked:
+    what the others add up to counts in full."""
+    q, k, v = _inputs(nq, nk, heads, kv, hs)
+    gone = np.random.default_rng(3).random(nk) < 0.3
+    gone[0] = False
+    q[..., 0], k[..., 0] = size, 0
+    k[gone, :, 0] = -1
+    if size == 1e5:
+        k[gone, :, 0] = -1e2
+    got = _run(dev, q, k, v)
+    want, tol = _want(q[..., 1:], k[..., 1:], v, gone, hs ** -0.5)
+    assert (np.abs(got - want) <= tol[..., None]).all(), float(np.max(np.abs(got - want) / tol[..., None]))
+    off = np.linalg.norm(got - want) / np.linalg.norm(want)
+    assert off < 2e-6, off
