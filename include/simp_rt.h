@@ -403,8 +403,15 @@ int32_t simp_rt_rope(
  * sequence stay as they are.  starts: i32, increasing, sequences + 1 of them;
  * values outside the rows are cut off at them.  head_size 1 to 256; rows of k and v
  * less than 2^23 elements apart.  out may share no memory range with the inputs.
- * Sums and statistics are fp32, and the products as close as fp32 ones; the values
- * of a query's keys, added up, have to stay below fp32's largest number. */
+ * Sums and statistics are fp32.  A number of q, k, v or a weight is taken as two f16 parts,
+ * 22 bits, and a product is within 3 * 2^-22 of itself: sums come out as close as
+ * fp32 ones.  The parts end 2^-39 below the largest number that they stand with:
+ * k and v, the largest of some 32 keys, and never less than 24 bits below a key's own
+ * largest; q, the query's (but a query most of whose elements are 2^-16 of its
+ * largest or less counts in full).  So a channel of v that is 2^-16 of its
+ * neighbours or less comes out with fewer bits, one of 2^-40 as 0, and so do the products
+ * of such channels of k and q.  The values of a query's keys, added up, have to stay
+ * below fp32's largest number. */
 int32_t simp_rt_attention_packed_f32(
     const float *q_alloc, const float *q, int64_t q_off, int64_t q_s0, int64_t q_s1, int64_t q_s2,
     int64_t q_st0, int64_t q_st1, int64_t q_st2,
@@ -480,11 +487,13 @@ int32_t simp_rt_kv8_read(
  * pointers, sizes 0) add up the weight that each token receives: seen_out =
  * seen_in + the sum of p over the heads that share the kv head, for the tokens
  * below the length; the rest stays as it is.  They may be the same array, and
- * share no range otherwise.  Sums and statistics are fp32; q is rounded to 24 bits of
- * its largest element, and the products with the codes are exact; the values
- * of a sequence's tokens, added up, have to stay below fp32's largest number, and
+ * share no range otherwise.  Sums and statistics are fp32.  q is rounded to 24 bits of
+ * its largest element, the weights (times the scales of V) to 24 bits of the largest
+ * among 64 tokens, and the products with the codes are exact; the values of a
+ * sequence's tokens, added up, have to stay below fp32's largest number, and
  * those below 2^-90 lose bits to gradual underflow.  At most 4096 query heads to a kv
- * head. */
+ * head.  The call takes device scratch that the library keeps: with seen, 4 bytes per query
+ * head and token of the capacity (in whole 64s), whatever the lengths. */
 int32_t simp_rt_kv8_attention(
     const simp_rt_kv8 *cache,
     const float *q_alloc, const float *q, int64_t q_off, int64_t q_s0, int64_t q_s1, int64_t q_s2,

@@ -216,3 +216,23 @@ def test_a_channel_that_masks_keys(dev, nq, nk, heads, kv, hs, size):
     assert (np.abs(got - want) <= tol[..., None]).all(), float(np.max(np.abs(got - want) / tol[..., None]))
     off = np.linalg.norm(got - want) / np.linalg.norm(want)
     assert off < 2e-6, off
+
+
+@pytest.mark.parametrize("power", [-12, -20, -28, -40, -60])
+@pytest.mark.parametrize("nq, nk, heads, kv, hs", FORMS + [(800, 811, 4, 1, 192)])
+def test_channels_far_below_the_others(dev, nq, nk, heads, kv, hs, power):
+    """Some channels of V are 2^power of the rest: off by no more than 2^-38 of the largest
+    value, besides what fp32 sums of their own size may be off.  So is the rest, by
+    channels of K that are that small."""
+    q, k, v = _inputs(nq, nk, heads, kv, hs)
+    top = np.abs(v).max()
+    small = np.arange(hs) % 7 == 3
+    v[..., small] *= np.float32(2.0 ** power)
+    k[..., np.arange(hs) % 5 == 2] *= np.float32(2.0 ** power)
+    got = _run(dev, q, k, v)
+    none = np.zeros(nk, bool)
+    want, tol = _want(q, k, v, none)
+    assert (np.abs(got - want) <= tol[..., None]).all()
+    want, tol = _want(q, k, v[..., small], none)
+    assert (np.abs(got[..., small] - want) <= tol[..., None] + 2.0 ** -38 * top).all()
+    assert np.linalg.norm(got[..., small] - want) <= (2e-6 * np.linalg.norm(want) + 2.0 ** -39 * top * want.size ** 0.5)
