@@ -410,8 +410,9 @@ int32_t simp_rt_rope(
  * largest; q, the query's (but a query most of whose elements are 2^-16 of its
  * largest or less counts in full).  So a channel of v that is 2^-16 of its
  * neighbours or less comes out with fewer bits, one of 2^-40 as 0, and so do the products
- * of such channels of k and q.  The values of a query's keys, added up, have to stay
- * below fp32's largest number. */
+ * of such channels of k and q.  Scores lose bits where scale times the query's largest
+ * element is subnormal.  The values of a query's keys, added up, have to stay below
+ * fp32's largest number. */
 int32_t simp_rt_attention_packed_f32(
     const float *q_alloc, const float *q, int64_t q_off, int64_t q_s0, int64_t q_s1, int64_t q_s2,
     int64_t q_st0, int64_t q_st1, int64_t q_st2,
