@@ -185,7 +185,7 @@ __device__ __forceinline__ void attend16(const PackedArgs &a, const float *qr, c
 // A block whose keys the split form does not serve (a value that is not finite, or sizes
 // too far apart), and a wave whose queries it does not, compute their rows in fp32 instead
 // (2048 tokens of 32 heads over 8, 128 wide, with a NaN in the last value and 1e30 in the
-// first: 979 us for 170).
+// first: 990 us for 151; with 1e9 in a channel of every query 1079).
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -1055,7 +1055,10 @@ int plan_packed(const PackedArgs &p, int heads, bool may_store, Plan &plan) {
   // make each stage: 1024 tokens of 32 heads over 8, 128 wide (32 blocks) 63 us against 77,
   // 4096 (128) 400 against 537; 512 (16) 46 against 39, 2048 of 16 over 16, 64 wide (16) 75
   // against 66.
-  const int64_t rows = cdiv(p.tq, p.n), keys = cdiv(p.tk, p.n);  // of a sequence, on average
+  // Lengths are on the device, so this and the split below go by the mean.  Batches of like
+  // sequences are what it was measured with; uneven ones pay (4096 tokens and 31 single ones
+  // beside them 499 us, alone 400; 64 single queries, one of them after 60000 tokens, 4.2 ms).
+  const int64_t rows = cdiv(p.tq, p.n), keys = cdiv(p.tk, p.n);
   const bool stored = plan.stored = may_store && rows * p.group >= 24 * 128;
   // Eight waves share a fetched stage where their registers leave room for two on a SIMD.
   const int nw = stored && p.hs <= 128 ? 8 : 4;
