@@ -407,7 +407,7 @@ int32_t simp_rt_rope(
  * 22 bits, and a product is within 3 * 2^-22 of itself: sums come out as close as
  * fp32 ones.  The parts end 2^-39 below the largest number that they stand with:
  * k and v, the largest of some 32 keys, and never less than 24 bits below a key's own
- * largest; q, the query's (but a query most of whose elements are 2^-16 of its
+ * largest; q, the query's (but a query half of whose elements are 2^-16 of its
  * largest or less counts in full).  So a channel of v that is 2^-16 of its
  * neighbours or less comes out with fewer bits, one of 2^-40 as 0, and so do the products
  * of such channels of k and q.  Scores lose bits where scale times the query's largest

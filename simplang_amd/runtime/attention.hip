@@ -802,7 +802,7 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
       permlane32_swap(u, v);
       top = max(__float_as_uint(u), __float_as_uint(v));
     }
-    // A query most of whose elements lie far below its largest: one channel masks keys, say,
+    // A query half of whose elements lie far below its largest: one channel masks keys, say,
     // and the others, which decide, would keep few bits in its scaling.
     {
       const uint32_t limit = (uint32_t)max((int)top - (kWide << 23), 1) - 1;
@@ -814,7 +814,7 @@ __global__ void __launch_bounds__(64 * NW, NB == 1 || (NB == 2 && STORED) ? 4 : 
       float u = __int_as_float(low), v = u;
       permlane32_swap(u, v);
       low = __float_as_int(u) + __float_as_int(v);
-      wide = __any(2 * low > a.hs && low > 1);
+      wide = __any(2 * low >= a.hs);
     }
     const int eq = top < 0x7f800000u ? lift(top) : 0;  // infinities and NaN come through
     const float sign = a.scale < 0.f ? -1.f : 1.f;

@@ -200,7 +200,7 @@ def test_capture_of_a_long_prompt_without_a_warm_up_call(dev):
 
 
 @pytest.mark.parametrize("size", [1e5, 1e9, 1e20])
-@pytest.mark.parametrize("nq, nk, heads, kv, hs", FORMS + [(5, 5, 1, 1, 33)])
+@pytest.mark.parametrize("nq, nk, heads, kv, hs", FORMS + [(5, 5, 1, 1, 33), (70, 70, 2, 1, 2)])
 def test_a_channel_that_masks_keys(dev, nq, nk, heads, kv, hs, size):
     """Channel 0 of a query is far above the others, and 0 in the keys that are not masked:
     what the others add up to counts in full."""
