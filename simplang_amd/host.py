@@ -616,7 +616,7 @@ class KV8Cache:
         ks, vs = _strides(_typed(fn, "k_scale", k_scale, "float32")), _strides(_typed(fn, "v_scale", v_scale, "float32"))
         if kd[1:] != vd[1:] or ks[1:] != vs[1:]:
             raise ValueError("KV8Cache: k and v, and their scales, must have the same strides")
-        if kd[4] != 1 or ks[3] > 1:
+        if kd[4] != 1 or (ks[3] != 1 and k_scale.shape[2] != 1):
             raise ValueError("KV8Cache: the innermost stride must be 1")
         self._tensors = (k, v, k_scale, v_scale)
         self.batch, self.kv_heads, self.capacity, self.head_size, self.block = b, h, cap, hs, block

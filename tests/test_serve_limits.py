@@ -146,3 +146,11 @@ def test_lists_of_one_element_have_any_stride():
 def test_no_head_size_is_refused():
     with pytest.raises(sa.SimpRTError, match="1..256"):
         sa.attention_packed(**_prompt(hs=0))
+
+
+def test_scales_whose_blocks_are_not_side_by_side_are_refused():
+    k, v = _cache(b=1, h=1)[:2]
+    s = np.zeros((1, 1, 6), F)
+    for x in (s[:, :, ::2], s[:, :, 2::-1], np.broadcast_to(s[:, :, :1], (1, 1, 3))):
+        with pytest.raises(ValueError, match="innermost"):
+            sa.KV8Cache(k, v, x, x, 16)
