@@ -252,6 +252,57 @@ int32_t simp_rt_matmul_w4s(
     float *o_alloc, float *o, int64_t o_off, int64_t o_s0, int64_t o_s1, int64_t o_st0, int64_t o_st1,
     int64_t group_size);
 
+/* ------------------------------------------------------------- MX4 -- */
+/* Microscaled 4-bit floating point (the MXFP4 format of the OCP Microscaling Formats
+ * specification 1.0); no counterparts in the reference, whose 4-bit formats are
+ * integers.  A row of K elements is ceil(K/2) bytes of E2M1 codes, two to a byte (low
+ * nibble = even element): bit 3 the sign, bits 0-2 one of 0, 0.5, 1, 1.5, 2, 3, 4, 6;
+ * and ceil(K/32) scale bytes, one for each block of 32 elements (the last may be
+ * shorter): s stands for 2^(s - 127), 255 for NaN, and an element for its code's
+ * value times that.  All rows may be strided, at any alignment.  Outputs share no
+ * element with another operand (rows of one array may lie between another's). */
+
+/* Codes and scales of fp32 rows x[rows, cols].  With m = max|x| of a block, its scale
+ * is 2^e, e = max(floor(log2 m) - 2, -127) (byte 0 for a block of zeros), and a code is
+ * x / 2^e rounded to the nearest value, ties to the even code, what lies above 6 to 6;
+ * the sign stays, also of what becomes 0.  A block with a NaN or an infinity has the
+ * scale byte 255 and codes 0: its values read NaN.  For odd cols the last byte's high
+ * nibble is 0. */
+int32_t simp_rt_quantize_mx4(
+    const float *x_alloc, const float *x, int64_t x_off, int64_t x_s0, int64_t x_s1, int64_t x_st0, int64_t x_st1,
+    uint8_t *c_alloc, uint8_t *codes, int64_t c_off, int64_t c_s0, int64_t c_s1, int64_t c_st0, int64_t c_st1,
+    uint8_t *s_alloc, uint8_t *scales, int64_t s_off, int64_t s_s0, int64_t s_s1, int64_t s_st0, int64_t s_st1);
+
+/* The values of codes and scales into fp32 rows out[rows, cols], exact (a scale of 2^126
+ * or more may give an infinity). */
+int32_t simp_rt_dequantize_mx4(
+    const uint8_t *c_alloc, const uint8_t *codes, int64_t c_off, int64_t c_s0, int64_t c_s1, int64_t c_st0, int64_t c_st1,
+    const uint8_t *s_alloc, const uint8_t *scales, int64_t s_off, int64_t s_s0, int64_t s_s1, int64_t s_st0, int64_t s_st1,
+    float *out_alloc, float *out, int64_t out_off, int64_t out_s0, int64_t out_s1, int64_t out_st0, int64_t out_st1);
+
+/* out[M,N] = A[M,K] x B[N,K]^T on MX4 rows (activations and weights alike), fp32 out,
+ * overwritten.  K is what the code bytes hold, so an odd K's last nibble has to be 0, as
+ * simp_rt_quantize_mx4 leaves it.  Products are exact and sums fp32 (of 128 products
+ * at a time, to nearest); a sum with a NaN scale in it is NaN.  K = 0 gives zeros. */
+int32_t simp_rt_matmul_mx4(
+    const uint8_t *a_alloc, const uint8_t *a, int64_t a_off, int64_t a_s0, int64_t a_s1, int64_t a_st0, int64_t a_st1,
+    const uint8_t *as_alloc, const uint8_t *a_scales, int64_t as_off, int64_t as_s0, int64_t as_s1, int64_t as_st0, int64_t as_st1,
+    const uint8_t *b_alloc, const uint8_t *b, int64_t b_off, int64_t b_s0, int64_t b_s1, int64_t b_st0, int64_t b_st1,
+    const uint8_t *bs_alloc, const uint8_t *b_scales, int64_t bs_off, int64_t bs_s0, int64_t bs_s1, int64_t bs_st0, int64_t bs_st1,
+    float *out_alloc, float *out, int64_t out_off, int64_t out_s0, int64_t out_s1, int64_t out_st0, int64_t out_st1);
+
+/* The gated half of a feed-forward block in one kernel: out[M,N] = silu(A W1^T) * (A W3^T)
+ * for A[M,K], W1[N,K] and W3[N,K] in MX4, silu(x) = x / (1 + exp(-x)) as simp_rt_swiglu
+ * computes it from the two products of simp_rt_matmul_mx4. */
+int32_t simp_rt_swiglu_mx4(
+    const uint8_t *a_alloc, const uint8_t *a, int64_t a_off, int64_t a_s0, int64_t a_s1, int64_t a_st0, int64_t a_st1,
+    const uint8_t *as_alloc, const uint8_t *a_scales, int64_t as_off, int64_t as_s0, int64_t as_s1, int64_t as_st0, int64_t as_st1,
+    const uint8_t *w1_alloc, const uint8_t *w1, int64_t w1_off, int64_t w1_s0, int64_t w1_s1, int64_t w1_st0, int64_t w1_st1,
+    const uint8_t *s1_alloc, const uint8_t *s1, int64_t s1_off, int64_t s1_s0, int64_t s1_s1, int64_t s1_st0, int64_t s1_st1,
+    const uint8_t *w3_alloc, const uint8_t *w3, int64_t w3_off, int64_t w3_s0, int64_t w3_s1, int64_t w3_st0, int64_t w3_st1,
+    const uint8_t *s3_alloc, const uint8_t *s3, int64_t s3_off, int64_t s3_s0, int64_t s3_s1, int64_t s3_st0, int64_t s3_st1,
+    float *out_alloc, float *out, int64_t out_off, int64_t out_s0, int64_t out_s1, int64_t out_st0, int64_t out_st1);
+
 /* --------------------------------------------------------------- fp32 -- */
 
 /* matmul(lhs, rhs, output, m, k, n, lhs_offset, rhs_offset, output_offset):

@@ -83,6 +83,10 @@ _sig("simp_rt_kv8_append", [_P] + _D3 * 2 + _D1 * 2)
 _sig("simp_rt_kv8_read", [_P] + _D1 * 2 + _D3 * 2)
 _sig("simp_rt_kv8_attention", [_P] + _D3 + _D1 + _D3 * 3 + [C.c_double])
 _sig("simp_rt_kv8_evict", [_P, _P] + _D1 + _D3 * 3 + [_I, _I])
+_sig("simp_rt_quantize_mx4", _D2 * 3)
+_sig("simp_rt_dequantize_mx4", _D2 * 3)
+_sig("simp_rt_matmul_mx4", _D2 * 5)
+_sig("simp_rt_swiglu_mx4", _D2 * 7)
 _sig("simp_rt_llama_create", [_P, _P, _P])
 _sig("simp_rt_llama_destroy", [_P])
 _sig("simp_rt_llama_forward", [_P, _I, _I, _P])
@@ -679,6 +683,60 @@ def _strides(x):
             raise ValueError("strides must be whole elements")
         p, st = x.ctypes.data, [s // x.itemsize for s in x.strides]
     return [p, *(0 if n == 1 else s for n, s in zip(x.shape, st))]
+
+
+# --------------------------------------------------------------------- MX4
+
+def _mat(fn, name, x, dtype="uint8"):
+    """The rank-2 descriptor of an operand of the given type."""
+    if _DTYPES.get(x.dtype) != dtype:
+        _typed(fn, name, x, dtype)
+    try:
+        p = x.data_ptr()
+    except AttributeError:
+        return descn(x, 2)
+    d = (p, p, 0, *x.shape, *x.stride())
+    if len(d) != 7:
+        raise ValueError(f"expected a rank-2 tensor, got shape {tuple(x.shape)}")
+    return d
+
+
+def quantize_mx4(x, codes, scales):
+    """Microscaled 4-bit floating point (MXFP4) of fp32 rows x [rows, cols]: codes uint8
+    [rows, ceil(cols / 2)], two E2M1 codes a byte, and one power of two for each 32 elements,
+    scales uint8 [rows, ceil(cols / 32)], as a byte s for 2^(s - 127)."""
+    fn = "quantize_mx4"
+    _check(fn, lib.simp_rt_quantize_mx4(*_mat(fn, "x", x, "float32"), *_mat(fn, "codes", codes),
+                                        *_mat(fn, "scales", scales)))
+    return codes, scales
+
+
+def dequantize_mx4(codes, scales, out):
+    """The fp32 values out [rows, cols] that :func:`quantize_mx4`'s codes and scales stand for."""
+    fn = "dequantize_mx4"
+    _check(fn, lib.simp_rt_dequantize_mx4(*_mat(fn, "codes", codes), *_mat(fn, "scales", scales),
+                                          *_mat(fn, "out", out, "float32")))
+    return out
+
+
+def matmul_mx4(a, a_scales, b, b_scales, out):
+    """out[M,N] = A[M,K] B[N,K]^T in fp32, both operands MX4 codes and scales as
+    :func:`quantize_mx4` writes them."""
+    fn = "matmul_mx4"
+    _check(fn, lib.simp_rt_matmul_mx4(
+        *_mat(fn, "a", a), *_mat(fn, "a_scales", a_scales), *_mat(fn, "b", b),
+        *_mat(fn, "b_scales", b_scales), *_mat(fn, "out", out, "float32")))
+    return out
+
+
+def swiglu_mx4(a, a_scales, w1, s1, w3, s3, out):
+    """out[M,N] = silu(A W1^T) * (A W3^T) in fp32 for A [M,K], W1 and W3 [N,K], all MX4: the
+    gated half of a feed-forward block in one kernel."""
+    fn = "swiglu_mx4"
+    _check(fn, lib.simp_rt_swiglu_mx4(
+        *_mat(fn, "a", a), *_mat(fn, "a_scales", a_scales), *_mat(fn, "w1", w1), *_mat(fn, "s1", s1),
+        *_mat(fn, "w3", w3), *_mat(fn, "s3", s3), *_mat(fn, "out", out, "float32")))
+    return out
 
 
 # ------------------------------------------------------------------ decode

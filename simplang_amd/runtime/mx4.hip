@@ -1,0 +1,450 @@
+// mx4.hip -- microscaled 4-bit floating point (MXFP4): quantisation, products and the
+// gated half of a feed-forward block.
+//
+// A value is an E2M1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) times a power of two
+// that 32 elements of a row share (OCP Microscaling Formats specification 1.0).
+// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies such operands as they are: lane l of a
+// wave holds the 32 codes (16 bytes) of block l / 16 of row l % 16, and their scale in a
+// byte of another register, so that an MX block is what one lane brings and nothing is
+// unpacked.  Checked on the device: products are exact, and the sum of 128 of them and
+// the accumulator is rounded to nearest in fp32, subnormals kept (two blocks' sums that
+// lie 2^24 apart are rounded where they meet); a scale byte of 255 makes the sum NaN,
+// also where the codes are 0.
+#include <algorithm>
+
+#include "rt_device.h"
+#include "rt_internal.h"
+#include "serve_args.h"
+
+namespace simp {
+namespace {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+// Loads and stores at any address their element allows (the type says so; the
+// compiler picks the instructions).
+typedef uint32_t u4any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u1any __attribute__((aligned(1)));
+typedef float f4any __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ uint32_t max_dpp4(uint32_t v) {  // over lanes 4i .. 4i+3
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor1, 0xF, 0xF, false));
+  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor2, 0xF, 0xF, false));
+}
+
+// 2^(s - 127) in fp32 (255: infinity)
+__device__ __forceinline__ float scale_of(uint32_t s) {
+  return __uint_as_float(s ? s << 23 : 0x00400000u);
+}
+
+// Row and column block of the i-th 32-element block of the rows, i counted from the
+// workgroup's first: one 64-bit division per workgroup, a 32-bit one per thread.
+struct BlockAt {
+  int64_t row0;
+  uint32_t rem, per;
+  __device__ BlockAt(int64_t first, int64_t per_row) {
+    row0 = first / per_row;
+    rem = (uint32_t)(first - row0 * per_row);
+    per = (uint32_t)per_row;
+  }
+  __device__ void get(uint32_t i, int64_t &row, int64_t &blk) const {
+    const uint32_t q = (rem + i) / per;
+    row = row0 + q;
+    blk = rem + i - q * per;
+  }
+};
+
+constexpr int kBlocksPerWg = 256;  // MX blocks of a workgroup of 256 threads
+
+// Four lanes to a block, eight elements each.
+__global__ void __launch_bounds__(256)
+    quantize_mx4_k(const float *__restrict__ x, int64_t ldx, uint8_t *__restrict__ codes,
+                   int64_t ldc, uint8_t *__restrict__ scales, int64_t lds, int64_t cols,
+                   int64_t per_row, int64_t blocks) {
+  const int64_t first = (int64_t)blockIdx.x * kBlocksPerWg;
+  const BlockAt at(first, per_row);
+#pragma unroll
+  for (int u = 0; u < kBlocksPerWg / 64; u++) {
+    const uint32_t i = u * 64 + (threadIdx.x >> 2);
+    if (first + i >= blocks) break;  // the four lanes of a block together
+    int64_t row, blk;
+    at.get(i, row, blk);
+    const int64_t c0 = 32 * blk + 8 * (threadIdx.x & 3);
+    const float *p = x + row * ldx + c0;
+    float v[8];
+    if (c0 + 8 <= cols) {
+      const f4any a = *(const f4any *)p, b = *(const f4any *)(p + 4);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = a[e], v[4 + e] = b[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = c0 + e < cols ? p[e] : 0.f;
+    }
+    uint32_t top = 0;  // sizes compare as whole numbers, NaN above infinity
+#pragma unroll
+    for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+    top = max_dpp4(top);
+    const bool bad = top >= 0x7F800000u;
+    const uint32_t ex = top >> 23, s = ex > 2 ? ex - 2 : 0;
+    const float unit = scale_of(s);
+    uint32_t c = 0;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], unit, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], unit, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], unit, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], unit, 3);
+    if (bad) c = 0;
+    uint8_t *o = codes + row * ldc + (c0 >> 1);
+    if (c0 + 8 <= cols) {
+      *(u1any *)o = c;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (c0 + 2 * e < cols) o[e] = (uint8_t)(c >> (8 * e));
+    }
+    if ((threadIdx.x & 3) == 0) scales[row * lds + blk] = bad ? 255 : (uint8_t)s;
+  }
+}
+
+__global__ void __launch_bounds__(256)
+    dequantize_mx4_k(const uint8_t *__restrict__ codes, int64_t ldc,
+                     const uint8_t *__restrict__ scales, int64_t lds, float *__restrict__ out,
+                     int64_t ldo, int64_t cols, int64_t per_row, int64_t blocks) {
+  const int64_t first = (int64_t)blockIdx.x * kBlocksPerWg;
+  const BlockAt at(first, per_row);
+#pragma unroll
+  for (int u = 0; u < kBlocksPerWg / 64; u++) {
+    const uint32_t i = u * 64 + (threadIdx.x >> 2);
+    if (first + i >= blocks) break;
+    int64_t row, blk;
+    at.get(i, row, blk);
+    const int64_t c0 = 32 * blk + 8 * (threadIdx.x & 3);
+    if (c0 >= cols) continue;
+    const bool whole = c0 + 8 <= cols;
+    const uint8_t *p = codes + row * ldc + (c0 >> 1);
+    uint32_t c = 0;
+    if (whole) {
+      c = *(const u1any *)p;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (c0 + 2 * e < cols) c |= (uint32_t)p[e] << (8 * e);
+    }
+    const uint32_t s = scales[row * lds + blk];
+    const float unit = scale_of(s);
+    float v[8];
+    const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, unit, 0),
+              b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, unit, 1),
+              d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, unit, 2),
+              f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, unit, 3);
+    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1];
+    v[4] = d[0], v[5] = d[1], v[6] = f[0], v[7] = f[1];
+    if (s == 255) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] = __uint_as_float(0x7FC00000u);
+    }
+    float *o = out + row * ldo + c0;
+    if (whole) {
+      *(f4any *)o = f4any{v[0], v[1], v[2], v[3]};
+      *(f4any *)(o + 4) = f4any{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (c0 + e < cols) o[e] = v[e];
+    }
+  }
+}
+
+// ------------------------------------------------------------------ products
+
+struct Mx4Args {
+  const uint8_t *a, *as, *b[2], *bs[2];  // codes and scales of A, and of B or W1 and W3
+  int64_t lda, ldas, ldb[2], ldbs[2];
+  float *out;
+  int64_t ldo;
+  int M, N, kb;  // kb: code bytes of a row
+};
+
+__device__ __forceinline__ v4f mfma_mx4(uint4 a, uint32_t sa, uint4 b, uint32_t sb, v4f c) {
+  const v8i x = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0},
+            y = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 0, (int)sa, 0, (int)sb);
+}
+
+__device__ __forceinline__ float swiglu(float g, float u) { return (g / (1.f + expf(-g))) * u; }
+
+// 16 code bytes of a row from byte k on, zeros behind its end.
+__device__ __forceinline__ uint4 row16(const uint8_t *row, int k, int kb) {
+  if (k + 16 <= kb) {
+    const u4any v = *(const u4any *)(row + k);
+    return make_uint4(v.x, v.y, v.z, v.w);
+  }
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 16; i++)
+    if (k + i < kb) w[i >> 2] |= (uint32_t)row[k + i] << (8 * (i & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// One wave to 16 x 16 outputs, operands straight from memory.
+template <int MATS>
+__global__ void __launch_bounds__(64) mx4_tile_k(const Mx4Args a) {
+  const int lane = threadIdx.x, r = lane & 15, q = lane >> 4;
+  const int tiles_n = (a.N + 15) >> 4;
+  const int m0 = 16 * (blockIdx.x / tiles_n), n0 = 16 * (blockIdx.x % tiles_n);
+  const int64_t m = min(m0 + r, a.M - 1), n = min(n0 + r, a.N - 1);
+  const uint8_t *ap = a.a + m * a.lda, *as = a.as + m * a.ldas;
+  v4f acc[MATS];
+#pragma unroll
+  for (int t = 0; t < MATS; t++) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < a.kb; k0 += 64) {
+    const int k = k0 + 16 * q;
+    const uint4 av = row16(ap, k, a.kb);
+    const uint32_t sa = k < a.kb ? as[k >> 4] : 127;
+#pragma unroll
+    for (int t = 0; t < MATS; t++) {
+      const uint4 bv = row16(a.b[t] + n * a.ldb[t], k, a.kb);
+      const uint32_t sb = k < a.kb ? a.bs[t][n * a.ldbs[t] + (k >> 4)] : 127;
+      acc[t] = mfma_mx4(bv, sb, av, sa, acc[t]);  // C^T: a lane has 4 columns of a row
+    }
+  }
+  if (m0 + r < a.M) {
+    float *o = a.out + m * a.ldo;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int col = n0 + 4 * q + e;
+      if (col < a.N) o[col] = MATS == 2 ? swiglu(acc[0][e], acc[MATS - 1][e]) : acc[0][e];
+    }
+  }
+}
+
+template <int MATS>
+int launch_mx4(const Mx4Args &a, hipStream_t st) {
+  const int64_t tiles = cdiv(a.M, 16) * cdiv(a.N, 16);
+  hipLaunchKernelGGL(mx4_tile_k<MATS>, dim3((unsigned)tiles), dim3(64), 0, st, a);
+  SIMP_HIP(hipGetLastError());
+  return SIMP_RT_OK;
+}
+
+// ------------------------------------------------------------- entry points
+
+// A rank-2 descriptor and its extent.  One row may have any stride.
+template <class T>
+struct Mat {
+  T *p;
+  int64_t off, s[2], st[2], span;
+  int check(const char *name) {
+    if (s[0] == 1) st[0] = s[1];
+    if (s[1] == 1) st[1] = 1;
+    if (const int rc = check_descn(name, p, off, 2, s, st, &span)) return rc;
+    if (s[0] > INT32_MAX - 4096 || s[1] > INT32_MAX - 4096)
+      return set_error(SIMP_RT_EUNSUPPORTED, "%s: dimension above 2^31 - 4097", name);
+    return SIMP_RT_OK;
+  }
+  T *data() const { return p + off; }
+  size_t bytes() const { return (size_t)span * sizeof(T); }
+};
+
+// Whether two arrays share an element: ranges that meet do not where both have rows of
+// one stride in bytes and each row lies in the gap between the other's.
+template <class T, class U>
+bool meets(const Mat<T> &a, const Mat<U> &b) {
+  if (!overlap(a.data(), a.bytes(), b.data(), b.bytes())) return false;
+  const int64_t st = a.st[0] * (int64_t)sizeof(T);
+  if (a.s[0] <= 1 || b.s[0] <= 1 || st != b.st[0] * (int64_t)sizeof(U)) return true;
+  const uintptr_t x = (uintptr_t)a.data(), y = (uintptr_t)b.data();
+  const int64_t d = y >= x ? (int64_t)((y - x) % (uintptr_t)st)
+                           : (st - (int64_t)((x - y) % (uintptr_t)st)) % st;
+  return d < a.s[1] * (int64_t)sizeof(T) || d + b.s[1] * (int64_t)sizeof(U) > st;
+}
+
+// K of the codes' bytes and the scales that go with them.
+int check_rows(const char *fn, const char *name, const Mat<const uint8_t> &c,
+               const Mat<const uint8_t> &s) {
+  if (s.s[0] != c.s[0] || s.s[1] != cdiv(c.s[1], 16))
+    return set_error(SIMP_RT_EINVAL,
+                     "%s: %s: shape mismatch, codes [%lld,%lld] and scales [%lld,%lld] (one for 16 bytes)",
+                     fn, name, (long long)c.s[0], (long long)c.s[1], (long long)s.s[0], (long long)s.s[1]);
+  return SIMP_RT_OK;
+}
+
+template <int MATS>
+int product(const char *fn, Mat<const uint8_t> &a, Mat<const uint8_t> &as,
+            Mat<const uint8_t> (&b)[MATS], Mat<const uint8_t> (&bs)[MATS], Mat<float> &o) {
+  static const char *const kB[2][2] = {{"b", "w1"}, {"", "w3"}},
+                           *const kS[2][2] = {{"b_scales", "s1"}, {"", "s3"}};
+  int rc;
+  if ((rc = a.check("a")) || (rc = as.check("a_scales")) || (rc = o.check("out")) ||
+      (rc = check_rows(fn, "a", a, as)))
+    return rc;
+  for (int t = 0; t < MATS; t++) {
+    const char *name = kB[t][MATS - 1];
+    if ((rc = b[t].check(name)) || (rc = bs[t].check(kS[t][MATS - 1])) ||
+        (rc = check_rows(fn, name, b[t], bs[t])))
+      return rc;
+    if (b[t].s[1] != a.s[1] || b[t].s[0] != o.s[1] || a.s[0] != o.s[0])
+      return set_error(SIMP_RT_EINVAL, "%s: shape mismatch a[%lld,%lld] %s[%lld,%lld] out[%lld,%lld]",
+                       fn, (long long)a.s[0], (long long)a.s[1], name, (long long)b[t].s[0],
+                       (long long)b[t].s[1], (long long)o.s[0], (long long)o.s[1]);
+  }
+  if (o.s[0] == 0 || o.s[1] == 0) return SIMP_RT_OK;
+  bool shared = meets(o, a) || meets(o, as);
+  for (int t = 0; t < MATS; t++) shared = shared || meets(o, b[t]) || meets(o, bs[t]);
+  if (shared) return set_error(SIMP_RT_EINVAL, "%s: out shares memory with another operand", fn);
+  const int dev = ensure_device();
+  if (dev < 0) return dev;
+  Operand oa, oas, ob[MATS], obs[MATS], oo;
+  if ((rc = bind_here(oa, a.data(), a.bytes(), Operand::kIn, dev, "a")) ||
+      (rc = bind_here(oas, as.data(), as.bytes(), Operand::kIn, dev, "a_scales")) ||
+      (rc = bind_here(oo, o.data(), o.bytes(), Operand::kOut, dev, "out")))
+    return rc;
+  Mx4Args g{};
+  g.a = (const uint8_t *)oa.dev(), g.as = (const uint8_t *)oas.dev();
+  g.lda = a.st[0], g.ldas = as.st[0];
+  for (int t = 0; t < MATS; t++) {
+    if ((rc = bind_here(ob[t], b[t].data(), b[t].bytes(), Operand::kIn, dev, kB[t][MATS - 1])) ||
+        (rc = bind_here(obs[t], bs[t].data(), bs[t].bytes(), Operand::kIn, dev, kS[t][MATS - 1])))
+      return rc;
+    g.b[t] = (const uint8_t *)ob[t].dev(), g.bs[t] = (const uint8_t *)obs[t].dev();
+    g.ldb[t] = b[t].st[0], g.ldbs[t] = bs[t].st[0];
+  }
+  g.out = (float *)oo.dev(), g.ldo = o.st[0];
+  g.M = (int)o.s[0], g.N = (int)o.s[1], g.kb = (int)a.s[1];
+  if ((rc = launch_mx4<MATS>(g, cur_stream()))) return rc;
+  Operand *ops[] = {&oa, &oas, &oo, &ob[0], &obs[0], &ob[MATS - 1], &obs[MATS - 1]};
+  return finish(ops, 3 + 2 * MATS);
+}
+
+// Blocks of the rows, and the grid for them.
+int block_grid(const char *fn, int64_t rows, int64_t per_row, int64_t *blocks, unsigned *grid) {
+  *blocks = rows * per_row;
+  const int64_t g = cdiv(*blocks, kBlocksPerWg);
+  if (g > INT32_MAX / 256) return set_error(SIMP_RT_EUNSUPPORTED, "%s: more elements than the grid holds", fn);
+  *grid = (unsigned)g;
+  return SIMP_RT_OK;
+}
+
+}  // namespace
+}  // namespace simp
+
+using namespace simp;
+
+extern "C" {
+
+int32_t simp_rt_quantize_mx4(
+    const float *x_alloc, const float *x, int64_t x_off, int64_t x_s0, int64_t x_s1, int64_t x_st0,
+    int64_t x_st1, uint8_t *c_alloc, uint8_t *codes, int64_t c_off, int64_t c_s0, int64_t c_s1,
+    int64_t c_st0, int64_t c_st1, uint8_t *s_alloc, uint8_t *scales, int64_t s_off, int64_t s_s0,
+    int64_t s_s1, int64_t s_st0, int64_t s_st1) {
+  (void)x_alloc; (void)c_alloc; (void)s_alloc;
+  static const char *fn = "quantize_mx4";
+  Mat<const float> mx{x, x_off, {x_s0, x_s1}, {x_st0, x_st1}, 0};
+  Mat<uint8_t> mc{codes, c_off, {c_s0, c_s1}, {c_st0, c_st1}, 0};
+  Mat<uint8_t> ms{scales, s_off, {s_s0, s_s1}, {s_st0, s_st1}, 0};
+  int rc;
+  if ((rc = mx.check("x")) || (rc = mc.check("codes")) || (rc = ms.check("scales"))) return rc;
+  if (c_s0 != x_s0 || s_s0 != x_s0 || c_s1 != cdiv(x_s1, 2) || s_s1 != cdiv(x_s1, 32))
+    return set_error(SIMP_RT_EINVAL,
+                     "%s: shape mismatch x[%lld,%lld] codes[%lld,%lld] scales[%lld,%lld]", fn,
+                     (long long)x_s0, (long long)x_s1, (long long)c_s0, (long long)c_s1,
+                     (long long)s_s0, (long long)s_s1);
+  if (x_s0 == 0 || x_s1 == 0) return SIMP_RT_OK;
+  if (meets(mc, mx) || meets(ms, mx) || meets(mc, ms))
+    return set_error(SIMP_RT_EINVAL, "%s: codes or scales share memory with another operand", fn);
+  int64_t blocks;
+  unsigned grid;
+  if ((rc = block_grid(fn, x_s0, s_s1, &blocks, &grid))) return rc;
+  const int dev = ensure_device();
+  if (dev < 0) return dev;
+  Operand ox, oc, os;
+  if ((rc = bind_here(ox, mx.data(), mx.bytes(), Operand::kIn, dev, "x")) ||
+      (rc = bind_here(oc, mc.data(), mc.bytes(), Operand::kOut, dev, "codes")) ||
+      (rc = bind_here(os, ms.data(), ms.bytes(), Operand::kOut, dev, "scales")))
+    return rc;
+  hipLaunchKernelGGL(quantize_mx4_k, dim3(grid), dim3(256), 0, cur_stream(), (const float *)ox.dev(),
+                     mx.st[0], (uint8_t *)oc.dev(), mc.st[0], (uint8_t *)os.dev(), ms.st[0], x_s1,
+                     s_s1, blocks);
+  SIMP_HIP(hipGetLastError());
+  Operand *ops[] = {&ox, &oc, &os};
+  return finish(ops, 3);
+}
+
+int32_t simp_rt_dequantize_mx4(
+    const uint8_t *c_alloc, const uint8_t *codes, int64_t c_off, int64_t c_s0, int64_t c_s1,
+    int64_t c_st0, int64_t c_st1, const uint8_t *s_alloc, const uint8_t *scales, int64_t s_off,
+    int64_t s_s0, int64_t s_s1, int64_t s_st0, int64_t s_st1, float *out_alloc, float *out,
+    int64_t out_off, int64_t out_s0, int64_t out_s1, int64_t out_st0, int64_t out_st1) {
+  (void)c_alloc; (void)s_alloc; (void)out_alloc;
+  static const char *fn = "dequantize_mx4";
+  Mat<const uint8_t> mc{codes, c_off, {c_s0, c_s1}, {c_st0, c_st1}, 0};
+  Mat<const uint8_t> ms{scales, s_off, {s_s0, s_s1}, {s_st0, s_st1}, 0};
+  Mat<float> mo{out, out_off, {out_s0, out_s1}, {out_st0, out_st1}, 0};
+  int rc;
+  if ((rc = mc.check("codes")) || (rc = ms.check("scales")) || (rc = mo.check("out"))) return rc;
+  if (c_s0 != out_s0 || s_s0 != out_s0 || c_s1 != cdiv(out_s1, 2) || s_s1 != cdiv(out_s1, 32))
+    return set_error(SIMP_RT_EINVAL,
+                     "%s: shape mismatch codes[%lld,%lld] scales[%lld,%lld] out[%lld,%lld]", fn,
+                     (long long)c_s0, (long long)c_s1, (long long)s_s0, (long long)s_s1,
+                     (long long)out_s0, (long long)out_s1);
+  if (out_s0 == 0 || out_s1 == 0) return SIMP_RT_OK;
+  if (meets(mo, mc) || meets(mo, ms))
+    return set_error(SIMP_RT_EINVAL, "%s: out shares memory with another operand", fn);
+  int64_t blocks;
+  unsigned grid;
+  if ((rc = block_grid(fn, out_s0, s_s1, &blocks, &grid))) return rc;
+  const int dev = ensure_device();
+  if (dev < 0) return dev;
+  Operand oc, os, oo;
+  if ((rc = bind_here(oc, mc.data(), mc.bytes(), Operand::kIn, dev, "codes")) ||
+      (rc = bind_here(os, ms.data(), ms.bytes(), Operand::kIn, dev, "scales")) ||
+      (rc = bind_here(oo, mo.data(), mo.bytes(), Operand::kOut, dev, "out")))
+    return rc;
+  hipLaunchKernelGGL(dequantize_mx4_k, dim3(grid), dim3(256), 0, cur_stream(),
+                     (const uint8_t *)oc.dev(), mc.st[0], (const uint8_t *)os.dev(), ms.st[0],
+                     (float *)oo.dev(), mo.st[0], out_s1, s_s1, blocks);
+  SIMP_HIP(hipGetLastError());
+  Operand *ops[] = {&oc, &os, &oo};
+  return finish(ops, 3);
+}
+
+int32_t simp_rt_matmul_mx4(
+    const uint8_t *a_alloc, const uint8_t *a, int64_t a_off, int64_t a_s0, int64_t a_s1,
+    int64_t a_st0, int64_t a_st1, const uint8_t *as_alloc, const uint8_t *a_scales, int64_t as_off,
+    int64_t as_s0, int64_t as_s1, int64_t as_st0, int64_t as_st1, const uint8_t *b_alloc,
+    const uint8_t *b, int64_t b_off, int64_t b_s0, int64_t b_s1, int64_t b_st0, int64_t b_st1,
+    const uint8_t *bs_alloc, const uint8_t *b_scales, int64_t bs_off, int64_t bs_s0, int64_t bs_s1,
+    int64_t bs_st0, int64_t bs_st1, float *out_alloc, float *out, int64_t out_off, int64_t out_s0,
+    int64_t out_s1, int64_t out_st0, int64_t out_st1) {
+  (void)a_alloc; (void)as_alloc; (void)b_alloc; (void)bs_alloc; (void)out_alloc;
+  Mat<const uint8_t> ma{a, a_off, {a_s0, a_s1}, {a_st0, a_st1}, 0};
+  Mat<const uint8_t> mas{a_scales, as_off, {as_s0, as_s1}, {as_st0, as_st1}, 0};
+  Mat<const uint8_t> mb[1] = {{b, b_off, {b_s0, b_s1}, {b_st0, b_st1}, 0}};
+  Mat<const uint8_t> mbs[1] = {{b_scales, bs_off, {bs_s0, bs_s1}, {bs_st0, bs_st1}, 0}};
+  Mat<float> mo{out, out_off, {out_s0, out_s1}, {out_st0, out_st1}, 0};
+  return product<1>("matmul_mx4", ma, mas, mb, mbs, mo);
+}
+
+int32_t simp_rt_swiglu_mx4(
+    const uint8_t *a_alloc, const uint8_t *a, int64_t a_off, int64_t a_s0, int64_t a_s1,
+    int64_t a_st0, int64_t a_st1, const uint8_t *as_alloc, const uint8_t *a_scales, int64_t as_off,
+    int64_t as_s0, int64_t as_s1, int64_t as_st0, int64_t as_st1, const uint8_t *w1_alloc,
+    const uint8_t *w1, int64_t w1_off, int64_t w1_s0, int64_t w1_s1, int64_t w1_st0, int64_t w1_st1,
+    const uint8_t *s1_alloc, const uint8_t *s1, int64_t s1_off, int64_t s1_s0, int64_t s1_s1,
+    int64_t s1_st0, int64_t s1_st1, const uint8_t *w3_alloc, const uint8_t *w3, int64_t w3_off,
+    int64_t w3_s0, int64_t w3_s1, int64_t w3_st0, int64_t w3_st1, const uint8_t *s3_alloc,
+    const uint8_t *s3, int64_t s3_off, int64_t s3_s0, int64_t s3_s1, int64_t s3_st0, int64_t s3_st1,
+    float *out_alloc, float *out, int64_t out_off, int64_t out_s0, int64_t out_s1, int64_t out_st0,
+    int64_t out_st1) {
+  (void)a_alloc; (void)as_alloc; (void)w1_alloc; (void)s1_alloc; (void)w3_alloc; (void)s3_alloc;
+  (void)out_alloc;
+  Mat<const uint8_t> ma{a, a_off, {a_s0, a_s1}, {a_st0, a_st1}, 0};
+  Mat<const uint8_t> mas{a_scales, as_off, {as_s0, as_s1}, {as_st0, as_st1}, 0};
+  Mat<const uint8_t> mb[2] = {{w1, w1_off, {w1_s0, w1_s1}, {w1_st0, w1_st1}, 0},
+                              {w3, w3_off, {w3_s0, w3_s1}, {w3_st0, w3_st1}, 0}};
+  Mat<const uint8_t> mbs[2] = {{s1, s1_off, {s1_s0, s1_s1}, {s1_st0, s1_st1}, 0},
+                               {s3, s3_off, {s3_s0, s3_s1}, {s3_st0, s3_st1}, 0}};
+  Mat<float> mo{out, out_off, {out_s0, out_s1}, {out_st0, out_st1}, 0};
+  return product<2>("swiglu_mx4", ma, mas, mb, mbs, mo);
+}
+
+}  // extern "C"

@@ -1,0 +1,359 @@
+"""The MX4 operators on the GPU against their plain 64-bit forms."""
+import threading
+
+import numpy as np
+import pytest
+
+import _mx4 as mx
+import simplang_amd as sa
+
+pytestmark = pytest.mark.gpu
+
+F, U = np.float32, np.uint8
+
+
+def _dev(x, dev, pad=0, shift=0, fill=0):
+    """x on the device in rows pad elements apart, the first shift elements into its memory."""
+    import torch
+    x = torch.from_numpy(np.ascontiguousarray(x))
+    m, k = x.shape
+    buf = torch.full((shift + m * (k + pad) + 1,), fill, dtype=x.dtype, device=dev)
+    v = buf[shift:shift + m * (k + pad)].view(m, k + pad)[:, :k]
+    v.copy_(x)
+    return v
+
+
+def _x(rng, m, k):
+    """Values of very different sizes, zeros, whole blocks of zeros, borders and subnormals."""
+    x = (rng.standard_normal((m, k)) * 2.0 ** rng.integers(-6, 7, (m, k))).astype(F)
+    x[rng.random((m, k)) < 0.05] = 0
+    half = np.concatenate([mx.VALUES, mx.MIDS, [7, 7.99, 5.0000005]])
+    on = rng.random((m, k)) < 0.3
+    x[on] = (half[rng.integers(0, len(half), on.sum())] * np.where(rng.random(on.sum()) < .5, -1, 1)).astype(F)
+    for j in range(mx.blocks(k)):
+        b = x[:, 32 * j:32 * j + 32]
+        p = rng.integers(0, 12, m)
+        b[p == 0] = 0
+        b[p == 1] *= F(2.0 ** -120)
+        b[p == 2] *= F(2.0 ** -60) * F(2.0 ** -70)
+        b[p == 3] *= F(2.0 ** 110)
+        b[p == 4] = F(-0.0)
+        b[p == 5] = F(2.0 ** -149)
+    return x
+
+
+SIZES = [1, 2, 7, 31, 32, 33, 63, 64, 65, 100, 255, 256, 768, 1533, 3200]
+
+
+@pytest.mark.parametrize("k", SIZES)
+@pytest.mark.parametrize("m", [1, 5, 130])
+def test_quantize_and_back(dev, m, k):
+    import torch
+    rng = np.random.default_rng(100 * k + m)
+    x = _x(rng, m, k)
+    codes, scales = mx.quantize(x)
+    for pad, shift in ((0, 0), (3, 1), (32, 16)):
+        dx = _dev(x, dev, pad, shift, 9)
+        c = _dev(np.zeros_like(codes), dev, pad, shift, 77)
+        s = _dev(np.zeros_like(scales), dev, pad, shift, 78)
+        out = _dev(np.zeros_like(x), dev, pad, shift, 5)
+        sa.quantize_mx4(dx, c, s)
+        sa.dequantize_mx4(c, s, out)
+        torch.cuda.synchronize()
+        assert np.array_equal(s.cpu().numpy(), scales)
+        assert np.array_equal(c.cpu().numpy(), codes)
+        assert np.array_equal(out.cpu().numpy(), mx.values(codes, scales)[:, :k])
+        for buf, n, f in ((c, codes.shape[1], 77), (s, scales.shape[1], 78), (out, k, 5)):
+            whole = buf._base[shift:shift + m * (n + pad)].view(m, n + pad)
+            assert (whole[:, n:] == f).all() and (buf._base[:shift] == f).all()
+
+
+def test_quantize_marks_blocks_that_are_not_finite(dev):
+    import torch
+    x = np.ones((6, 100), F)
+    x[0, 3], x[1, 40], x[2, 99], x[3, 64:96] = np.nan, np.inf, -np.inf, np.nan
+    x[4, 31] = np.float32(3.4e38)
+    codes, scales = mx.quantize(x)
+    c, s = (torch.zeros(v.shape, dtype=torch.uint8, device=dev) for v in (codes, scales))
+    out = torch.zeros(x.shape, device=dev)
+    sa.quantize_mx4(torch.from_numpy(x).to(dev), c, s)
+    sa.dequantize_mx4(c, s, out)
+    assert np.array_equal(s.cpu().numpy(), scales) and np.array_equal(c.cpu().numpy(), codes)
+    assert (scales == 255).sum() == 4
+    assert np.array_equal(out.cpu().numpy(), mx.values(codes, scales)[:, :100], equal_nan=True)
+
+
+def test_dequantize_all_codes_and_scales(dev):
+    import torch
+    c = np.tile(np.arange(256, dtype=U), (256, 1))
+    s = np.repeat(np.arange(256, dtype=U)[:, None], 16, 1)
+    out = torch.zeros((256, 512), device=dev)
+    sa.dequantize_mx4(torch.from_numpy(c).to(dev), torch.from_numpy(s).to(dev), out)
+    with np.errstate(over="ignore"):
+        want = mx.values(c, s).astype(F)
+    assert np.array_equal(out.cpu().numpy(), want, equal_nan=True)
+
+
+def _call(dev, gate, a, sa_, bs, pads=(0, 0), shifts=(0, 0), out_pad=0):
+    """The product of A and the matrices bs on the device, out's gaps and ends checked."""
+    import torch
+    m, n = a.shape[0], bs[0][0].shape[0]
+    args = []
+    for c, s in ((a, sa_), *bs):
+        # the bytes behind the rows are codes and scales that would show
+        args += [_dev(c, dev, pads[0], shifts[0], 0x77), _dev(s, dev, pads[1], shifts[1], 255)]
+    buf = torch.full((m + 2, n + out_pad), 12345.0, device=dev)
+    out = buf[1:m + 1, :n]
+    (sa.swiglu_mx4 if gate else sa.matmul_mx4)(*args, out)
+    torch.cuda.synchronize()
+    got = buf.cpu().numpy()
+    assert (got[0] == 12345).all() and (got[-1] == 12345).all() and (got[:, n:] == 12345).all()
+    return got[1:m + 1, :n]
+
+
+def _check(got, want, tol):
+    with np.errstate(all="ignore"):
+        bad = ~((np.abs(got - want) <= tol) | (np.isnan(got) & np.isnan(want)) | (got == want))
+    assert not bad.any(), (np.argwhere(bad)[:3], got[bad][:3], want[bad][:3])
+
+
+def _want(gate, a, s, bs):
+    g, tg = mx.product(a, s, *bs[0])
+    return mx.gated(g, tg, *mx.product(a, s, *bs[1])) if gate else (g, tg)
+
+
+MS = [1, 2, 3, 8, 15, 16, 17, 31, 32, 33, 48, 64, 65, 100, 128, 129, 200, 257]
+KBS = [1, 2, 8, 15, 16, 17, 32, 33, 48, 63, 64, 65, 80, 127, 128, 144, 208, 255, 256, 272, 384, 767, 1024]
+NS = [1, 3, 15, 16, 17, 31, 32, 33, 64, 65, 100, 127, 128, 129, 200, 255, 256, 257, 300]
+
+
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("i", range(69))
+def test_product_sizes(dev, gate, i):
+    """Every row count, width and column count with several others, rows at any address."""
+    m, kb, n = MS[i % len(MS)], KBS[i % len(KBS)], NS[(i * 7 + i // 19) % len(NS)]
+    rng = np.random.default_rng(i)
+    a, s = mx.codes(rng, m, kb)
+    bs = [mx.codes(rng, n, kb) for _ in range(1 + gate)]
+    got = _call(dev, gate, a, s, bs, *[((0, 0), (0, 0)), ((16, 16), (16, 16)), ((3, 1), (1, 1)), ((0, 2), (4, 2))][i % 4],
+                out_pad=(0, 0, 1, 4)[i // 4 % 4])
+    want, tol = _want(gate, a, s, bs)
+    if not gate:
+        assert np.array_equal(got, want)  # sums of these codes are exact in fp32
+    _check(got, want, tol)
+
+
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("lo, hi", [(100, 150), (60, 190), (0, 40), (200, 255), (0, 255)])
+@pytest.mark.parametrize("m, kb, n", [(1, 400, 70), (16, 1000, 40), (40, 321, 65), (150, 640, 140), (300, 1024, 300)])
+def test_product_of_scales_far_apart(dev, gate, lo, hi, m, kb, n):
+    rng = np.random.default_rng(lo + hi + m)
+    a, s = mx.codes(rng, m, kb, lo, hi)
+    bs = [mx.codes(rng, n, kb, lo, hi) for _ in range(1 + gate)]
+    got = _call(dev, gate, a, s, bs)
+    want, tol = _want(gate, a, s, bs)
+    with np.errstate(all="ignore"):
+        # where a partial sum may pass fp32's range, infinities and what follows from them are right
+        size = sum(np.abs(mx.values(a, s)) @ np.abs(mx.values(*b)).T for b in bs)
+        if gate:
+            size = np.maximum(size, np.abs(want) + tol)
+    ok = size < 3e38
+    _check(got[ok], want[ok], tol[ok])
+
+
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("m, kb, n", [(1, 100, 33), (20, 272, 65), (140, 256, 130), (300, 512, 300)])
+def test_nan_scales_touch_their_rows_only(dev, gate, m, kb, n):
+    rng = np.random.default_rng(m)
+    a, s = mx.codes(rng, m, kb)
+    bs = [mx.codes(rng, n, kb) for _ in range(1 + gate)]
+    s[m // 2, -1] = 255
+    bs[-1][1][n // 3, 0] = 255
+    got = _call(dev, gate, a, s, bs)
+    assert np.isnan(got[m // 2]).all() and np.isnan(got[:, n // 3]).all()
+    s[m // 2, -1] = 0
+    bs[-1][1][n // 3, 0] = 0
+    want, tol = _want(gate, a, s, bs)
+    keep = np.ix_(np.arange(m) != m // 2, np.arange(n) != n // 3)
+    _check(got[keep], want[keep], tol[keep])
+
+
+def test_product_of_nothing_is_zero(dev):
+    import torch
+    for m, n in ((1, 1), (20, 300)):
+        e = lambda r: torch.zeros((r, 0), dtype=torch.uint8, device=dev)
+        for f, k in ((sa.matmul_mx4, 1), (sa.swiglu_mx4, 2)):
+            out = torch.full((m, n), 7.0, device=dev)
+            f(e(m), e(m), *[x for _ in range(k) for x in (e(n), e(n))], out)
+            assert (out == 0).all()
+
+
+@pytest.mark.parametrize("m, k, h", [(1, 768, 2048), (5, 100, 333), (33, 512, 288), (200, 768, 2048)])
+def test_feed_forward_block(dev, m, k, h):
+    """quantize, swiglu_mx4, quantize, matmul_mx4, each on what the one before left."""
+    import torch
+    rng = np.random.default_rng(m)
+    x = rng.standard_normal((m, k)).astype(F)
+    w1, w3 = ((rng.standard_normal((h, k)) * 0.05).astype(F) for _ in range(2))
+    w2 = (rng.standard_normal((k, h)) * 0.05).astype(F)
+
+    def q(t):
+        c = torch.empty((t.shape[0], (t.shape[1] + 1) // 2), dtype=torch.uint8, device=dev)
+        s = torch.empty((t.shape[0], mx.blocks(t.shape[1])), dtype=torch.uint8, device=dev)
+        return sa.quantize_mx4(t, c, s)
+
+    on = lambda v: torch.from_numpy(v).to(dev)
+    W1, W3, W2, X = q(on(w1)), q(on(w3)), q(on(w2)), q(on(x))
+    hid = sa.swiglu_mx4(*X, *W1, *W3, torch.empty((m, h), device=dev))
+    out = sa.matmul_mx4(*q(hid), *W2, torch.empty((m, k), device=dev))
+    want, tol = mx.gated(*mx.product(*mx.quantize(x), *mx.quantize(w1)),
+                         *mx.product(*mx.quantize(x), *mx.quantize(w3)))
+    _check(hid.cpu().numpy(), want, tol)
+    # the second half from the hidden values that the first half left: a code may lie on
+    # either side of a border that the last bit of a hidden value crosses
+    want, tol = mx.product(*mx.quantize(hid.cpu().numpy()), *mx.quantize(w2))
+    _check(out.cpu().numpy(), want, tol)
+
+
+def test_gate_is_swiglu_of_the_two_products(dev):
+    import torch
+    rng = np.random.default_rng(3)
+    for m, kb, n in ((1, 384, 300), (40, 384, 300), (200, 1024, 520)):
+        t = [torch.from_numpy(v).to(dev) for r in (m, n, n) for v in mx.codes(rng, r, kb, 118, 124)]
+        g, u, both, want = (torch.empty((m, n), device=dev) for _ in range(4))
+        sa.matmul_mx4(*t[:4], g)
+        sa.matmul_mx4(*t[:2], *t[4:], u)
+        sa.swiglu_mx4(*t, both)
+        sa.swiglu(g.view(-1), u.view(-1), want.view(-1), m * n)
+        assert torch.equal(both, want)
+
+
+def test_host_arrays(dev):
+    rng = np.random.default_rng(5)
+    x, w = rng.standard_normal((5, 100)).astype(F), rng.standard_normal((17, 100)).astype(F)
+    q = lambda v: sa.quantize_mx4(v, np.empty((v.shape[0], 50), U), np.empty((v.shape[0], 4), U))
+    X, W = q(x), q(w)
+    for got, want in zip((*X, *W), (*mx.quantize(x), *mx.quantize(w))):
+        assert np.array_equal(got, want)
+    assert np.array_equal(sa.dequantize_mx4(*X, np.empty((5, 100), F)), mx.values(*X))
+    _check(sa.matmul_mx4(*X, *W, np.empty((5, 17), F)), *mx.product(*X, *W))
+    g, tg = mx.product(*X, *W)
+    _check(sa.swiglu_mx4(*X, *W, *W, np.empty((5, 17), F)), *mx.gated(g, tg, g, tg))
+
+
+def test_rows_far_apart(dev):
+    """Rows whose offsets pass 32 bits, in every operand."""
+    import torch
+    rng = np.random.default_rng(8)
+    far = (1 << 31) + 64
+    big = torch.empty(3 * far, dtype=torch.uint8, device=dev)
+
+    def spread(v, at):
+        t = torch.as_strided(big, v.shape, (far, 1), at)
+        t.copy_(torch.from_numpy(v))
+        return t
+
+    for m, n, kb in ((3, 3, 100), (3, 3, 256)):
+        a, s = mx.codes(rng, m, kb)
+        b, t = mx.codes(rng, n, kb)
+        d = [spread(a, 0), spread(s, 1024), spread(b, 2048), spread(t, 4096)]
+        out = torch.as_strided(big.view(torch.float32), (m, n), (far // 4, 1), 2048)
+        want, _ = mx.product(a, s, b, t)
+        sa.matmul_mx4(*d, out)
+        assert np.array_equal(out.cpu().numpy(), want)
+        x = torch.as_strided(big.view(torch.float32), (m, 2 * kb), (far // 4, 1), 8192)
+        sa.dequantize_mx4(*d[:2], x)
+        assert np.array_equal(x.cpu().numpy(), mx.values(a, s))
+        x.copy_(torch.from_numpy(_x(rng, m, 2 * kb)))
+        codes, scales = mx.quantize(x.cpu().numpy())
+        sa.quantize_mx4(x, *d[:2])
+        assert np.array_equal(d[0].cpu().numpy(), codes) and np.array_equal(d[1].cpu().numpy(), scales)
+
+
+SHAPES = [(1, 400, 300), (16, 1080, 160), (40, 767, 65), (200, 400, 540), (300, 1024, 512), (1100, 256, 1100)]
+
+
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("m, kb, n", SHAPES)
+def test_captured_and_replayed(dev, gate, m, kb, n):
+    """Replays on new inputs, with eager work between them, against eager results; another
+    graph of the stream replayed in turn."""
+    import torch
+    rng = np.random.default_rng(m)
+    f = sa.swiglu_mx4 if gate else sa.matmul_mx4
+    sizes = (m, n, n) if gate else (m, n)
+    new = lambda: [torch.from_numpy(v).to(dev) for r in sizes for v in mx.codes(rng, r, kb, 120, 125)]
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        sa.set_stream(st)
+        try:
+            t, t2 = new(), new()
+            out, out2 = (torch.zeros((m, n), device=dev) for _ in range(2))
+            f(*t, out)  # the warm-up call of this size
+            st.synchronize()
+            graphs = []
+            for args in ((t, out), (t2, out2)):
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=st):
+                    f(*args[0], args[1])
+                graphs.append(g)
+            for _ in range(3):
+                for a, b in zip(t + t2, new() + new()):
+                    a.copy_(b)
+                want = [f(*t, torch.empty_like(out)), f(*t2, torch.empty_like(out))]
+                st.synchronize()
+                for o in (out, out2):
+                    o.fill_(9)
+                for g in graphs:
+                    g.replay()
+                st.synchronize()
+                assert torch.equal(out, want[0]) and torch.equal(out2, want[1])
+        finally:
+            sa.set_stream(torch.cuda.default_stream())
+
+
+def test_two_threads_on_their_own_streams(dev):
+    import torch
+    rng = np.random.default_rng(9)
+    jobs = []
+    for m, kb, n in ((3, 767, 333), (260, 767, 333)):
+        (a, s), (b, t) = mx.codes(rng, m, kb), mx.codes(rng, n, kb)
+        jobs.append(([torch.from_numpy(v).to(dev) for v in (a, s, b, t)], mx.product(a, s, b, t)[0]))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(job):
+        torch.cuda.set_device(0)
+        st = torch.cuda.Stream()
+        sa.set_stream(st)
+        try:
+            with torch.cuda.stream(st):
+                for _ in range(20):
+                    out = torch.zeros(job[1].shape, device=dev)
+                    sa.matmul_mx4(*job[0], out)
+                    st.synchronize()
+                    if not np.array_equal(out.cpu().numpy(), job[1]):
+                        bad.append(job[1].shape)
+        except Exception as e:  # a thread's error is the test's
+            bad.append(e)
+        finally:
+            sa.set_stream(None)
+
+    ts = [threading.Thread(target=work, args=(j,)) for j in jobs for _ in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad, bad
+
+
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("m, kb, n", SHAPES + [(2, 4320, 3200), (520, 1600, 2051)])
+def test_the_same_call_gives_the_same_bits(dev, gate, m, kb, n):
+    import torch
+    rng = np.random.default_rng(m)
+    t = [torch.from_numpy(v).to(dev) for r in ((m, n, n) if gate else (m, n)) for v in mx.codes(rng, r, kb, 90, 150)]
+    f = sa.swiglu_mx4 if gate else sa.matmul_mx4
+    first = f(*t, torch.empty((m, n), device=dev))
+    for _ in range(5):
+        assert torch.equal(f(*t, torch.empty((m, n), device=dev)).nan_to_num(), first.nan_to_num())
