@@ -11,6 +11,7 @@
 // lie 2^24 apart are rounded where they meet); a scale byte of 255 makes the sum NaN,
 // also where the codes are 0.
 #include <algorithm>
+#include <type_traits>
 
 #include "rt_device.h"
 #include "rt_internal.h"
@@ -218,8 +219,259 @@ __global__ void __launch_bounds__(64) mx4_tile_k(const Mx4Args a) {
   }
 }
 
+// ---- large products: 256 x 256 tiles on an LDS-DMA ring
+
+// dma16 (rt_device.h) from a wave's base address and a lane's offset: one register instead
+// of two, so that nothing of the tile kernel's loop is spilled.
+__device__ __forceinline__ void dma16_at(const void *base, uint32_t off, uint32_t lds_off) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %2, %3\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(__builtin_amdgcn_readfirstlane(lds_off)), "v"(off), "s"(base)
+      : "memory");
+}
+
+// Scale bytes as the tile kernel reads them: for 64 rows and 4 K-steps of 128 (one
+// "group") 1 KB, 16 bytes a row, dword q of which has block q of the steps 0 .. 3 in its
+// bytes 0 .. 3.  So one DMA instruction brings a wave the scales of 64 rows for four
+// steps, a lane (row, q) keeps one register for them, and the matrix instruction
+// picks the step's byte.  Row v of W1 and W3 together: 16 rows of one, then 16 of the
+// other.  Blocks behind a row's end get 2^-127: the codes that the last stage reads in their
+// place (its first block again) then add up to less than 2^-240, which no sum notices.
+template <int MATS>
+__global__ void __launch_bounds__(256)
+    mx4_pack_scales_k(const Mx4Args a, uint4 *__restrict__ pa, uint4 *__restrict__ pb, int ga,
+                      int gb, int groups) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int r = (int)(i & 63);
+  const int64_t t = i >> 6;
+  const int g = (int)(t % groups);
+  const int64_t rg = t / groups;  // of the ga + gb row groups
+  if (rg >= ga + gb) return;
+  const bool is_a = rg < ga;
+  const int v = (int)(is_a ? rg : rg - ga) * 64 + r;
+  const int mat = !is_a && MATS == 2 ? (v >> 4) & 1 : 0;
+  const int row = !is_a && MATS == 2 ? (v >> 5) * 16 + (v & 15) : v;
+  const uint8_t *s = is_a ? a.as + (int64_t)row * a.ldas : a.bs[mat] + (int64_t)row * a.ldbs[mat];
+  const int nb = (a.kb + 15) >> 4;
+  uint32_t w[4];  // w[j]: blocks 4j .. 4j+3 of the group
+  const bool in = row < (is_a ? a.M : a.N);
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const int b0 = 16 * g + 4 * j;
+    w[j] = 0;
+    if (in && b0 + 4 <= nb) {
+      w[j] = *(const u1any *)(s + b0);
+    } else if (in) {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (b0 + e < nb) w[j] = (w[j] & ~(255u << (8 * e))) | (uint32_t)s[b0 + e] << (8 * e);
+    }
+  }
+  // 4 x 4 byte transpose
+  const uint32_t x0 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u),
+                 x1 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u),
+                 y0 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u),
+                 y1 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  const uint4 o = make_uint4(__builtin_amdgcn_perm(y0, x0, 0x05040100u),
+                             __builtin_amdgcn_perm(y0, x0, 0x07060302u),
+                             __builtin_amdgcn_perm(y1, x1, 0x05040100u),
+                             __builtin_amdgcn_perm(y1, x1, 0x07060302u));
+  (is_a ? pa + t * 64 : pb + (t - (int64_t)ga * groups) * 64)[r] = o;
+}
+
+template <int P>
+__device__ __forceinline__ v4f mfma_step(const uint4 &b, uint32_t sb, const uint4 &a, uint32_t sa, v4f c) {
+  const v8i x = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0},
+            y = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(y, x, c, 4, 4, P, (int)sb, P, (int)sa);
+}
+
+// Persistent 256 x 256 tiles (MATS == 2: of 128 columns of W1 and W3 each), 8 waves of
+// 128 x 64, K-steps of 64 code bytes through a ring of 4 stages that
+// global_load_lds_dwordx4 fills three steps ahead.
+template <int MATS>
+__global__ void __launch_bounds__(512)
+    mx4_dma_k(const Mx4Args a, const uint4 *__restrict__ pa, const uint4 *__restrict__ pb,
+              int tiles_m, int tiles_n, int groups, int stream) {
+  constexpr int BM = 256, BN = 256, BK = 64, WGN = 4, STAGES = 4;
+  constexpr int WM = 128, WN = 64, FM = WM / 16, FN = WN / 16;
+  constexpr int STAGE = (BM + BN) * BK, SCALES = (BM + BN) * 16;  // bytes
+  __shared__ uint4 lds[(STAGES * STAGE + 2 * SCALES) / 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm0 = (wave / WGN) * WM, wn0 = (wave % WGN) * WN;
+  const int nk = (a.kb + BK - 1) / BK;
+  const int ntiles = tiles_m * tiles_n;
+  const int lrow = lane & 15, lkc = lane >> 4;
+  const int drow = lane >> 2, dkc = (lane & 3) ^ ((drow >> 1) & 3);  // DMA lane -> row, chunk
+  const int rslot = lrow * 4 + (lkc ^ ((lrow >> 1) & 3));          // operand lane -> slot
+  const uint32_t lds_wave = lds_offset(lds) + 2048 * wave;  // wave w fills blocks 2w, 2w+1
+  const uint32_t lds_scale = lds_offset(lds) + STAGES * STAGE + 1024 * wave;
+  const uint32_t *sl = (const uint32_t *)(lds + STAGES * STAGE / 16) + lrow * 4 + lkc;
+
+  for (int vb = blockIdx.x; vb < ntiles; vb += gridDim.x) {
+    int tm, tn;
+    tile_of_block(vb, ntiles, tiles_m, tiles_n, tm, tn);
+    const int m0 = tm * BM, n0 = tn * (BN / MATS);
+    // a lane's rows, from the tile's first: two of A, two of B or one each of W1 and W3
+    const uint8_t *baseA = a.a + (int64_t)m0 * a.lda, *baseB0 = a.b[0] + (int64_t)n0 * a.ldb[0],
+                  *baseB1 = a.b[MATS - 1] + (int64_t)n0 * a.ldb[MATS - 1];
+    auto off = [&](int r, int rows, int64_t ld) { return (uint32_t)(min(r, rows - 1) * (uint32_t)ld) + 16 * dkc; };
+    const uint32_t offA0 = off(32 * wave + drow, a.M - m0, a.lda),
+                   offA1 = off(32 * wave + 16 + drow, a.M - m0, a.lda),
+                   offB0 = off((MATS == 2 ? 16 : 32) * wave + drow, a.N - n0, a.ldb[0]),
+                   offB1 = off((MATS == 2 ? 16 * wave : 32 * wave + 16) + drow, a.N - n0, a.ldb[MATS - 1]);
+    const uint4 *baseS = wave < 4 ? pa + (int64_t)(4 * tm + wave) * groups * 64
+                                  : pb + (int64_t)(4 * tn + wave - 4) * groups * 64;
+    // The scales of a group go ahead of its first stage.  `last`: kt may be the last
+    // stage, which can be shorter.
+    auto issue = [&](int kt, auto last) {
+      const uint32_t st = lds_wave + (kt % STAGES) * STAGE;
+      const int64_t k0 = (int64_t)kt * BK;
+      if ((kt & 3) == 0) dma16_at(baseS + (kt >> 2) * 64, 16 * lane, lds_scale + ((kt >> 2) & 1) * SCALES);
+      uint32_t back = 0;
+      if constexpr (decltype(last)::value) back = k0 + 16 * dkc < a.kb ? 0 : 16 * dkc;
+      dma16_at(baseA + k0, offA0 - back, st);
+      dma16_at(baseA + k0, offA1 - back, st + 1024);
+      dma16_at(baseB0 + k0, offB0 - back, st + BM * BK);
+      dma16_at(baseB1 + k0, offB1 - back, st + BM * BK + 1024);
+    };
+    v4f acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+      for (int j = 0; j < FN; j++) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    uint4 fa[FM], fb[2][FN];
+    uint32_t ra[FM], rb[FN], rbn[FN];  // scales of four steps
+    auto frag = [&](int kt, int blk) { return lds[(kt % STAGES) * (STAGE / 16) + blk * 64 + rslot]; };
+    constexpr int BOFF = BM * BK / 1024;  // first B block of a stage
+    auto scale = [&](int g, int row) { return sl[(g & 1) * (SCALES / 4) + 4 * row]; };
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // the previous tile's stores
+    using T = std::true_type;
+    using F = std::false_type;
+    for (int p = 0; p < min(STAGES, nk); p++) issue(p, T{});
+    if (nk >= STAGES) __builtin_amdgcn_s_waitcnt(waitcnt_vm(4 * (STAGES - 1)));
+    else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    block_barrier();
+#pragma unroll
+    for (int j = 0; j < FN; j++) fb[0][j] = frag(0, BOFF + wn0 / 16 + j), rb[j] = scale(0, BM + wn0 + 16 * j);
+#pragma unroll
+    for (int i = 0; i < FM; i++) fa[i] = frag(0, wm0 / 16 + i), ra[i] = scale(0, wm0 + 16 * i);
+    // Step kt: certify stage kt + 1, read its fragments while the MFMAs of stage kt run, and
+    // refill the buffer of stage kt.  Steady: stage kt + 4 is there and not the last.
+    // (Behind the last stage the reads bring stale LDS that is not used.)
+    auto step = [&](int kt, auto phase, auto steady) {
+      constexpr int P = decltype(phase)::value, cb = P & 1;
+      constexpr bool S = decltype(steady)::value;
+      // a group's scales are ahead of its first stage: kt + 3 or kt + 2 here
+      constexpr int vm = 4 * (STAGES - 2) + (P == 1 || P == 2);
+      if (S || kt + STAGES - 1 < nk) __builtin_amdgcn_s_waitcnt(waitcnt_vm(vm));
+      else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0);
+      block_barrier();
+#pragma unroll
+      for (int j = 0; j < FN; j++) {
+        fb[cb ^ 1][j] = frag(kt + 1, BOFF + wn0 / 16 + j);
+        if constexpr (P == 3) rbn[j] = scale((kt + 1) >> 2, BM + wn0 + 16 * j);
+      }
+#pragma unroll
+      for (int i = 0; i < FM; i++) {
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = mfma_step<P>(fb[cb][j], rb[j], fa[i], ra[i], acc[i][j]);
+        fa[i] = frag(kt + 1, wm0 / 16 + i);
+        if constexpr (P == 3) ra[i] = scale((kt + 1) >> 2, wm0 + 16 * i);
+        if (i == 3) {
+          if constexpr (S) issue(kt + STAGES, F{});
+          else if (kt + STAGES < nk) issue(kt + STAGES, T{});
+        }
+      }
+      if constexpr (P == 3) {
+#pragma unroll
+        for (int j = 0; j < FN; j++) rb[j] = rbn[j];
+      }
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I3 = std::integral_constant<int, 3>;
+    int kt = 0;
+    for (; kt + 8 < nk; kt += 4) {
+      step(kt, I0{}, T{});
+      step(kt + 1, I1{}, T{});
+      step(kt + 2, I2{}, T{});
+      step(kt + 3, I3{}, T{});
+    }
+    for (; kt < nk; kt += 4) {
+      step(kt, I0{}, F{});
+      if (kt + 1 < nk) step(kt + 1, I1{}, F{});
+      if (kt + 2 < nk) step(kt + 2, I2{}, F{});
+      if (kt + 3 < nk) step(kt + 3, I3{}, F{});
+    }
+    // acc[i][j][r] = C[m0 + wm0 + 16 i + l%16][v0 + wn0 + 16 j + 4 (l/16) + r]
+#pragma unroll
+    for (int j = 0; j < FN; j += MATS) {
+      const int col = n0 + (wn0 + 16 * j) / MATS + 4 * lkc;
+#pragma unroll
+      for (int i = 0; i < FM; i++) {
+        const int row = m0 + wm0 + 16 * i + lrow;
+        if (row >= a.M || col >= a.N) continue;
+        v4f v = acc[i][j];
+        if constexpr (MATS == 2) {
+#pragma unroll
+          for (int r = 0; r < 4; r++) v[r] = swiglu(v[r], acc[i][j + 1][r]);
+        }
+        float *dst = a.out + (int64_t)row * a.ldo + col;
+        if (stream) {
+          __builtin_nontemporal_store(v, (v4f *)dst);
+        } else if (col + 3 < a.N) {
+          *(f4any *)dst = v;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            if (col + r < a.N) dst[r] = v[r];
+        }
+      }
+    }
+  }
+}
+
+// Whether the tile kernel can read the codes: 16-byte pieces of aligned rows.
+template <int MATS>
+bool aligned16(const Mx4Args &a) {
+  uintptr_t x = (uintptr_t)a.a | (uintptr_t)a.lda | (uintptr_t)a.kb;
+  for (int t = 0; t < MATS; t++) x |= (uintptr_t)a.b[t] | (uintptr_t)a.ldb[t];
+  return (x & 15) == 0;
+}
+
 template <int MATS>
 int launch_mx4(const Mx4Args &a, hipStream_t st) {
+  const int64_t cus = num_cus();
+  const int64_t tm = cdiv(a.M, 256), tn = cdiv(a.N, 256 / MATS);
+  // (offsets within a tile are 32-bit)
+  const int64_t ld = std::max({a.lda, a.ldb[0], a.ldb[MATS - 1]});
+  if (a.kb > 0 && tm * tn >= cus / 2 && tm * tn <= INT32_MAX && ld < (1 << 23) && aligned16<MATS>(a)) {
+    const int groups = (int)cdiv(a.kb, 256), ga = (int)(4 * tm), gb = (int)(4 * tn);
+    const int64_t rgs = (int64_t)(ga + gb) * groups;
+    Workspace ws;
+    void *p;
+    if (rgs <= INT32_MAX && ws.try_get(st, (size_t)rgs * 1024, &p, 4)) {
+      uint4 *pa = (uint4 *)p, *pb = pa + (int64_t)ga * groups * 64;
+      hipLaunchKernelGGL(mx4_pack_scales_k<MATS>, dim3((unsigned)cdiv(rgs, 4)), dim3(256), 0, st, a,
+                         pa, pb, ga, gb, groups);
+      SIMP_HIP(hipGetLastError());
+      const int stream = a.N % 16 == 0 && ((uintptr_t)a.out & 63) == 0 && a.ldo % 16 == 0;
+      KernelTimer kt(st, "mx4_dma");
+      hipLaunchKernelGGL(mx4_dma_k<MATS>, dim3((unsigned)std::min(tm * tn, cus)), dim3(512), 0, st, a,
+                         pa, pb, (int)tm, (int)tn, groups, stream);
+      SIMP_HIP(hipGetLastError());
+      return SIMP_RT_OK;
+    }
+  }
   const int64_t tiles = cdiv(a.M, 16) * cdiv(a.N, 16);
   hipLaunchKernelGGL(mx4_tile_k<MATS>, dim3((unsigned)tiles), dim3(64), 0, st, a);
   SIMP_HIP(hipGetLastError());

@@ -178,6 +178,47 @@ def test_nan_scales_touch_their_rows_only(dev, gate, m, kb, n):
     _check(got[keep], want[keep], tol[keep])
 
 
+def _values64(codes, scales):
+    """mx.values on the device."""
+    import torch
+    c = torch.stack([codes & 15, codes >> 4], -1).view(codes.shape[0], -1).int()
+    v = torch.from_numpy(mx.VALUES).to(codes.device)[c & 7]
+    v = torch.where(c > 7, -v, v)
+    two = ((scales.long() - 127 + 1023) << 52).view(torch.float64)
+    return v * two.repeat_interleave(32, 1)[:, :v.shape[1]]
+
+
+LARGE = [(2900, 16, 3100), (2817, 32, 3089), (3000, 80, 2900), (2900, 208, 3001), (3100, 272, 2900),
+         (3000, 528, 3000), (257, 640, 16640), (8200, 144, 700), (2900, 1040, 3008)]
+
+
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("m, kb, n", LARGE)
+def test_large_products(dev, gate, m, kb, n):
+    """Against 64 bits on the device: every output of products that fill the chip."""
+    import torch
+    g = torch.Generator(device=dev)
+    g.manual_seed(m + kb)
+    n //= 1 + gate
+
+    def codes(r):
+        return (torch.randint(0, 256, (r, kb), generator=g, device=dev, dtype=torch.uint8),
+                torch.randint(126, 129, (r, -(-kb // 16)), generator=g, device=dev, dtype=torch.uint8))
+
+    a, *bs = [codes(r) for r in (m, n, n)[:2 + gate]]
+    out = torch.full((m + 2, n), 5.0, device=dev)
+    (sa.swiglu_mx4 if gate else sa.matmul_mx4)(*a, *[x for b in bs for x in b], out[1:-1])
+    want = [_values64(*a) @ _values64(*b).t().contiguous() for b in bs]
+    assert (out[0] == 5).all() and (out[-1] == 5).all()
+    if not gate:
+        assert torch.equal(out[1:-1].double(), want[0])
+    else:
+        silu = want[0] / (1 + torch.exp(-want[0]))
+        w = silu * want[1]
+        # the two sums are exact in fp32: what is left is the gate's rounding (mx.gated)
+        assert ((out[1:-1].double() - w).abs() <= 8 * mx.EPS * w.abs() + 2.0 ** -121 * want[1].abs()).all()
+
+
 def test_product_of_nothing_is_zero(dev):
     import torch
     for m, n in ((1, 1), (20, 300)):
