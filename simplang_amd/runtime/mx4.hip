@@ -187,36 +187,155 @@ __device__ __forceinline__ uint4 row16(const uint8_t *row, int k, int kb) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One wave to 16 x 16 outputs, operands straight from memory.
-template <int MATS>
-__global__ void __launch_bounds__(64) mx4_tile_k(const Mx4Args a) {
-  const int lane = threadIdx.x, r = lane & 15, q = lane >> 4;
-  const int tiles_n = (a.N + 15) >> 4;
-  const int m0 = 16 * (blockIdx.x / tiles_n), n0 = 16 * (blockIdx.x % tiles_n);
-  const int64_t m = min(m0 + r, a.M - 1), n = min(n0 + r, a.N - 1);
-  const uint8_t *ap = a.a + m * a.lda, *as = a.as + m * a.ldas;
-  v4f acc[MATS];
+// 16 NT columns of each matrix and all 16 MT rows to a block, whose waves split K: a wave
+// takes every byte of its rows' piece once, straight from memory into the lanes that
+// feed the matrix instruction (16 rows of 64 bytes, and a byte of scales to a lane), and
+// the waves' sums meet in LDS, in the order of K.
+template <int MT, int NT, int MATS>
+__global__ void __launch_bounds__(1024) mx4_skinny_k(const Mx4Args a, int span) {
+  constexpr int T = MATS * MT * NT;
+  extern __shared__ v4f part[];  // [waves][T][64]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int r = lane & 15, q = lane >> 4;
+  const int n0 = 16 * NT * blockIdx.x, m0 = 16 * MT * blockIdx.y;
+  const uint8_t *ap[MT], *as[MT], *bp[MATS][NT], *bs[MATS][NT];
 #pragma unroll
-  for (int t = 0; t < MATS; t++) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
-  for (int k0 = 0; k0 < a.kb; k0 += 64) {
-    const int k = k0 + 16 * q;
-    const uint4 av = row16(ap, k, a.kb);
-    const uint32_t sa = k < a.kb ? as[k >> 4] : 127;
+  for (int i = 0; i < MT; i++) {
+    const int64_t m = min(m0 + 16 * i + r, a.M - 1);
+    ap[i] = a.a + m * a.lda + 16 * q, as[i] = a.as + m * a.ldas + q;
+  }
+#pragma unroll
+  for (int t = 0; t < MATS; t++)
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+      const int64_t n = min(n0 + 16 * j + r, a.N - 1);
+      bp[t][j] = a.b[t] + n * a.ldb[t] + 16 * q, bs[t][j] = a.bs[t] + n * a.ldbs[t] + q;
+    }
+  v4f acc[MATS][MT][NT];
+#pragma unroll
+  for (int t = 0; t < MATS; t++)
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) acc[t][i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  struct Step {
+    uint4 a[MT], b[MATS][NT];
+    uint32_t as[MT], bs[MATS][NT];
+  };
+  auto run = [&](const Step &s) {
+#pragma unroll
+    for (int t = 0; t < MATS; t++)
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+          acc[t][i][j] = mfma_mx4(s.b[t][j], s.bs[t][j], s.a[i], s.as[i], acc[t][i][j]);
+  };
+  auto load = [&](int s) {
+    Step x;
+#pragma unroll
+    for (int t = 0; t < MATS; t++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        const u4any v = *(const u4any *)(bp[t][j] + 64 * s);
+        x.b[t][j] = make_uint4(v.x, v.y, v.z, v.w);
+        x.bs[t][j] = bs[t][j][4 * s];
+      }
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+      const u4any v = *(const u4any *)(ap[i] + 64 * s);
+      x.a[i] = make_uint4(v.x, v.y, v.z, v.w);
+      x.as[i] = as[i][4 * s];
+    }
+    return x;
+  };
+  const int whole = a.kb >> 6;
+  int s = wave * span;
+  const int end = min(s + span, whole);
+  constexpr int U = T >= 4 ? 2 : 4;
+  for (; s + U <= end; s += U) {
+    Step x[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) x[u] = load(s + u);
+#pragma unroll
+    for (int u = 0; u < U; u++) run(x[u]);
+  }
+  for (; s < end; s++) run(load(s));
+  if (wave == waves - 1 && (a.kb & 63)) {  // the last step, which rows end in
+    const int k = 64 * whole + 16 * q;
+    Step x;
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+      x.a[i] = row16(ap[i] - 16 * q, k, a.kb);
+      x.as[i] = k < a.kb ? as[i][4 * whole] : 127;
+    }
+#pragma unroll
+    for (int t = 0; t < MATS; t++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        x.b[t][j] = row16(bp[t][j] - 16 * q, k, a.kb);
+        x.bs[t][j] = k < a.kb ? bs[t][j][4 * whole] : 127;
+      }
+    run(x);
+  }
+  if (waves > 1) {
+#pragma unroll
+    for (int t = 0; t < MATS; t++)
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) part[(wave * T + (t * MT + i) * NT + j) * 64 + lane] = acc[t][i][j];
+    __syncthreads();
+  }
+  // a wave stores every `waves`-th 16 x 16 tile
+  for (int o = wave; o < MT * NT; o += waves) {
+    const int i = o / NT, j = o - i * NT;
+    v4f v[MATS];
 #pragma unroll
     for (int t = 0; t < MATS; t++) {
-      const uint4 bv = row16(a.b[t] + n * a.ldb[t], k, a.kb);
-      const uint32_t sb = k < a.kb ? a.bs[t][n * a.ldbs[t] + (k >> 4)] : 127;
-      acc[t] = mfma_mx4(bv, sb, av, sa, acc[t]);  // C^T: a lane has 4 columns of a row
-    }
-  }
-  if (m0 + r < a.M) {
-    float *o = a.out + m * a.ldo;
+      if (waves > 1) {
+        v[t] = part[((t * MT + i) * NT + j) * 64 + lane];
+        for (int w = 1; w < waves; w++) v[t] += part[(w * T + (t * MT + i) * NT + j) * 64 + lane];
+      } else {
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int col = n0 + 4 * q + e;
-      if (col < a.N) o[col] = MATS == 2 ? swiglu(acc[0][e], acc[MATS - 1][e]) : acc[0][e];
+        for (int ii = 0; ii < MT; ii++)
+#pragma unroll
+          for (int jj = 0; jj < NT; jj++)
+            if (ii == i && jj == j) v[t] = acc[t][ii][jj];
+      }
+    }
+    const int row = m0 + 16 * i + r, col = n0 + 16 * j + 4 * q;
+    if (row >= a.M) continue;
+    v4f y = v[0];
+    if constexpr (MATS == 2) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = swiglu(v[0][e], v[1][e]);
+    }
+    float *dst = a.out + (int64_t)row * a.ldo + col;
+    if (col + 3 < a.N) {
+      *(f4any *)dst = y;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (col + e < a.N) dst[e] = y[e];
     }
   }
+}
+
+constexpr int kSkinnyWaves = 4096;
+
+template <int MT, int NT, int MATS>
+int launch_skinny(const Mx4Args &a, hipStream_t st) {
+  const int64_t blocks = cdiv(a.N, 16 * NT) * cdiv(a.M, 16 * MT);
+  const int steps = a.kb >> 6;
+  int waves = (int)std::min<int64_t>({cdiv(kSkinnyWaves, blocks), 16, std::max(steps, 1), 64 / (MATS * MT * NT)});
+  const int span = (int)cdiv(steps, waves);
+  if (span) waves = (int)cdiv(steps, span);
+  KernelTimer kt(st, "mx4_skinny");
+  hipLaunchKernelGGL((mx4_skinny_k<MT, NT, MATS>), dim3((unsigned)cdiv(a.N, 16 * NT), (unsigned)cdiv(a.M, 16 * MT)),
+                     dim3(64 * waves), waves > 1 ? waves * MATS * MT * NT * 1024 : 0, st, a, span);
+  SIMP_HIP(hipGetLastError());
+  return SIMP_RT_OK;
 }
 
 // ---- large products: 256 x 256 tiles on an LDS-DMA ring
@@ -472,10 +591,9 @@ int launch_mx4(const Mx4Args &a, hipStream_t st) {
       return SIMP_RT_OK;
     }
   }
-  const int64_t tiles = cdiv(a.M, 16) * cdiv(a.N, 16);
-  hipLaunchKernelGGL(mx4_tile_k<MATS>, dim3((unsigned)tiles), dim3(64), 0, st, a);
-  SIMP_HIP(hipGetLastError());
-  return SIMP_RT_OK;
+  if (a.M <= 16) return launch_skinny<1, 1, MATS>(a, st);
+  if (a.M <= 32) return launch_skinny<2, 1, MATS>(a, st);
+  return launch_skinny<4, 1, MATS>(a, st);
 }
 
 // ------------------------------------------------------------- entry points
