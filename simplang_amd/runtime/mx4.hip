@@ -174,6 +174,29 @@ __device__ __forceinline__ v4f mfma_mx4(uint4 a, uint32_t sa, uint4 b, uint32_t 
 
 __device__ __forceinline__ float swiglu(float g, float u) { return (g / (1.f + expf(-g))) * u; }
 
+// Exchanges registers and lanes: of n = 2 or 4 neighbouring lanes, lane t gets in y[s] what
+// lane s has in x[t].  A fragment of the products leaves a lane four columns of one row, 64
+// bytes for each of 16 rows to a store; of n fragments side by side this makes n stores of
+// 64 n bytes for each of 16 / n rows, whole lines, which the memory takes in half the time.
+template <int N>
+__device__ __forceinline__ void lane_transpose(v4f (&x)[N]) {
+  const int t = threadIdx.x;
+  auto swap = [&](v4f &a, v4f &b, auto ctrl, bool odd) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float u = dpp_mov<decltype(ctrl)::value>(b[e]), v = dpp_mov<decltype(ctrl)::value>(a[e]);
+      a[e] = odd ? u : a[e];
+      b[e] = odd ? b[e] : v;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < N; i += 2) swap(x[i], x[i + 1], std::integral_constant<int, kDppXor1>{}, t & 1);
+  if constexpr (N == 4) {
+    swap(x[0], x[2], std::integral_constant<int, kDppXor2>{}, t & 2);
+    swap(x[1], x[3], std::integral_constant<int, kDppXor2>{}, t & 2);
+  }
+}
+
 // 16 code bytes of a row from byte k on, zeros behind its end.
 __device__ __forceinline__ uint4 row16(const uint8_t *row, int k, int kb) {
   if (k + 16 <= kb) {
@@ -192,12 +215,13 @@ __device__ __forceinline__ uint4 row16(const uint8_t *row, int k, int kb) {
 // feed the matrix instruction (16 rows of 64 bytes, and a byte of scales to a lane), and
 // the waves' sums meet in LDS, in the order of K.
 template <int MT, int NT, int MATS>
-__global__ void __launch_bounds__(1024) mx4_skinny_k(const Mx4Args a, int span) {
+__global__ void __launch_bounds__(1024) mx4_skinny_k(const Mx4Args a, int span, int blocks_n) {
   constexpr int T = MATS * MT * NT;
   extern __shared__ v4f part[];  // [waves][T][64]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int r = lane & 15, q = lane >> 4;
-  const int n0 = 16 * NT * blockIdx.x, m0 = 16 * MT * blockIdx.y;
+  const int bm = blockIdx.x / blocks_n;
+  const int n0 = 16 * NT * (blockIdx.x - bm * blocks_n), m0 = 16 * MT * bm;
   const uint8_t *ap[MT], *as[MT], *bp[MATS][NT], *bs[MATS][NT];
 #pragma unroll
   for (int i = 0; i < MT; i++) {
@@ -322,19 +346,24 @@ __global__ void __launch_bounds__(1024) mx4_skinny_k(const Mx4Args a, int span) 
   }
 }
 
-constexpr int kSkinnyWaves = 4096;
-
 template <int MT, int NT, int MATS>
-int launch_skinny(const Mx4Args &a, hipStream_t st) {
-  const int64_t blocks = cdiv(a.N, 16 * NT) * cdiv(a.M, 16 * MT);
+int launch_skinny(Mx4Args a, hipStream_t st) {
+  const int64_t bn = cdiv(a.N, 16 * NT), bm = cdiv(a.M, 16 * MT);
+  // about 4096 waves on the chip, up to 16 to a block (64 KiB of sums)
   const int steps = a.kb >> 6;
-  int waves = (int)std::min<int64_t>({cdiv(kSkinnyWaves, blocks), 16, std::max(steps, 1), 64 / (MATS * MT * NT)});
+  int waves = (int)std::min<int64_t>({cdiv(4096, bn * bm), 16, std::max(steps, 1), 64 / (MATS * MT * NT)});
   const int span = (int)cdiv(steps, waves);
   if (span) waves = (int)cdiv(steps, span);
+  const int64_t most = std::max<int64_t>(INT32_MAX / (64 * waves) / bn, 1);  // row blocks of a launch
   KernelTimer kt(st, "mx4_skinny");
-  hipLaunchKernelGGL((mx4_skinny_k<MT, NT, MATS>), dim3((unsigned)cdiv(a.N, 16 * NT), (unsigned)cdiv(a.M, 16 * MT)),
-                     dim3(64 * waves), waves > 1 ? waves * MATS * MT * NT * 1024 : 0, st, a, span);
-  SIMP_HIP(hipGetLastError());
+  for (int64_t b = 0; b < bm; b += most) {
+    Mx4Args c = a;
+    const int64_t row = b * 16 * MT, rows = std::min<int64_t>(most * 16 * MT, a.M - row);
+    c.a += row * a.lda, c.as += row * a.ldas, c.out += row * a.ldo, c.M = (int)rows;
+    hipLaunchKernelGGL((mx4_skinny_k<MT, NT, MATS>), dim3((unsigned)(bn * cdiv(rows, 16 * MT))),
+                       dim3(64 * waves), waves > 1 ? waves * MATS * MT * NT * 1024 : 0, st, c, span, (int)bn);
+    SIMP_HIP(hipGetLastError());
+  }
   return SIMP_RT_OK;
 }
 
@@ -355,53 +384,56 @@ __device__ __forceinline__ void dma16_at(const void *base, uint32_t off, uint32_
       : "memory");
 }
 
-// Scale bytes as the tile kernel reads them: for 64 rows and 4 K-steps of 128 (one
-// "group") 1 KB, 16 bytes a row, dword q of which has block q of the steps 0 .. 3 in its
-// bytes 0 .. 3.  So one DMA instruction brings a wave the scales of 64 rows for four
-// steps, a lane (row, q) keeps one register for them, and the matrix instruction
-// picks the step's byte.  Row v of W1 and W3 together: 16 rows of one, then 16 of the
-// other.  Blocks behind a row's end get 2^-127: the codes that the last stage reads in their
-// place (its first block again) then add up to less than 2^-240, which no sum notices.
-template <int MATS>
-__global__ void __launch_bounds__(256)
-    mx4_pack_scales_k(const Mx4Args a, uint4 *__restrict__ pa, uint4 *__restrict__ pb, int ga,
-                      int gb, int groups) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int r = (int)(i & 63);
-  const int64_t t = i >> 6;
-  const int g = (int)(t % groups);
-  const int64_t rg = t / groups;  // of the ga + gb row groups
-  if (rg >= ga + gb) return;
-  const bool is_a = rg < ga;
-  const int v = (int)(is_a ? rg : rg - ga) * 64 + r;
-  const int mat = !is_a && MATS == 2 ? (v >> 4) & 1 : 0;
-  const int row = !is_a && MATS == 2 ? (v >> 5) * 16 + (v & 15) : v;
-  const uint8_t *s = is_a ? a.as + (int64_t)row * a.ldas : a.bs[mat] + (int64_t)row * a.ldbs[mat];
-  const int nb = (a.kb + 15) >> 4;
+// The scale bytes of blocks 16g .. 16g + 15 of a row of nb blocks, for four K-steps of 128:
+// dword q has block q of the steps 0 .. 3 in its bytes 0 .. 3, so a lane (row, q) keeps
+// one register for the four and the matrix instruction picks the step's byte.  Blocks
+// behind the row's end get 2^-127: the codes that the last stage reads in their place
+// (its first block again) then add up to less than 2^-240, which no sum notices.
+__device__ __forceinline__ uint4 scale_group(const uint8_t *s, int g, int nb) {
   uint32_t w[4];  // w[j]: blocks 4j .. 4j+3 of the group
-  const bool in = row < (is_a ? a.M : a.N);
+  if (16 * g + 16 <= nb) {
+    const u4any v = *(const u4any *)(s + 16 * g);
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int b0 = 16 * g + 4 * j;
-    w[j] = 0;
-    if (in && b0 + 4 <= nb) {
-      w[j] = *(const u1any *)(s + b0);
-    } else if (in) {
+    for (int j = 0; j < 4; j++) w[j] = v[j];
+  } else if (nb >= 4) {  // the row's last four bytes, shifted down
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (b0 + e < nb) w[j] = (w[j] & ~(255u << (8 * e))) | (uint32_t)s[b0 + e] << (8 * e);
+    for (int j = 0; j < 4; j++) {
+      const int b0 = 16 * g + 4 * j, at = min(b0, nb - 4);
+      const uint32_t v = *(const u1any *)(s + at);
+      w[j] = b0 - at < 4 ? v >> (8 * (b0 - at)) : 0;
     }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = 0;
+    for (int e = 0; e < nb && g == 0; e++) w[0] |= (uint32_t)s[e] << (8 * e);
   }
   // 4 x 4 byte transpose
   const uint32_t x0 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u),
                  x1 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u),
                  y0 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u),
                  y1 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
-  const uint4 o = make_uint4(__builtin_amdgcn_perm(y0, x0, 0x05040100u),
-                             __builtin_amdgcn_perm(y0, x0, 0x07060302u),
-                             __builtin_amdgcn_perm(y1, x1, 0x05040100u),
-                             __builtin_amdgcn_perm(y1, x1, 0x07060302u));
-  (is_a ? pa + t * 64 : pb + (t - (int64_t)ga * groups) * 64)[r] = o;
+  return make_uint4(__builtin_amdgcn_perm(y0, x0, 0x05040100u),
+                    __builtin_amdgcn_perm(y0, x0, 0x07060302u),
+                    __builtin_amdgcn_perm(y1, x1, 0x05040100u),
+                    __builtin_amdgcn_perm(y1, x1, 0x07060302u));
+}
+
+// Scale bytes as the 256 x 256 tiles read them: for 64 rows and a group of four K-steps
+// 1 KB, 16 bytes a row (scale_group), so that one DMA instruction brings a wave the scales
+// of 64 rows for four steps.  Row v of W1 and W3 together: 16 rows of one, then 16 of the
+// other.
+template <int MATS>
+__global__ void __launch_bounds__(256)
+    mx4_pack_scales_k(const Mx4Args a, uint4 *__restrict__ pa, uint4 *__restrict__ pb, int ga, int groups) {
+  const int r = threadIdx.x & 63, g = 4 * blockIdx.y + (threadIdx.x >> 6);
+  if (g >= groups) return;
+  const bool is_a = (int)blockIdx.x < ga;
+  const int rg = is_a ? blockIdx.x : blockIdx.x - ga, v = rg * 64 + r;
+  const int mat = !is_a && MATS == 2 ? (v >> 4) & 1 : 0;
+  const int row = !is_a && MATS == 2 ? (v >> 5) * 16 + (v & 15) : v;
+  const uint8_t *s = is_a ? a.as + (int64_t)row * a.ldas : a.bs[mat] + (int64_t)row * a.ldbs[mat];
+  (is_a ? pa : pb)[((int64_t)rg * groups + g) * 64 + r] =
+      scale_group(s, g, row < (is_a ? a.M : a.N) ? (a.kb + 15) >> 4 : 0);
 }
 
 template <int P>
@@ -411,17 +443,19 @@ __device__ __forceinline__ v4f mfma_step(const uint4 &b, uint32_t sb, const uint
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(y, x, c, 4, 4, P, (int)sb, P, (int)sa);
 }
 
-// Persistent 256 x 256 tiles (MATS == 2: of 128 columns of W1 and W3 each), 8 waves of
-// 128 x 64, K-steps of 64 code bytes through a ring of 4 stages that
+// Persistent 256 x 256 tiles (MATS == 2: of 128 columns of W1 and W3 each), 8 waves of 128 x
+// 64, K-steps of 64 code bytes through a ring of four stages that
 // global_load_lds_dwordx4 fills three steps ahead.
 template <int MATS>
 __global__ void __launch_bounds__(512)
     mx4_dma_k(const Mx4Args a, const uint4 *__restrict__ pa, const uint4 *__restrict__ pb,
-              int tiles_m, int tiles_n, int groups, int stream) {
-  constexpr int BM = 256, BN = 256, BK = 64, WGN = 4, STAGES = 4;
+              int tiles_m, int tiles_n, int groups, int stream, int stagger) {
+  constexpr int BM = 256, BN = 256, BK = 64, STAGES = 4, WGN = 4;
   constexpr int WM = 128, WN = 64, FM = WM / 16, FN = WN / 16;
   constexpr int STAGE = (BM + BN) * BK, SCALES = (BM + BN) * 16;  // bytes
-  __shared__ uint4 lds[(STAGES * STAGE + 2 * SCALES) / 16];
+  constexpr int DA = 2, DB = 2, DPW = DA + DB;  // DMA instructions of a wave
+  // a group's scales are issued when the group before has been read: one buffer
+  __shared__ uint4 lds[(STAGES * STAGE + SCALES) / 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm0 = (wave / WGN) * WM, wn0 = (wave % WGN) * WN;
   const int nk = (a.kb + BK - 1) / BK;
@@ -429,36 +463,46 @@ __global__ void __launch_bounds__(512)
   const int lrow = lane & 15, lkc = lane >> 4;
   const int drow = lane >> 2, dkc = (lane & 3) ^ ((drow >> 1) & 3);  // DMA lane -> row, chunk
   const int rslot = lrow * 4 + (lkc ^ ((lrow >> 1) & 3));          // operand lane -> slot
-  const uint32_t lds_wave = lds_offset(lds) + 2048 * wave;  // wave w fills blocks 2w, 2w+1
-  const uint32_t lds_scale = lds_offset(lds) + STAGES * STAGE + 1024 * wave;
+  const uint32_t lds0 = lds_offset(lds);
+  // Workgroups of equal tiles store at the same time, and all wait for the memory then; with
+  // eight starts, `stagger` of about 1 us apart, the others of an XCD compute meanwhile.
+  for (int z = stagger * ((blockIdx.x >> 3) & 7); z > 0; z--) __builtin_amdgcn_s_sleep(32);
   const uint32_t *sl = (const uint32_t *)(lds + STAGES * STAGE / 16) + lrow * 4 + lkc;
 
   for (int vb = blockIdx.x; vb < ntiles; vb += gridDim.x) {
     int tm, tn;
     tile_of_block(vb, ntiles, tiles_m, tiles_n, tm, tn);
     const int m0 = tm * BM, n0 = tn * (BN / MATS);
-    // a lane's rows, from the tile's first: two of A, two of B or one each of W1 and W3
-    const uint8_t *baseA = a.a + (int64_t)m0 * a.lda, *baseB0 = a.b[0] + (int64_t)n0 * a.ldb[0],
-                  *baseB1 = a.b[MATS - 1] + (int64_t)n0 * a.ldb[MATS - 1];
-    auto off = [&](int r, int rows, int64_t ld) { return (uint32_t)(min(r, rows - 1) * (uint32_t)ld) + 16 * dkc; };
-    const uint32_t offA0 = off(32 * wave + drow, a.M - m0, a.lda),
-                   offA1 = off(32 * wave + 16 + drow, a.M - m0, a.lda),
-                   offB0 = off((MATS == 2 ? 16 : 32) * wave + drow, a.N - n0, a.ldb[0]),
-                   offB1 = off((MATS == 2 ? 16 * wave : 32 * wave + 16) + drow, a.N - n0, a.ldb[MATS - 1]);
+    // blocks of 16 rows of A and of B (16 rows of W1, 16 of W3 in turn): a lane's row of each,
+    // from the tile's first
+    const uint8_t *baseA = a.a + (int64_t)m0 * a.lda, *baseB[MATS];
+#pragma unroll
+    for (int t = 0; t < MATS; t++) baseB[t] = a.b[t] + (int64_t)n0 * a.ldb[t];
+    uint32_t offA[DA], offB[DB];
+#pragma unroll
+    for (int i = 0; i < DA; i++)
+      offA[i] = (uint32_t)min(16 * (DA * wave + i) + drow, a.M - 1 - m0) * (uint32_t)a.lda + 16 * dkc;
+#pragma unroll
+    for (int i = 0; i < DB; i++) {
+      const int blk = DB * wave + i;
+      offB[i] = (uint32_t)min(16 * (blk / MATS) + drow, a.N - 1 - n0) * (uint32_t)a.ldb[blk % MATS] + 16 * dkc;
+    }
+    // 64 rows of scales to a wave: A's, then B's
     const uint4 *baseS = wave < 4 ? pa + (int64_t)(4 * tm + wave) * groups * 64
                                   : pb + (int64_t)(4 * tn + wave - 4) * groups * 64;
     // The scales of a group go ahead of its first stage.  `last`: kt may be the last
     // stage, which can be shorter.
     auto issue = [&](int kt, auto last) {
-      const uint32_t st = lds_wave + (kt % STAGES) * STAGE;
+      const uint32_t st = lds0 + (kt % STAGES) * STAGE;
       const int64_t k0 = (int64_t)kt * BK;
-      if ((kt & 3) == 0) dma16_at(baseS + (kt >> 2) * 64, 16 * lane, lds_scale + ((kt >> 2) & 1) * SCALES);
+      if ((kt & 3) == 0) dma16_at(baseS + (kt >> 2) * 64, 16 * lane, lds0 + STAGES * STAGE + 1024 * wave);
       uint32_t back = 0;
       if constexpr (decltype(last)::value) back = k0 + 16 * dkc < a.kb ? 0 : 16 * dkc;
-      dma16_at(baseA + k0, offA0 - back, st);
-      dma16_at(baseA + k0, offA1 - back, st + 1024);
-      dma16_at(baseB0 + k0, offB0 - back, st + BM * BK);
-      dma16_at(baseB1 + k0, offB1 - back, st + BM * BK + 1024);
+#pragma unroll
+      for (int i = 0; i < DA; i++) dma16_at(baseA + k0, offA[i] - back, st + 1024 * (DA * wave + i));
+#pragma unroll
+      for (int i = 0; i < DB; i++)
+        dma16_at(baseB[(DB * wave + i) % MATS] + k0, offB[i] - back, st + BM * BK + 1024 * (DB * wave + i));
     };
     v4f acc[FM][FN];
 #pragma unroll
@@ -467,43 +511,44 @@ __global__ void __launch_bounds__(512)
       for (int j = 0; j < FN; j++) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
     uint4 fa[FM], fb[2][FN];
     uint32_t ra[FM], rb[FN], rbn[FN];  // scales of four steps
-    auto frag = [&](int kt, int blk) { return lds[(kt % STAGES) * (STAGE / 16) + blk * 64 + rslot]; };
+    auto frag = [&](int slot, int blk) { return lds[slot * (STAGE / 16) + blk * 64 + rslot]; };
     constexpr int BOFF = BM * BK / 1024;  // first B block of a stage
-    auto scale = [&](int g, int row) { return sl[(g & 1) * (SCALES / 4) + 4 * row]; };
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // the previous tile's stores
+    auto scale = [&](int row) { return sl[4 * row]; };
     using T = std::true_type;
     using F = std::false_type;
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // the previous tile's stores
     for (int p = 0; p < min(STAGES, nk); p++) issue(p, T{});
-    if (nk >= STAGES) __builtin_amdgcn_s_waitcnt(waitcnt_vm(4 * (STAGES - 1)));
+    if (nk >= STAGES) __builtin_amdgcn_s_waitcnt(waitcnt_vm(DPW * (STAGES - 1)));
     else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     block_barrier();
 #pragma unroll
-    for (int j = 0; j < FN; j++) fb[0][j] = frag(0, BOFF + wn0 / 16 + j), rb[j] = scale(0, BM + wn0 + 16 * j);
+    for (int j = 0; j < FN; j++) fb[0][j] = frag(0, BOFF + wn0 / 16 + j), rb[j] = scale(BM + wn0 + 16 * j);
 #pragma unroll
-    for (int i = 0; i < FM; i++) fa[i] = frag(0, wm0 / 16 + i), ra[i] = scale(0, wm0 + 16 * i);
+    for (int i = 0; i < FM; i++) fa[i] = frag(0, wm0 / 16 + i), ra[i] = scale(wm0 + 16 * i);
     // Step kt: certify stage kt + 1, read its fragments while the MFMAs of stage kt run, and
-    // refill the buffer of stage kt.  Steady: stage kt + 4 is there and not the last.
+    // refill the buffer of stage kt.  Steady: stage kt + STAGES is there and not the last.
     // (Behind the last stage the reads bring stale LDS that is not used.)
     auto step = [&](int kt, auto phase, auto steady) {
       constexpr int P = decltype(phase)::value, cb = P & 1;
       constexpr bool S = decltype(steady)::value;
-      // a group's scales are ahead of its first stage: kt + 3 or kt + 2 here
-      constexpr int vm = 4 * (STAGES - 2) + (P == 1 || P == 2);
+      // stages kt + 2 and kt + 3 may be on their way, and the scales ahead of one
+      constexpr int vm = DPW * (STAGES - 2) + (P == 1 || P == 2);
       if (S || kt + STAGES - 1 < nk) __builtin_amdgcn_s_waitcnt(waitcnt_vm(vm));
       else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
       __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0);
       block_barrier();
+      constexpr int next = (P + 1) % STAGES;  // slot of stage kt + 1
 #pragma unroll
       for (int j = 0; j < FN; j++) {
-        fb[cb ^ 1][j] = frag(kt + 1, BOFF + wn0 / 16 + j);
-        if constexpr (P == 3) rbn[j] = scale((kt + 1) >> 2, BM + wn0 + 16 * j);
+        fb[cb ^ 1][j] = frag(next, BOFF + wn0 / 16 + j);
+        if constexpr (P == 3) rbn[j] = scale(BM + wn0 + 16 * j);
       }
 #pragma unroll
       for (int i = 0; i < FM; i++) {
 #pragma unroll
         for (int j = 0; j < FN; j++) acc[i][j] = mfma_step<P>(fb[cb][j], rb[j], fa[i], ra[i], acc[i][j]);
-        fa[i] = frag(kt + 1, wm0 / 16 + i);
-        if constexpr (P == 3) ra[i] = scale((kt + 1) >> 2, wm0 + 16 * i);
+        fa[i] = frag(next, wm0 / 16 + i);
+        if constexpr (P == 3) ra[i] = scale(wm0 + 16 * i);
         if (i == 3) {
           if constexpr (S) issue(kt + STAGES, F{});
           else if (kt + STAGES < nk) issue(kt + STAGES, T{});
@@ -532,63 +577,391 @@ __global__ void __launch_bounds__(512)
       if (kt + 3 < nk) step(kt + 3, I3{}, F{});
     }
     // acc[i][j][r] = C[m0 + wm0 + 16 i + l%16][v0 + wn0 + 16 j + 4 (l/16) + r]
+    constexpr int NF = FN / MATS;  // fragments side by side in out
+    const int col = n0 + (wn0 / MATS) + 16 * (lrow & (NF - 1)) + 4 * lkc;
 #pragma unroll
-    for (int j = 0; j < FN; j += MATS) {
-      const int col = n0 + (wn0 + 16 * j) / MATS + 4 * lkc;
+    for (int i = 0; i < FM; i++) {
+      v4f v[NF];
 #pragma unroll
-      for (int i = 0; i < FM; i++) {
-        const int row = m0 + wm0 + 16 * i + lrow;
-        if (row >= a.M || col >= a.N) continue;
-        v4f v = acc[i][j];
+      for (int j = 0; j < NF; j++) {
+        v[j] = acc[i][j * MATS];
         if constexpr (MATS == 2) {
 #pragma unroll
-          for (int r = 0; r < 4; r++) v[r] = swiglu(v[r], acc[i][j + 1][r]);
+          for (int r = 0; r < 4; r++) v[j][r] = swiglu(v[j][r], acc[i][2 * j + 1][r]);
         }
+      }
+      lane_transpose<NF>(v);
+#pragma unroll
+      for (int j = 0; j < NF; j++) {
+        const int row = m0 + wm0 + 16 * i + (lrow & ~(NF - 1)) + j;
+        if (row >= a.M || col >= a.N) continue;
         float *dst = a.out + (int64_t)row * a.ldo + col;
         if (stream) {
-          __builtin_nontemporal_store(v, (v4f *)dst);
+          __builtin_nontemporal_store(v[j], (v4f *)dst);
         } else if (col + 3 < a.N) {
-          *(f4any *)dst = v;
+          *(f4any *)dst = v[j];
         } else {
 #pragma unroll
           for (int r = 0; r < 4; r++)
-            if (col + r < a.N) dst[r] = v[r];
+            if (col + r < a.N) dst[r] = v[j][r];
         }
       }
     }
   }
 }
 
-// Whether the tile kernel can read the codes: 16-byte pieces of aligned rows.
+// ---- products between the two: BM x BN tiles, stages of 128 code bytes
+
+// KS groups of WGM x WGN waves have a part of K each, with a ring of SLOTS stages of their
+// own, and their sums meet in LDS in the order of K: the chain of stages, each of which
+// costs a round trip and a barrier, is KS times shorter, and a tile that has a CU to
+// itself keeps it busy.  A stage is two K-steps; a DMA instruction is 8 rows of 128 bytes,
+// whole lines.  The scales of RG groups of a part are staged through registers into
+// LDS as scale_group gives them (RG odd: rows of scales then start in different banks),
+// and those of the next RG when they are used up.
+template <int BM, int BN, int WGM, int WGN, int KS, int RG, int MATS>
+__global__ void __launch_bounds__(64 * WGM * WGN * KS)
+    mx4_ring_k(const Mx4Args a, int tiles_m, int tiles_n, int per) {
+  constexpr int NW = WGM * WGN, NT = 64 * NW * KS;
+  constexpr int WM = BM / WGM, WN = BN / WGN, FM = WM / 16, FN = WN / 16;
+  constexpr int BK = 128;
+  constexpr int SA = BM * BK, SB = BN * BK, STAGE = SA + SB;  // bytes
+  constexpr int DA = SA / 1024 / NW, DB = SB / 1024 / NW;     // DMA instructions per wave
+  constexpr int SLOTS = 2;
+  static_assert(DA >= 1 && DB >= 1 && FN % MATS == 0, "ring shape");
+  static_assert(RG % 2 == 1 && BM * BN * 4 <= SLOTS * STAGE, "scales and sums");
+  __shared__ uint4 lds[KS * SLOTS * STAGE / 16];
+  __shared__ uint4 sc[KS * (BM + BN) * RG];
+  const int lane = threadIdx.x & 63, wall = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = wall % NW, part = wall / NW;
+  const int wm0 = (wave / WGN) * WM, wn0 = (wave % WGN) * WN;
+  const int lrow = lane & 15, lkc = lane >> 4;
+  uint4 *ring = lds + part * (SLOTS * STAGE / 16);
+  const uint32_t lds_base = lds_offset(ring);
+  const int fsw = (lrow >> 1) & 7;  // chunk swizzle of this lane's operand rows
+  const int ns = (a.kb + BK - 1) / BK, nb = (a.kb + 15) >> 4;
+  const int s0 = part * per, s1 = min(s0 + per, ns);  // this part's stages (per is even)
+  int tm, tn;
+  tile_of_block(blockIdx.x, tiles_m * tiles_n, tiles_m, tiles_n, tm, tn);
+  const int m0 = tm * BM, n0 = tn * (BN / MATS);
+  const uint8_t *baseA = a.a + (int64_t)m0 * a.lda;
+  const uint8_t *baseB[MATS];
+#pragma unroll
+  for (int t = 0; t < MATS; t++) baseB[t] = a.b[t] + (int64_t)n0 * a.ldb[t];
+  uint32_t offA[DA], offB[DB];
+#pragma unroll
+  for (int i = 0; i < DA; i++) {
+    const int r = 8 * (wave * DA + i) + (lane >> 3);
+    offA[i] = (uint32_t)min(r, a.M - 1 - m0) * (uint32_t)a.lda + 16 * ((lane & 7) ^ ((r >> 1) & 7));
+  }
+#pragma unroll
+  for (int i = 0; i < DB; i++) {
+    const int v = 8 * (wave * DB + i) + (lane >> 3);
+    const int r = MATS == 2 ? (v >> 5) * 16 + (v & 15) : v;
+    const int t = MATS == 2 ? ((wave * DB + i) >> 1) & 1 : 0;
+    offB[i] = (uint32_t)min(r, a.N - 1 - n0) * (uint32_t)a.ldb[t] + 16 * ((lane & 7) ^ ((v >> 1) & 7));
+  }
+  // `last`: st may be the last stage, where blocks behind the row's end are its first again
+  auto issue = [&](int st, int slot, auto last) {
+    const uint32_t dst = lds_base + slot * STAGE;
+    const int64_t k0 = (int64_t)st * BK;
+    auto go = [&](const uint8_t *base, uint32_t off, int i, uint32_t d) {
+      if constexpr (decltype(last)::value) {
+        const int c = 16 * ((lane & 7) ^ ((4 * i + (lane >> 4)) & 7));  // the lane's chunk, as above
+        off -= k0 + c < a.kb ? 0 : c;
+      }
+      dma16_at(base + k0, off, d);
+    };
+#pragma unroll
+    for (int i = 0; i < DA; i++) go(baseA, offA[i], wave * DA + i, dst + 1024 * (wave * DA + i));
+#pragma unroll
+    for (int i = 0; i < DB; i++)
+      go(baseB[MATS == 2 ? ((wave * DB + i) >> 1) & 1 : 0], offB[i], wave * DB + i,
+         dst + SA + 1024 * (wave * DB + i));
+  };
+  // (slot and row part constant: the reads' immediate offsets)
+  const uint4 *fA[2], *fB[2];
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    fA[h] = ring + wm0 * 8 + lrow * 8 + ((4 * h + lkc) ^ fsw);
+    fB[h] = fA[h] + (BM + wn0 - wm0) * 8;
+  }
+  const uint32_t *sl = (const uint32_t *)(sc + part * (BM + BN) * RG) + lrow * 4 * RG + lkc;
+  auto scale = [&](int g, int row) { return sl[row * 4 * RG + 4 * g]; };
+  v4f acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; i++)
+#pragma unroll
+    for (int j = 0; j < FN; j++) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  using T = std::true_type;
+  using F = std::false_type;
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+
+  // the row whose scales this thread stages: A's, then B's, of every part
+  constexpr int ROWS = KS * (BM + BN), TPR = NT / ROWS > 0 ? NT / ROWS : 1, U = (RG + TPR - 1) / TPR;
+  static_assert(NT >= ROWS, "a thread to each row");
+  const int srow = threadIdx.x % ROWS, sg = threadIdx.x / ROWS;
+  const uint8_t *sp;
+  {
+    const int p = srow / (BM + BN), row = srow - p * (BM + BN);
+    if (row < BM) {
+      sp = a.as + (int64_t)min(m0 + row, a.M - 1) * a.ldas;
+    } else {
+      const int v = row - BM, r = MATS == 2 ? (v >> 5) * 16 + (v & 15) : v;
+      const int64_t n = min(n0 + r, a.N - 1);
+      sp = MATS == 2 && (v & 16) ? a.bs[MATS - 1] + n * a.ldbs[MATS - 1] : a.bs[0] + n * a.ldbs[0];
+    }
+    sp += 8 * p * per;  // a stage is 8 blocks
+  }
+  const int snb = nb - 8 * (srow / (BM + BN)) * per;  // the row's blocks from there on
+
+  for (int d0 = 0; d0 < per; d0 += 2 * RG) {  // spans of every part whose scales are staged
+    const int len = min(per - d0, 2 * RG), groups = len >> 1;  // the same for all parts
+    const int c0 = s0 + d0, c1 = min(c0 + len, s1);
+    if (d0) block_barrier();  // the span before is read
+    const int first = max(min(SLOTS, c1 - c0), 0);
+    for (int i = 0; i < first; i++) issue(c0 + i, i, T{});
+    // scales: a thread has one row (and part) and takes its groups all at once
+    uint4 sv[U];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (u * TPR + sg < groups) sv[u] = scale_group(sp, (d0 >> 1) + u * TPR + sg, snb);
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (u * TPR + sg < groups) sc[srow * RG + u * TPR + sg] = sv[u];
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    lds_barrier();
+    uint4 fra[2][FM], frb[2][FN];
+    uint32_t sa[FM], sb[FN], na[FM], nb_[FN];
+    auto read = [&](auto slot, auto half) {
+      constexpr int h = decltype(half)::value, at = decltype(slot)::value * (STAGE / 16);
+#pragma unroll
+      for (int j = 0; j < FN; j++) frb[h][j] = fB[h][at + j * 128];
+#pragma unroll
+      for (int i = 0; i < FM; i++) fra[h][i] = fA[h][at + i * 128];
+    };
+    auto mul = [&](auto phase) {
+      constexpr int P = decltype(phase)::value, h = P & 1;
+#pragma unroll
+      for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = mfma_step<P>(frb[h][j], sb[j], fra[h][i], sa[i], acc[i][j]);
+    };
+#pragma unroll
+    for (int j = 0; j < FN; j++) sb[j] = scale(0, BM + wn0 + 16 * j);
+#pragma unroll
+    for (int i = 0; i < FM; i++) sa[i] = scale(0, wm0 + 16 * i);
+    read(I0{}, I0{});
+    // Stage st: its second step is read while its first is multiplied; then stage st + 1
+    // is waited for, stage st is read on every wave, and its slot is filled again while
+    // the second step is multiplied.  (c0 is even: an even stage lies in slot 0.)
+    // Steady: stage st + 2 is there and not the last.  (Reads behind the last stage and
+    // group bring stale LDS that is not used.)  One barrier a stage, in every part.  The
+    // scheduling barriers keep the reads ahead of the products that they run beside.
+    auto stage = [&](int st, auto odd, auto steady) {
+      constexpr int o = decltype(odd)::value;
+      constexpr bool S = decltype(steady)::value;
+      using Other = std::integral_constant<int, o ^ 1>;
+      const bool in = S || st < c1;  // (a part may have fewer stages)
+      read(odd, I1{});
+      __builtin_amdgcn_sched_barrier(0);
+      if (in) mul(std::integral_constant<int, 2 * o>{});
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+      __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0);
+      block_barrier();
+      read(Other{}, I0{});
+      if constexpr (o == 1) {
+        const int g = min((st + 1 - c0) >> 1, RG - 1);
+#pragma unroll
+        for (int j = 0; j < FN; j++) nb_[j] = scale(g, BM + wn0 + 16 * j);
+#pragma unroll
+        for (int i = 0; i < FM; i++) na[i] = scale(g, wm0 + 16 * i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (S) issue(st + 2, o, F{});
+      else if (st + 2 < c1) issue(st + 2, o, T{});
+      if (in) mul(std::integral_constant<int, 2 * o + 1>{});
+      if constexpr (o == 1) {
+#pragma unroll
+        for (int j = 0; j < FN; j++) sb[j] = nb_[j];
+#pragma unroll
+        for (int i = 0; i < FM; i++) sa[i] = na[i];
+      }
+    };
+    int st = c0;
+    for (; st + 4 < c1; st += 2) {
+      stage(st, I0{}, T{});
+      stage(st + 1, I1{}, T{});
+    }
+    for (; st < c0 + len; st += 2) {
+      stage(st, I0{}, F{});
+      stage(st + 1, I1{}, F{});
+    }
+  }
+  // acc[i][j][r] = C[m0 + wm0 + 16 i + l%16][v0 + wn0 + 16 j + 4 (l/16) + r]
+  auto store = [&](int i, int j, v4f v, v4f w) {
+    const int row = m0 + wm0 + 16 * i + lrow, col = n0 + (wn0 + 16 * j) / MATS + 4 * lkc;
+    if (row >= a.M || col >= a.N) return;
+    if constexpr (MATS == 2) {
+#pragma unroll
+      for (int r = 0; r < 4; r++) v[r] = swiglu(v[r], w[r]);
+    }
+    float *dst = a.out + (int64_t)row * a.ldo + col;
+    if (col + 3 < a.N) {
+      *(f4any *)dst = v;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        if (col + r < a.N) dst[r] = v[r];
+    }
+  };
+  if constexpr (KS == 1) {
+#pragma unroll
+    for (int j = 0; j < FN; j += MATS)
+#pragma unroll
+      for (int i = 0; i < FM; i++) store(i, j, acc[i][j], acc[i][j + MATS - 1]);
+  } else {
+    v4f *sums = (v4f *)lds;  // [part][wave][i][j][lane]
+    lds_barrier();           // every wave is through with its ring
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+      for (int j = 0; j < FN; j++) sums[((part * NW + wave) * FM * FN + i * FN + j) * 64 + lane] = acc[i][j];
+    lds_barrier();
+    auto sum = [&](int i, int j) {
+      v4f v = sums[(wave * FM * FN + i * FN + j) * 64 + lane];
+#pragma unroll
+      for (int p = 1; p < KS; p++) v += sums[((p * NW + wave) * FM * FN + i * FN + j) * 64 + lane];
+      return v;
+    };
+    // the parts share a wave's fragments out between them
+#pragma unroll
+    for (int o = 0; o < FM * FN / MATS; o += KS) {
+      if (o + part < FM * FN / MATS) {
+        const int i = (o + part) / (FN / MATS), j = (o + part) % (FN / MATS) * MATS;
+        store(i, j, sum(i, j), sum(i, j + MATS - 1));
+      }
+    }
+  }
+}
+
+template <int BM, int BN, int WGM, int WGN, int KS, int RG, int MATS>
+int launch_ring(const Mx4Args &a, hipStream_t st) {
+  const int64_t tm = cdiv(a.M, BM), tn = cdiv(a.N, BN / MATS);
+  const int per = (int)(2 * cdiv(cdiv(a.kb, 128), 2 * KS));  // stages of a part, even
+  KernelTimer kt(st, BN == 128 ? "mx4_ring128" : KS == 2 ? "mx4_ring64x2" : "mx4_ring64");
+  hipLaunchKernelGGL((mx4_ring_k<BM, BN, WGM, WGN, KS, RG, MATS>), dim3((unsigned)(tm * tn)),
+                     dim3(64 * WGM * WGN * KS), 0, st, a, (int)tm, (int)tn, per);
+  SIMP_HIP(hipGetLastError());
+  return SIMP_RT_OK;
+}
+
+// Codes of rows whose bytes the tile kernels cannot read in place (any address and length)
+// into rows of whole aligned 16 bytes, zeros behind their ends.
+__global__ void __launch_bounds__(256)
+    mx4_pad_k(const uint8_t *__restrict__ codes, int64_t ld, uint4 *__restrict__ out, int kb, int per,
+              int64_t chunks) {
+  const int64_t first = (int64_t)blockIdx.x * 1024;
+  const BlockAt at(first, per);
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const uint32_t i = u * 256 + threadIdx.x;
+    if (first + i >= chunks) break;
+    int64_t row, c;
+    at.get(i, row, c);
+    out[first + i] = row16(codes + row * ld, 16 * (int)c, kb);
+  }
+}
+
+// 256 x 256 tiles; false where their scales cannot be packed (no memory, or a captured call
+// whose warm-up left too little).
 template <int MATS>
-bool aligned16(const Mx4Args &a) {
-  uintptr_t x = (uintptr_t)a.a | (uintptr_t)a.lda | (uintptr_t)a.kb;
-  for (int t = 0; t < MATS; t++) x |= (uintptr_t)a.b[t] | (uintptr_t)a.ldb[t];
-  return (x & 15) == 0;
+bool launch_dma(const Mx4Args &a, hipStream_t st, int *rc) {
+  const int64_t tm = cdiv(a.M, 256), tn = cdiv(a.N, 256 / MATS);
+  const int groups = (int)cdiv(a.kb, 256), ga = (int)(4 * tm), gb = (int)(4 * tn);
+  const int64_t rgs = (int64_t)(ga + gb) * groups;
+  Workspace ws;
+  void *p;
+  if (tm * tn > INT32_MAX || (int64_t)(ga + gb) * 256 > INT32_MAX || groups > 4 * 65535 ||
+      !ws.try_get(st, (size_t)rgs * 1024, &p, 10))
+    return false;
+  uint4 *pa = (uint4 *)p, *pb = pa + (int64_t)ga * groups * 64;
+  hipLaunchKernelGGL(mx4_pack_scales_k<MATS>, dim3((unsigned)(ga + gb), (unsigned)cdiv(groups, 4)),
+                     dim3(256), 0, st, a, pa, pb, ga, groups);
+  const int stream = a.N % 16 == 0 && ((uintptr_t)a.out & 63) == 0 && a.ldo % 16 == 0;
+  const int64_t grid = std::min<int64_t>(tm * tn, num_cus());
+  const int stagger = tm * tn >= 2 * grid && MATS == 1 ? 2 : tm * tn >= 4 * grid ? 1 : 0;
+  KernelTimer kt(st, "mx4_dma");
+  hipLaunchKernelGGL((mx4_dma_k<MATS>), dim3((unsigned)grid), dim3(512), 0, st, a, pa, pb, (int)tm,
+                     (int)tn, groups, stream, stagger);
+  const hipError_t e = hipGetLastError();
+  *rc = e == hipSuccess ? SIMP_RT_OK : hip_fail(e, "launch");
+  return true;
+}
+
+// What each form takes in us, fitted to whole calls (graph replay) of 1 to 8192 rows,
+// K = 768 to 8192 and up to 32000 columns; `steps` of 128 elements, `out` the outputs'
+// time to memory.  The choice by it is within about 10% of the best form's time.
+enum Form { kSkinny, kRing64, kRing64x2, kRing128, kTiles256 };
+template <int MATS>
+Form pick(const Mx4Args &a, int64_t cus) {
+  const double steps = (double)cdiv(a.kb, 64), out = 4e-6 * a.M * a.N / 6.5;
+  const int mt = a.M <= 16 ? 16 : a.M <= 32 ? 32 : 64;
+  auto tiles = [&](int m, int n) { return cdiv(a.M, m) * cdiv(a.N, n / MATS); };
+  auto rounds = [&](int64_t t) { return (double)cdiv(t, cus); };
+  double us[5];
+  us[kSkinny] = 3.0 + (double)cdiv(a.M, mt) * cdiv(a.N, 16) * (std::min(a.M, mt) + 16 * MATS) * steps * 68 / 6.6e6;
+  const int64_t t64 = tiles(64, 64), t256 = tiles(256, 256);
+  us[kRing64] = 3.7 + steps / 2 * std::max(0.33, 0.23 * rounds(t64)) + out;
+  us[kRing64x2] = 4.0 + steps / 2 * 0.2 * (t64 <= cus ? 1. : 1.3 * rounds(t64)) + out;
+  us[kRing128] = 3.7 + steps / 2 * 0.42 * rounds(tiles(64, 128)) + out;
+  us[kTiles256] = 8.0 + steps * (0.95 * (t256 / cus) + (t256 % cus ? 0.3 + 0.65 * (t256 % cus) / cus : 0.)) + out;
+  return (Form)(std::min_element(us, us + 5) - us);
+}
+
+// The form that `pick` names, where the codes can be read as they lie; false where not.
+template <int MATS>
+bool launch_tiles(const Mx4Args &a, Form f, hipStream_t st, int *rc) {
+  if (f == kTiles256 && launch_dma<MATS>(a, st, rc)) return true;
+  if (cdiv(a.M, 64) * cdiv(a.N, 64 / MATS) > INT32_MAX / 512) return false;
+  *rc = f == kRing64 ? launch_ring<64, 64, 2, 2, 1, 9, MATS>(a, st)
+        : f == kRing64x2 ? launch_ring<64, 64, 2, 2, 2, 9, MATS>(a, st)
+                         : launch_ring<64, 128, 2, 4, 1, 9, MATS>(a, st);
+  return true;
 }
 
 template <int MATS>
 int launch_mx4(const Mx4Args &a, hipStream_t st) {
-  const int64_t cus = num_cus();
-  const int64_t tm = cdiv(a.M, 256), tn = cdiv(a.N, 256 / MATS);
-  // (offsets within a tile are 32-bit)
-  const int64_t ld = std::max({a.lda, a.ldb[0], a.ldb[MATS - 1]});
-  if (a.kb > 0 && tm * tn >= cus / 2 && tm * tn <= INT32_MAX && ld < (1 << 23) && aligned16<MATS>(a)) {
-    const int groups = (int)cdiv(a.kb, 256), ga = (int)(4 * tm), gb = (int)(4 * tn);
-    const int64_t rgs = (int64_t)(ga + gb) * groups;
-    Workspace ws;
-    void *p;
-    if (rgs <= INT32_MAX && ws.try_get(st, (size_t)rgs * 1024, &p, 4)) {
-      uint4 *pa = (uint4 *)p, *pb = pa + (int64_t)ga * groups * 64;
-      hipLaunchKernelGGL(mx4_pack_scales_k<MATS>, dim3((unsigned)cdiv(rgs, 4)), dim3(256), 0, st, a,
-                         pa, pb, ga, gb, groups);
-      SIMP_HIP(hipGetLastError());
-      const int stream = a.N % 16 == 0 && ((uintptr_t)a.out & 63) == 0 && a.ldo % 16 == 0;
-      KernelTimer kt(st, "mx4_dma");
-      hipLaunchKernelGGL(mx4_dma_k<MATS>, dim3((unsigned)std::min(tm * tn, cus)), dim3(512), 0, st, a,
-                         pa, pb, (int)tm, (int)tn, groups, stream);
-      SIMP_HIP(hipGetLastError());
-      return SIMP_RT_OK;
+  int rc;
+  const Form f = pick<MATS>(a, num_cus());
+  if (f != kSkinny && a.kb > 0) {
+    // the tile kernels read aligned 16-byte pieces, and their offsets within a tile are 32-bit
+    uintptr_t low = (uintptr_t)a.a | (uintptr_t)a.lda | (uintptr_t)a.kb;
+    for (int t = 0; t < MATS; t++) low |= (uintptr_t)a.b[t] | (uintptr_t)a.ldb[t];
+    const int64_t ld = std::max({a.lda, a.ldb[0], a.ldb[MATS - 1]});
+    if ((low & 15) == 0 && ld < (1 << 23)) {
+      if (launch_tiles<MATS>(a, f, st, &rc)) return rc;
+    } else if (a.kb < (1 << 23) - 16) {
+      const int per = (int)cdiv(a.kb, 16);
+      const int64_t ca = (int64_t)a.M * per, cb = (int64_t)a.N * per;
+      Workspace ws;
+      void *p;
+      if (std::max(ca, cb) / 4 < INT32_MAX - 256 && ws.try_get(st, 16 * (size_t)(ca + MATS * cb), &p, 11)) {
+        Mx4Args c = a;
+        uint4 *q = (uint4 *)p;
+        auto pad = [&](const uint8_t *&codes, int64_t &row, int64_t chunks) {
+          hipLaunchKernelGGL(mx4_pad_k, dim3((unsigned)cdiv(chunks, 1024)), dim3(256), 0, st, codes, row, q,
+                             a.kb, per, chunks);
+          codes = (const uint8_t *)q, row = 16 * (int64_t)per;
+          q += chunks;
+        };
+        pad(c.a, c.lda, ca);
+        for (int t = 0; t < MATS; t++) pad(c.b[t], c.ldb[t], cb);
+        SIMP_HIP(hipGetLastError());
+        if (launch_tiles<MATS>(c, f, st, &rc)) return rc;
+      }
     }
   }
   if (a.M <= 16) return launch_skinny<1, 1, MATS>(a, st);

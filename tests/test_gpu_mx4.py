@@ -188,35 +188,106 @@ def _values64(codes, scales):
     return v * two.repeat_interleave(32, 1)[:, :v.shape[1]]
 
 
-LARGE = [(2900, 16, 3100), (2817, 32, 3089), (3000, 80, 2900), (2900, 208, 3001), (3100, 272, 2900),
-         (3000, 528, 3000), (257, 640, 16640), (8200, 144, 700), (2900, 1040, 3008)]
+# rows, code bytes of a row, columns, and the kernel that takes the product and the gate
+FORMS = [
+    (64, 1600, 2800, "skinny", "ring64x2"),
+    (33, 2320, 3000, "skinny", "skinny"),
+    (129, 2304, 1500, "ring64x2", "ring64x2"),
+    (300, 1024, 3000, "ring64x2", "ring128"),
+    (250, 912, 3000, "ring64x2", "ring128"),
+    (100, 1088, 8200, "ring128", "ring64"),
+    (257, 640, 8320, "ring64", "ring128"),
+    (600, 272, 4100, "ring64", "ring128"),
+    (513, 2448, 2050, "ring128", "ring64"),
+    (700, 767, 2051, "ring128", "ring64"),
+    (900, 80, 9000, "ring64", "ring128"),
+    (300, 1100, 2051, "ring64x2", "ring128"),
+    (65, 2500, 3001, "ring64x2", "ring64x2"),
+    (130, 640, 9000, "ring128", "ring128"),
+    (1100, 1104, 1100, "ring128", "ring64"),
+    (1000, 144, 6000, "ring128", "ring128"),
+    (600, 2336, 2000, "ring128", "ring64"),
+    (200, 1601, 4000, "ring64x2", "ring128"),
+    (65, 6000, 1000, "skinny", "ring64x2"),
+    (3000, 800, 2900, "dma", "dma"),
+    (2900, 1040, 3008, "dma", "dma"),
+    (2817, 1088, 3089, "dma", "dma"),
+    (3100, 1200, 2900, "dma", "dma"),
+    (2900, 1001, 3000, "dma", "dma"),
+    (6000, 1024, 6000, "dma", "dma"),
+    (3000, 2064, 2900, "dma", "dma"),
+    (70, 2048, 4096, "ring64x2", "ring64x2"),
+    (200, 768, 12000, "ring64", "ring128"),
+]
+
+
+def _on_device(dev, seed, m, kb, n, gate, lo=126, hi=129, pad=0, shift=0):
+    import torch
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+
+    def codes(r):
+        out = []
+        for w, a, b in ((kb, 0, 256), (-(-kb // 16), lo, hi)):
+            buf = torch.randint(a, b, (shift + r * (w + pad) + 1,), generator=g, device=dev, dtype=torch.uint8)
+            out.append(buf[shift:shift + r * (w + pad)].view(r, w + pad)[:, :w])
+        return out
+
+    return [codes(r) for r in (m, n, n)[:2 + gate]]
 
 
 @pytest.mark.parametrize("gate", [False, True])
-@pytest.mark.parametrize("m, kb, n", LARGE)
-def test_large_products(dev, gate, m, kb, n):
-    """Against 64 bits on the device: every output of products that fill the chip."""
+@pytest.mark.parametrize("pad, shift, opad", [(0, 0, 0), (32, 16, 4), (3, 1, 1)])
+@pytest.mark.parametrize("m, kb, n, plain, gated", FORMS)
+def test_every_form(dev, gate, m, kb, n, plain, gated, pad, shift, opad):
+    """Against 64 bits on the device, every output; rows as they lie, padded, and at odd addresses."""
     import torch
-    g = torch.Generator(device=dev)
-    g.manual_seed(m + kb)
-    n //= 1 + gate
-
-    def codes(r):
-        return (torch.randint(0, 256, (r, kb), generator=g, device=dev, dtype=torch.uint8),
-                torch.randint(126, 129, (r, -(-kb // 16)), generator=g, device=dev, dtype=torch.uint8))
-
-    a, *bs = [codes(r) for r in (m, n, n)[:2 + gate]]
-    out = torch.full((m + 2, n), 5.0, device=dev)
-    (sa.swiglu_mx4 if gate else sa.matmul_mx4)(*a, *[x for b in bs for x in b], out[1:-1])
+    a, *bs = _on_device(dev, m + kb, m, kb, n, gate, pad=pad, shift=shift)
+    buf = torch.full((m + 2, n + opad), 5.0, device=dev)
+    out = buf[1:-1, :n]
+    f = sa.swiglu_mx4 if gate else sa.matmul_mx4
+    f(*a, *[x for b in bs for x in b], out)  # (makes room for the scratch that the form takes)
+    out.fill_(6)
+    sa.timing(True)
+    try:
+        f(*a, *[x for b in bs for x in b], out)
+        assert sa.timing_query("mx4_" + (gated if gate else plain))[1] == 1
+    finally:
+        sa.timing(False)
+    assert (buf[0] == 5).all() and (buf[-1] == 5).all() and (buf[:, n:] == 5).all()
     want = [_values64(*a) @ _values64(*b).t().contiguous() for b in bs]
-    assert (out[0] == 5).all() and (out[-1] == 5).all()
     if not gate:
-        assert torch.equal(out[1:-1].double(), want[0])
+        assert torch.equal(out.double(), want[0])  # the sums are exact in fp32
     else:
-        silu = want[0] / (1 + torch.exp(-want[0]))
-        w = silu * want[1]
-        # the two sums are exact in fp32: what is left is the gate's rounding (mx.gated)
-        assert ((out[1:-1].double() - w).abs() <= 8 * mx.EPS * w.abs() + 2.0 ** -121 * want[1].abs()).all()
+        w = want[0] / (1 + torch.exp(-want[0])) * want[1]
+        assert ((out.double() - w).abs() <= 8 * mx.EPS * w.abs() + 2.0 ** -121 * want[1].abs()).all()
+
+
+@pytest.mark.parametrize("lo, hi", [(100, 150), (40, 200), (0, 40)])
+@pytest.mark.parametrize("m, kb, n", [(129, 2304, 1500), (600, 272, 4100), (130, 640, 9000), (2900, 1040, 3008)])
+def test_every_form_with_scales_far_apart(dev, m, kb, n, lo, hi):
+    import torch
+    a, b = _on_device(dev, m + lo, m, kb, n, False, lo, hi)
+    a[1][m // 2, -1] = 255  # one row with a NaN
+    out = sa.matmul_mx4(*a, *b, torch.empty((m, n), device=dev))
+    assert out[m // 2].isnan().all()
+    a[1][m // 2, -1] = 0
+    va, vb = _values64(*a), _values64(*b)
+    size = va.abs() @ vb.abs().t().contiguous()
+    tol = (a[1].shape[1] + 20) * (mx.EPS * size + 2.0 ** -150)
+    off = (out.double() - va @ vb.t().contiguous()).abs()
+    off[m // 2] = 0
+    # beyond fp32's range infinities and what follows from them are right
+    assert ((off <= tol) | (size > 3e38)).all()
+
+
+def test_millions_of_rows(dev):
+    import torch
+    m, kb = 2_200_000, 3
+    a, b = _on_device(dev, 1, m, kb, 300, False)
+    out = sa.matmul_mx4(*a, *b, torch.empty((m, 300), device=dev))
+    assert torch.equal(out[-5000:].double(), _values64(*[x[-5000:] for x in a]) @ _values64(*b).t().contiguous())
+    assert torch.equal(out[:5000].double(), _values64(*[x[:5000] for x in a]) @ _values64(*b).t().contiguous())
 
 
 def test_product_of_nothing_is_zero(dev):
@@ -311,7 +382,8 @@ def test_rows_far_apart(dev):
         assert np.array_equal(d[0].cpu().numpy(), codes) and np.array_equal(d[1].cpu().numpy(), scales)
 
 
-SHAPES = [(1, 400, 300), (16, 1080, 160), (40, 767, 65), (200, 400, 540), (300, 1024, 512), (1100, 256, 1100)]
+SHAPES = [(1, 400, 300), (16, 1080, 160), (40, 767, 65), (129, 2304, 1500), (700, 767, 2051), (130, 640, 9000),
+          (2900, 1040, 3008), (2900, 1001, 3000)]
 
 
 @pytest.mark.parametrize("gate", [False, True])
@@ -389,7 +461,7 @@ def test_two_threads_on_their_own_streams(dev):
 
 
 @pytest.mark.parametrize("gate", [False, True])
-@pytest.mark.parametrize("m, kb, n", SHAPES + [(2, 4320, 3200), (520, 1600, 2051)])
+@pytest.mark.parametrize("m, kb, n", SHAPES + [(2, 4320, 3200), (600, 272, 4100)])
 def test_the_same_call_gives_the_same_bits(dev, gate, m, kb, n):
     import torch
     rng = np.random.default_rng(m)
