@@ -27,11 +27,13 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 // compiler picks the instructions).
 typedef uint32_t u4any __attribute__((ext_vector_type(4), aligned(1)));
 typedef uint32_t u1any __attribute__((aligned(1)));
+typedef uint16_t u2any __attribute__((aligned(1)));
 typedef float f4any __attribute__((ext_vector_type(4), aligned(4)));
 
-__device__ __forceinline__ uint32_t max_dpp4(uint32_t v) {  // over lanes 4i .. 4i+3
+__device__ __forceinline__ uint32_t max_dpp8(uint32_t v) {  // over lanes 8i .. 8i+7
   v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor1, 0xF, 0xF, false));
-  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor2, 0xF, 0xF, false));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor2, 0xF, 0xF, false));
+  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppHalfMirror, 0xF, 0xF, false));
 }
 
 // 2^(s - 127) in fp32 (255: infinity)
@@ -40,14 +42,15 @@ __device__ __forceinline__ float scale_of(uint32_t s) {
 }
 
 // Row and column block of the i-th 32-element block of the rows, i counted from the
-// workgroup's first: one 64-bit division per workgroup, a 32-bit one per thread.
+// workgroup's first (per_row below 2^31).
 struct BlockAt {
   int64_t row0;
   uint32_t rem, per;
   __device__ BlockAt(int64_t first, int64_t per_row) {
-    row0 = first / per_row;
-    rem = (uint32_t)(first - row0 * per_row);
     per = (uint32_t)per_row;
+    if ((uint64_t)first >> 32 == 0) row0 = (uint32_t)first / per;
+    else row0 = first / per_row;
+    rem = (uint32_t)(first - row0 * per_row);
   }
   __device__ void get(uint32_t i, int64_t &row, int64_t &blk) const {
     const uint32_t q = (rem + i) / per;
@@ -56,101 +59,110 @@ struct BlockAt {
   }
 };
 
-constexpr int kBlocksPerWg = 256;  // MX blocks of a workgroup of 256 threads
-
-// Four lanes to a block, eight elements each.
+// Eight lanes to a block, four elements each, so that a wave's loads and stores of values are
+// 1 KB in lane order; a thread takes RUN blocks, their loads together.  STREAM: values are
+// taken and left past the caches (they lie on 16 bytes).  8192 x 8192: 59 us (5.1 TB/s) and
+// back 44 us (6.9; a copy reaches 4.9); with eight elements to a lane, 32 bytes apart, 75
+// and 78.  RUN = 4 for many blocks, 1 where few leave CUs idle (one row of 3200: 1.9 us, not 2.7).
+template <int RUN, bool STREAM>
 __global__ void __launch_bounds__(256)
     quantize_mx4_k(const float *__restrict__ x, int64_t ldx, uint8_t *__restrict__ codes,
                    int64_t ldc, uint8_t *__restrict__ scales, int64_t lds, int64_t cols,
                    int64_t per_row, int64_t blocks) {
-  const int64_t first = (int64_t)blockIdx.x * kBlocksPerWg;
+  const int64_t first = (int64_t)blockIdx.x * (32 * RUN);
   const BlockAt at(first, per_row);
+  const int lane8 = threadIdx.x & 7;
+  int64_t row[RUN], blk[RUN];
+  v4f v[RUN];
 #pragma unroll
-  for (int u = 0; u < kBlocksPerWg / 64; u++) {
-    const uint32_t i = u * 64 + (threadIdx.x >> 2);
-    if (first + i >= blocks) break;  // the four lanes of a block together
-    int64_t row, blk;
-    at.get(i, row, blk);
-    const int64_t c0 = 32 * blk + 8 * (threadIdx.x & 3);
-    const float *p = x + row * ldx + c0;
-    float v[8];
-    if (c0 + 8 <= cols) {
-      const f4any a = *(const f4any *)p, b = *(const f4any *)(p + 4);
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = a[e], v[4 + e] = b[e];
+  for (int u = 0; u < RUN; u++) {
+    const uint32_t i = u * 32 + (threadIdx.x >> 3);
+    at.get(i, row[u], blk[u]);
+    const int64_t c0 = 32 * blk[u] + 4 * lane8;
+    const float *p = x + row[u] * ldx + c0;
+    v[u] = v4f{0.f, 0.f, 0.f, 0.f};
+    if (first + i >= blocks) continue;  // the eight lanes of a block together
+    if (c0 + 4 <= cols) {
+      if constexpr (STREAM) v[u] = __builtin_nontemporal_load((const v4f *)p);
+      else v[u] = *(const f4any *)p;
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = c0 + e < cols ? p[e] : 0.f;
+      for (int e = 0; e < 3; e++)
+        if (c0 + e < cols) v[u][e] = p[e];
     }
+  }
+#pragma unroll
+  for (int u = 0; u < RUN; u++) {
+    if (first + u * 32 + (threadIdx.x >> 3) >= blocks) break;
+    const int64_t c0 = 32 * blk[u] + 4 * lane8;
     uint32_t top = 0;  // sizes compare as whole numbers, NaN above infinity
 #pragma unroll
-    for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[e]) & 0x7FFFFFFFu);
-    top = max_dpp4(top);
+    for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(v[u][e]) & 0x7FFFFFFFu);
+    top = max_dpp8(top);
     const bool bad = top >= 0x7F800000u;
     const uint32_t ex = top >> 23, s = ex > 2 ? ex - 2 : 0;
     const float unit = scale_of(s);
     uint32_t c = 0;
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], unit, 0);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], unit, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], unit, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], unit, 3);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[u][0], v[u][1], unit, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[u][2], v[u][3], unit, 1);
     if (bad) c = 0;
-    uint8_t *o = codes + row * ldc + (c0 >> 1);
-    if (c0 + 8 <= cols) {
-      *(u1any *)o = c;
+    uint8_t *o = codes + row[u] * ldc + (c0 >> 1);
+    if (c0 + 4 <= cols) {
+      *(u2any *)o = (uint16_t)c;
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++)
+      for (int e = 0; e < 2; e++)
         if (c0 + 2 * e < cols) o[e] = (uint8_t)(c >> (8 * e));
     }
-    if ((threadIdx.x & 3) == 0) scales[row * lds + blk] = bad ? 255 : (uint8_t)s;
+    if (lane8 == 0) scales[row[u] * lds + blk[u]] = bad ? 255 : (uint8_t)s;
   }
 }
 
+template <int RUN, bool STREAM>
 __global__ void __launch_bounds__(256)
     dequantize_mx4_k(const uint8_t *__restrict__ codes, int64_t ldc,
                      const uint8_t *__restrict__ scales, int64_t lds, float *__restrict__ out,
                      int64_t ldo, int64_t cols, int64_t per_row, int64_t blocks) {
-  const int64_t first = (int64_t)blockIdx.x * kBlocksPerWg;
+  const int64_t first = (int64_t)blockIdx.x * (32 * RUN);
   const BlockAt at(first, per_row);
+  const int lane8 = threadIdx.x & 7;
+  int64_t row[RUN], blk[RUN];
+  uint32_t c[RUN], s[RUN];
 #pragma unroll
-  for (int u = 0; u < kBlocksPerWg / 64; u++) {
-    const uint32_t i = u * 64 + (threadIdx.x >> 2);
-    if (first + i >= blocks) break;
-    int64_t row, blk;
-    at.get(i, row, blk);
-    const int64_t c0 = 32 * blk + 8 * (threadIdx.x & 3);
-    if (c0 >= cols) continue;
-    const bool whole = c0 + 8 <= cols;
-    const uint8_t *p = codes + row * ldc + (c0 >> 1);
-    uint32_t c = 0;
-    if (whole) {
-      c = *(const u1any *)p;
+  for (int u = 0; u < RUN; u++) {
+    const uint32_t i = u * 32 + (threadIdx.x >> 3);
+    at.get(i, row[u], blk[u]);
+    const int64_t c0 = 32 * blk[u] + 4 * lane8;
+    const uint8_t *p = codes + row[u] * ldc + (c0 >> 1);
+    c[u] = s[u] = 0;
+    if (first + i >= blocks || c0 >= cols) continue;
+    if (c0 + 4 <= cols) {
+      c[u] = *(const u2any *)p;
+    } else {
+      c[u] = p[0];
+      if (c0 + 2 < cols) c[u] |= (uint32_t)p[1] << 8;
+    }
+    s[u] = scales[row[u] * lds + blk[u]];
+  }
+#pragma unroll
+  for (int u = 0; u < RUN; u++) {
+    const int64_t c0 = 32 * blk[u] + 4 * lane8;
+    if (first + u * 32 + (threadIdx.x >> 3) >= blocks || c0 >= cols) continue;
+    const float unit = scale_of(s[u]);
+    const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], unit, 0),
+              b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], unit, 1);
+    v4f v = {a[0], a[1], b[0], b[1]};
+    if (s[u] == 255) {
+      const float nan = __uint_as_float(0x7FC00000u);
+      v = v4f{nan, nan, nan, nan};
+    }
+    float *o = out + row[u] * ldo + c0;
+    if (c0 + 4 <= cols) {
+      if constexpr (STREAM) __builtin_nontemporal_store(v, (v4f *)o);
+      else *(f4any *)o = v;
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (c0 + 2 * e < cols) c |= (uint32_t)p[e] << (8 * e);
-    }
-    const uint32_t s = scales[row * lds + blk];
-    const float unit = scale_of(s);
-    float v[8];
-    const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, unit, 0),
-              b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, unit, 1),
-              d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, unit, 2),
-              f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, unit, 3);
-    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1];
-    v[4] = d[0], v[5] = d[1], v[6] = f[0], v[7] = f[1];
-    if (s == 255) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[e] = __uint_as_float(0x7FC00000u);
-    }
-    float *o = out + row * ldo + c0;
-    if (whole) {
-      *(f4any *)o = f4any{v[0], v[1], v[2], v[3]};
-      *(f4any *)(o + 4) = f4any{v[4], v[5], v[6], v[7]};
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; e++)
+      for (int e = 0; e < 3; e++)
         if (c0 + e < cols) o[e] = v[e];
     }
   }
@@ -197,15 +209,20 @@ __device__ __forceinline__ void lane_transpose(v4f (&x)[N]) {
   }
 }
 
-// 16 code bytes of a row from byte k on, zeros behind its end.
+// 16 code bytes of a row from byte k on, zeros behind its end: with fewer left, the row's
+// last 16 shifted down.
 __device__ __forceinline__ uint4 row16(const uint8_t *row, int k, int kb) {
-  if (k + 16 <= kb) {
-    const u4any v = *(const u4any *)(row + k);
-    return make_uint4(v.x, v.y, v.z, v.w);
+  if (kb >= 16) {
+    const int at = min(k, kb - 16), sh = min(k - at, 16);
+    const u4any v = *(const u4any *)(row + at);
+    uint64_t lo = v.x | (uint64_t)v.y << 32, hi = v.z | (uint64_t)v.w << 32;
+    if (sh >= 8) lo = sh < 16 ? hi >> (8 * (sh - 8)) : 0, hi = 0;
+    else if (sh > 0) lo = lo >> (8 * sh) | hi << (64 - 8 * sh), hi >>= 8 * sh;
+    return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
   }
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < 16; i++)
+  for (int i = 0; i < 15; i++)
     if (k + i < kb) w[i >> 2] |= (uint32_t)row[k + i] << (8 * (i & 3));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
@@ -214,26 +231,30 @@ __device__ __forceinline__ uint4 row16(const uint8_t *row, int k, int kb) {
 // takes every byte of its rows' piece once, straight from memory into the lanes that
 // feed the matrix instruction (16 rows of 64 bytes, and a byte of scales to a lane), and
 // the waves' sums meet in LDS, in the order of K.
+constexpr int skinny_waves(int MT) { return MT >= 4 ? 8 : 16; }  // of a block at most
 template <int MT, int NT, int MATS>
-__global__ void __launch_bounds__(1024) mx4_skinny_k(const Mx4Args a, int span, int blocks_n) {
+__global__ void __launch_bounds__(64 * skinny_waves(MT)) mx4_skinny_k(const Mx4Args a, int span, int blocks_n) {
   constexpr int T = MATS * MT * NT;
+  constexpr int U = MT == 4 ? 2 : 4;
   extern __shared__ v4f part[];  // [waves][T][64]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int r = lane & 15, q = lane >> 4;
   const int bm = blockIdx.x / blocks_n;
   const int n0 = 16 * NT * (blockIdx.x - bm * blocks_n), m0 = 16 * MT * bm;
   const uint8_t *ap[MT], *as[MT], *bp[MATS][NT], *bs[MATS][NT];
+  bool in[MT];  // rows behind the last are not asked for
 #pragma unroll
   for (int i = 0; i < MT; i++) {
+    in[i] = m0 + 16 * i + r < a.M;
     const int64_t m = min(m0 + 16 * i + r, a.M - 1);
-    ap[i] = a.a + m * a.lda + 16 * q, as[i] = a.as + m * a.ldas + q;
+    ap[i] = a.a + m * a.lda + 16 * q, as[i] = a.as + m * a.ldas;
   }
 #pragma unroll
   for (int t = 0; t < MATS; t++)
 #pragma unroll
     for (int j = 0; j < NT; j++) {
       const int64_t n = min(n0 + 16 * j + r, a.N - 1);
-      bp[t][j] = a.b[t] + n * a.ldb[t] + 16 * q, bs[t][j] = a.bs[t] + n * a.ldbs[t] + q;
+      bp[t][j] = a.b[t] + n * a.ldb[t] + 16 * q, bs[t][j] = a.bs[t] + n * a.ldbs[t];
     }
   v4f acc[MATS][MT][NT];
 #pragma unroll
@@ -255,51 +276,79 @@ __global__ void __launch_bounds__(1024) mx4_skinny_k(const Mx4Args a, int span, 
         for (int j = 0; j < NT; j++)
           acc[t][i][j] = mfma_mx4(s.b[t][j], s.bs[t][j], s.a[i], s.as[i], acc[t][i][j]);
   };
-  auto load = [&](int s) {
-    Step x;
+  auto load16 = [](const uint8_t *p) {
+    const u4any v = *(const u4any *)p;
+    return make_uint4(v.x, v.y, v.z, v.w);
+  };
+  auto codes = [&](Step &x, int s) {
 #pragma unroll
     for (int t = 0; t < MATS; t++)
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
-        const u4any v = *(const u4any *)(bp[t][j] + 64 * s);
-        x.b[t][j] = make_uint4(v.x, v.y, v.z, v.w);
-        x.bs[t][j] = bs[t][j][4 * s];
-      }
+      for (int j = 0; j < NT; j++) x.b[t][j] = load16(bp[t][j] + 64 * s);
 #pragma unroll
     for (int i = 0; i < MT; i++) {
-      const u4any v = *(const u4any *)(ap[i] + 64 * s);
-      x.a[i] = make_uint4(v.x, v.y, v.z, v.w);
-      x.as[i] = as[i][4 * s];
+      x.a[i] = make_uint4(0, 0, 0, 0);
+      if (in[i]) x.a[i] = load16(ap[i] + 64 * s);
     }
-    return x;
   };
   const int whole = a.kb >> 6;
   int s = wave * span;
   const int end = min(s + span, whole);
-  constexpr int U = T >= 4 ? 2 : 4;
-  for (; s + U <= end; s += U) {
-    Step x[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) x[u] = load(s + u);
-#pragma unroll
-    for (int u = 0; u < U; u++) run(x[u]);
-  }
-  for (; s < end; s++) run(load(s));
-  if (wave == waves - 1 && (a.kb & 63)) {  // the last step, which rows end in
-    const int k = 64 * whole + 16 * q;
-    Step x;
-#pragma unroll
-    for (int i = 0; i < MT; i++) {
-      x.a[i] = row16(ap[i] - 16 * q, k, a.kb);
-      x.as[i] = k < a.kb ? as[i][4 * whole] : 127;
-    }
+  // Four steps at a time: a lane's four scale bytes come out of 16 of its row.  What bounds
+  // the loop is the path from the caches, 64 bytes a cycle and a row to a cycle: a byte
+  // of scales for each fragment and step would cost as much as the codes.
+  for (; s + 4 <= end; s += 4) {
+    uint4 sa[MT], sb[MATS][NT];
 #pragma unroll
     for (int t = 0; t < MATS; t++)
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
-        x.b[t][j] = row16(bp[t][j] - 16 * q, k, a.kb);
-        x.bs[t][j] = k < a.kb ? bs[t][j][4 * whole] : 127;
+      for (int j = 0; j < NT; j++) sb[t][j] = load16(bs[t][j] + 4 * s);
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+      sa[i] = make_uint4(0, 0, 0, 0);
+      if (in[i]) sa[i] = load16(as[i] + 4 * s);
+    }
+    Step x[U];
+#pragma unroll
+    for (int h = 0; h < 4; h += U) {
+#pragma unroll
+      for (int u = 0; u < U; u++) codes(x[u], s + h + u);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        auto byte = [&](const uint4 &v) {
+          return (h + u == 0 ? v.x : h + u == 1 ? v.y : h + u == 2 ? v.z : v.w) >> (8 * q);
+        };
+#pragma unroll
+        for (int t = 0; t < MATS; t++)
+#pragma unroll
+          for (int j = 0; j < NT; j++) x[u].bs[t][j] = byte(sb[t][j]);
+#pragma unroll
+        for (int i = 0; i < MT; i++) x[u].as[i] = byte(sa[i]);
+        run(x[u]);
       }
+    }
+  }
+  // single steps; the last of all, which rows end in, by the last wave
+  const bool tail = wave == waves - 1 && (a.kb & 63);
+  for (; s < end + tail; s++) {
+    Step x;
+    const int k = 64 * s + 16 * q;
+    if (s < whole) {
+      codes(x, s);
+    } else {
+#pragma unroll
+      for (int i = 0; i < MT; i++) x.a[i] = row16(ap[i] - 16 * q, k, a.kb);
+#pragma unroll
+      for (int t = 0; t < MATS; t++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) x.b[t][j] = row16(bp[t][j] - 16 * q, k, a.kb);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; i++) x.as[i] = k < a.kb ? as[i][4 * s + q] : 127;
+#pragma unroll
+    for (int t = 0; t < MATS; t++)
+#pragma unroll
+      for (int j = 0; j < NT; j++) x.bs[t][j] = k < a.kb ? bs[t][j][4 * s + q] : 127;
     run(x);
   }
   if (waves > 1) {
@@ -349,10 +398,10 @@ __global__ void __launch_bounds__(1024) mx4_skinny_k(const Mx4Args a, int span, 
 template <int MT, int NT, int MATS>
 int launch_skinny(Mx4Args a, hipStream_t st) {
   const int64_t bn = cdiv(a.N, 16 * NT), bm = cdiv(a.M, 16 * MT);
-  // about 4096 waves on the chip, up to 16 to a block (64 KiB of sums)
+  // about 3072 waves on the chip, up to 16 to a block (64 KiB of sums)
   const int steps = a.kb >> 6;
-  int waves = (int)std::min<int64_t>({cdiv(4096, bn * bm), 16, std::max(steps, 1), 64 / (MATS * MT * NT)});
-  const int span = (int)cdiv(steps, waves);
+  int waves = (int)std::min<int64_t>({cdiv(3072, bn * bm), skinny_waves(MT), std::max(steps, 1), 64 / (MATS * MT * NT)});
+  const int span = (int)cdiv(cdiv(steps, waves), 4) * 4;
   if (span) waves = (int)cdiv(steps, span);
   const int64_t most = std::max<int64_t>(INT32_MAX / (64 * waves) / bn, 1);  // row blocks of a launch
   KernelTimer kt(st, "mx4_skinny");
@@ -859,20 +908,18 @@ int launch_ring(const Mx4Args &a, hipStream_t st) {
 }
 
 // Codes of rows whose bytes the tile kernels cannot read in place (any address and length)
-// into rows of whole aligned 16 bytes, zeros behind their ends.
-__global__ void __launch_bounds__(256)
-    mx4_pad_k(const uint8_t *__restrict__ codes, int64_t ld, uint4 *__restrict__ out, int kb, int per,
-              int64_t chunks) {
-  const int64_t first = (int64_t)blockIdx.x * 1024;
-  const BlockAt at(first, per);
-#pragma unroll
-  for (int u = 0; u < 4; u++) {
-    const uint32_t i = u * 256 + threadIdx.x;
-    if (first + i >= chunks) break;
-    int64_t row, c;
-    at.get(i, row, c);
-    out[first + i] = row16(codes + row * ld, 16 * (int)c, kb);
-  }
+// into rows of whole aligned 16 bytes, zeros behind their ends: A's, then each B's.
+template <int MATS>
+__global__ void __launch_bounds__(256) mx4_pad_k(const Mx4Args a, uint4 *__restrict__ out, int per, int ga, int gb) {
+  const int w = (int)blockIdx.x < ga ? 0 : MATS == 2 && (int)blockIdx.x >= ga + gb ? 2 : 1;
+  const int64_t first = (int64_t)((int)blockIdx.x - (w > 0 ? ga : 0) - (w > 1 ? gb : 0)) * 256;
+  const int64_t ca = (int64_t)a.M * per, cb = (int64_t)a.N * per;
+  if (first + threadIdx.x >= (w ? cb : ca)) return;
+  int64_t row, c;
+  BlockAt(first, per).get(threadIdx.x, row, c);
+  const uint8_t *p = w == 0 ? a.a + row * a.lda
+                            : a.b[w > 1 ? MATS - 1 : 0] + row * a.ldb[w > 1 ? MATS - 1 : 0];
+  out[(w > 0 ? ca : 0) + (w > 1 ? cb : 0) + first + threadIdx.x] = row16(p, 16 * (int)c, a.kb);
 }
 
 // 256 x 256 tiles; false where their scales cannot be packed (no memory, or a captured call
@@ -912,11 +959,14 @@ Form pick(const Mx4Args &a, int64_t cus) {
   auto tiles = [&](int m, int n) { return cdiv(a.M, m) * cdiv(a.N, n / MATS); };
   auto rounds = [&](int64_t t) { return (double)cdiv(t, cus); };
   double us[5];
-  us[kSkinny] = 3.0 + (double)cdiv(a.M, mt) * cdiv(a.N, 16) * (std::min(a.M, mt) + 16 * MATS) * steps * 68 / 6.6e6;
+  const double mem = (a.M + (double)MATS * a.N) * steps * 68 / 5.2e6;  // the operands' time from memory
+  // its blocks' operands from the caches: every row block reads B, every column block A
+  const double path = (double)cdiv(a.M, mt) * cdiv(a.N, 16) * (std::min(a.M, mt) + 16 * MATS) * steps * 68 / 8.5e6;
+  us[kSkinny] = 2.5 + std::max(path, mem);
   const int64_t t64 = tiles(64, 64), t256 = tiles(256, 256);
-  us[kRing64] = 3.7 + steps / 2 * std::max(0.33, 0.23 * rounds(t64)) + out;
-  us[kRing64x2] = 4.0 + steps / 2 * 0.2 * (t64 <= cus ? 1. : 1.3 * rounds(t64)) + out;
-  us[kRing128] = 3.7 + steps / 2 * 0.42 * rounds(tiles(64, 128)) + out;
+  us[kRing64] = 3.7 + std::max(mem, steps / 2 * std::max(0.33, 0.23 * rounds(t64))) + out;
+  us[kRing64x2] = 4.0 + std::max(mem, steps / 2 * 0.2 * (t64 <= cus ? 1. : 1.3 * rounds(t64))) + out;
+  us[kRing128] = 4.0 + std::max(mem, steps / 2 * 0.42 * rounds(tiles(64, 128))) + out;
   us[kTiles256] = 8.0 + steps * (0.95 * (t256 / cus) + (t256 % cus ? 0.3 + 0.65 * (t256 % cus) / cus : 0.)) + out;
   return (Form)(std::min_element(us, us + 5) - us);
 }
@@ -948,18 +998,16 @@ int launch_mx4(const Mx4Args &a, hipStream_t st) {
       const int64_t ca = (int64_t)a.M * per, cb = (int64_t)a.N * per;
       Workspace ws;
       void *p;
-      if (std::max(ca, cb) / 4 < INT32_MAX - 256 && ws.try_get(st, 16 * (size_t)(ca + MATS * cb), &p, 11)) {
-        Mx4Args c = a;
+      const int64_t ga = cdiv(ca, 256), gb = cdiv(cb, 256);
+      if ((ga + MATS * gb) * 256 <= INT32_MAX && ws.try_get(st, 16 * (size_t)(ca + MATS * cb), &p, 11)) {
         uint4 *q = (uint4 *)p;
-        auto pad = [&](const uint8_t *&codes, int64_t &row, int64_t chunks) {
-          hipLaunchKernelGGL(mx4_pad_k, dim3((unsigned)cdiv(chunks, 1024)), dim3(256), 0, st, codes, row, q,
-                             a.kb, per, chunks);
-          codes = (const uint8_t *)q, row = 16 * (int64_t)per;
-          q += chunks;
-        };
-        pad(c.a, c.lda, ca);
-        for (int t = 0; t < MATS; t++) pad(c.b[t], c.ldb[t], cb);
+        hipLaunchKernelGGL(mx4_pad_k<MATS>, dim3((unsigned)(ga + MATS * gb)), dim3(256), 0, st, a, q, per,
+                           (int)ga, (int)gb);
         SIMP_HIP(hipGetLastError());
+        Mx4Args c = a;
+        c.a = (const uint8_t *)q, c.lda = 16 * (int64_t)per;
+        for (int t = 0; t < MATS; t++)
+          c.b[t] = (const uint8_t *)(q + ca + t * cb), c.ldb[t] = 16 * (int64_t)per;
         if (launch_tiles<MATS>(c, f, st, &rc)) return rc;
       }
     }
@@ -1058,13 +1106,24 @@ int product(const char *fn, Mat<const uint8_t> &a, Mat<const uint8_t> &as,
   return finish(ops, 3 + 2 * MATS);
 }
 
-// Blocks of the rows, and the grid for them.
-int block_grid(const char *fn, int64_t rows, int64_t per_row, int64_t *blocks, unsigned *grid) {
-  *blocks = rows * per_row;
-  const int64_t g = cdiv(*blocks, kBlocksPerWg);
-  if (g > INT32_MAX / 256) return set_error(SIMP_RT_EUNSUPPORTED, "%s: more elements than the grid holds", fn);
-  *grid = (unsigned)g;
-  return SIMP_RT_OK;
+// Launches a kernel over the blocks of rows.
+struct BlockLaunch {
+  int64_t blocks;
+  int run;
+  unsigned grid;
+  int plan(const char *fn, int64_t rows, int64_t per_row) {
+    blocks = rows * per_row;
+    run = blocks <= (1 << 15) ? 1 : 4;
+    const int64_t g = cdiv(blocks, 32 * run);
+    if (g > INT32_MAX / 256) return set_error(SIMP_RT_EUNSUPPORTED, "%s: more elements than the grid holds", fn);
+    grid = (unsigned)g;
+    return SIMP_RT_OK;
+  }
+};
+
+// Values that go past the caches: too many to stay there for the next operator, rows on 16 bytes.
+bool streams(const void *p, int64_t ld, int64_t n) {
+  return n >= (int64_t(1) << 24) && ((uintptr_t)p & 15) == 0 && (ld & 3) == 0;
 }
 
 }  // namespace
@@ -1094,9 +1153,8 @@ int32_t simp_rt_quantize_mx4(
   if (x_s0 == 0 || x_s1 == 0) return SIMP_RT_OK;
   if (meets(mc, mx) || meets(ms, mx) || meets(mc, ms))
     return set_error(SIMP_RT_EINVAL, "%s: codes or scales share memory with another operand", fn);
-  int64_t blocks;
-  unsigned grid;
-  if ((rc = block_grid(fn, x_s0, s_s1, &blocks, &grid))) return rc;
+  BlockLaunch bl;
+  if ((rc = bl.plan(fn, x_s0, s_s1))) return rc;
   const int dev = ensure_device();
   if (dev < 0) return dev;
   Operand ox, oc, os;
@@ -1104,9 +1162,10 @@ int32_t simp_rt_quantize_mx4(
       (rc = bind_here(oc, mc.data(), mc.bytes(), Operand::kOut, dev, "codes")) ||
       (rc = bind_here(os, ms.data(), ms.bytes(), Operand::kOut, dev, "scales")))
     return rc;
-  hipLaunchKernelGGL(quantize_mx4_k, dim3(grid), dim3(256), 0, cur_stream(), (const float *)ox.dev(),
-                     mx.st[0], (uint8_t *)oc.dev(), mc.st[0], (uint8_t *)os.dev(), ms.st[0], x_s1,
-                     s_s1, blocks);
+  auto kernel = bl.run == 1 ? quantize_mx4_k<1, false>
+                : streams(ox.dev(), mx.st[0], x_s0 * x_s1) ? quantize_mx4_k<4, true> : quantize_mx4_k<4, false>;
+  hipLaunchKernelGGL(kernel, dim3(bl.grid), dim3(256), 0, cur_stream(), (const float *)ox.dev(), mx.st[0],
+                     (uint8_t *)oc.dev(), mc.st[0], (uint8_t *)os.dev(), ms.st[0], x_s1, s_s1, bl.blocks);
   SIMP_HIP(hipGetLastError());
   Operand *ops[] = {&ox, &oc, &os};
   return finish(ops, 3);
@@ -1132,9 +1191,8 @@ int32_t simp_rt_dequantize_mx4(
   if (out_s0 == 0 || out_s1 == 0) return SIMP_RT_OK;
   if (meets(mo, mc) || meets(mo, ms))
     return set_error(SIMP_RT_EINVAL, "%s: out shares memory with another operand", fn);
-  int64_t blocks;
-  unsigned grid;
-  if ((rc = block_grid(fn, out_s0, s_s1, &blocks, &grid))) return rc;
+  BlockLaunch bl;
+  if ((rc = bl.plan(fn, out_s0, s_s1))) return rc;
   const int dev = ensure_device();
   if (dev < 0) return dev;
   Operand oc, os, oo;
@@ -1142,9 +1200,10 @@ int32_t simp_rt_dequantize_mx4(
       (rc = bind_here(os, ms.data(), ms.bytes(), Operand::kIn, dev, "scales")) ||
       (rc = bind_here(oo, mo.data(), mo.bytes(), Operand::kOut, dev, "out")))
     return rc;
-  hipLaunchKernelGGL(dequantize_mx4_k, dim3(grid), dim3(256), 0, cur_stream(),
-                     (const uint8_t *)oc.dev(), mc.st[0], (const uint8_t *)os.dev(), ms.st[0],
-                     (float *)oo.dev(), mo.st[0], out_s1, s_s1, blocks);
+  auto kernel = bl.run == 1 ? dequantize_mx4_k<1, false>
+                : streams(oo.dev(), mo.st[0], out_s0 * out_s1) ? dequantize_mx4_k<4, true> : dequantize_mx4_k<4, false>;
+  hipLaunchKernelGGL(kernel, dim3(bl.grid), dim3(256), 0, cur_stream(), (const uint8_t *)oc.dev(), mc.st[0],
+                     (const uint8_t *)os.dev(), ms.st[0], (float *)oo.dev(), mo.st[0], out_s1, s_s1, bl.blocks);
   SIMP_HIP(hipGetLastError());
   Operand *ops[] = {&oc, &os, &oo};
   return finish(ops, 3);

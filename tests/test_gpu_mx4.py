@@ -190,25 +190,25 @@ def _values64(codes, scales):
 
 # rows, code bytes of a row, columns, and the kernel that takes the product and the gate
 FORMS = [
-    (64, 1600, 2800, "skinny", "ring64x2"),
+    (64, 1600, 2800, "skinny", "skinny"),
     (33, 2320, 3000, "skinny", "skinny"),
     (129, 2304, 1500, "ring64x2", "ring64x2"),
     (300, 1024, 3000, "ring64x2", "ring128"),
-    (250, 912, 3000, "ring64x2", "ring128"),
+    (250, 912, 3000, "ring64x2", "ring64"),
     (100, 1088, 8200, "ring128", "ring64"),
     (257, 640, 8320, "ring64", "ring128"),
-    (600, 272, 4100, "ring64", "ring128"),
+    (600, 272, 4100, "ring64", "ring64"),
     (513, 2448, 2050, "ring128", "ring64"),
-    (700, 767, 2051, "ring128", "ring64"),
-    (900, 80, 9000, "ring64", "ring128"),
+    (700, 767, 2051, "ring64", "ring64"),
+    (900, 80, 9000, "ring64", "ring64"),
     (300, 1100, 2051, "ring64x2", "ring128"),
     (65, 2500, 3001, "ring64x2", "ring64x2"),
-    (130, 640, 9000, "ring128", "ring128"),
+    (130, 640, 9000, "ring64", "ring128"),
     (1100, 1104, 1100, "ring128", "ring64"),
-    (1000, 144, 6000, "ring128", "ring128"),
+    (1000, 144, 6000, "ring64", "ring128"),
     (600, 2336, 2000, "ring128", "ring64"),
     (200, 1601, 4000, "ring64x2", "ring128"),
-    (65, 6000, 1000, "skinny", "ring64x2"),
+    (65, 6000, 1000, "skinny", "skinny"),
     (3000, 800, 2900, "dma", "dma"),
     (2900, 1040, 3008, "dma", "dma"),
     (2817, 1088, 3089, "dma", "dma"),
@@ -218,6 +218,8 @@ FORMS = [
     (3000, 2064, 2900, "dma", "dma"),
     (70, 2048, 4096, "ring64x2", "ring64x2"),
     (200, 768, 12000, "ring64", "ring128"),
+    (150, 1600, 8200, "ring128", "ring128"),
+    (300, 2400, 1500, "ring64x2", "ring64x2"),
 ]
 
 
