@@ -30,6 +30,20 @@ typedef uint32_t u1any __attribute__((aligned(1)));
 typedef uint16_t u2any __attribute__((aligned(1)));
 typedef float f4any __attribute__((ext_vector_type(4), aligned(4)));
 
+// Sixteen bytes at any address.  `shift` (uniform): aligned dwords put together, which may
+// begin up to three bytes ahead of p; a load that the memory path splits takes longer.
+__device__ __forceinline__ uint4 load16(const uint8_t *p, bool shift = false) {
+  if (shift) {
+    const uint32_t sh = (uintptr_t)p & 3;
+    const u4any u = *(const u4any *)__builtin_assume_aligned(p - sh, 4);
+    const uint32_t w = *(const u1any *)(p + 12);
+    return make_uint4(__builtin_amdgcn_alignbyte(u.y, u.x, sh), __builtin_amdgcn_alignbyte(u.z, u.y, sh),
+                      __builtin_amdgcn_alignbyte(u.w, u.z, sh), w);
+  }
+  const u4any v = *(const u4any *)p;
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+
 __device__ __forceinline__ uint32_t max_dpp8(uint32_t v) {  // over lanes 8i .. 8i+7
   v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor1, 0xF, 0xF, false));
   v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, kDppXor2, 0xF, 0xF, false));
@@ -176,6 +190,7 @@ struct Mx4Args {
   float *out;
   int64_t ldo;
   int M, N, kb;  // kb: code bytes of a row
+  bool shift;    // rows of scales not on 4 bytes, but the arrays' first bytes are
 };
 
 __device__ __forceinline__ v4f mfma_mx4(uint4 a, uint32_t sa, uint4 b, uint32_t sb, v4f c) {
@@ -276,10 +291,6 @@ __global__ void __launch_bounds__(64 * skinny_waves(MT)) mx4_skinny_k(const Mx4A
         for (int j = 0; j < NT; j++)
           acc[t][i][j] = mfma_mx4(s.b[t][j], s.bs[t][j], s.a[i], s.as[i], acc[t][i][j]);
   };
-  auto load16 = [](const uint8_t *p) {
-    const u4any v = *(const u4any *)p;
-    return make_uint4(v.x, v.y, v.z, v.w);
-  };
   auto codes = [&](Step &x, int s) {
 #pragma unroll
     for (int t = 0; t < MATS; t++)
@@ -302,11 +313,11 @@ __global__ void __launch_bounds__(64 * skinny_waves(MT)) mx4_skinny_k(const Mx4A
 #pragma unroll
     for (int t = 0; t < MATS; t++)
 #pragma unroll
-      for (int j = 0; j < NT; j++) sb[t][j] = load16(bs[t][j] + 4 * s);
+      for (int j = 0; j < NT; j++) sb[t][j] = load16(bs[t][j] + 4 * s, a.shift);
 #pragma unroll
     for (int i = 0; i < MT; i++) {
       sa[i] = make_uint4(0, 0, 0, 0);
-      if (in[i]) sa[i] = load16(as[i] + 4 * s);
+      if (in[i]) sa[i] = load16(as[i] + 4 * s, a.shift);
     }
     Step x[U];
 #pragma unroll
@@ -438,12 +449,11 @@ __device__ __forceinline__ void dma16_at(const void *base, uint32_t off, uint32_
 // one register for the four and the matrix instruction picks the step's byte.  Blocks
 // behind the row's end get 2^-127: the codes that the last stage reads in their place
 // (its first block again) then add up to less than 2^-240, which no sum notices.
-__device__ __forceinline__ uint4 scale_group(const uint8_t *s, int g, int nb) {
+__device__ __forceinline__ uint4 scale_group(const uint8_t *s, int g, int nb, bool shift) {
   uint32_t w[4];  // w[j]: blocks 4j .. 4j+3 of the group
   if (16 * g + 16 <= nb) {
-    const u4any v = *(const u4any *)(s + 16 * g);
-#pragma unroll
-    for (int j = 0; j < 4; j++) w[j] = v[j];
+    const uint4 v = load16(s + 16 * g, shift);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
   } else if (nb >= 4) {  // the row's last four bytes, shifted down
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -482,7 +492,7 @@ __global__ void __launch_bounds__(256)
   const int row = !is_a && MATS == 2 ? (v >> 5) * 16 + (v & 15) : v;
   const uint8_t *s = is_a ? a.as + (int64_t)row * a.ldas : a.bs[mat] + (int64_t)row * a.ldbs[mat];
   (is_a ? pa : pb)[((int64_t)rg * groups + g) * 64 + r] =
-      scale_group(s, g, row < (is_a ? a.M : a.N) ? (a.kb + 15) >> 4 : 0);
+      scale_group(s, g, row < (is_a ? a.M : a.N) ? (a.kb + 15) >> 4 : 0, a.shift);
 }
 
 template <int P>
@@ -775,7 +785,7 @@ __global__ void __launch_bounds__(64 * WGM * WGN * KS)
     uint4 sv[U];
 #pragma unroll
     for (int u = 0; u < U; u++)
-      if (u * TPR + sg < groups) sv[u] = scale_group(sp, (d0 >> 1) + u * TPR + sg, snb);
+      if (u * TPR + sg < groups) sv[u] = scale_group(sp, (d0 >> 1) + u * TPR + sg, snb, a.shift);
 #pragma unroll
     for (int u = 0; u < U; u++)
       if (u * TPR + sg < groups) sc[srow * RG + u * TPR + sg] = sv[u];
@@ -1101,6 +1111,9 @@ int product(const char *fn, Mat<const uint8_t> &a, Mat<const uint8_t> &as,
   }
   g.out = (float *)oo.dev(), g.ldo = o.st[0];
   g.M = (int)o.s[0], g.N = (int)o.s[1], g.kb = (int)a.s[1];
+  uintptr_t base = (uintptr_t)g.as, rows = (uintptr_t)g.ldas;
+  for (int t = 0; t < MATS; t++) base |= (uintptr_t)g.bs[t], rows |= (uintptr_t)g.ldbs[t];
+  g.shift = (base & 3) == 0 && (rows & 3) != 0;
   if ((rc = launch_mx4<MATS>(g, cur_stream()))) return rc;
   Operand *ops[] = {&oa, &oas, &oo, &ob[0], &obs[0], &ob[MATS - 1], &obs[MATS - 1]};
   return finish(ops, 3 + 2 * MATS);
