@@ -970,9 +970,10 @@ Form pick(const Mx4Args &a, int64_t cus) {
   auto rounds = [&](int64_t t) { return (double)cdiv(t, cus); };
   double us[5];
   const double mem = (a.M + (double)MATS * a.N) * steps * 68 / 5.2e6;  // the operands' time from memory
-  // its blocks' operands from the caches: every row block reads B, every column block A
-  const double path = (double)cdiv(a.M, mt) * cdiv(a.N, 16) * (std::min(a.M, mt) + 16 * MATS) * steps * 68 / 8.5e6;
-  us[kSkinny] = 2.5 + std::max(path, mem);
+  // a block's operands from the caches, 33 KB a us to a CU: every row block reads B, every
+  // column block A
+  const double blocks = (double)cdiv(a.M, mt) * cdiv(a.N, 16) / cus;
+  us[kSkinny] = 2.5 + std::max(std::max(1., blocks) * (std::min(a.M, mt) + 16 * MATS) * steps * 68 / 33.2e3, mem);
   const int64_t t64 = tiles(64, 64), t256 = tiles(256, 256);
   us[kRing64] = 3.7 + std::max(mem, steps / 2 * std::max(0.33, 0.23 * rounds(t64))) + out;
   us[kRing64x2] = 4.0 + std::max(mem, steps / 2 * 0.2 * (t64 <= cus ? 1. : 1.3 * rounds(t64))) + out;

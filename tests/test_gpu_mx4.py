@@ -190,7 +190,7 @@ def _values64(codes, scales):
 
 # rows, code bytes of a row, columns, and the kernel that takes the product and the gate
 FORMS = [
-    (64, 1600, 2800, "skinny", "skinny"),
+    (64, 1600, 2800, "skinny", "ring64x2"),
     (33, 2320, 3000, "skinny", "skinny"),
     (129, 2304, 1500, "ring64x2", "ring64x2"),
     (300, 1024, 3000, "ring64x2", "ring128"),
@@ -208,7 +208,7 @@ FORMS = [
     (1000, 144, 6000, "ring64", "ring128"),
     (600, 2336, 2000, "ring128", "ring64"),
     (200, 1601, 4000, "ring64x2", "ring128"),
-    (65, 6000, 1000, "skinny", "skinny"),
+    (65, 6000, 1000, "ring64x2", "ring64x2"),
     (3000, 800, 2900, "dma", "dma"),
     (2900, 1040, 3008, "dma", "dma"),
     (2817, 1088, 3089, "dma", "dma"),
