@@ -61,12 +61,17 @@ def product(a, sa, b, sb):
         return va @ vb.T, n * (EPS * size + 2.0 ** -150)
 
 
+# The gate's roundings in EPS: exp(-|g|) is within 3 (a unit of the instruction, 2, and one of the
+# correction), its product with g rounds (1), the divisor 1 + exp takes at most half of those 3
+# and rounds (2.5), its reciprocal is within 1 after a step, and two products round: 9.5.
+GATE = 10
+
+
 def gated(g, tg, u, tu):
-    """silu(g) * u and its bound: silu's slope is below 1.1, exp is within 2 units (4 EPS) of
-    itself, and an addition, a division and a product round.  exp(-g) passes fp32's range below
-    g = -88.7, where the silu of 2^-121 or less becomes 0."""
+    """silu(g) * u and its bound: silu's slope is below 1.1, and the gate's own roundings.
+    exp(-|g|) becomes 0 below g = -87.3, where silu is less than 2^-119."""
     with np.errstate(all="ignore"):
         s = g / (1 + np.exp(-g))
         out = s * u
-        tol = (1.1 * tg * (np.abs(u) + tu) + np.abs(s) * tu) + 8 * EPS * np.abs(out) + 2.0 ** -121 * np.abs(u) + 2.0 ** -148
+        tol = (1.1 * tg * (np.abs(u) + tu) + np.abs(s) * tu) + GATE * EPS * np.abs(out) + 2.0 ** -119 * np.abs(u) + 2.0 ** -148
     return out, tol

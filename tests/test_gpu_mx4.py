@@ -262,7 +262,7 @@ def test_every_form(dev, gate, m, kb, n, plain, gated, pad, shift, opad):
         assert torch.equal(out.double(), want[0])  # the sums are exact in fp32
     else:
         w = want[0] / (1 + torch.exp(-want[0])) * want[1]
-        assert ((out.double() - w).abs() <= 8 * mx.EPS * w.abs() + 2.0 ** -121 * want[1].abs()).all()
+        assert ((out.double() - w).abs() <= mx.GATE * mx.EPS * w.abs() + 2.0 ** -119 * want[1].abs()).all()
 
 
 @pytest.mark.parametrize("lo, hi", [(100, 150), (40, 200), (0, 40)])
@@ -329,17 +329,45 @@ def test_feed_forward_block(dev, m, k, h):
     _check(out.cpu().numpy(), want, tol)
 
 
-def test_gate_is_swiglu_of_the_two_products(dev):
+@pytest.mark.parametrize("m, kb, n", [(1, 384, 300), (40, 384, 300), (200, 1024, 520), (2900, 1040, 1500)])
+def test_gate_of_the_two_products(dev, m, kb, n):
+    """The gate of what matmul_mx4 gives, and near the swiglu operator's (whose expf, sum,
+    quotient and product are within 2 units, 2, 2.5 and 1 EPS)."""
     import torch
-    rng = np.random.default_rng(3)
-    for m, kb, n in ((1, 384, 300), (40, 384, 300), (200, 1024, 520)):
-        t = [torch.from_numpy(v).to(dev) for r in (m, n, n) for v in mx.codes(rng, r, kb, 118, 124)]
-        g, u, both, want = (torch.empty((m, n), device=dev) for _ in range(4))
-        sa.matmul_mx4(*t[:4], g)
-        sa.matmul_mx4(*t[:2], *t[4:], u)
-        sa.swiglu_mx4(*t, both)
-        sa.swiglu(g.view(-1), u.view(-1), want.view(-1), m * n)
-        assert torch.equal(both, want)
+    a, *bs = _on_device(dev, m, m, kb, n, True, 116, 122)
+    g, u, both, other = (torch.empty((m, n), device=dev) for _ in range(4))
+    sa.matmul_mx4(*a, *bs[0], g)
+    sa.matmul_mx4(*a, *bs[1], u)
+    sa.swiglu_mx4(*a, *bs[0], *bs[1], both)
+    sa.swiglu(g.view(-1), u.view(-1), other.view(-1), m * n)
+    gd, ud = g.double(), u.double()
+    want = gd / (1 + torch.exp(-gd)) * ud
+    low = 2.0 ** -119 * ud.abs()
+    assert ((both.double() - want).abs() <= mx.GATE * mx.EPS * want.abs() + low).all()
+    assert ((both.double() - other.double()).abs() <= (mx.GATE + 10) * mx.EPS * want.abs() + low).all()
+
+
+def test_gate_at_its_ends(dev):
+    """Sums that are large, subnormal and infinite through the gate."""
+    import torch
+    # row i of A is 2^e_i in one element; W1's columns have +-1, W3's 1
+    es = [-140, -126, -20, -1, 0, 3, 4, 5, 6, 6.5, 7, 20, 100, 120]
+    m = len(es)
+    a, s = np.zeros((m, 16), U), np.full((m, 1), 127, U)
+    a[:, 0] = 2                                       # 1.0
+    s[:, 0] = [max(int(e), -127) + 127 for e in es]
+    w1, w3 = np.zeros((2, 16), U), np.zeros((2, 16), U)
+    w1[:, 0], w3[:, 0] = [2, 10], 2
+    t = np.full((2, 1), 127, U)
+    got = _call(dev, True, a, s, [(w1, t), (w3, t)])
+    want, tol = _want(True, a, s, [(w1, t), (w3, t)])
+    ok = np.abs(want) < 3e38
+    _check(got[ok], want[ok], tol[ok])
+    assert (got[-1] == [np.inf, 0]).all() and (got[-2] == [np.inf, 0]).all()
+    big = np.full((1, 1), 254, U)
+    a[0, 0] = 7                                       # 6 * 2^127: infinite in fp32
+    got = _call(dev, True, a[:1], big, [(w1[:1], t[:1]), (w3[:1], np.full((1, 1), 1, U))])
+    assert np.isinf(got[0, 0]) and got[0, 0] > 0
 
 
 def test_host_arrays(dev):
