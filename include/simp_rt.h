@@ -260,7 +260,10 @@ int32_t simp_rt_matmul_w4s(
  * and ceil(K/32) scale bytes, one for each block of 32 elements (the last may be
  * shorter): s stands for 2^(s - 127), 255 for NaN, and an element for its code's
  * value times that.  All rows may be strided, at any alignment.  Outputs share no
- * element with another operand (rows of one array may lie between another's). */
+ * element with another operand (rows of one array may lie between another's).  Products of
+ * many rows use device scratch where they have it: a captured call to which no call of its
+ * size on the stream has left some goes on without, slower, and may add the same products
+ * up in another order.  Equal calls give equal bits, as do replays of one graph. */
 
 /* Codes and scales of fp32 rows x[rows, cols].  With m = max|x| of a block, its scale
  * is 2^e, e = max(floor(log2 m) - 2, -127) (byte 0 for a block of zeros), and a code is

@@ -419,20 +419,27 @@ __global__ void __launch_bounds__(64 * skinny_waves(MT)) mx4_skinny_k(const Mx4A
 template <int MT, int NT, int MATS>
 int launch_skinny(Mx4Args a, hipStream_t st) {
   const int64_t bn = cdiv(a.N, 16 * NT), bm = cdiv(a.M, 16 * MT);
-  // about 3072 waves on the chip, up to 16 to a block (64 KiB of sums)
+  // about twelve waves to a CU, up to 16 to a block (64 KiB of sums)
   const int steps = a.kb >> 6;
-  int waves = (int)std::min<int64_t>({cdiv(3072, bn * bm), skinny_waves(MT), std::max(steps, 1), 64 / (MATS * MT * NT)});
+  int waves = (int)std::min<int64_t>({cdiv(12 * num_cus(), bn * bm), skinny_waves(MT), std::max(steps, 1), 64 / (MATS * MT * NT)});
   const int span = (int)cdiv(cdiv(steps, waves), 4) * 4;
   if (span) waves = (int)cdiv(steps, span);
-  const int64_t most = std::max<int64_t>(INT32_MAX / (64 * waves) / bn, 1);  // row blocks of a launch
+  // a launch has below 2^31 threads: in turn, runs of column blocks, and of row blocks where
+  // one run has all columns
+  const int64_t most = INT32_MAX / (64 * waves), cb = std::min(bn, most), rb = std::max<int64_t>(most / bn, 1);
   KernelTimer kt(st, "mx4_skinny");
-  for (int64_t b = 0; b < bm; b += most) {
-    Mx4Args c = a;
-    const int64_t row = b * 16 * MT, rows = std::min<int64_t>(most * 16 * MT, a.M - row);
-    c.a += row * a.lda, c.as += row * a.ldas, c.out += row * a.ldo, c.M = (int)rows;
-    hipLaunchKernelGGL((mx4_skinny_k<MT, NT, MATS>), dim3((unsigned)(bn * cdiv(rows, 16 * MT))),
-                       dim3(64 * waves), waves > 1 ? waves * MATS * MT * NT * 1024 : 0, st, c, span, (int)bn);
-    SIMP_HIP(hipGetLastError());
+  for (int64_t i = 0; i < bm; i += rb) {
+    for (int64_t j = 0; j < bn; j += cb) {
+      Mx4Args c = a;
+      const int64_t row = 16 * MT * i, col = 16 * NT * j;
+      const int64_t rows = std::min(16 * MT * rb, a.M - row), cols = std::min(16 * NT * cb, a.N - col);
+      c.a += row * a.lda, c.as += row * a.ldas, c.out += row * a.ldo + col, c.M = (int)rows, c.N = (int)cols;
+      for (int t = 0; t < MATS; t++) c.b[t] += col * a.ldb[t], c.bs[t] += col * a.ldbs[t];
+      const int64_t blocks_n = cdiv(cols, 16 * NT);
+      hipLaunchKernelGGL((mx4_skinny_k<MT, NT, MATS>), dim3((unsigned)(blocks_n * cdiv(rows, 16 * MT))),
+                         dim3(64 * waves), waves > 1 ? waves * MATS * MT * NT * 1024 : 0, st, c, span, (int)blocks_n);
+      SIMP_HIP(hipGetLastError());
+    }
   }
   return SIMP_RT_OK;
 }
@@ -1020,7 +1027,9 @@ int launch_mx4(const Mx4Args &a, hipStream_t st) {
       Workspace ws;
       void *p;
       const int64_t ga = cdiv(ca, 256), gb = cdiv(cb, 256);
-      if ((ga + MATS * gb) * 256 <= INT32_MAX && ws.try_get(st, 16 * (size_t)(ca + MATS * cb), &p, 11)) {
+      // (no more than 4 GiB, which stay the library's)
+      if ((ga + MATS * gb) * 256 <= INT32_MAX && ca + MATS * cb <= (1 << 28) &&
+          ws.try_get(st, 16 * (size_t)(ca + MATS * cb), &p, 11)) {
         uint4 *q = (uint4 *)p;
         hipLaunchKernelGGL(mx4_pad_k<MATS>, dim3((unsigned)(ga + MATS * gb)), dim3(256), 0, st, a, q, per,
                            (int)ga, (int)gb);

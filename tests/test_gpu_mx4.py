@@ -292,6 +292,34 @@ def test_millions_of_rows(dev):
     assert torch.equal(out[:5000].double(), _values64(*[x[:5000] for x in a]) @ _values64(*b).t().contiguous())
 
 
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("m, n", [(1, 540_000_000), (1_080_000_000, 17)])
+def test_more_blocks_than_a_launch_has(dev, gate, m, n):
+    """Below K = 2 every sum is exact; the ends, the middle, and where a launch ends."""
+    import torch
+    if torch.cuda.mem_get_info()[0] < (100 << 30):
+        pytest.skip("needs 100 GB")
+    g = torch.Generator(device=dev).manual_seed(m)
+    ops = [[torch.randint(0, 256, (r, 1), dtype=torch.uint8, device=dev, generator=g),
+            torch.randint(122, 128, (r, 1), dtype=torch.uint8, device=dev, generator=g)]
+           for r in ((m, n, n) if gate else (m, n))]
+    f = sa.swiglu_mx4 if gate else sa.matmul_mx4
+    out = f(*sum(ops, []), torch.full((m, n), float("nan"), device=dev))
+    many = max(m, n)
+    blocks = (2**31 - 1) // 64  # of a launch, of one wave
+    for at in (0, many // 2, (16 * blocks if m == 1 else 64 * (blocks // 2)) - 500, many - 1000):
+        cut = slice(at, at + 1000)
+        rows, cols = (cut, slice(None)) if m > 1 else (slice(None), cut)
+        h = [_values64(*[x[r] for x in o]) for o, r in zip(ops, (rows, cols, cols))]
+        want = h[0] @ h[1].t().contiguous()
+        got = out[rows, cols].double()
+        if gate:
+            want = want / (1 + torch.exp(-want)) * (h[0] @ h[2].t().contiguous())
+            assert ((got - want).abs() <= mx.GATE * 2.0**-24 * want.abs()).all()
+        else:
+            assert torch.equal(got, want)
+
+
 def test_product_of_nothing_is_zero(dev):
     import torch
     for m, n in ((1, 1), (20, 300)):
@@ -451,6 +479,35 @@ def test_captured_and_replayed(dev, gate, m, kb, n):
                     g.replay()
                 st.synchronize()
                 assert torch.equal(out, want[0]) and torch.equal(out2, want[1])
+        finally:
+            sa.set_stream(torch.cuda.default_stream())
+
+
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("m, kb, n", [(9000, 1001, 9000), (9000, 2064, 9000)])
+def test_captured_without_a_call_before(dev, gate, m, kb, n):
+    """More scratch than any other test leaves: the captured call goes on without it."""
+    import torch
+    rng = np.random.default_rng(kb)
+    f = sa.swiglu_mx4 if gate else sa.matmul_mx4
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        sa.set_stream(st)
+        try:
+            t = [torch.from_numpy(v).to(dev) for r in ((m, n, n) if gate else (m, n))
+                 for v in mx.codes(rng, r, kb, 120, 122)]
+            out, want = (torch.zeros((m, n), device=dev) for _ in range(2))
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                f(*t, out)
+            f(*t, want)
+            for _ in range(3):
+                out.fill_(9)
+                g.replay()
+                st.synchronize()
+                # sums are multiples of 2^-16 (products of 2^-2 at least, times 2^-14) and
+                # below 2^6 (36 * 2^-12 for each of 4128): exact in either order
+                assert torch.equal(out, want)
         finally:
             sa.set_stream(torch.cuda.default_stream())
 
