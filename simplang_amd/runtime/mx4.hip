@@ -520,65 +520,64 @@ __device__ __forceinline__ v4f mfma_step(const uint4 &b, uint32_t sb, const uint
 }
 
 // Persistent 256 x 256 tiles (MATS == 2: of 128 columns of W1 and W3 each), 8 waves of 128 x
-// 64, K-steps of 64 code bytes through a ring of four stages that
-// global_load_lds_dwordx4 fills three steps ahead.
+// 64 in K-steps of 64 code bytes.  global_load_lds_dwordx4 fills a ring of two slots of two
+// steps each, so that every request is a whole line of 128 bytes: half lines, in four slots
+// of one step, cost 8192^3 184 us for the loads alone, not 129 (whole: 267, not 260).
 template <int MATS>
 __global__ void __launch_bounds__(512)
     mx4_dma_k(const Mx4Args a, const uint4 *__restrict__ pa, const uint4 *__restrict__ pb,
               int tiles_m, int tiles_n, int groups, int stream, int stagger) {
-  constexpr int BM = 256, BN = 256, BK = 64, STAGES = 4, WGN = 4;
+  constexpr int BM = 256, BN = 256, BK = 128, SLOTS = 2, WGN = 4;  // BK: bytes of a slot's rows
   constexpr int WM = 128, WN = 64, FM = WM / 16, FN = WN / 16;
-  constexpr int STAGE = (BM + BN) * BK, SCALES = (BM + BN) * 16;  // bytes
-  constexpr int DA = 2, DB = 2, DPW = DA + DB;  // DMA instructions of a wave
+  constexpr int SLOT = (BM + BN) * BK, SCALES = (BM + BN) * 16;  // bytes
+  constexpr int DA = 4, DB = 4, DPW = DA + DB;  // DMA instructions of a wave
   // a group's scales are issued when the group before has been read: one buffer
-  __shared__ uint4 lds[(STAGES * STAGE + SCALES) / 16];
+  __shared__ uint4 lds[(SLOTS * SLOT + SCALES) / 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm0 = (wave / WGN) * WM, wn0 = (wave % WGN) * WN;
-  const int nk = (a.kb + BK - 1) / BK;
+  const int nk = (a.kb + 63) / 64, ns = (a.kb + BK - 1) / BK;
   const int ntiles = tiles_m * tiles_n;
   const int lrow = lane & 15, lkc = lane >> 4;
-  const int drow = lane >> 2, dkc = (lane & 3) ^ ((drow >> 1) & 3);  // DMA lane -> row, chunk
-  const int rslot = lrow * 4 + (lkc ^ ((lrow >> 1) & 3));          // operand lane -> slot
+  // chunk c of row r lies at c ^ ((r >> 1) & 7)
+  const int drow = lane >> 3, dkc[2] = {16 * ((lane & 7) ^ (lane >> 4)), 16 * ((lane & 7) ^ (4 + (lane >> 4)))};
+  const int rslot[2] = {lrow * 8 + (lkc ^ (lrow >> 1)), lrow * 8 + ((4 + lkc) ^ (lrow >> 1))};
   const uint32_t lds0 = lds_offset(lds);
   // Workgroups of equal tiles store at the same time, and all wait for the memory then; with
   // eight starts, `stagger` of about 1 us apart, the others of an XCD compute meanwhile.
   for (int z = stagger * ((blockIdx.x >> 3) & 7); z > 0; z--) __builtin_amdgcn_s_sleep(32);
-  const uint32_t *sl = (const uint32_t *)(lds + STAGES * STAGE / 16) + lrow * 4 + lkc;
+  const uint32_t *sl = (const uint32_t *)(lds + SLOTS * SLOT / 16) + lrow * 4 + lkc;
 
   for (int vb = blockIdx.x; vb < ntiles; vb += gridDim.x) {
     int tm, tn;
     tile_of_block(vb, ntiles, tiles_m, tiles_n, tm, tn);
     const int m0 = tm * BM, n0 = tn * (BN / MATS);
-    // blocks of 16 rows of A and of B (16 rows of W1, 16 of W3 in turn): a lane's row of each,
-    // from the tile's first
+    // a lane's rows of the wave's blocks of 8, from the tile's first (B: 16 rows of W1, 16 of W3
+    // in turn)
     const uint8_t *baseA = a.a + (int64_t)m0 * a.lda, *baseB[MATS];
 #pragma unroll
     for (int t = 0; t < MATS; t++) baseB[t] = a.b[t] + (int64_t)n0 * a.ldb[t];
     uint32_t offA[DA], offB[DB];
 #pragma unroll
     for (int i = 0; i < DA; i++)
-      offA[i] = (uint32_t)min(16 * (DA * wave + i) + drow, a.M - 1 - m0) * (uint32_t)a.lda + 16 * dkc;
+      offA[i] = (uint32_t)min(8 * (DA * wave + i) + drow, a.M - 1 - m0) * (uint32_t)a.lda + dkc[i & 1];
 #pragma unroll
     for (int i = 0; i < DB; i++) {
-      const int blk = DB * wave + i;
-      offB[i] = (uint32_t)min(16 * (blk / MATS) + drow, a.N - 1 - n0) * (uint32_t)a.ldb[blk % MATS] + 16 * dkc;
+      const int r = MATS == 2 ? 16 * wave + 8 * (i & 1) + drow : 8 * (DB * wave + i) + drow;
+      offB[i] = (uint32_t)min(r, a.N - 1 - n0) * (uint32_t)a.ldb[i / 2 % MATS] + dkc[i & 1];
     }
     // 64 rows of scales to a wave: A's, then B's
     const uint4 *baseS = wave < 4 ? pa + (int64_t)(4 * tm + wave) * groups * 64
                                   : pb + (int64_t)(4 * tn + wave - 4) * groups * 64;
-    // The scales of a group go ahead of its first stage.  `last`: kt may be the last
-    // stage, which can be shorter.
-    auto issue = [&](int kt, auto last) {
-      const uint32_t st = lds0 + (kt % STAGES) * STAGE;
-      const int64_t k0 = (int64_t)kt * BK;
-      if ((kt & 3) == 0) dma16_at(baseS + (kt >> 2) * 64, 16 * lane, lds0 + STAGES * STAGE + 1024 * wave);
+    // Part i of a slot; the scales of a group of four steps go ahead of its first slot.  `last`: s
+    // may be the last, which can be shorter.
+    auto issue = [&](int s, auto last, int i) {
+      const uint32_t st = lds0 + (s & 1) * SLOT;
+      const int64_t k0 = (int64_t)s * BK;
       uint32_t back = 0;
-      if constexpr (decltype(last)::value) back = k0 + 16 * dkc < a.kb ? 0 : 16 * dkc;
-#pragma unroll
-      for (int i = 0; i < DA; i++) dma16_at(baseA + k0, offA[i] - back, st + 1024 * (DA * wave + i));
-#pragma unroll
-      for (int i = 0; i < DB; i++)
-        dma16_at(baseB[(DB * wave + i) % MATS] + k0, offB[i] - back, st + BM * BK + 1024 * (DB * wave + i));
+      if constexpr (decltype(last)::value) back = k0 + dkc[i & 1] < a.kb ? 0 : dkc[i & 1];
+      if (i == 0 && (s & 1) == 0) dma16_at(baseS + (s >> 1) * 64, 16 * lane, lds0 + SLOTS * SLOT + 1024 * wave);
+      dma16_at(baseA + k0, offA[i] - back, st + 1024 * (DA * wave + i));
+      dma16_at(baseB[i / 2 % MATS] + k0, offB[i] - back, st + BM * BK + 1024 * (DB * wave + i));
     };
     v4f acc[FM][FN];
 #pragma unroll
@@ -587,33 +586,43 @@ __global__ void __launch_bounds__(512)
       for (int j = 0; j < FN; j++) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
     uint4 fa[FM], fb[2][FN];
     uint32_t ra[FM], rb[FN], rbn[FN];  // scales of four steps
-    auto frag = [&](int slot, int blk) { return lds[slot * (STAGE / 16) + blk * 64 + rslot]; };
-    constexpr int BOFF = BM * BK / 1024;  // first B block of a stage
+    // step `at` of the ring's four, 16 rows from 16 blk on (A, then B)
+    auto frag = [&](int at, int blk) { return lds[(at >> 1) * (SLOT / 16) + blk * 128 + rslot[at & 1]]; };
+    constexpr int BOFF = BM / 16;  // first B block of a slot
     auto scale = [&](int row) { return sl[4 * row]; };
     using T = std::true_type;
     using F = std::false_type;
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // the previous tile's stores
-    for (int p = 0; p < min(STAGES, nk); p++) issue(p, T{});
-    if (nk >= STAGES) __builtin_amdgcn_s_waitcnt(waitcnt_vm(DPW * (STAGES - 1)));
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // the previous tile's stores, and its last reads
+    __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0);
+    block_barrier();
+    for (int p = 0; p < min(SLOTS, ns); p++)
+#pragma unroll
+      for (int i = 0; i < DA; i++) issue(p, T{}, i);
+    if (ns >= SLOTS) __builtin_amdgcn_s_waitcnt(waitcnt_vm(DPW));
     else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     block_barrier();
 #pragma unroll
     for (int j = 0; j < FN; j++) fb[0][j] = frag(0, BOFF + wn0 / 16 + j), rb[j] = scale(BM + wn0 + 16 * j);
 #pragma unroll
     for (int i = 0; i < FM; i++) fa[i] = frag(0, wm0 / 16 + i), ra[i] = scale(wm0 + 16 * i);
-    // Step kt: certify stage kt + 1, read its fragments while the MFMAs of stage kt run, and
-    // refill the buffer of stage kt.  Steady: stage kt + STAGES is there and not the last.
-    // (Behind the last stage the reads bring stale LDS that is not used.)
+    // Step kt: the fragments of step kt + 1 are read while the products of step kt run.  In an
+    // odd step every wave has read this slot: the next is waited for, and this one filled
+    // again, ahead of the products (spread over them 268 us).  Steady: slot kt / 2 + 2 is
+    // there and not the last.  (Behind the last step the reads bring stale LDS that is not used.)
     auto step = [&](int kt, auto phase, auto steady) {
       constexpr int P = decltype(phase)::value, cb = P & 1;
       constexpr bool S = decltype(steady)::value;
-      // stages kt + 2 and kt + 3 may be on their way, and the scales ahead of one
-      constexpr int vm = DPW * (STAGES - 2) + (P == 1 || P == 2);
-      if (S || kt + STAGES - 1 < nk) __builtin_amdgcn_s_waitcnt(waitcnt_vm(vm));
-      else __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-      __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0);
-      block_barrier();
-      constexpr int next = (P + 1) % STAGES;  // slot of stage kt + 1
+      if constexpr (P & 1) {
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+        __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0);
+        block_barrier();
+#pragma unroll
+        for (int i = 0; i < DA; i++) {
+          if constexpr (S) issue((kt >> 1) + 2, F{}, i);
+          else if ((kt >> 1) + 2 < ns) issue((kt >> 1) + 2, T{}, i);
+        }
+      }
+      constexpr int next = (P + 1) & 3;
 #pragma unroll
       for (int j = 0; j < FN; j++) {
         fb[cb ^ 1][j] = frag(next, BOFF + wn0 / 16 + j);
@@ -625,10 +634,6 @@ __global__ void __launch_bounds__(512)
         for (int j = 0; j < FN; j++) acc[i][j] = mfma_step<P>(fb[cb][j], rb[j], fa[i], ra[i], acc[i][j]);
         fa[i] = frag(next, wm0 / 16 + i);
         if constexpr (P == 3) ra[i] = scale(wm0 + 16 * i);
-        if (i == 3) {
-          if constexpr (S) issue(kt + STAGES, F{});
-          else if (kt + STAGES < nk) issue(kt + STAGES, T{});
-        }
       }
       if constexpr (P == 3) {
 #pragma unroll
@@ -640,7 +645,7 @@ __global__ void __launch_bounds__(512)
     using I2 = std::integral_constant<int, 2>;
     using I3 = std::integral_constant<int, 3>;
     int kt = 0;
-    for (; kt + 8 < nk; kt += 4) {
+    for (; (kt >> 1) + 4 < ns; kt += 4) {
       step(kt, I0{}, T{});
       step(kt + 1, I1{}, T{});
       step(kt + 2, I2{}, T{});
