@@ -199,16 +199,16 @@ __device__ __forceinline__ v4f mfma_mx4(uint4 a, uint32_t sa, uint4 b, uint32_t 
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 0, (int)sa, 0, (int)sb);
 }
 
-// silu(g) * u within 9.5 half units: with e = exp(-|g|) in (0, 1], silu(g) is g / (1 + e), and
-// g e / (1 + e) below 0, so nothing overflows and the divisor lies in (1, 2], where one step
-// on the reciprocal is enough.  (-|g| log2(e) is carried in two parts: a rounding of it would
-// count |g| times.)  Half the instructions of expf and a division: 4096 x 2048 x 8192 103 -> 96 us.
+// silu(g) * u = g / (1 + exp(-g)) * u within 8 half units: with t = fl(x log2(e)), exp(x) is
+// 2^t (1 + x - t ln 2), which leaves the rounding of t (it would count |x| times) out.  Above
+// x = 88.7228394, the first for which t reaches 128, exp is infinite and silu 0.  A gate costs
+// what its instructions do, 64 to a lane and tile with the matrix cores idle: with expf and a
+// division 4096 x 2048 x 8192 takes 100 us in the 256 x 256 tiles, not 87.
 __device__ __forceinline__ float swiglu(float g, float u) {
-  const float x = fmaxf(-fabsf(g), -200.f), t = x * 1.44269504f;
-  const float low = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269504f, -t));  // log2(e) = 1.44269504 + 1.9e-8
-  const float p = __builtin_amdgcn_exp2f(t), e = fmaf(p, low * 0.693147182f, p);
-  const float d = 1.f + e, c = __builtin_amdgcn_rcpf(d);
-  return (g < 0.f ? g * e : g) * fmaf(fmaf(-d, c, 1.f), c, c) * u;
+  const float x = __builtin_amdgcn_fmed3f(-g, -200.f, 88.7228394f), t = x * 1.44269504f;
+  const float low = fmaf(-t, -1.90465421e-9f, fmaf(-t, 0.693147182f, x));  // ln 2 in two parts
+  const float p = __builtin_amdgcn_exp2f(t), e = fmaf(p, low, p);
+  return g * __builtin_amdgcn_rcpf(1.f + e) * u;
 }
 
 // Exchanges registers and lanes: of n = 2 or 4 neighbouring lanes, lane t gets in y[s] what

@@ -61,15 +61,15 @@ def product(a, sa, b, sb):
         return va @ vb.T, n * (EPS * size + 2.0 ** -150)
 
 
-# The gate's roundings in EPS: exp(-|g|) is within 3 (a unit of the instruction, 2, and one of the
-# correction), its product with g rounds (1), the divisor 1 + exp takes at most half of those 3
-# and rounds (2.5), its reciprocal is within 1 after a step, and two products round: 9.5.
-GATE = 10
+# The gate's roundings in EPS: exp(-g) is within 3 (a unit of the instruction, 2, and one of the
+# correction), the divisor 1 + exp takes at most those 3 and rounds (4), its reciprocal is
+# within a unit (2), and two products round: 8, and what their products add.
+GATE = 9
 
 
 def gated(g, tg, u, tu):
     """silu(g) * u and its bound: silu's slope is below 1.1, and the gate's own roundings.
-    exp(-|g|) becomes 0 below g = -87.3, where silu is less than 2^-119."""
+    1 / (1 + exp(-g)) becomes 0 below g = -87.3, where silu is less than 2^-119."""
     with np.errstate(all="ignore"):
         s = g / (1 + np.exp(-g))
         out = s * u

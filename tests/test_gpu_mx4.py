@@ -398,6 +398,26 @@ def test_gate_at_its_ends(dev):
     assert np.isinf(got[0, 0]) and got[0, 0] > 0
 
 
+def test_gate_where_exp_overflows(dev):
+    """g = -96 to -80 in steps of 1/64, from binary digits in blocks of their own (exact)."""
+    n = np.arange(80 * 64, 96 * 64 + 1)
+    digits = n[:, None] >> np.arange(12, -1, -1) & 1
+    a, s = np.zeros((len(n), 13 * 16), U), np.tile(127 + 6 - np.arange(13), (len(n), 1)).astype(U)
+    a[:, ::16] = 2 * digits                           # 1.0
+    w1, w3, t = np.zeros((1, 13 * 16), U), np.zeros((1, 13 * 16), U), np.full((1, 13), 127, U)
+    w1[:, ::16], w3[:, 0] = 10, 2                     # -1.0; 64 (every n has that digit)
+    for m in (len(n), 5):
+        for at in range(0, len(n), m):
+            cut = slice(at, at + m)
+            got = _call(dev, True, a[cut], s[cut], [(w1, t), (w3, t)])[:, 0]
+            g = -n[cut] / 64
+            want = g / (1 + np.exp(-g)) * 64
+            assert (np.abs(got - want) <= mx.GATE * mx.EPS * np.abs(want) + 2.0 ** -119 * 64).all()
+            assert (got[g < -88.73] == 0).all()
+            if at > 200:
+                break
+
+
 def test_host_arrays(dev):
     rng = np.random.default_rng(5)
     x, w = rng.standard_normal((5, 100)).astype(F), rng.standard_normal((17, 100)).astype(F)
