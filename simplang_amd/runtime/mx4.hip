@@ -191,6 +191,7 @@ struct Mx4Args {
   int64_t ldo;
   int M, N, kb;  // kb: code bytes of a row
   bool shift;    // rows of scales not on 4 bytes, but the arrays' first bytes are
+  bool shift_codes;  // the same for rows of codes, and no array's first byte is in the way
 };
 
 __device__ __forceinline__ v4f mfma_mx4(uint4 a, uint32_t sa, uint4 b, uint32_t sb, v4f c) {
@@ -234,31 +235,32 @@ __device__ __forceinline__ void lane_transpose(v4f (&x)[N]) {
   }
 }
 
-// 16 code bytes of a row from byte k on, zeros behind its end: with fewer left, the row's
-// last 16 shifted down.
-__device__ __forceinline__ uint4 row16(const uint8_t *row, int k, int kb) {
-  if (kb >= 16) {
-    const int at = min(k, kb - 16), sh = min(k - at, 16);
-    const u4any v = *(const u4any *)(row + at);
-    uint64_t lo = v.x | (uint64_t)v.y << 32, hi = v.z | (uint64_t)v.w << 32;
-    if (sh >= 8) lo = sh < 16 ? hi >> (8 * (sh - 8)) : 0, hi = 0;
-    else if (sh > 0) lo = lo >> (8 * sh) | hi << (64 - 8 * sh), hi >>= 8 * sh;
-    return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
-  }
+// 16 bytes of a row of kb from byte k on, zeros behind its end: with fewer left, the row's last
+// 16 shifted down.  In two parts, so that many loads can be on their way: what to load, ...
+__device__ __forceinline__ uint4 row_load(const uint8_t *row, int k, int kb) {
+  if (kb >= 16) return load16(row + min(k, kb - 16));
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < 15; i++)
     if (k + i < kb) w[i >> 2] |= (uint32_t)row[k + i] << (8 * (i & 3));
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+// ... and what to make of it.
+__device__ __forceinline__ uint4 row_shift(uint4 v, int k, int kb) {
+  const int sh = kb >= 16 ? min(max(k - kb + 16, 0), 16) : 0;
+  uint64_t lo = v.x | (uint64_t)v.y << 32, hi = v.z | (uint64_t)v.w << 32;
+  if (sh >= 8) lo = sh < 16 ? hi >> (8 * (sh - 8)) : 0, hi = 0;
+  else if (sh > 0) lo = lo >> (8 * sh) | hi << (64 - 8 * sh), hi >>= 8 * sh;
+  return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+}
 
 // 16 NT columns of each matrix and all 16 MT rows to a block, whose waves split K: a wave
 // takes every byte of its rows' piece once, straight from memory into the lanes that
 // feed the matrix instruction (16 rows of 64 bytes, and a byte of scales to a lane), and
 // the waves' sums meet in LDS, in the order of K.
-constexpr int skinny_waves(int MT) { return MT >= 4 ? 8 : 16; }  // of a block at most
-template <int MT, int NT, int MATS>
-__global__ void __launch_bounds__(64 * skinny_waves(MT)) mx4_skinny_k(const Mx4Args a, int span, int blocks_n) {
+constexpr int skinny_waves(int MT, int MATS) { return MT * MATS >= 4 ? 8 : 16; }  // of a block at most
+template <int MT, int NT, int MATS, int SHIFT>
+__global__ void __launch_bounds__(64 * skinny_waves(MT, MATS)) mx4_skinny_k(const Mx4Args a, int span, int blocks_n) {
   constexpr int T = MATS * MT * NT;
   constexpr int U = MT == 4 ? 2 : 4;
   extern __shared__ v4f part[];  // [waves][T][64]
@@ -272,14 +274,14 @@ __global__ void __launch_bounds__(64 * skinny_waves(MT)) mx4_skinny_k(const Mx4A
   for (int i = 0; i < MT; i++) {
     in[i] = m0 + 16 * i + r < a.M;
     const int64_t m = min(m0 + 16 * i + r, a.M - 1);
-    ap[i] = a.a + m * a.lda + 16 * q, as[i] = a.as + m * a.ldas;
+    ap[i] = a.a + m * a.lda, as[i] = a.as + m * a.ldas;
   }
 #pragma unroll
   for (int t = 0; t < MATS; t++)
 #pragma unroll
     for (int j = 0; j < NT; j++) {
       const int64_t n = min(n0 + 16 * j + r, a.N - 1);
-      bp[t][j] = a.b[t] + n * a.ldb[t] + 16 * q, bs[t][j] = a.bs[t] + n * a.ldbs[t];
+      bp[t][j] = a.b[t] + n * a.ldb[t], bs[t][j] = a.bs[t] + n * a.ldbs[t];
     }
   v4f acc[MATS][MT][NT];
 #pragma unroll
@@ -301,43 +303,57 @@ __global__ void __launch_bounds__(64 * skinny_waves(MT)) mx4_skinny_k(const Mx4A
         for (int j = 0; j < NT; j++)
           acc[t][i][j] = mfma_mx4(s.b[t][j], s.bs[t][j], s.a[i], s.as[i], acc[t][i][j]);
   };
-  auto codes = [&](Step &x, int s) {
+  // Four steps: a lane's four scale bytes come out of 16 of its row.  What bounds the loop is
+  // the path from the caches, 64 bytes a cycle and a row to a cycle: a byte of scales for
+  // each fragment and step would cost as much as the codes.  `edge`: rows may end in them.
+  const int nb = (a.kb + 15) >> 4;
+  auto four = [&](int s, int end, auto edge) {
+    constexpr int E = decltype(edge)::value;  // 2: rows shorter than 16 bytes
+    auto load = [&](const uint8_t *row, int k, int size) {
+      if constexpr (E == 2) return row_load(row, k, size);
+      else return load16(row + (E ? min(k, size - 16) : k), SHIFT == 2);
+    };
+    auto scales = [&](const uint8_t *row) {  // (rows of scales have 16 bytes less often)
+      if constexpr (E == 0) return load16(row + 4 * s, SHIFT >= 1);
+      uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int t = 0; t < MATS; t++)
-#pragma unroll
-      for (int j = 0; j < NT; j++) x.b[t][j] = load16(bp[t][j] + 64 * s);
-#pragma unroll
-    for (int i = 0; i < MT; i++) {
-      x.a[i] = make_uint4(0, 0, 0, 0);
-      if (in[i]) x.a[i] = load16(ap[i] + 64 * s);
-    }
-  };
-  const int whole = a.kb >> 6;
-  int s = wave * span;
-  const int end = min(s + span, whole);
-  // Four steps at a time: a lane's four scale bytes come out of 16 of its row.  What bounds
-  // the loop is the path from the caches, 64 bytes a cycle and a row to a cycle: a byte
-  // of scales for each fragment and step would cost as much as the codes.
-  for (; s + 4 <= end; s += 4) {
+      for (int u = 0; u < 4; u++)
+        if (SHIFT == 2 || s + u < end) w[u] = row[min(4 * (s + u) + q, nb - 1)];
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    };
     uint4 sa[MT], sb[MATS][NT];
 #pragma unroll
     for (int t = 0; t < MATS; t++)
 #pragma unroll
-      for (int j = 0; j < NT; j++) sb[t][j] = load16(bs[t][j] + 4 * s, a.shift);
+      for (int j = 0; j < NT; j++) sb[t][j] = scales(bs[t][j]);
 #pragma unroll
     for (int i = 0; i < MT; i++) {
       sa[i] = make_uint4(0, 0, 0, 0);
-      if (in[i]) sa[i] = load16(as[i] + 4 * s, a.shift);
+      if (in[i]) sa[i] = scales(as[i]);
     }
     Step x[U];
 #pragma unroll
     for (int h = 0; h < 4; h += U) {
 #pragma unroll
-      for (int u = 0; u < U; u++) codes(x[u], s + h + u);
+      for (int u = 0; u < U; u++) {
+        const int k = 64 * (s + h + u) + 16 * q;
+        // (a load that is put together here would be waited for here)
+        if (E && SHIFT != 2 && s + h + u >= end) break;
+#pragma unroll
+        for (int t = 0; t < MATS; t++)
+#pragma unroll
+          for (int j = 0; j < NT; j++) x[u].b[t][j] = load(bp[t][j], k, a.kb);
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+          x[u].a[i] = make_uint4(0, 0, 0, 0);
+          if (in[i]) x[u].a[i] = load(ap[i], k, a.kb);
+        }
+      }
 #pragma unroll
       for (int u = 0; u < U; u++) {
+        if (E && s + h + u >= end) break;
         auto byte = [&](const uint4 &v) {
-          return (h + u == 0 ? v.x : h + u == 1 ? v.y : h + u == 2 ? v.z : v.w) >> (8 * q);
+          return (h + u == 0 ? v.x : h + u == 1 ? v.y : h + u == 2 ? v.z : v.w) >> (E ? 0 : 8 * q);
         };
 #pragma unroll
         for (int t = 0; t < MATS; t++)
@@ -345,32 +361,32 @@ __global__ void __launch_bounds__(64 * skinny_waves(MT)) mx4_skinny_k(const Mx4A
           for (int j = 0; j < NT; j++) x[u].bs[t][j] = byte(sb[t][j]);
 #pragma unroll
         for (int i = 0; i < MT; i++) x[u].as[i] = byte(sa[i]);
+        if (E == 1 && 64 * (s + h + u + 1) > a.kb) {
+          const int k = 64 * (s + h + u) + 16 * q;
+#pragma unroll
+          for (int t = 0; t < MATS; t++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) x[u].b[t][j] = row_shift(x[u].b[t][j], k, a.kb);
+#pragma unroll
+          for (int i = 0; i < MT; i++) x[u].a[i] = row_shift(x[u].a[i], k, a.kb);
+          // (a block behind the end must not bring the last one's scale, which may be NaN)
+#pragma unroll
+          for (int t = 0; t < MATS; t++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) x[u].bs[t][j] = k < a.kb ? x[u].bs[t][j] : 127;
+#pragma unroll
+          for (int i = 0; i < MT; i++) x[u].as[i] = k < a.kb ? x[u].as[i] : 127;
+        }
         run(x[u]);
       }
     }
-  }
-  // single steps; the last of all, which rows end in, by the last wave
-  const bool tail = wave == waves - 1 && (a.kb & 63);
-  for (; s < end + tail; s++) {
-    Step x;
-    const int k = 64 * s + 16 * q;
-    if (s < whole) {
-      codes(x, s);
-    } else {
-#pragma unroll
-      for (int i = 0; i < MT; i++) x.a[i] = row16(ap[i] - 16 * q, k, a.kb);
-#pragma unroll
-      for (int t = 0; t < MATS; t++)
-#pragma unroll
-        for (int j = 0; j < NT; j++) x.b[t][j] = row16(bp[t][j] - 16 * q, k, a.kb);
-    }
-#pragma unroll
-    for (int i = 0; i < MT; i++) x.as[i] = k < a.kb ? as[i][4 * s + q] : 127;
-#pragma unroll
-    for (int t = 0; t < MATS; t++)
-#pragma unroll
-      for (int j = 0; j < NT; j++) x.bs[t][j] = k < a.kb ? bs[t][j][4 * s + q] : 127;
-    run(x);
+  };
+  int s = wave * span;
+  const int end = min(s + span, (a.kb + 63) >> 6);
+  for (; 64 * (s + 4) <= a.kb && s < end; s += 4) four(s, end, std::integral_constant<int, 0>{});
+  if (s < end) {
+    if (a.kb >= 16) four(s, end, std::integral_constant<int, 1>{});
+    else four(s, end, std::integral_constant<int, 2>{});
   }
   if (waves > 1) {
 #pragma unroll
@@ -420,8 +436,8 @@ template <int MT, int NT, int MATS>
 int launch_skinny(Mx4Args a, hipStream_t st) {
   const int64_t bn = cdiv(a.N, 16 * NT), bm = cdiv(a.M, 16 * MT);
   // about twelve waves to a CU, up to 16 to a block (64 KiB of sums)
-  const int steps = a.kb >> 6;
-  int waves = (int)std::min<int64_t>({cdiv(12 * num_cus(), bn * bm), skinny_waves(MT), std::max(steps, 1), 64 / (MATS * MT * NT)});
+  const int steps = (a.kb + 63) >> 6;
+  int waves = (int)std::min<int64_t>({cdiv(12 * num_cus(), bn * bm), skinny_waves(MT, MATS), std::max(steps, 1), 64 / (MATS * MT * NT)});
   const int span = (int)cdiv(cdiv(steps, waves), 4) * 4;
   if (span) waves = (int)cdiv(steps, span);
   // a launch has below 2^31 threads: in turn, runs of column blocks, and of row blocks where
@@ -436,8 +452,9 @@ int launch_skinny(Mx4Args a, hipStream_t st) {
       c.a += row * a.lda, c.as += row * a.ldas, c.out += row * a.ldo + col, c.M = (int)rows, c.N = (int)cols;
       for (int t = 0; t < MATS; t++) c.b[t] += col * a.ldb[t], c.bs[t] += col * a.ldbs[t];
       const int64_t blocks_n = cdiv(cols, 16 * NT);
-      hipLaunchKernelGGL((mx4_skinny_k<MT, NT, MATS>), dim3((unsigned)(blocks_n * cdiv(rows, 16 * MT))),
-                         dim3(64 * waves), waves > 1 ? waves * MATS * MT * NT * 1024 : 0, st, c, span, (int)blocks_n);
+      hipLaunchKernelGGL((a.shift_codes ? mx4_skinny_k<MT, NT, MATS, 2> : a.shift ? mx4_skinny_k<MT, NT, MATS, 1> : mx4_skinny_k<MT, NT, MATS, 0>),
+                         dim3((unsigned)(blocks_n * cdiv(rows, 16 * MT))), dim3(64 * waves),
+                         waves > 1 ? waves * MATS * MT * NT * 1024 : 0, st, c, span, (int)blocks_n);
       SIMP_HIP(hipGetLastError());
     }
   }
@@ -951,7 +968,7 @@ __global__ void __launch_bounds__(256) mx4_pad_k(const Mx4Args a, uint4 *__restr
   BlockAt(first, per).get(threadIdx.x, row, c);
   const uint8_t *p = w == 0 ? a.a + row * a.lda
                             : a.b[w > 1 ? MATS - 1 : 0] + row * a.ldb[w > 1 ? MATS - 1 : 0];
-  out[(w > 0 ? ca : 0) + (w > 1 ? cb : 0) + first + threadIdx.x] = row16(p, 16 * (int)c, a.kb);
+  out[(w > 0 ? ca : 0) + (w > 1 ? cb : 0) + first + threadIdx.x] = row_shift(row_load(p, 16 * (int)c, a.kb), 16 * (int)c, a.kb);
 }
 
 // 256 x 256 tiles; false where their scales cannot be packed (no memory, or a captured call
@@ -1136,9 +1153,13 @@ int product(const char *fn, Mat<const uint8_t> &a, Mat<const uint8_t> &as,
   }
   g.out = (float *)oo.dev(), g.ldo = o.st[0];
   g.M = (int)o.s[0], g.N = (int)o.s[1], g.kb = (int)a.s[1];
-  uintptr_t base = (uintptr_t)g.as, rows = (uintptr_t)g.ldas;
-  for (int t = 0; t < MATS; t++) base |= (uintptr_t)g.bs[t], rows |= (uintptr_t)g.ldbs[t];
+  uintptr_t base = (uintptr_t)g.as, rows = (uintptr_t)g.ldas, cbase = (uintptr_t)g.a, crows = (uintptr_t)g.lda;
+  for (int t = 0; t < MATS; t++) {
+    base |= (uintptr_t)g.bs[t], rows |= (uintptr_t)g.ldbs[t];
+    cbase |= (uintptr_t)g.b[t], crows |= (uintptr_t)g.ldb[t];
+  }
   g.shift = (base & 3) == 0 && (rows & 3) != 0;
+  g.shift_codes = ((base | cbase) & 3) == 0 && (crows & 3) != 0;
   if ((rc = launch_mx4<MATS>(g, cur_stream()))) return rc;
   Operand *ops[] = {&oa, &oas, &oo, &ob[0], &obs[0], &ob[MATS - 1], &obs[MATS - 1]};
   return finish(ops, 3 + 2 * MATS);
