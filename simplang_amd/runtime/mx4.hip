@@ -257,7 +257,10 @@ __device__ __forceinline__ uint4 row_shift(uint4 v, int k, int kb) {
 // 16 NT columns of each matrix and all 16 MT rows to a block, whose waves split K: a wave
 // takes every byte of its rows' piece once, straight from memory into the lanes that
 // feed the matrix instruction (16 rows of 64 bytes, and a byte of scales to a lane), and
-// the waves' sums meet in LDS, in the order of K.
+// the waves' sums meet in LDS, in the order of K.  SHIFT: rows of scales (1), of codes too (2),
+// that are not on 4 bytes are read as aligned dwords (16 x 8641 x 3200: 9.1 us, 14.6 as
+// they lie; 16 x 8640 x 3200, where only the scales are not, 6.6).  Memory bounds it, 1 x 3200 x 32000:
+// 10.0 us, 5.4 TB/s of weights that lie in the last cache; 16 x 3200 x 8640 gated 7.6.
 constexpr int skinny_waves(int MT, int MATS) { return MT * MATS >= 4 ? 8 : 16; }  // of a block at most
 template <int MT, int NT, int MATS, int SHIFT>
 __global__ void __launch_bounds__(64 * skinny_waves(MT, MATS)) mx4_skinny_k(const Mx4Args a, int span, int blocks_n) {
@@ -513,8 +516,8 @@ __device__ __forceinline__ uint4 scale_group(const uint8_t *s, int g, int nb, bo
 
 // Scale bytes as the 256 x 256 tiles read them: for 64 rows and a group of four K-steps
 // 1 KB, 16 bytes a row (scale_group), so that one DMA instruction brings a wave the scales
-// of 64 rows for four steps.  Row v of W1 and W3 together: 16 rows of one, then 16 of the
-// other.
+// of 64 rows for four steps (8192 + 8192 rows of K = 8192: 4 us).  Row v of W1 and W3 together:
+// 16 rows of one, then 16 of the other.
 template <int MATS>
 __global__ void __launch_bounds__(256)
     mx4_pack_scales_k(const Mx4Args a, uint4 *__restrict__ pa, uint4 *__restrict__ pb, int ga, int groups) {
@@ -540,6 +543,8 @@ __device__ __forceinline__ v4f mfma_step(const uint4 &b, uint32_t sb, const uint
 // 64 in K-steps of 64 code bytes.  global_load_lds_dwordx4 fills a ring of two slots of two
 // steps each, so that every request is a whole line of 128 bytes: half lines, in four slots
 // of one step, cost 8192^3 184 us for the loads alone, not 129 (whole: 267, not 260).
+// 8192^3: 254 us, 4.3 POP/s; the matrix instructions take 57% of the cycles at 2.0 GHz, and
+// alone, from registers, 164 us, for the clock falls with them (6.7 POP/s).
 template <int MATS>
 __global__ void __launch_bounds__(512)
     mx4_dma_k(const Mx4Args a, const uint4 *__restrict__ pa, const uint4 *__restrict__ pb,
@@ -710,6 +715,9 @@ __global__ void __launch_bounds__(512)
 
 // ---- products between the two: BM x BN tiles, stages of 128 code bytes
 
+// What bounds them is the path that brings the operands into LDS, 16 KB for a 64 x 64 tile and
+// stage (200 x 3200 x 8640: 12.9 us, 110 MB at 70% of the rate that DMA alone reaches), and below
+// one tile to a CU a stage's round trip.
 // KS groups of WGM x WGN waves have a part of K each, with a ring of SLOTS stages of their
 // own, and their sums meet in LDS in the order of K: the chain of stages, each of which
 // costs a round trip and a barrier, is KS times shorter, and a tile that has a CU to
@@ -957,7 +965,8 @@ int launch_ring(const Mx4Args &a, hipStream_t st) {
 }
 
 // Codes of rows whose bytes the tile kernels cannot read in place (any address and length)
-// into rows of whole aligned 16 bytes, zeros behind their ends: A's, then each B's.
+// into rows of whole aligned 16 bytes, zeros behind their ends: A's, then each B's (717 and 2051
+// rows of 767 bytes 4 us, of the 11.3 of their product).
 template <int MATS>
 __global__ void __launch_bounds__(256) mx4_pad_k(const Mx4Args a, uint4 *__restrict__ out, int per, int ga, int gb) {
   const int w = (int)blockIdx.x < ga ? 0 : MATS == 2 && (int)blockIdx.x >= ga + gb ? 2 : 1;
@@ -999,7 +1008,8 @@ bool launch_dma(const Mx4Args &a, hipStream_t st, int *rc) {
 
 // What each form takes in us, fitted to whole calls (graph replay) of 1 to 8192 rows,
 // K = 768 to 8192 and up to 32000 columns; `steps` of 128 elements, `out` the outputs'
-// time to memory.  The choice by it is within about 10% of the best form's time.
+// time to memory.  The choice by it is within about 10% of the best form's time (odd K,
+// padded first: within 15%, 2% on average).
 enum Form { kSkinny, kRing64, kRing64x2, kRing128, kTiles256 };
 template <int MATS>
 Form pick(const Mx4Args &a, int64_t cus) {
