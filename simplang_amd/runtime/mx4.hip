@@ -246,12 +246,14 @@ __device__ __forceinline__ uint4 row_load(const uint8_t *row, int k, int kb) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 // ... and what to make of it.
-__device__ __forceinline__ uint4 row_shift(uint4 v, int k, int kb) {
-  const int sh = kb >= 16 ? min(max(k - kb + 16, 0), 16) : 0;
+__device__ __forceinline__ uint4 shift_down(uint4 v, int bytes) {  // 0 to 16
   uint64_t lo = v.x | (uint64_t)v.y << 32, hi = v.z | (uint64_t)v.w << 32;
-  if (sh >= 8) lo = sh < 16 ? hi >> (8 * (sh - 8)) : 0, hi = 0;
-  else if (sh > 0) lo = lo >> (8 * sh) | hi << (64 - 8 * sh), hi >>= 8 * sh;
+  if (bytes >= 8) lo = bytes < 16 ? hi >> (8 * (bytes - 8)) : 0, hi = 0;
+  else if (bytes > 0) lo = lo >> (8 * bytes) | hi << (64 - 8 * bytes), hi >>= 8 * bytes;
   return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+}
+__device__ __forceinline__ uint4 row_shift(uint4 v, int k, int kb) {
+  return kb >= 16 ? shift_down(v, min(max(k - kb + 16, 0), 16)) : v;
 }
 
 // 16 NT columns of each matrix and all 16 MT rows to a block, whose waves split K: a wave
@@ -725,7 +727,7 @@ __global__ void __launch_bounds__(512)
 // whole lines.  The scales of RG groups of a part are staged through registers into
 // LDS as scale_group gives them (RG odd: rows of scales then start in different banks),
 // and those of the next RG when they are used up.
-template <int BM, int BN, int WGM, int WGN, int KS, int RG, int MATS>
+template <int BM, int BN, int WGM, int WGN, int KS, int RG, int MATS, bool REG>
 __global__ void __launch_bounds__(64 * WGM * WGN * KS)
     mx4_ring_k(const Mx4Args a, int tiles_m, int tiles_n, int per) {
   constexpr int NW = WGM * WGN, NT = 64 * NW * KS;
@@ -785,6 +787,42 @@ __global__ void __launch_bounds__(64 * WGM * WGN * KS)
       go(baseB[MATS == 2 ? ((wave * DB + i) >> 1) & 1 : 0], offB[i], wave * DB + i,
          dst + SA + 1024 * (wave * DB + i));
   };
+  // REG: a stage's pieces on their way through registers, as aligned dwords, and into the slot.
+  struct Piece {
+    uint4 u;
+    uint32_t w, sh;
+  };
+  Piece pieces[REG ? DA + DB : 1];
+  // the bytes of a lane's piece i that lie behind the row's end
+  auto behind = [&](int st, int i) {
+    return max(st * BK + 16 * ((lane & 7) ^ ((4 * i + (lane >> 4)) & 7)) + 16 - a.kb, 0);
+  };
+  auto fetch = [&](int st, auto last) {
+    const int64_t k0 = (int64_t)st * BK;
+    auto go = [&](const uint8_t *base, uint32_t off, int i, Piece &x) {
+      const uint8_t *p = base + k0 + off;
+      if constexpr (decltype(last)::value) p -= behind(st, i);
+      x.sh = (uintptr_t)p & 3;
+      const u4any u = *(const u4any *)__builtin_assume_aligned(p - x.sh, 4);
+      x.u = make_uint4(u.x, u.y, u.z, u.w), x.w = *(const u1any *)(p + 12);
+    };
+#pragma unroll
+    for (int i = 0; i < DA; i++) go(baseA, offA[i], wave * DA + i, pieces[i]);
+#pragma unroll
+    for (int i = 0; i < DB; i++)
+      go(baseB[MATS == 2 ? ((wave * DB + i) >> 1) & 1 : 0], offB[i], wave * DB + i, pieces[DA + i]);
+  };
+  auto put = [&](int st, int slot, auto last) {
+#pragma unroll
+    for (int i = 0; i < DA + DB; i++) {
+      const Piece &x = pieces[i];
+      const int at = i < DA ? wave * DA + i : wave * DB + i - DA;
+      uint4 v = make_uint4(__builtin_amdgcn_alignbyte(x.u.y, x.u.x, x.sh), __builtin_amdgcn_alignbyte(x.u.z, x.u.y, x.sh),
+                           __builtin_amdgcn_alignbyte(x.u.w, x.u.z, x.sh), x.w);
+      if constexpr (decltype(last)::value) v = shift_down(v, min(behind(st, at), 16));
+      ring[slot * (STAGE / 16) + (i < DA ? 0 : SA / 16) + at * 64 + lane] = v;
+    }
+  };
   // (slot and row part constant: the reads' immediate offsets)
   const uint4 *fA[2], *fB[2];
 #pragma unroll
@@ -827,7 +865,12 @@ __global__ void __launch_bounds__(64 * WGM * WGN * KS)
     const int c0 = s0 + d0, c1 = min(c0 + len, s1);
     if (d0) block_barrier();  // the span before is read
     const int first = max(min(SLOTS, c1 - c0), 0);
-    for (int i = 0; i < first; i++) issue(c0 + i, i, T{});
+    if constexpr (REG) {
+      if (first > 0) fetch(c0, T{}), put(c0, 0, T{});
+      if (first > 1) fetch(c0 + 1, T{});
+    } else {
+      for (int i = 0; i < first; i++) issue(c0 + i, i, T{});
+    }
     // scales: a thread has one row (and part) and takes its groups all at once
     uint4 sv[U];
 #pragma unroll
@@ -874,9 +917,15 @@ __global__ void __launch_bounds__(64 * WGM * WGN * KS)
       __builtin_amdgcn_sched_barrier(0);
       if (in) mul(std::integral_constant<int, 2 * o>{});
       __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-      __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0);
-      block_barrier();
+      if constexpr (REG) {
+        if constexpr (S) put(st + 1, o ^ 1, F{});
+        else if (st + 1 < c1) put(st + 1, o ^ 1, T{});
+        lds_barrier();
+      } else {
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+        __builtin_amdgcn_s_waitcnt(waitcnt_lgkm0);
+        block_barrier();
+      }
       read(Other{}, I0{});
       if constexpr (o == 1) {
         const int g = min((st + 1 - c0) >> 1, RG - 1);
@@ -886,8 +935,13 @@ __global__ void __launch_bounds__(64 * WGM * WGN * KS)
         for (int i = 0; i < FM; i++) na[i] = scale(g, wm0 + 16 * i);
       }
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (S) issue(st + 2, o, F{});
-      else if (st + 2 < c1) issue(st + 2, o, T{});
+      if constexpr (REG) {
+        if constexpr (S) fetch(st + 2, F{});
+        else if (st + 2 < c1) fetch(st + 2, T{});
+      } else {
+        if constexpr (S) issue(st + 2, o, F{});
+        else if (st + 2 < c1) issue(st + 2, o, T{});
+      }
       if (in) mul(std::integral_constant<int, 2 * o + 1>{});
       if constexpr (o == 1) {
 #pragma unroll
@@ -953,12 +1007,14 @@ __global__ void __launch_bounds__(64 * WGM * WGN * KS)
   }
 }
 
-template <int BM, int BN, int WGM, int WGN, int KS, int RG, int MATS>
+template <int BM, int BN, int WGM, int WGN, int KS, int RG, int MATS, bool REG>
 int launch_ring(const Mx4Args &a, hipStream_t st) {
   const int64_t tm = cdiv(a.M, BM), tn = cdiv(a.N, BN / MATS);
   const int per = (int)(2 * cdiv(cdiv(a.kb, 128), 2 * KS));  // stages of a part, even
-  KernelTimer kt(st, BN == 128 ? "mx4_ring128" : KS == 2 ? "mx4_ring64x2" : "mx4_ring64");
-  hipLaunchKernelGGL((mx4_ring_k<BM, BN, WGM, WGN, KS, RG, MATS>), dim3((unsigned)(tm * tn)),
+  static const char *const kNames[2][3] = {{"mx4_ring64", "mx4_ring64x2", "mx4_ring128"},
+                                           {"mx4_ring64d", "mx4_ring64x2d", "mx4_ring128d"}};
+  KernelTimer kt(st, kNames[REG][BN == 128 ? 2 : KS - 1]);
+  hipLaunchKernelGGL((mx4_ring_k<BM, BN, WGM, WGN, KS, RG, MATS, REG>), dim3((unsigned)(tm * tn)),
                      dim3(64 * WGM * WGN * KS), 0, st, a, (int)tm, (int)tn, per);
   SIMP_HIP(hipGetLastError());
   return SIMP_RT_OK;
@@ -1008,51 +1064,74 @@ bool launch_dma(const Mx4Args &a, hipStream_t st, int *rc) {
 
 // What each form takes in us, fitted to whole calls (graph replay) of 1 to 8192 rows,
 // K = 768 to 8192 and up to 32000 columns; `steps` of 128 elements, `out` the outputs'
-// time to memory.  The choice by it is within about 10% of the best form's time (odd K,
-// padded first: within 15%, 2% on average).
+// time to memory.  The choice by it is within about 10% of the best form's time.
 enum Form { kSkinny, kRing64, kRing64x2, kRing128, kTiles256 };
+// What the tile kernels make of rows that do not lie on 16 bytes: they read them as dwords
+// (the rings' stages go through registers, and take about twice as long: 60 x 2899 x 23360
+// gated 23 us, with the copy 40, on 16 bytes 16), or rows are copied first (600 x 3201 x 8640 39.5
+// us; as dwords 41).
+enum Rows { kDirect, kDwords, kPadded };
+struct Choice {
+  Form form;
+  Rows rows;
+};
+// `can`: kDirect where rows do lie on 16 bytes, kPadded where they cannot be read as dwords.
 template <int MATS>
-Form pick(const Mx4Args &a, int64_t cus) {
+Choice pick(const Mx4Args &a, int64_t cus, Rows can) {
   const double steps = (double)cdiv(a.kb, 64), out = 4e-6 * a.M * a.N / 6.5;
   const int mt = a.M <= 16 ? 16 : a.M <= 32 ? 32 : 64;
   auto tiles = [&](int m, int n) { return cdiv(a.M, m) * cdiv(a.N, n / MATS); };
   auto rounds = [&](int64_t t) { return (double)cdiv(t, cus); };
-  double us[5];
   const double mem = (a.M + (double)MATS * a.N) * steps * 68 / 5.2e6;  // the operands' time from memory
   // a block's operands from the caches, 33 KB a us to a CU: every row block reads B, every
   // column block A
   const double blocks = (double)cdiv(a.M, mt) * cdiv(a.N, 16) / cus;
-  us[kSkinny] = 2.5 + std::max(std::max(1., blocks) * (std::min(a.M, mt) + 16 * MATS) * steps * 68 / 33.2e3, mem);
-  const int64_t t64 = tiles(64, 64), t256 = tiles(256, 256);
-  us[kRing64] = 3.7 + std::max(mem, steps / 2 * std::max(0.33, 0.23 * rounds(t64))) + out;
-  us[kRing64x2] = 4.0 + std::max(mem, steps / 2 * 0.2 * (t64 <= cus ? 1. : 1.3 * rounds(t64))) + out;
-  us[kRing128] = 4.0 + std::max(mem, steps / 2 * 0.42 * rounds(tiles(64, 128))) + out;
-  us[kTiles256] = 8.0 + steps * (0.95 * (t256 / cus) + (t256 % cus ? 0.3 + 0.65 * (t256 % cus) / cus : 0.)) + out;
-  return (Form)(std::min_element(us, us + 5) - us);
+  const double cache = std::max(1., blocks) * (std::min(a.M, mt) + 16 * MATS) * steps * 68 / 33.2e3;
+  const int64_t t64 = tiles(64, 64), t128 = tiles(64, 128), t256 = tiles(256, 256);
+  double us[5] = {2.5 + std::max(cache, mem),
+                  3.7 + std::max(mem, steps / 2 * std::max(0.33, 0.23 * rounds(t64))) + out,
+                  4.0 + std::max(mem, steps / 2 * 0.2 * (t64 <= cus ? 1. : 1.3 * rounds(t64))) + out,
+                  4.0 + std::max(mem, steps / 2 * 0.42 * rounds(t128)) + out,
+                  8.0 + steps * (0.95 * (t256 / cus) + (t256 % cus ? 0.3 + 0.65 * (t256 % cus) / cus : 0.)) + out};
+  const auto least = [](const double *v) { return (int)(std::min_element(v, v + 5) - v); };
+  if (can != kDwords) return {(Form)least(us), can};
+  const double copy = 6 + (a.M + (double)MATS * a.N) * 2 * a.kb / 4.5e6;
+  us[kSkinny] = 2.5 + std::max((a.shift_codes ? 1.9 : a.M > 32 ? 1.6 : 1.1) * cache, (a.shift_codes ? 1.45 : 1.) * mem);
+  for (int f = kRing64; f <= kTiles256; f++) us[f] += copy;
+  const double dwords[5] = {us[kSkinny],
+                            3.7 + std::max(mem, steps / 2 * std::max(0.6, 0.45 * rounds(t64))) + out,
+                            4.0 + std::max(mem, steps / 2 * 0.5 * (t64 <= cus ? 1. : 1.6 * rounds(t64))) + out,
+                            4.0 + std::max(mem, steps / 2 * (t128 <= cus ? 0.82 : 0.95 * rounds(t128))) + out,
+                            us[kTiles256]};
+  const int f = least(us), d = least(dwords);
+  return us[f] <= dwords[d] ? Choice{(Form)f, kPadded} : Choice{(Form)d, kDwords};
 }
 
-// The form that `pick` names, where the codes can be read as they lie; false where not.
-template <int MATS>
+// A form on tiles; false where its grid has no room.
+template <int MATS, bool REG>
 bool launch_tiles(const Mx4Args &a, Form f, hipStream_t st, int *rc) {
-  if (f == kTiles256 && launch_dma<MATS>(a, st, rc)) return true;
+  if (!REG && f == kTiles256 && launch_dma<MATS>(a, st, rc)) return true;
   if (cdiv(a.M, 64) * cdiv(a.N, 64 / MATS) > INT32_MAX / 512) return false;
-  *rc = f == kRing64 ? launch_ring<64, 64, 2, 2, 1, 9, MATS>(a, st)
-        : f == kRing64x2 ? launch_ring<64, 64, 2, 2, 2, 9, MATS>(a, st)
-                         : launch_ring<64, 128, 2, 4, 1, 9, MATS>(a, st);
+  *rc = f == kRing64 ? launch_ring<64, 64, 2, 2, 1, 9, MATS, REG>(a, st)
+        : f == kRing64x2 ? launch_ring<64, 64, 2, 2, 2, 9, MATS, REG>(a, st)
+                         : launch_ring<64, 128, 2, 4, 1, 9, MATS, REG>(a, st);
   return true;
 }
 
 template <int MATS>
 int launch_mx4(const Mx4Args &a, hipStream_t st) {
   int rc;
-  const Form f = pick<MATS>(a, num_cus());
-  if (f != kSkinny && a.kb > 0) {
-    // the tile kernels read aligned 16-byte pieces, and their offsets within a tile are 32-bit
-    uintptr_t low = (uintptr_t)a.a | (uintptr_t)a.lda | (uintptr_t)a.kb;
-    for (int t = 0; t < MATS; t++) low |= (uintptr_t)a.b[t] | (uintptr_t)a.ldb[t];
-    const int64_t ld = std::max({a.lda, a.ldb[0], a.ldb[MATS - 1]});
-    if ((low & 15) == 0 && ld < (1 << 23)) {
-      if (launch_tiles<MATS>(a, f, st, &rc)) return rc;
+  // the tile kernels' offsets within a tile are 32-bit
+  uintptr_t base = (uintptr_t)a.a, rows = (uintptr_t)a.lda | (uintptr_t)a.kb;
+  for (int t = 0; t < MATS; t++) base |= (uintptr_t)a.b[t], rows |= (uintptr_t)a.ldb[t];
+  const bool near = std::max({a.lda, a.ldb[0], a.ldb[MATS - 1]}) < (1 << 23);
+  const Choice c = pick<MATS>(a, num_cus(), near && ((base | rows) & 15) == 0 ? kDirect
+                                            : near && (base & 3) == 0 && a.kb >= 16 ? kDwords : kPadded);
+  if (c.form != kSkinny && a.kb > 0) {
+    if (c.rows == kDirect) {
+      if (launch_tiles<MATS, false>(a, c.form, st, &rc)) return rc;
+    } else if (c.rows == kDwords) {
+      if (launch_tiles<MATS, true>(a, c.form, st, &rc)) return rc;
     } else if (a.kb < (1 << 23) - 16) {
       const int per = (int)cdiv(a.kb, 16);
       const int64_t ca = (int64_t)a.M * per, cb = (int64_t)a.N * per;
@@ -1066,11 +1145,11 @@ int launch_mx4(const Mx4Args &a, hipStream_t st) {
         hipLaunchKernelGGL(mx4_pad_k<MATS>, dim3((unsigned)(ga + MATS * gb)), dim3(256), 0, st, a, q, per,
                            (int)ga, (int)gb);
         SIMP_HIP(hipGetLastError());
-        Mx4Args c = a;
-        c.a = (const uint8_t *)q, c.lda = 16 * (int64_t)per;
+        Mx4Args o = a;
+        o.a = (const uint8_t *)q, o.lda = 16 * (int64_t)per;
         for (int t = 0; t < MATS; t++)
-          c.b[t] = (const uint8_t *)(q + ca + t * cb), c.ldb[t] = 16 * (int64_t)per;
-        if (launch_tiles<MATS>(c, f, st, &rc)) return rc;
+          o.b[t] = (const uint8_t *)(q + ca + t * cb), o.ldb[t] = 16 * (int64_t)per;
+        if (launch_tiles<MATS, false>(o, c.form, st, &rc)) return rc;
       }
     }
   }

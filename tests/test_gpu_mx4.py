@@ -199,27 +199,57 @@ FORMS = [
     (257, 640, 8320, "ring64", "ring128"),
     (600, 272, 4100, "ring64", "ring64"),
     (513, 2448, 2050, "ring128", "ring64"),
-    (700, 767, 2051, "ring64", "ring64"),
     (900, 80, 9000, "ring64", "ring64"),
-    (300, 1100, 2051, "ring64x2", "ring128"),
-    (65, 2500, 3001, "ring64x2", "ring64x2"),
     (130, 640, 9000, "ring64", "ring128"),
     (1100, 1104, 1100, "ring128", "ring64"),
     (1000, 144, 6000, "ring64", "ring128"),
     (600, 2336, 2000, "ring128", "ring64"),
-    (200, 1601, 4000, "ring64x2", "ring128"),
     (65, 6000, 1000, "ring64x2", "ring64x2"),
     (3000, 800, 2900, "dma", "dma"),
     (2900, 1040, 3008, "dma", "dma"),
     (2817, 1088, 3089, "dma", "dma"),
     (3100, 1200, 2900, "dma", "dma"),
-    (2900, 1001, 3000, "dma", "dma"),
     (6000, 1024, 6000, "dma", "dma"),
     (3000, 2064, 2900, "dma", "dma"),
     (70, 2048, 4096, "ring64x2", "ring64x2"),
     (200, 768, 12000, "ring64", "ring128"),
     (150, 1600, 8200, "ring128", "ring128"),
     (300, 2400, 1500, "ring64x2", "ring64x2"),
+]
+# pad, shift: rows that do not lie on 16 bytes
+ODD = [
+    (600, 272, 4100, 1, 0, "ring64d", "ring64d"),
+    (1000, 144, 6000, 1, 0, "ring64d", "ring64d"),
+    (200, 768, 12000, 1, 0, "ring64d", "ring64d"),
+    (250, 912, 3000, 3, 4, "ring64x2d", "ring128d"),
+    (300, 2400, 1500, 3, 0, "ring64x2d", "ring64x2d"),
+    (64, 1600, 2800, 1, 0, "skinny", "ring64x2d"),
+    (300, 1100, 2051, 0, 0, "ring64x2d", "ring128d"),
+    (300, 1101, 2051, 0, 0, "ring64x2d", "ring128d"),
+    (65, 2500, 3001, 0, 0, "ring64x2d", "ring64x2d"),
+    (65, 6001, 1000, 0, 0, "ring64x2", "ring64x2"),
+    (700, 767, 2051, 0, 0, "ring128d", "ring64d"),
+    (700, 767, 2051, 2, 0, "ring128d", "ring64d"),
+    (200, 1601, 4000, 0, 0, "ring64x2d", "ring128d"),
+    (513, 2447, 2050, 0, 0, "ring128d", "ring64"),
+    (100, 1087, 8200, 0, 4, "ring128d", "ring64d"),
+    (33, 2319, 3000, 0, 0, "skinny", "skinny"),
+    (2900, 1001, 3000, 0, 0, "dma", "dma"),
+    (120, 17, 3000, 0, 0, "skinny", "skinny"),
+    (120, 31, 3000, 0, 0, "skinny", "skinny"),
+    (120, 16, 3000, 3, 0, "skinny", "skinny"),
+    (120, 15, 3000, 0, 0, "skinny", "skinny"),
+    (130, 385, 9000, 0, 0, "ring64d", "ring64d"),
+    (20, 1451, 9000, 0, 0, "skinny", "skinny"),
+    (200, 129, 5000, 0, 0, "ring64d", "ring64d"),
+    (200, 1153, 5000, 0, 0, "ring128d", "ring64d"),
+    (700, 767, 2051, 0, 1, "ring64", "ring64"),
+    (200, 1601, 4000, 0, 3, "ring64x2", "ring128"),
+    (300, 1100, 2051, 0, 2, "ring64x2", "ring128"),
+    (2900, 1001, 3000, 0, 5, "dma", "dma"),
+    (65, 1250, 3001, 0, 0, "ring64x2d", "ring64x2d"),
+    (150, 1252, 3001, 0, 0, "ring64x2d", "ring128d"),
+    (65, 1250, 3001, 1, 0, "ring64x2d", "ring64x2d"),
 ]
 
 
@@ -239,10 +269,21 @@ def _on_device(dev, seed, m, kb, n, gate, lo=126, hi=129, pad=0, shift=0):
 
 
 @pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("m, kb, n, pad, shift, plain, gated", ODD)
+def test_every_form_of_odd_rows(dev, gate, m, kb, n, pad, shift, plain, gated):
+    _form(dev, gate, m, kb, n, pad, shift, 1, gated if gate else plain)
+
+
+@pytest.mark.parametrize("gate", [False, True])
 @pytest.mark.parametrize("pad, shift, opad", [(0, 0, 0), (32, 16, 4), (3, 1, 1)])
 @pytest.mark.parametrize("m, kb, n, plain, gated", FORMS)
 def test_every_form(dev, gate, m, kb, n, plain, gated, pad, shift, opad):
-    """Against 64 bits on the device, every output; rows as they lie, padded, and at odd addresses."""
+    """Rows as they lie, padded, and at odd addresses."""
+    _form(dev, gate, m, kb, n, pad, shift, opad, gated if gate else plain)
+
+
+def _form(dev, gate, m, kb, n, pad, shift, opad, form):
+    """Against 64 bits on the device, every output, by the form that is expected."""
     import torch
     a, *bs = _on_device(dev, m + kb, m, kb, n, gate, pad=pad, shift=shift)
     buf = torch.full((m + 2, n + opad), 5.0, device=dev)
@@ -253,7 +294,7 @@ def test_every_form(dev, gate, m, kb, n, plain, gated, pad, shift, opad):
     sa.timing(True)
     try:
         f(*a, *[x for b in bs for x in b], out)
-        assert sa.timing_query("mx4_" + (gated if gate else plain))[1] == 1
+        assert sa.timing_query("mx4_" + form)[1] == 1
     finally:
         sa.timing(False)
     assert (buf[0] == 5).all() and (buf[-1] == 5).all() and (buf[:, n:] == 5).all()
