@@ -960,48 +960,52 @@ __global__ void __launch_bounds__(64 * WGM * WGN * KS)
       stage(st + 1, I1{}, F{});
     }
   }
-  // acc[i][j][r] = C[m0 + wm0 + 16 i + l%16][v0 + wn0 + 16 j + 4 (l/16) + r]
-  auto store = [&](int i, int j, v4f v, v4f w) {
-    const int row = m0 + wm0 + 16 * i + lrow, col = n0 + (wn0 + 16 * j) / MATS + 4 * lkc;
-    if (row >= a.M || col >= a.N) return;
-    if constexpr (MATS == 2) {
-#pragma unroll
-      for (int r = 0; r < 4; r++) v[r] = swiglu(v[r], w[r]);
-    }
-    float *dst = a.out + (int64_t)row * a.ldo + col;
-    if (col + 3 < a.N) {
-      *(f4any *)dst = v;
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; r++)
-        if (col + r < a.N) dst[r] = v[r];
-    }
-  };
-  if constexpr (KS == 1) {
-#pragma unroll
-    for (int j = 0; j < FN; j += MATS)
-#pragma unroll
-      for (int i = 0; i < FM; i++) store(i, j, acc[i][j], acc[i][j + MATS - 1]);
-  } else {
-    v4f *sums = (v4f *)lds;  // [part][wave][i][j][lane]
-    lds_barrier();           // every wave is through with its ring
+  // acc[i][j][r] = C[m0 + wm0 + 16 i + l%16][v0 + wn0 + 16 j + 4 (l/16) + r]; the parts share the
+  // wave's fragments out between them, NF side by side in out
+  constexpr int NF = FN / MATS;
+  v4f *sums = (v4f *)lds;  // [part][wave][i][j][lane]
+  if constexpr (KS > 1) {
+    lds_barrier();  // every wave is through with its ring
 #pragma unroll
     for (int i = 0; i < FM; i++)
 #pragma unroll
       for (int j = 0; j < FN; j++) sums[((part * NW + wave) * FM * FN + i * FN + j) * 64 + lane] = acc[i][j];
     lds_barrier();
-    auto sum = [&](int i, int j) {
-      v4f v = sums[(wave * FM * FN + i * FN + j) * 64 + lane];
+  }
+  auto sum = [&](int i, int j) {
+    if constexpr (KS == 1) return acc[i][j];
+    v4f v = sums[(wave * FM * FN + i * FN + j) * 64 + lane];
 #pragma unroll
-      for (int p = 1; p < KS; p++) v += sums[((p * NW + wave) * FM * FN + i * FN + j) * 64 + lane];
-      return v;
-    };
-    // the parts share a wave's fragments out between them
+    for (int p = 1; p < KS; p++) v += sums[((p * NW + wave) * FM * FN + i * FN + j) * 64 + lane];
+    return v;
+  };
 #pragma unroll
-    for (int o = 0; o < FM * FN / MATS; o += KS) {
-      if (o + part < FM * FN / MATS) {
-        const int i = (o + part) / (FN / MATS), j = (o + part) % (FN / MATS) * MATS;
-        store(i, j, sum(i, j), sum(i, j + MATS - 1));
+  for (int o = 0; o < FM; o += KS) {
+    if (KS > 1 && o + part >= FM) break;
+    const int i = KS > 1 ? o + part : o;
+    v4f v[NF];
+#pragma unroll
+    for (int j = 0; j < NF; j++) {
+      v[j] = sum(i, j * MATS);
+      if constexpr (MATS == 2) {
+        const v4f w = sum(i, j * MATS + 1);
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[j][r] = swiglu(v[j][r], w[r]);
+      }
+    }
+    if constexpr (NF > 1) lane_transpose<NF>(v);
+    const int col = n0 + wn0 / MATS + 16 * (lrow & (NF - 1)) + 4 * lkc;
+#pragma unroll
+    for (int j = 0; j < NF; j++) {
+      const int row = m0 + wm0 + 16 * i + (lrow & ~(NF - 1)) + j;
+      if (row >= a.M || col >= a.N) continue;
+      float *dst = a.out + (int64_t)row * a.ldo + col;
+      if (col + 3 < a.N) {
+        *(f4any *)dst = v[j];
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          if (col + r < a.N) dst[r] = v[j][r];
       }
     }
   }
@@ -1063,8 +1067,8 @@ bool launch_dma(const Mx4Args &a, hipStream_t st, int *rc) {
 }
 
 // What each form takes in us, fitted to whole calls (graph replay) of 1 to 8192 rows,
-// K = 768 to 8192 and up to 32000 columns; `steps` of 128 elements, `out` the outputs'
-// time to memory.  The choice by it is within about 10% of the best form's time.
+// K = 768 to 8192 and up to 32000 columns; `steps` of 128 elements.
+// The choice by it is within about 10% of the best form's time.
 enum Form { kSkinny, kRing64, kRing64x2, kRing128, kTiles256 };
 // What the tile kernels make of rows that do not lie on 16 bytes: they read them as dwords
 // (the rings' stages go through registers, and take about twice as long: 60 x 2899 x 23360
@@ -1088,20 +1092,23 @@ Choice pick(const Mx4Args &a, int64_t cus, Rows can) {
   const double blocks = (double)cdiv(a.M, mt) * cdiv(a.N, 16) / cus;
   const double cache = std::max(1., blocks) * (std::min(a.M, mt) + 16 * MATS) * steps * 68 / 33.2e3;
   const int64_t t64 = tiles(64, 64), t128 = tiles(64, 128), t256 = tiles(256, 256);
-  double us[5] = {2.5 + std::max(cache, mem),
-                  3.7 + std::max(mem, steps / 2 * std::max(0.33, 0.23 * rounds(t64))) + out,
-                  4.0 + std::max(mem, steps / 2 * 0.2 * (t64 <= cus ? 1. : 1.3 * rounds(t64))) + out,
-                  4.0 + std::max(mem, steps / 2 * 0.42 * rounds(t128)) + out,
-                  8.0 + steps * (0.95 * (t256 / cus) + (t256 % cus ? 0.3 + 0.65 * (t256 % cus) / cus : 0.)) + out};
+  // outputs' time to memory, and the ends of tiles that nothing hides
+  const double out64 = out + (MATS == 2 ? 0.45 : 0.2) * rounds(t64), out128 = out + (MATS == 2 ? 0.55 : 0.1) * rounds(t128);
+  const double out256 = out + (MATS == 2 ? 2. * (rounds(t256) - 1) - 1. : 0.);
+  double us[5] = {2.5 + std::max(cache, mem) + out,
+                  3.5 + std::max(mem, steps / 2 * std::max(0.33, 0.23 * rounds(t64))) + out64,
+                  3.8 + std::max(mem, steps / 2 * 0.2 * (t64 <= cus ? 1. : 1.3 * rounds(t64))) + out64,
+                  4.0 + std::max(mem, steps / 2 * 0.42 * rounds(t128)) + out128,
+                  8.0 + steps * (0.95 * (t256 / cus) + (t256 % cus ? 0.6 + 0.35 * (t256 % cus) / cus : 0.)) + out256};
   const auto least = [](const double *v) { return (int)(std::min_element(v, v + 5) - v); };
   if (can != kDwords) return {(Form)least(us), can};
   const double copy = 6 + (a.M + (double)MATS * a.N) * 2 * a.kb / 4.5e6;
-  us[kSkinny] = 2.5 + std::max((a.shift_codes ? 1.9 : a.M > 32 ? 1.6 : 1.1) * cache, (a.shift_codes ? 1.45 : 1.) * mem);
+  us[kSkinny] = 2.5 + std::max((a.shift_codes ? 1.9 : a.M > 32 ? 1.6 : 1.1) * cache, (a.shift_codes ? 1.45 : 1.) * mem) + out;
   for (int f = kRing64; f <= kTiles256; f++) us[f] += copy;
   const double dwords[5] = {us[kSkinny],
-                            3.7 + std::max(mem, steps / 2 * std::max(0.6, 0.45 * rounds(t64))) + out,
-                            4.0 + std::max(mem, steps / 2 * 0.5 * (t64 <= cus ? 1. : 1.6 * rounds(t64))) + out,
-                            4.0 + std::max(mem, steps / 2 * (t128 <= cus ? 0.82 : 0.95 * rounds(t128))) + out,
+                            3.5 + std::max(mem, steps / 2 * std::max(0.6, 0.45 * rounds(t64))) + out64,
+                            3.8 + std::max(mem, steps / 2 * 0.5 * (t64 <= cus ? 1. : 1.6 * rounds(t64))) + out64,
+                            4.0 + std::max(mem, steps / 2 * (t128 <= cus ? 0.82 : 0.95 * rounds(t128))) + out128,
                             us[kTiles256]};
   const int f = least(us), d = least(dwords);
   return us[f] <= dwords[d] ? Choice{(Form)f, kPadded} : Choice{(Form)d, kDwords};

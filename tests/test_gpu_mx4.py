@@ -190,22 +190,22 @@ def _values64(codes, scales):
 
 # rows, code bytes of a row, columns, and the kernel that takes the product and the gate
 FORMS = [
-    (64, 1600, 2800, "skinny", "ring64x2"),
+    (64, 1600, 2800, "ring64x2", "ring64x2"),
     (33, 2320, 3000, "skinny", "skinny"),
     (129, 2304, 1500, "ring64x2", "ring64x2"),
     (300, 1024, 3000, "ring64x2", "ring128"),
-    (250, 912, 3000, "ring64x2", "ring64"),
+    (250, 912, 3000, "ring64x2", "ring128"),
     (100, 1088, 8200, "ring128", "ring64"),
     (257, 640, 8320, "ring64", "ring128"),
-    (600, 272, 4100, "ring64", "ring64"),
+    (600, 272, 4100, "ring64", "ring128"),
     (513, 2448, 2050, "ring128", "ring64"),
-    (900, 80, 9000, "ring64", "ring64"),
-    (130, 640, 9000, "ring64", "ring128"),
+    (900, 80, 9000, "ring128", "dma"),
+    (130, 640, 9000, "ring128", "ring128"),
     (1100, 1104, 1100, "ring128", "ring64"),
-    (1000, 144, 6000, "ring64", "ring128"),
+    (1000, 144, 6000, "ring128", "dma"),
     (600, 2336, 2000, "ring128", "ring64"),
     (65, 6000, 1000, "ring64x2", "ring64x2"),
-    (3000, 800, 2900, "dma", "dma"),
+    (3000, 800, 2900, "ring128", "dma"),
     (2900, 1040, 3008, "dma", "dma"),
     (2817, 1088, 3089, "dma", "dma"),
     (3100, 1200, 2900, "dma", "dma"),
@@ -218,12 +218,12 @@ FORMS = [
 ]
 # pad, shift: rows that do not lie on 16 bytes
 ODD = [
-    (600, 272, 4100, 1, 0, "ring64d", "ring64d"),
-    (1000, 144, 6000, 1, 0, "ring64d", "ring64d"),
+    (600, 272, 4100, 1, 0, "ring64d", "ring128d"),
+    (1000, 144, 6000, 1, 0, "ring128d", "ring128d"),
     (200, 768, 12000, 1, 0, "ring64d", "ring64d"),
     (250, 912, 3000, 3, 4, "ring64x2d", "ring128d"),
     (300, 2400, 1500, 3, 0, "ring64x2d", "ring64x2d"),
-    (64, 1600, 2800, 1, 0, "skinny", "ring64x2d"),
+    (64, 1600, 2800, 1, 0, "ring64x2d", "ring64x2d"),
     (300, 1100, 2051, 0, 0, "ring64x2d", "ring128d"),
     (300, 1101, 2051, 0, 0, "ring64x2d", "ring128d"),
     (65, 2500, 3001, 0, 0, "ring64x2d", "ring64x2d"),
@@ -239,11 +239,11 @@ ODD = [
     (120, 31, 3000, 0, 0, "skinny", "skinny"),
     (120, 16, 3000, 3, 0, "skinny", "skinny"),
     (120, 15, 3000, 0, 0, "skinny", "skinny"),
-    (130, 385, 9000, 0, 0, "ring64d", "ring64d"),
+    (130, 385, 9000, 0, 0, "ring128d", "ring64d"),
     (20, 1451, 9000, 0, 0, "skinny", "skinny"),
     (200, 129, 5000, 0, 0, "ring64d", "ring64d"),
     (200, 1153, 5000, 0, 0, "ring128d", "ring64d"),
-    (700, 767, 2051, 0, 1, "ring64", "ring64"),
+    (700, 767, 2051, 0, 1, "ring128", "ring64"),
     (200, 1601, 4000, 0, 3, "ring64x2", "ring128"),
     (300, 1100, 2051, 0, 2, "ring64x2", "ring128"),
     (2900, 1001, 3000, 0, 5, "dma", "dma"),
