@@ -718,8 +718,10 @@ __global__ void __launch_bounds__(512)
 // ---- products between the two: BM x BN tiles, stages of 128 code bytes
 
 // What bounds them is the path that brings the operands into LDS, 16 KB for a 64 x 64 tile and
-// stage (200 x 3200 x 8640: 12.9 us, 110 MB at 70% of the rate that DMA alone reaches), and below
-// one tile to a CU a stage's round trip.
+// stage (200 x 3200 x 8640: 11.5 us, 110 MB at 80% of the rate that DMA alone reaches), and below
+// one tile to a CU a stage's round trip.  (64 bytes of a row to a store instead of 128: 12.3.)
+// REG: rows that do not lie on 16 bytes; a stage is loaded as aligned dwords, waits in registers while
+// the one before is multiplied, and is put together on its way into LDS.
 // KS groups of WGM x WGN waves have a part of K each, with a ring of SLOTS stages of their
 // own, and their sums meet in LDS in the order of K: the chain of stages, each of which
 // costs a round trip and a barrier, is KS times shorter, and a tile that has a CU to
@@ -1026,7 +1028,7 @@ int launch_ring(const Mx4Args &a, hipStream_t st) {
 
 // Codes of rows whose bytes the tile kernels cannot read in place (any address and length)
 // into rows of whole aligned 16 bytes, zeros behind their ends: A's, then each B's (717 and 2051
-// rows of 767 bytes 4 us, of the 11.3 of their product).
+// rows of 767 bytes: 4 us).
 template <int MATS>
 __global__ void __launch_bounds__(256) mx4_pad_k(const Mx4Args a, uint4 *__restrict__ out, int per, int ga, int gb) {
   const int w = (int)blockIdx.x < ga ? 0 : MATS == 2 && (int)blockIdx.x >= ga + gb ? 2 : 1;
