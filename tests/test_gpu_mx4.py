@@ -324,6 +324,18 @@ def test_every_form_with_scales_far_apart(dev, m, kb, n, lo, hi):
     assert ((off <= tol) | (size > 3e38)).all()
 
 
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("shifts", [(0, 0), (4, 0), (1, 0), (0, 3), (2, 8)])
+@pytest.mark.parametrize("pads", [(0, 0), (1, 0), (2, 1), (3, 3), (4, 2)])
+@pytest.mark.parametrize("m, kb, n", [(5, 97, 60), (20, 129, 40), (40, 130, 100), (130, 259, 300), (300, 388, 500)])
+def test_codes_and_scales_at_addresses_of_their_own(dev, gate, m, kb, n, pads, shifts):
+    rng = np.random.default_rng(m + kb)
+    a, *bs = [mx.codes(rng, r, kb) for r in (m, n, n)[:2 + gate]]
+    got = _call(dev, gate, *a, bs, pads, shifts, 3)
+    want, tol = _want(gate, *a, bs)
+    _check(got, want, tol)
+
+
 def test_millions_of_rows(dev):
     import torch
     m, kb = 2_200_000, 3
