@@ -695,10 +695,11 @@ def _mat(fn, name, x, dtype="uint8"):
         p = x.data_ptr()
     except AttributeError:
         return descn(x, 2)
-    d = (p, p, 0, *x.shape, *x.stride())
-    if len(d) != 7:
-        raise ValueError(f"expected a rank-2 tensor, got shape {tuple(x.shape)}")
-    return d
+    try:
+        (rows, cols), (s0, s1) = x.shape, x.stride()
+    except ValueError:
+        raise ValueError(f"expected a rank-2 tensor, got shape {tuple(x.shape)}") from None
+    return p, p, 0, rows, cols, s0, s1
 
 
 def quantize_mx4(x, codes, scales):
