@@ -1136,8 +1136,9 @@ int launch_mx4(const Mx4Args &a, hipStream_t st) {
   uintptr_t base = (uintptr_t)a.a, rows = (uintptr_t)a.lda | (uintptr_t)a.kb;
   for (int t = 0; t < MATS; t++) base |= (uintptr_t)a.b[t], rows |= (uintptr_t)a.ldb[t];
   const bool near = std::max({a.lda, a.ldb[0], a.ldb[MATS - 1]}) < (1 << 23);
-  const Choice c = pick<MATS>(a, num_cus(), near && ((base | rows) & 15) == 0 ? kDirect
-                                            : near && (base & 3) == 0 && a.kb >= 16 ? kDwords : kPadded);
+  const Rows can = near && ((base | rows) & 15) == 0 ? kDirect
+                   : near && (base & 3) == 0 && a.kb >= 16 ? kDwords : kPadded;
+  const Choice c = pick<MATS>(a, num_cus(), can);
   if (c.form != kSkinny && a.kb > 0) {
     if (c.rows == kDirect) {
       if (launch_tiles<MATS, false>(a, c.form, st, &rc)) return rc;
@@ -1162,6 +1163,7 @@ int launch_mx4(const Mx4Args &a, hipStream_t st) {
           o.b[t] = (const uint8_t *)(q + ca + t * cb), o.ldb[t] = 16 * (int64_t)per;
         if (launch_tiles<MATS, false>(o, c.form, st, &rc)) return rc;
       }
+      if (can == kDwords && launch_tiles<MATS, true>(a, c.form, st, &rc)) return rc;  // no room for copies
     }
   }
   if (a.M <= 16) return launch_skinny<1, 1, MATS>(a, st);
