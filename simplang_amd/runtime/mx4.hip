@@ -1188,6 +1188,7 @@ struct Mat {
   }
   T *data() const { return p + off; }
   size_t bytes() const { return (size_t)span * sizeof(T); }
+  void rows_of(Operand &o) const { o.set_rows(1, 0, s[0], st[0] * (int64_t)sizeof(T), (size_t)s[1] * sizeof(T)); }
 };
 
 // Whether two arrays share an element: ranges that meet do not where both have rows of
@@ -1323,6 +1324,7 @@ int32_t simp_rt_quantize_mx4(
       (rc = bind_here(oc, mc.data(), mc.bytes(), Operand::kOut, dev, "codes")) ||
       (rc = bind_here(os, ms.data(), ms.bytes(), Operand::kOut, dev, "scales")))
     return rc;
+  mc.rows_of(oc), ms.rows_of(os);  // they may lie between each other's
   auto kernel = bl.run == 1 ? quantize_mx4_k<1, false>
                 : streams(ox.dev(), mx.st[0], x_s0 * x_s1) ? quantize_mx4_k<4, true> : quantize_mx4_k<4, false>;
   hipLaunchKernelGGL(kernel, dim3(bl.grid), dim3(256), 0, cur_stream(), (const float *)ox.dev(), mx.st[0],

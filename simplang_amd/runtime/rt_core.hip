@@ -10,8 +10,10 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <vector>
 
@@ -222,8 +224,27 @@ int Operand::bind(const void *p, size_t bytes, Dir dir, const char *name, bool s
   return SIMP_RT_OK;
 }
 
+void Operand::set_rows(int64_t n0, int64_t st0, int64_t n1, int64_t st1, size_t row) {
+  rows_[0] = n0, rows_[1] = n1, row_st_[0] = st0, row_st_[1] = st1, row_ = row;
+}
+
 int Operand::commit() {
   if (!staged_ || !(dir_ & kOut) || bytes_ == 0) return SIMP_RT_OK;
+  if (row_ && (size_t)(rows_[0] * rows_[1]) * row_ < bytes_) {
+    // The bytes between the rows came in with the stage: they are what the caller had before
+    // the call, and another output of it may be there by now.
+    std::unique_ptr<char, void (*)(void *)> all((char *)std::malloc(bytes_), std::free);
+    if (!all) return set_error(SIMP_RT_ENOMEM, "staging %zu bytes back: out of host memory", bytes_);
+    SIMP_HIP(hipMemcpyAsync(all.get(), dev_, bytes_, hipMemcpyDeviceToHost, cur_stream()));
+    SIMP_HIP(hipStreamSynchronize(cur_stream()));
+    char *host = (char *)const_cast<void *>(host_);
+    for (int64_t i = 0; i < rows_[0]; i++)
+      for (int64_t j = 0; j < rows_[1]; j++) {
+        const int64_t at = i * row_st_[0] + j * row_st_[1];
+        std::memcpy(host + at, all.get() + at, row_);
+      }
+    return SIMP_RT_OK;
+  }
   SIMP_HIP(hipMemcpyAsync(const_cast<void *>(host_), dev_, bytes_,
                           hipMemcpyDeviceToHost, cur_stream()));
   return SIMP_RT_OK;

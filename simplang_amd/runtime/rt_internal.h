@@ -50,13 +50,17 @@ class Operand {
   bool staged() const { return staged_; }
   // The GPU that the caller's device memory lies on; -1 for anything else.
   int device() const { return device_; }
+  // Says that an output is n0 x n1 rows of `row` bytes, st0 and st1 bytes apart: commit() then
+  // leaves the host bytes between them alone, where a call's other output may lie.
+  void set_rows(int64_t n0, int64_t st0, int64_t n1, int64_t st1, size_t row);
   // Copies a staged output back to its host range (on the current stream).
   int commit();
 
  private:
   const void *host_ = nullptr;
   void *dev_ = nullptr;
-  size_t bytes_ = 0;
+  size_t bytes_ = 0, row_ = 0;  // row_: of rows_, 0 without
+  int64_t rows_[2] = {0, 0}, row_st_[2] = {0, 0};
   Dir dir_ = kIn;
   bool staged_ = false;
   int device_ = -1;

@@ -484,6 +484,34 @@ def test_host_arrays(dev):
     _check(sa.swiglu_mx4(*X, *W, *W, np.empty((5, 17), F)), *mx.gated(g, tg, g, tg))
 
 
+@pytest.mark.parametrize("m, k", [(1, 64), (2, 32), (4, 64), (7, 100), (33, 3199), (700, 1533)])
+@pytest.mark.parametrize("torch_tensors", [False, True])
+def test_codes_and_scales_in_one_host_array(dev, m, k, torch_tensors):
+    """Rows of codes and of scales between each other in plain host memory, either first, next to
+    each other and apart: every row is there, and the bytes between them stay."""
+    import torch
+    rng = np.random.default_rng(m)
+    x = _x(rng, m, k)
+    codes, scales = mx.quantize(x)
+    nc, ns = codes.shape[1], scales.shape[1]
+    for at_c, at_s, width in ((0, nc, nc + ns), (ns, 0, nc + ns), (1, nc + 3, nc + ns + 8), (ns + 5, 2, nc + ns + 6)):
+        before = rng.integers(0, 256, (m, width)).astype(U)
+        buf = before.copy()
+        c, s = buf[:, at_c:at_c + nc], buf[:, at_s:at_s + ns]
+        want = before.copy()
+        want[:, at_c:at_c + nc], want[:, at_s:at_s + ns] = codes, scales
+        if torch_tensors:
+            b = torch.from_numpy(buf)
+            sa.quantize_mx4(torch.from_numpy(x), b[:, at_c:at_c + nc], b[:, at_s:at_s + ns])
+        else:
+            sa.quantize_mx4(x, c, s)
+        assert np.array_equal(buf, want), (at_c, at_s, np.argwhere(buf != want)[:3])
+        # and read from there, into rows of which the ends belong to someone else
+        out = np.full((m, k + 3), 7, F)
+        sa.dequantize_mx4(c, s, out[:, :k])
+        assert np.array_equal(out[:, :k], mx.values(codes, scales)[:, :k]) and (out[:, k:] == 7).all()
+
+
 def test_rows_far_apart(dev):
     """Rows whose offsets pass 32 bits, in every operand."""
     import torch
