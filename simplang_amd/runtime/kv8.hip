@@ -1269,6 +1269,7 @@ int32_t simp_rt_kv8_read(
       (rc = bind_here(os, starts + st_off, 4 * (size_t)st_size, Operand::kIn, dev, "starts")) ||
       (rc = bind_here(ol, lengths + len_off, 4 * (size_t)len_size, Operand::kIn, dev, "lengths")))
     return rc;
+  dk.rows_of(ok), dv.rows_of(ov);  // they may lie between each other's
   const ReadArgs a{bc.c, (const int *)os.dev(), (const int *)ol.dev(), (float *)ok.dev(),
                    (float *)ov.dev(), dk.st[0], dk.st[1], dv.st[0], dv.st[1], (int)k_s0};
   const dim3 grid((unsigned)cdiv(k_s0, kReadRows), (unsigned)bc.c.hk);

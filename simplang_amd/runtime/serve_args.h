@@ -26,6 +26,10 @@ struct Desc3 {
   bool is(int64_t a, int64_t b, int64_t c) const { return s[0] == a && s[1] == b && s[2] == c; }
   T *data() const { return p + off; }
   size_t bytes() const { return (size_t)span * sizeof(T); }
+  void rows_of(Operand &o) const {
+    constexpr int64_t n = sizeof(T);
+    o.set_rows(s[0], st[0] * n, s[1], st[1] * n, (size_t)(s[2] * n));
+  }
 };
 
 // The kernels take the scale in fp32, times log2(e) for powers of two.

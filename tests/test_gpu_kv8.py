@@ -573,6 +573,24 @@ def test_read_into_parts_of_one_tensor(dev):
         assert np.array_equal(kt.cpu().numpy(), k) and np.array_equal(vt.cpu().numpy(), v)
 
 
+def test_read_into_parts_of_one_host_array(dev):
+    """The same in host memory: neither part's way back goes over the other."""
+    import torch
+    p = Pair(dev, 2, 3, 40, 32, 16)
+    st, ln = S.starts([9, 20]), np.array([30, 33], np.int32)
+    p.append(*_rows(29, 3, 32), [9, 20], ln)
+    k, v = np.zeros((29, 3, 32), np.float32), np.zeros((29, 3, 32), np.float32)
+    p.np.read(st, ln, k, v)
+    for shape, axis in (((29, 2, 3, 32), 1), ((29, 3, 2, 32), 2)):
+        x = np.full(shape[:-1] + (35,), 8, np.float32)  # three elements behind each head stay
+        kt, vt = (np.moveaxis(x, axis, 0)[i][..., :32] for i in (0, 1))
+        p.gpu.read(st, ln, kt, vt)
+        assert np.array_equal(kt, k) and np.array_equal(vt, v) and (x[..., 32:] == 8).all()
+        y = torch.full(shape, 8.0)
+        p.gpu.read(torch.from_numpy(st), torch.from_numpy(ln), *y.unbind(axis)[::-1])
+        assert np.array_equal(y.select(axis, 1).numpy(), k) and np.array_equal(y.select(axis, 0).numpy(), v)
+
+
 def test_read_over_many_empty_sequences(dev):
     import torch
     n = 3000
