@@ -296,8 +296,9 @@ int32_t simp_rt_matmul_mx4(
 
 /* The gated half of a feed-forward block in one kernel: out[M,N] = silu(A W1^T) * (A W3^T)
  * for A[M,K], W1[N,K] and W3[N,K] in MX4, silu(x) = x / (1 + exp(-x)): of the two products
- * that simp_rt_matmul_mx4 gives, within 9 * 2^-24 (0 for x below -87, where silu is
- * less than 2^-119; NaN for -inf, as in simp_rt_swiglu). */
+ * that simp_rt_matmul_mx4 gives, within 9 * 2^-24 of the result and 2^-148 of the second
+ * product, as long as exp(-x) is finite in fp32 (0 for x below -88.7228394, where silu is
+ * less than 2^-121; NaN for -inf, as in simp_rt_swiglu). */
 int32_t simp_rt_swiglu_mx4(
     const uint8_t *a_alloc, const uint8_t *a, int64_t a_off, int64_t a_s0, int64_t a_s1, int64_t a_st0, int64_t a_st1,
     const uint8_t *as_alloc, const uint8_t *a_scales, int64_t as_off, int64_t as_s0, int64_t as_s1, int64_t as_st0, int64_t as_st1,

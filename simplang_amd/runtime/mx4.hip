@@ -201,15 +201,17 @@ __device__ __forceinline__ v4f mfma_mx4(uint4 a, uint32_t sa, uint4 b, uint32_t 
 }
 
 // silu(g) * u = g / (1 + exp(-g)) * u within 8 half units: with t = fl(x log2(e)), exp(x) is
-// 2^t (1 + x - t ln 2), which leaves the rounding of t (it would count |x| times) out.  Above
-// x = 88.7228394, the first for which t reaches 128, exp is infinite and silu 0.  A gate costs
-// what its instructions do, 64 to a lane and tile with the matrix cores idle: with expf and a
-// division 4096 x 2048 x 8192 takes 100 us in the 256 x 256 tiles, not 87.
+// 2^t (1 + x - t ln 2), which leaves the rounding of t (it would count |x| times) out.  From
+// x = 88.7228394 on, the first for which t reaches 128, exp is infinite and silu 0.  Quarters of
+// g and of the divisor: the reciprocal of a number above 2^126 is subnormal, and comes out as 0.
+// A gate costs what its instructions do, 64 to a lane and tile with the matrix cores idle:
+// 4096 x 2048 x 8192 takes 87 us in the 256 x 256 tiles, with expf and a division 98, with a
+// Newton step for the reciprocal 90 (error in the 2-norm 5.25e-8, 4.95e-8, 5.20e-8).
 __device__ __forceinline__ float swiglu(float g, float u) {
   const float x = __builtin_amdgcn_fmed3f(-g, -200.f, 88.7228394f), t = x * 1.44269504f;
   const float low = fmaf(-t, -1.90465421e-9f, fmaf(-t, 0.693147182f, x));  // ln 2 in two parts
   const float p = __builtin_amdgcn_exp2f(t), e = fmaf(p, low, p);
-  return g * __builtin_amdgcn_rcpf(1.f + e) * u;
+  return 0.25f * g * __builtin_amdgcn_rcpf(fmaf(e, 0.25f, 0.25f)) * u;
 }
 
 // Exchanges registers and lanes: of n = 2 or 4 neighbouring lanes, lane t gets in y[s] what

@@ -471,6 +471,55 @@ def test_gate_where_exp_overflows(dev):
                 break
 
 
+@pytest.mark.parametrize("m, n", [(5, 1), (1025, 1), (1025, 300), (1025, 6000)])
+def test_gate_keeps_what_a_large_factor_brings_back(dev, m, n):
+    """g = -96 to -80 as above with u = +-2^120: silu is 2^-108 to 2^-122 and normal in fp32, and zero
+    only where exp(-g) overflows (-88.7228394).  The bound is the gate's own roundings, and
+    two for the halves of the smallest subnormal in g / 4 and in silu."""
+    import torch
+    d = np.arange(80 * 64, 96 * 64 + 1)[-m:] if m > 5 else np.array([5595, 5620, 5650, 5678, 5679])
+    digits = d[:, None] >> np.arange(12, -1, -1) & 1
+    a, s = np.zeros((m, 13 * 16), U), np.tile(127 + 6 - np.arange(13), (m, 1)).astype(U)
+    a[:, ::16] = 2 * digits                           # 1.0
+    w1, w3 = np.zeros((n, 13 * 16), U), np.zeros((n, 13 * 16), U)
+    t, t3 = np.full((n, 13), 127, U), np.full((n, 13), 127 + 114, U)
+    sign = np.where(np.arange(n) % 3 == 1, -1, 1)
+    w1[:, ::16], w3[:, 0] = 10, np.where(sign < 0, 10, 2)  # -1.0; 64 (every d has that digit) times 2^114
+    on = [torch.from_numpy(v).to(dev) for v in (a, s, w1, t, w3, t3)]
+    out = sa.swiglu_mx4(*on, torch.full((m, n), 3.0, device=dev)).double()
+    g = torch.from_numpy(-d / 64).to(dev)
+    u = torch.from_numpy(sign * 2.0 ** 120).to(dev)
+    silu = g / (1 + torch.exp(-g)) * (g > -88.7228394)
+    want = silu[:, None] * u
+    assert ((out - want).abs() <= mx.GATE * mx.EPS * want.abs() + 2.0 ** -148 * u.abs()).all()
+
+
+@pytest.mark.parametrize("m, n", [(3, 700), (1500, 700), (1500, 4000)])
+def test_gate_over_its_range(dev, m, n):
+    """g from -128 to 128 and down to 2^-36, u from 2^-100 to 2^19."""
+    import torch
+    rng = np.random.default_rng(m + n)
+    # g = the sum of 13 digits times 2^(6 - j), exact; columns turn the sign and scale it by 2^-c
+    d = rng.integers(0, 2 ** 13, m)
+    a, s = np.zeros((m, 14 * 16), U), np.tile(127 + 6 - np.arange(14), (m, 1)).astype(U)
+    a[:, :13 * 16:16] = 2 * (d[:, None] >> np.arange(12, -1, -1) & 1)
+    a[:, 13 * 16], s[:, 13] = 2, 127                  # 1.0: u's
+    w1, w3 = np.zeros((n, 14 * 16), U), np.zeros((n, 14 * 16), U)
+    t, t3 = np.full((n, 14), 127, U), np.full((n, 14), 127, U)
+    minus = rng.random(n) < 0.6
+    c = rng.integers(0, 31, n) * (rng.random(n) < 0.7)
+    w1[:, :13 * 16:16] = np.where(minus, 10, 2)[:, None]
+    t[:] = 127 - c[:, None]
+    e = rng.integers(-100, 20, n)
+    w3[:, 13 * 16], t3[:] = 2, (127 + e)[:, None]
+    on = [torch.from_numpy(v).to(dev) for v in (a, s, w1, t, w3, t3)]
+    out = sa.swiglu_mx4(*on, torch.full((m, n), 3.0, device=dev)).double()
+    g = torch.from_numpy(np.where(minus, -1, 1) * 2.0 ** -c * (d / 64)[:, None]).to(dev)
+    u = torch.from_numpy(2.0 ** e).to(dev)
+    want = g / (1 + torch.exp(-g)) * (g > -88.7228394) * u
+    assert ((out - want).abs() <= mx.GATE * mx.EPS * want.abs() + 2.0 ** -148 * u.abs() + 2.0 ** -150).all()
+
+
 def test_host_arrays(dev):
     rng = np.random.default_rng(5)
     x, w = rng.standard_normal((5, 100)).astype(F), rng.standard_normal((17, 100)).astype(F)
