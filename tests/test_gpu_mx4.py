@@ -68,6 +68,40 @@ def test_quantize_and_back(dev, m, k):
             assert (whole[:, n:] == f).all() and (buf._base[:shift] == f).all()
 
 
+# sizes with more than 2^15 blocks of 32, in four blocks to a thread, the last workgroup's not all
+# there: small rows and long ones, rows that end inside a block, a byte and four elements
+MANY = [(717, 1533), (33000, 30), (1100, 1024), (5, 250007)]
+# 2^24 elements and more, values past the caches where rows lie on 16 bytes: rows of 4099 elements 4100
+# apart and of 4096; the same where the rows' stride or the first row is off 16 bytes
+LARGE = [(4100, 4099, 1, 0), (4100, 4099, 5, 0), (4100, 4096, 0, 4), (4100, 4099, 2, 0), (4100, 4099, 1, 1),
+         (4100, 4096, 0, 3), (17_000_000, 1, 3, 0)]
+
+
+@pytest.mark.parametrize("m, k, pad, shift", [(m, k, *p) for m, k in MANY for p in ((0, 0), (3, 1), (32, 16))] + LARGE)
+def test_quantize_and_back_of_many_blocks(dev, m, k, pad, shift):
+    import torch
+    rng = np.random.default_rng(m + k)
+    some = min(m, 3000)  # rows of their own; the others repeat them
+    x = _x(rng, some, k)
+    codes, scales = mx.quantize(x)
+    vals = mx.values(codes, scales)[:, :k].astype(F)
+    idx = torch.from_numpy(rng.integers(0, some, m)).to(dev)
+
+    def rows(v, fill):
+        buf = torch.full((shift + m * (v.shape[1] + pad) + 1,), fill, dtype=torch.from_numpy(v).dtype, device=dev)
+        return buf, buf[shift:-1].view(m, -1)[:, :v.shape[1]]
+
+    _, dx = rows(x, 9)
+    dx.copy_(torch.from_numpy(x).to(dev)[idx])
+    outs = [rows(v, f) for v, f in ((codes, 77), (scales, 78), (vals, 5))]
+    sa.quantize_mx4(dx, outs[0][1], outs[1][1])
+    sa.dequantize_mx4(outs[0][1], outs[1][1], outs[2][1])
+    for (buf, got), want, f in zip(outs, (codes, scales, vals), (77, 78, 5)):
+        assert torch.equal(got, torch.from_numpy(want).to(dev)[idx])
+        gaps = buf[shift:-1].view(m, -1)[:, want.shape[1]:]
+        assert (gaps == f).all() and (buf[:shift] == f).all() and (buf[-1] == f).all()
+
+
 def test_quantize_marks_blocks_that_are_not_finite(dev):
     import torch
     x = np.ones((6, 100), F)
