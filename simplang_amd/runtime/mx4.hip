@@ -55,15 +55,14 @@ __device__ __forceinline__ float scale_of(uint32_t s) {
   return __uint_as_float(s ? s << 23 : 0x00400000u);
 }
 
-// Row and column block of the i-th 32-element block of the rows, i counted from the
-// workgroup's first (per_row below 2^31).
+// Row and column block of the i-th 32-element block (or 16-byte piece) of the rows, i counted from
+// the workgroup's first, which is below 2^31 (the callers hold the grid to it), as is per_row.
 struct BlockAt {
   int64_t row0;
   uint32_t rem, per;
   __device__ BlockAt(int64_t first, int64_t per_row) {
     per = (uint32_t)per_row;
-    if ((uint64_t)first >> 32 == 0) row0 = (uint32_t)first / per;
-    else row0 = first / per_row;
+    row0 = (uint32_t)first / per;
     rem = (uint32_t)(first - row0 * per_row);
   }
   __device__ void get(uint32_t i, int64_t &row, int64_t &blk) const {
@@ -258,7 +257,7 @@ __device__ __forceinline__ uint4 row_shift(uint4 v, int k, int kb) {
   return kb >= 16 ? shift_down(v, min(max(k - kb + 16, 0), 16)) : v;
 }
 
-// 16 NT columns of each matrix and all 16 MT rows to a block, whose waves split K: a wave
+// 16 columns of each matrix and all 16 MT rows to a block, whose waves split K: a wave
 // takes every byte of its rows' piece once, straight from memory into the lanes that
 // feed the matrix instruction (16 rows of 64 bytes, and a byte of scales to a lane), and
 // the waves' sums meet in LDS, in the order of K.  SHIFT: rows of scales (1), of codes too (2),
@@ -266,16 +265,16 @@ __device__ __forceinline__ uint4 row_shift(uint4 v, int k, int kb) {
 // they lie; 16 x 8640 x 3200, where only the scales are not, 6.6).  Memory bounds it, 1 x 3200 x 32000:
 // 10.0 us, 5.4 TB/s of weights that lie in the last cache; 16 x 3200 x 8640 gated 7.6.
 constexpr int skinny_waves(int MT, int MATS) { return MT * MATS >= 4 ? 8 : 16; }  // of a block at most
-template <int MT, int NT, int MATS, int SHIFT>
+template <int MT, int MATS, int SHIFT>
 __global__ void __launch_bounds__(64 * skinny_waves(MT, MATS)) mx4_skinny_k(const Mx4Args a, int span, int blocks_n) {
-  constexpr int T = MATS * MT * NT;
+  constexpr int T = MATS * MT;
   constexpr int U = MT == 4 ? 2 : 4;
   extern __shared__ v4f part[];  // [waves][T][64]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int r = lane & 15, q = lane >> 4;
   const int bm = blockIdx.x / blocks_n;
-  const int n0 = 16 * NT * (blockIdx.x - bm * blocks_n), m0 = 16 * MT * bm;
-  const uint8_t *ap[MT], *as[MT], *bp[MATS][NT], *bs[MATS][NT];
+  const int n0 = 16 * (blockIdx.x - bm * blocks_n), m0 = 16 * MT * bm;
+  const uint8_t *ap[MT], *as[MT], *bp[MATS], *bs[MATS];
   bool in[MT];  // rows behind the last are not asked for
 #pragma unroll
   for (int i = 0; i < MT; i++) {
@@ -284,31 +283,24 @@ __global__ void __launch_bounds__(64 * skinny_waves(MT, MATS)) mx4_skinny_k(cons
     ap[i] = a.a + m * a.lda, as[i] = a.as + m * a.ldas;
   }
 #pragma unroll
-  for (int t = 0; t < MATS; t++)
-#pragma unroll
-    for (int j = 0; j < NT; j++) {
-      const int64_t n = min(n0 + 16 * j + r, a.N - 1);
-      bp[t][j] = a.b[t] + n * a.ldb[t], bs[t][j] = a.bs[t] + n * a.ldbs[t];
-    }
-  v4f acc[MATS][MT][NT];
+  for (int t = 0; t < MATS; t++) {
+    const int64_t n = min(n0 + r, a.N - 1);
+    bp[t] = a.b[t] + n * a.ldb[t], bs[t] = a.bs[t] + n * a.ldbs[t];
+  }
+  v4f acc[MATS][MT];
 #pragma unroll
   for (int t = 0; t < MATS; t++)
 #pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-      for (int j = 0; j < NT; j++) acc[t][i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < MT; i++) acc[t][i] = v4f{0.f, 0.f, 0.f, 0.f};
   struct Step {
-    uint4 a[MT], b[MATS][NT];
-    uint32_t as[MT], bs[MATS][NT];
+    uint4 a[MT], b[MATS];
+    uint32_t as[MT], bs[MATS];
   };
   auto run = [&](const Step &s) {
 #pragma unroll
     for (int t = 0; t < MATS; t++)
 #pragma unroll
-      for (int i = 0; i < MT; i++)
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-          acc[t][i][j] = mfma_mx4(s.b[t][j], s.bs[t][j], s.a[i], s.as[i], acc[t][i][j]);
+      for (int i = 0; i < MT; i++) acc[t][i] = mfma_mx4(s.b[t], s.bs[t], s.a[i], s.as[i], acc[t][i]);
   };
   // Four steps: a lane's four scale bytes come out of 16 of its row.  What bounds the loop is
   // the path from the caches, 64 bytes a cycle and a row to a cycle: a byte of scales for
@@ -328,11 +320,9 @@ __global__ void __launch_bounds__(64 * skinny_waves(MT, MATS)) mx4_skinny_k(cons
         if (SHIFT == 2 || s + u < end) w[u] = row[min(4 * (s + u) + q, nb - 1)];
       return make_uint4(w[0], w[1], w[2], w[3]);
     };
-    uint4 sa[MT], sb[MATS][NT];
+    uint4 sa[MT], sb[MATS];
 #pragma unroll
-    for (int t = 0; t < MATS; t++)
-#pragma unroll
-      for (int j = 0; j < NT; j++) sb[t][j] = scales(bs[t][j]);
+    for (int t = 0; t < MATS; t++) sb[t] = scales(bs[t]);
 #pragma unroll
     for (int i = 0; i < MT; i++) {
       sa[i] = make_uint4(0, 0, 0, 0);
@@ -347,9 +337,7 @@ __global__ void __launch_bounds__(64 * skinny_waves(MT, MATS)) mx4_skinny_k(cons
         // (a load that is put together here would be waited for here)
         if (E && SHIFT != 2 && s + h + u >= end) break;
 #pragma unroll
-        for (int t = 0; t < MATS; t++)
-#pragma unroll
-          for (int j = 0; j < NT; j++) x[u].b[t][j] = load(bp[t][j], k, a.kb);
+        for (int t = 0; t < MATS; t++) x[u].b[t] = load(bp[t], k, a.kb);
 #pragma unroll
         for (int i = 0; i < MT; i++) {
           x[u].a[i] = make_uint4(0, 0, 0, 0);
@@ -363,24 +351,18 @@ __global__ void __launch_bounds__(64 * skinny_waves(MT, MATS)) mx4_skinny_k(cons
           return (h + u == 0 ? v.x : h + u == 1 ? v.y : h + u == 2 ? v.z : v.w) >> (E ? 0 : 8 * q);
         };
 #pragma unroll
-        for (int t = 0; t < MATS; t++)
-#pragma unroll
-          for (int j = 0; j < NT; j++) x[u].bs[t][j] = byte(sb[t][j]);
+        for (int t = 0; t < MATS; t++) x[u].bs[t] = byte(sb[t]);
 #pragma unroll
         for (int i = 0; i < MT; i++) x[u].as[i] = byte(sa[i]);
         if (E == 1 && 64 * (s + h + u + 1) > a.kb) {
           const int k = 64 * (s + h + u) + 16 * q;
 #pragma unroll
-          for (int t = 0; t < MATS; t++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) x[u].b[t][j] = row_shift(x[u].b[t][j], k, a.kb);
+          for (int t = 0; t < MATS; t++) x[u].b[t] = row_shift(x[u].b[t], k, a.kb);
 #pragma unroll
           for (int i = 0; i < MT; i++) x[u].a[i] = row_shift(x[u].a[i], k, a.kb);
           // (a block behind the end must not bring the last one's scale, which may be NaN)
 #pragma unroll
-          for (int t = 0; t < MATS; t++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) x[u].bs[t][j] = k < a.kb ? x[u].bs[t][j] : 127;
+          for (int t = 0; t < MATS; t++) x[u].bs[t] = k < a.kb ? x[u].bs[t] : 127;
 #pragma unroll
           for (int i = 0; i < MT; i++) x[u].as[i] = k < a.kb ? x[u].as[i] : 127;
         }
@@ -399,29 +381,24 @@ __global__ void __launch_bounds__(64 * skinny_waves(MT, MATS)) mx4_skinny_k(cons
 #pragma unroll
     for (int t = 0; t < MATS; t++)
 #pragma unroll
-      for (int i = 0; i < MT; i++)
-#pragma unroll
-        for (int j = 0; j < NT; j++) part[(wave * T + (t * MT + i) * NT + j) * 64 + lane] = acc[t][i][j];
+      for (int i = 0; i < MT; i++) part[(wave * T + t * MT + i) * 64 + lane] = acc[t][i];
     __syncthreads();
   }
   // a wave stores every `waves`-th 16 x 16 tile
-  for (int o = wave; o < MT * NT; o += waves) {
-    const int i = o / NT, j = o - i * NT;
+  for (int i = wave; i < MT; i += waves) {
     v4f v[MATS];
 #pragma unroll
     for (int t = 0; t < MATS; t++) {
       if (waves > 1) {
-        v[t] = part[((t * MT + i) * NT + j) * 64 + lane];
-        for (int w = 1; w < waves; w++) v[t] += part[(w * T + (t * MT + i) * NT + j) * 64 + lane];
+        v[t] = part[(t * MT + i) * 64 + lane];
+        for (int w = 1; w < waves; w++) v[t] += part[(w * T + t * MT + i) * 64 + lane];
       } else {
 #pragma unroll
         for (int ii = 0; ii < MT; ii++)
-#pragma unroll
-          for (int jj = 0; jj < NT; jj++)
-            if (ii == i && jj == j) v[t] = acc[t][ii][jj];
+          if (ii == i) v[t] = acc[t][ii];
       }
     }
-    const int row = m0 + 16 * i + r, col = n0 + 16 * j + 4 * q;
+    const int row = m0 + 16 * i + r, col = n0 + 4 * q;
     if (row >= a.M) continue;
     v4f y = v[0];
     if constexpr (MATS == 2) {
@@ -439,12 +416,12 @@ __global__ void __launch_bounds__(64 * skinny_waves(MT, MATS)) mx4_skinny_k(cons
   }
 }
 
-template <int MT, int NT, int MATS>
+template <int MT, int MATS>
 int launch_skinny(Mx4Args a, hipStream_t st) {
-  const int64_t bn = cdiv(a.N, 16 * NT), bm = cdiv(a.M, 16 * MT);
+  const int64_t bn = cdiv(a.N, 16), bm = cdiv(a.M, 16 * MT);
   // about twelve waves to a CU, up to 16 to a block (64 KiB of sums)
   const int steps = (a.kb + 63) >> 6;
-  int waves = (int)std::min<int64_t>({cdiv(12 * num_cus(), bn * bm), skinny_waves(MT, MATS), std::max(steps, 1), 64 / (MATS * MT * NT)});
+  int waves = (int)std::min<int64_t>({cdiv(12 * num_cus(), bn * bm), skinny_waves(MT, MATS), std::max(steps, 1), 64 / (MATS * MT)});
   const int span = (int)cdiv(cdiv(steps, waves), 4) * 4;
   if (span) waves = (int)cdiv(steps, span);
   // a launch has below 2^31 threads: in turn, runs of column blocks, and of row blocks where
@@ -454,14 +431,14 @@ int launch_skinny(Mx4Args a, hipStream_t st) {
   for (int64_t i = 0; i < bm; i += rb) {
     for (int64_t j = 0; j < bn; j += cb) {
       Mx4Args c = a;
-      const int64_t row = 16 * MT * i, col = 16 * NT * j;
-      const int64_t rows = std::min(16 * MT * rb, a.M - row), cols = std::min(16 * NT * cb, a.N - col);
+      const int64_t row = 16 * MT * i, col = 16 * j;
+      const int64_t rows = std::min(16 * MT * rb, a.M - row), cols = std::min(16 * cb, a.N - col);
       c.a += row * a.lda, c.as += row * a.ldas, c.out += row * a.ldo + col, c.M = (int)rows, c.N = (int)cols;
       for (int t = 0; t < MATS; t++) c.b[t] += col * a.ldb[t], c.bs[t] += col * a.ldbs[t];
-      const int64_t blocks_n = cdiv(cols, 16 * NT);
-      hipLaunchKernelGGL((a.shift_codes ? mx4_skinny_k<MT, NT, MATS, 2> : a.shift ? mx4_skinny_k<MT, NT, MATS, 1> : mx4_skinny_k<MT, NT, MATS, 0>),
+      const int64_t blocks_n = cdiv(cols, 16);
+      hipLaunchKernelGGL((a.shift_codes ? mx4_skinny_k<MT, MATS, 2> : a.shift ? mx4_skinny_k<MT, MATS, 1> : mx4_skinny_k<MT, MATS, 0>),
                          dim3((unsigned)(blocks_n * cdiv(rows, 16 * MT))), dim3(64 * waves),
-                         waves > 1 ? waves * MATS * MT * NT * 1024 : 0, st, c, span, (int)blocks_n);
+                         waves > 1 ? waves * MATS * MT * 1024 : 0, st, c, span, (int)blocks_n);
       SIMP_HIP(hipGetLastError());
     }
   }
@@ -1168,9 +1145,9 @@ int launch_mx4(const Mx4Args &a, hipStream_t st) {
       if (can == kDwords && launch_tiles<MATS, true>(a, c.form, st, &rc)) return rc;  // no room for copies
     }
   }
-  if (a.M <= 16) return launch_skinny<1, 1, MATS>(a, st);
-  if (a.M <= 32) return launch_skinny<2, 1, MATS>(a, st);
-  return launch_skinny<4, 1, MATS>(a, st);
+  if (a.M <= 16) return launch_skinny<1, MATS>(a, st);
+  if (a.M <= 32) return launch_skinny<2, MATS>(a, st);
+  return launch_skinny<4, MATS>(a, st);
 }
 
 // ------------------------------------------------------------- entry points
