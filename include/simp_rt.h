@@ -261,9 +261,12 @@ int32_t simp_rt_matmul_w4s(
  * shorter): s stands for 2^(s - 127), 255 for NaN, and an element for its code's
  * value times that.  All rows may be strided, at any alignment.  Outputs share no
  * element with another operand (rows of one array may lie between another's).  Products of
- * many rows use device scratch where they have it: a captured call to which no call of its
- * size on the stream has left some goes on without, slower, and may add the same products
- * up in another order.  Equal calls give equal bits, as do replays of one graph. */
+ * many rows use device scratch where they have it, which the library keeps (for each stream
+ * up to 4 GiB of copies of rows that do not lie on 16 bytes, made anew by every call, and a copy of
+ * the scales): a captured call to which no call of its size on the stream has left some
+ * goes on without, slower, and may add the same products up in another order.  Equal calls
+ * give equal bits, as do replays of one graph.  Dimensions up to 2^31 - 4097; fewer
+ * than 2^30 - 127 blocks in a call that quantises, or back. */
 
 /* Codes and scales of fp32 rows x[rows, cols].  With m = max|x| of a block, its scale
  * is 2^e, e = max(floor(log2 m) - 2, -127) (byte 0 for a block of zeros), and a code is

@@ -76,7 +76,10 @@ struct BlockAt {
 // 1 KB in lane order; a thread takes RUN blocks, their loads together.  STREAM: values are
 // taken and left past the caches (they lie on 16 bytes).  8192 x 8192: 59 us (5.1 TB/s) and
 // back 44 us (6.9; a copy reaches 4.9); with eight elements to a lane, 32 bytes apart, 75
-// and 78.  RUN = 4 for many blocks, 1 where few leave CUs idle (one row of 3200: 1.9 us, not 2.7).
+// and 78.  RUN: 1 to 2^15 blocks, where few leave CUs idle (in a graph 1 x 3200: 2.3 us and back
+// 2.5, with 4 3.2 and 3.1; 1024 x 992: 2.8 and 3.1, with 4 3.7 and 3.9), above it 4, which the
+// largest are better with (4096 x 4096 back: 12.4 us, with 1 13.6; 8192 x 8192 44, with 1 68, not past
+// the caches).  Just above 2^15 it costs a microsecond (717 x 1533: 4.1 and 4.1, with 1 3.1 and 3.4).
 template <int RUN, bool STREAM>
 __global__ void __launch_bounds__(256)
     quantize_mx4_k(const float *__restrict__ x, int64_t ldx, uint8_t *__restrict__ codes,
@@ -697,8 +700,9 @@ __global__ void __launch_bounds__(512)
 // ---- products between the two: BM x BN tiles, stages of 128 code bytes
 
 // What bounds them is the path that brings the operands into LDS, 16 KB for a 64 x 64 tile and
-// stage (200 x 3200 x 8640: 11.5 us, 110 MB at 80% of the rate that DMA alone reaches), and below
-// one tile to a CU a stage's round trip.  (64 bytes of a row to a store instead of 128: 12.3.)
+// stage (200 x 3200 x 8640: 12.2 us a call, 10.9 one behind the other in a graph, 110 MB at about
+// 80% of the rate that DMA alone reaches), and below one tile to a CU a stage's round trip.
+// (64 bytes of a row to a store instead of 128: 11.5 in a graph; 700 rows 27.4, not 26.0.)
 // REG: rows that do not lie on 16 bytes; a stage is loaded as aligned dwords, waits in registers while
 // the one before is multiplied, and is put together on its way into LDS.
 // KS groups of WGM x WGN waves have a part of K each, with a ring of SLOTS stages of their
@@ -1040,6 +1044,8 @@ bool launch_dma(const Mx4Args &a, hipStream_t st, int *rc) {
   // past them; x 26432: 188, 226 into them)
   const int stream = a.N % 16 == 0 && ((uintptr_t)a.out & 63) == 0 && a.ldo % 16 == 0;
   const int64_t grid = std::min<int64_t>(tm * tn, num_cus());
+  // (in a graph, without: 8192^3 270 us, 286; 8192 x 256 x 8192 61, 84; 6000 x 1024 x 6000 53, 55;
+  // gated 4096 x 2048 x 8192 89, 103; 8192 x 768 x 8192 110, 120; 8192 x 256 x 8192 69, 85)
   const int stagger = tm * tn >= 2 * grid && MATS == 1 ? 2 : tm * tn >= 4 * grid ? 1 : 0;
   KernelTimer kt(st, "mx4_dma");
   hipLaunchKernelGGL((mx4_dma_k<MATS>), dim3((unsigned)grid), dim3(512), 0, st, a, pa, pb, (int)tm,
@@ -1051,7 +1057,9 @@ bool launch_dma(const Mx4Args &a, hipStream_t st, int *rc) {
 
 // What each form takes in us, fitted to whole calls (graph replay) of 1 to 8192 rows,
 // K = 768 to 8192 and up to 32000 columns; `steps` of 128 elements.
-// The choice by it is within about 10% of the best form's time.
+// Over 168 products and gates of 1 to 8192 rows the chosen form takes 1% longer than the best one at
+// the median and 9% at the ninetieth percentile; the most are 32% (gated, 300 x 768 x 2048: 7.0 us,
+// 64 x 64 tiles 5.3; 64 x 8192 x 8192: 21.7, K in two parts 16.5).
 enum Form { kSkinny, kRing64, kRing64x2, kRing128, kTiles256 };
 // What the tile kernels make of rows that do not lie on 16 bytes: they read them as dwords
 // (the rings' stages go through registers, and take about twice as long: 60 x 2899 x 23360
@@ -1062,7 +1070,10 @@ struct Choice {
   Form form;
   Rows rows;
 };
-// `can`: kDirect where rows do lie on 16 bytes, kPadded where they cannot be read as dwords.
+// `can`: kDirect where rows do lie on 16 bytes, kPadded where they cannot be read as dwords.  Then
+// the choice is the one of rows in place: the copy comes on top of every form but the few-row one,
+// whose loads take longer in turn (first byte off 4 bytes, 16 x 8640 x 32000: 77 us with the
+// copy, 95 without; 64 x 3200 x 8640 gated 24 and 31; 64 x 3200 x 2800 13 and 11, the wrong one).
 template <int MATS>
 Choice pick(const Mx4Args &a, int64_t cus, Rows can) {
   const double steps = (double)cdiv(a.kb, 64), out = 4e-6 * a.M * a.N / 6.5;
