@@ -1178,6 +1178,7 @@ struct Mat {
   }
   T *data() const { return p + off; }
   size_t bytes() const { return (size_t)span * sizeof(T); }
+  // (an array's rows may lie between those of another output, of this call or of another thread's)
   void rows_of(Operand &o) const { o.set_rows(1, 0, s[0], st[0] * (int64_t)sizeof(T), (size_t)s[1] * sizeof(T)); }
 };
 
@@ -1234,6 +1235,7 @@ int product(const char *fn, Mat<const uint8_t> &a, Mat<const uint8_t> &as,
       (rc = bind_here(oas, as.data(), as.bytes(), Operand::kIn, dev, "a_scales")) ||
       (rc = bind_here(oo, o.data(), o.bytes(), Operand::kOut, dev, "out")))
     return rc;
+  o.rows_of(oo);
   Mx4Args g{};
   g.a = (const uint8_t *)oa.dev(), g.as = (const uint8_t *)oas.dev();
   g.lda = a.st[0], g.ldas = as.st[0];
@@ -1314,7 +1316,7 @@ int32_t simp_rt_quantize_mx4(
       (rc = bind_here(oc, mc.data(), mc.bytes(), Operand::kOut, dev, "codes")) ||
       (rc = bind_here(os, ms.data(), ms.bytes(), Operand::kOut, dev, "scales")))
     return rc;
-  mc.rows_of(oc), ms.rows_of(os);  // they may lie between each other's
+  mc.rows_of(oc), ms.rows_of(os);
   auto kernel = bl.run == 1 ? quantize_mx4_k<1, false>
                 : streams(ox.dev(), mx.st[0], x_s0 * x_s1) ? quantize_mx4_k<4, true> : quantize_mx4_k<4, false>;
   hipLaunchKernelGGL(kernel, dim3(bl.grid), dim3(256), 0, cur_stream(), (const float *)ox.dev(), mx.st[0],
@@ -1353,6 +1355,7 @@ int32_t simp_rt_dequantize_mx4(
       (rc = bind_here(os, ms.data(), ms.bytes(), Operand::kIn, dev, "scales")) ||
       (rc = bind_here(oo, mo.data(), mo.bytes(), Operand::kOut, dev, "out")))
     return rc;
+  mo.rows_of(oo);
   auto kernel = bl.run == 1 ? dequantize_mx4_k<1, false>
                 : streams(oo.dev(), mo.st[0], out_s0 * out_s1) ? dequantize_mx4_k<4, true> : dequantize_mx4_k<4, false>;
   hipLaunchKernelGGL(kernel, dim3(bl.grid), dim3(256), 0, cur_stream(), (const uint8_t *)oc.dev(), mc.st[0],

@@ -232,7 +232,7 @@ int Operand::commit() {
   if (!staged_ || !(dir_ & kOut) || bytes_ == 0) return SIMP_RT_OK;
   if (row_ && (size_t)(rows_[0] * rows_[1]) * row_ < bytes_) {
     // The bytes between the rows came in with the stage: they are what the caller had before
-    // the call, and another output of it may be there by now.
+    // the call, and another output may be there by now.
     std::unique_ptr<char, void (*)(void *)> all((char *)std::malloc(bytes_), std::free);
     if (!all) return set_error(SIMP_RT_ENOMEM, "staging %zu bytes back: out of host memory", bytes_);
     SIMP_HIP(hipMemcpyAsync(all.get(), dev_, bytes_, hipMemcpyDeviceToHost, cur_stream()));

@@ -51,7 +51,8 @@ class Operand {
   // The GPU that the caller's device memory lies on; -1 for anything else.
   int device() const { return device_; }
   // Says that an output is n0 x n1 rows of `row` bytes, st0 and st1 bytes apart: commit() then
-  // leaves the host bytes between them alone, where a call's other output may lie.
+  // leaves the host bytes between them alone, where the call's other output may lie, or
+  // that of another thread's call.
   void set_rows(int64_t n0, int64_t st0, int64_t n1, int64_t st1, size_t row);
   // Copies a staged output back to its host range (on the current stream).
   int commit();

@@ -595,6 +595,62 @@ def test_codes_and_scales_in_one_host_array(dev, m, k, torch_tensors):
         assert np.array_equal(out[:, :k], mx.values(codes, scales)[:, :k]) and (out[:, k:] == 7).all()
 
 
+@pytest.mark.parametrize("op", ["quantize", "dequantize", "product", "gate"])
+def test_two_threads_into_parts_of_one_host_array(dev, op):
+    """Each call writes its own columns of the rows that both share, in plain host memory, and
+    nothing of the other's."""
+    import torch
+    m, k, n = 300, 1024, 400
+    rng = np.random.default_rng(3)
+    x = [_x(rng, m, k) for _ in range(2)]
+    rows = [mx.codes(rng, r, k // 2) for r in (m, n, n)]
+    gate = op == "gate"
+    if op == "quantize":
+        buf = np.zeros((m, 2, k // 2), U)
+        want = [mx.quantize(v)[0] for v in x]
+        calls = [lambda i=i: sa.quantize_mx4(x[i], buf[:, i], np.empty((m, k // 32), U)) for i in range(2)]
+    elif op == "dequantize":
+        q = [mx.quantize(v) for v in x]
+        buf = np.zeros((m, 2, k), F)
+        want = [mx.values(*v) for v in q]
+        calls = [lambda i=i: sa.dequantize_mx4(*q[i], buf[:, i]) for i in range(2)]
+    else:
+        buf = np.zeros((m, 2, n), F)
+        a, *bs = rows[:2 + gate]
+        f = sa.swiglu_mx4 if gate else sa.matmul_mx4
+        flat = [*a, *[v for b in bs for v in b]]
+        want = [f(*flat, np.empty((m, n), F))] * 2  # (other tests say that it is right)
+        calls = [lambda i=i: f(*flat, buf[:, i]) for i in range(2)]
+    bad, meet = [], threading.Barrier(2)
+
+    def work(i):
+        torch.cuda.set_device(0)
+        st = torch.cuda.Stream()
+        sa.set_stream(st)
+        try:
+            for _ in range(30):
+                buf[:, i] = 0
+                meet.wait(60)
+                calls[i]()
+                if not np.array_equal(buf[:, i], want[i]):
+                    bad.append(i)
+                meet.wait(60)
+                if not np.array_equal(buf[:, i], want[i]):
+                    bad.append(i)
+        except Exception as e:  # a thread's error is the test's
+            bad.append(e)
+            meet.abort()
+        finally:
+            sa.set_stream(None)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad, bad[:4]
+
+
 def test_rows_far_apart(dev):
     """Rows whose offsets pass 32 bits, in every operand."""
     import torch
